@@ -489,6 +489,75 @@ int pla_kda_prefill_launch_states(
 int pla_kda_prefill_halved_sequences(const int32_t* raw_cu_seqlens, int N, int T, int H);
 
 /*
+ * Block tables and slot maps of a serving step from the requests' lengths (no counterpart in the reference).  Entry n of the
+ * batch has context[n] cached and query[n] new tokens and owns row mapping[n] (NULL: n) of block_table [table_rows, table_cols],
+ * of which held_blocks[row] entries are in use.  Index vectors are dense int32 or int64 (is_int64 flags).
+ *   Blocks held beyond ceil((context + query) / block_size) go back on the stack free_blocks[0 .. *free_count), in the order of
+ *   the batch, then of the row; then missing ones come off it in that order.  An entry is granted if the running sum of what
+ *   entries ask for, its own included, is on the stack (after the returns), and changes nothing if not.  Refused as well, and
+ *   asking for nothing: negative lengths, query > token_capacity, positions beyond the row, rows outside the table, a row that an
+ *   earlier entry names, token rows that end beyond token_capacity.
+ *   offsets [batch + 1] running sum of the query lengths in 0 .. token_capacity (others count 0), at most token_capacity;
+ *   seq_lens [batch] context + query, 0 if refused; positions and slots [token_capacity]: of token rows of granted entries, 0 and
+ *   -1 of all others.  With a mapping at most 8192 table rows.  Outputs and the four tables share no memory with the inputs.
+ */
+int pla_paged_kv_plan_launch(
+    const void* context, int context_wide, const void* query, int query_wide, const void* mapping, int mapping_wide,
+    int32_t* block_table, int64_t table_row_stride, int table_rows, int table_cols, int32_t* held_blocks,
+    int32_t* free_blocks, int32_t* free_count, int free_capacity, int batch, int block_size, int token_capacity,
+    int32_t* offsets, int32_t* seq_lens, int32_t* positions, int64_t* slots, void* stream);
+
+/*
+ * Norms of queries and keys for each head, position rotation and the write into a paged cache (no counterpart in the reference).
+ *   q [tokens,HQ,D], k, v [tokens,HKV,D] in act_dtype (PLA_BF16 or PLA_F16), D 64, 128 or 256; v NULL: no values
+ *   strides [16] in elements, multiples of 8: (token, head) of q, k, v, q_out, k_out, (block, token, head) of k_cache, v_cache
+ *   x rsqrt(mean(x^2) + eps) (weight + weight_offset) where the weight [D] (act_dtype, or float32) is not NULL
+ *   the first rotary_dim channels (a multiple of 16; 0: none) are turned by positions[t] * inv_freq[i], cosine and sine times
+ *       attention_factor; pairs (i, i + rotary_dim / 2), interleaved: (2i, 2i + 1)
+ *   q_out (may be q), k_out (may be k; NULL: not wanted), k_cache / v_cache [blocks,block_size,HKV,D] at slots[t] (negative or
+ *       past the cache: nowhere; no two tokens the same).  All pointers are 16-byte aligned, index vectors int32 or int64.
+ */
+int pla_qk_norm_rope_launch(
+    const void* q, const void* k, const void* v, const int64_t* strides, const void* positions, int positions_wide,
+    const void* q_weight, const void* k_weight, int weights_f32, float eps, float weight_offset,
+    const float* inv_freq, int rotary_dim, float attention_factor, int interleaved,
+    void* q_out, void* k_out, void* k_cache, void* v_cache, const void* slots, int slots_wide, int blocks, int block_size,
+    int tokens, int HQ, int HKV, int D, int act_dtype, void* stream);
+
+/* Workspace bytes (16-byte aligned; 0: none) of pla_paged_attention_launch, positions = table_cols * block_size; -1: not a valid shape. */
+int64_t pla_paged_attention_workspace_bytes(int batch, int HQ, int HKV, int head_dim, int max_query_len, int64_t positions);
+
+/*
+ * Attention of new tokens over a paged cache (no counterpart in the reference).
+ *   q, out, gate (NULL: none) [tokens,HQ,D] in act_dtype, (token, head) strides; k_cache, v_cache [blocks,block_size,HKV,D] with
+ *       common (block, token, head) strides; all strides multiples of 8 elements, pointers 16-byte aligned, block_size a
+ *       multiple of 16, D 64, 128 or 256, HQ a multiple of HKV
+ *   block_table int32 [table_rows,table_cols]; request n reads row mapping[n] (NULL: n)
+ *   offsets [batch + 1]: rows of request n's window, 1 .. max_query_len (at most 32) tokens (NULL: row n); a request whose
+ *       window is empty, longer or outside [0, tokens) is passed over.  seq_lens [batch]: cached tokens, window included.
+ *   token j of m sees positions below seq_len - m + j + 1 whose block is in the cache; a row that sees none is zeros.
+ *   out = softmax(scale q k^T) v [* sigmoid(gate)].  Calls that overlap in time need workspaces of their own.
+ */
+int pla_paged_attention_launch(
+    const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,
+    int64_t kv_block, int64_t kv_token, int64_t kv_head, int blocks, int block_size,
+    const int32_t* block_table, int64_t table_row_stride, int table_rows, int table_cols,
+    const void* mapping, int mapping_wide, const void* offsets, int offsets_wide, const void* seq_lens, int seq_lens_wide,
+    const void* gate, int64_t gate_token, int64_t gate_head, void* out, int64_t out_token, int64_t out_head,
+    float scale, int batch, int tokens, int max_query_len, int HQ, int HKV, int head_dim, int act_dtype,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * How pla_paged_attention_launch deals a batch out, from HOST copies of its offsets and lengths (host arithmetic only, for tests
+ * and for callers who log the plan): the segments of workgroup `worker`, up to `capacity` rows of (request, key-value head, block
+ * of query rows, first tile of 128 keys, tiles, workspace slot or -1 for a whole run, pieces of the run if this is its first).
+ * Returns their number, 0 for a worker without work, -1 for an invalid shape.
+ */
+int pla_paged_attention_segments(
+    const int32_t* offsets, const int32_t* seq_lens, int batch, int tokens, int HQ, int HKV, int head_dim, int max_query_len,
+    int64_t positions, int worker, int64_t* segments, int capacity);
+
+/*
  * Rows of the 128-row state tile a wavefront owns (8, 16 or 32) that a k-last launch with
  * rows_per_wave = 0 takes for a shape: the row count the auto-tuner measured for the nearest batch size
  * of the same (kernel, heads, dtypes) if the built-in table holds the shape, else the size thresholds.

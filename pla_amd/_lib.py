@@ -119,6 +119,28 @@ SIGNATURES = {
         _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64,
         _c_p, _c_p, _c_i64,
         _c_int, _c_int, _c_int, _c_int, _c_p, _c_p],
+    "pla_paged_kv_plan_launch": [
+        _c_p, _c_int, _c_p, _c_int, _c_p, _c_int,
+        _c_p, _c_i64, _c_int, _c_int, _c_p,
+        _c_p, _c_p, _c_int, _c_int, _c_int, _c_int,
+        _c_p, _c_p, _c_p, _c_p, _c_p],
+    "pla_qk_norm_rope_launch": [
+        _c_p, _c_p, _c_p, _c_p, _c_p, _c_int,
+        _c_p, _c_p, _c_int, _c_f, _c_f,
+        _c_p, _c_int, _c_f, _c_int,
+        _c_p, _c_p, _c_p, _c_p, _c_p, _c_int, _c_int, _c_int,
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_p],
+    "pla_paged_attention_segments": [
+        _c_p, _c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+        _c_i64, _c_int, _c_p, _c_int],
+    "pla_paged_attention_launch": [
+        _c_p, _c_i64, _c_i64, _c_p, _c_p,
+        _c_i64, _c_i64, _c_i64, _c_int, _c_int,
+        _c_p, _c_i64, _c_int, _c_int,
+        _c_p, _c_int, _c_p, _c_int, _c_p, _c_int,
+        _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+        _c_f, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+        _c_p, _c_i64, _c_p],
 }
 
 _lib = None
@@ -150,6 +172,8 @@ def load():
     lib.pla_kda_prefill_halved_sequences.argtypes = [_c_p, _c_int, _c_int, _c_int]
     lib.pla_kda_prefill_workspace_bytes.restype = _c_i64
     lib.pla_kda_prefill_workspace_bytes.argtypes = [_c_int, _c_int, _c_int]
+    lib.pla_paged_attention_workspace_bytes.restype = _c_i64
+    lib.pla_paged_attention_workspace_bytes.argtypes = [_c_int, _c_int, _c_int, _c_int, _c_int, _c_i64]
     lib.pla_tuned_rows_per_wave.restype = _c_int
     lib.pla_tuned_rows_per_wave.argtypes = [_c_int] * 7
     for name, argtypes in SIGNATURES.items():

@@ -17,7 +17,8 @@ LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libpla_gfx950.so")
 OBJ_DIR = os.path.join(HERE, "build")
 
-SOURCES = ["api.hip", "decode_k_last.hip", "decode_kda_mega.hip", "decode_kda_replay.hip", "commit_plan.hip", "prefill_gdn.hip", "prefill_kda.hip"]
+SOURCES = ["api.hip", "decode_k_last.hip", "decode_kda_mega.hip", "decode_kda_replay.hip", "commit_plan.hip", "prefill_gdn.hip", "prefill_kda.hip",
+           "paged_plan.hip", "qk_norm_rope.hip", "paged_attention.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-inline-asm",
@@ -63,10 +64,12 @@ def build_library(verbose=True):
 
 BINDING_SRC = os.path.join(CSRC, "decode_binding.cpp")
 PREFILL_BINDING_SRC = os.path.join(CSRC, "prefill_binding.cpp")
+PAGED_BINDING_SRC = os.path.join(CSRC, "paged_binding.cpp")
 
 # compiled host modules: package directory (relative to pla_amd) -> (source, extra defines)
 BINDINGS = {
     "decode": (BINDING_SRC, []),
+    os.path.join("decode", "paged"): (PAGED_BINDING_SRC, []),
     os.path.join("prefill", "flashqla"): (PREFILL_BINDING_SRC, ["-DPLA_BIND_FLASHQLA"]),
     os.path.join("prefill", "flashkdapro"): (PREFILL_BINDING_SRC, ["-DPLA_BIND_FLASHKDAPRO"]),
 }
@@ -111,7 +114,7 @@ def build_binding(verbose=True, package="decode"):
 
 
 def build_bindings(verbose=True):
-    """All compiled host modules (three g++ runs side by side)."""
+    """All compiled host modules (g++ runs side by side)."""
     with ThreadPoolExecutor(max_workers=len(BINDINGS)) as pool:
         return list(pool.map(lambda package: build_binding(verbose, package), BINDINGS))
 

@@ -1,0 +1,710 @@
+// Attention of one new token, or of a window of draft tokens, over a paged key-value cache:
+//
+//   o = sum_p softmax_p(scale q.k_p) v_p  [* sigmoid(gate)]      over the keys p that the token sees: p < length - window + j + 1
+//
+// for token j of a request's window.  The query heads of a key-value head and the tokens of the window are the rows of one
+// product, so keys and values are read once for all of them (blocks of 16 or 32 rows).
+//
+// Each wavefront takes 32 keys at a time, alone: keys and values go from memory to the registers in which the matrix
+// instructions want them, through no LDS, and nothing waits for another wavefront until the end of a run.
+//
+//   S^T = K Q^T    keys are the rows: lane (r, kb) loads 16 bytes of key r a step, any channels, as Q holds the same ones.
+//                  It gets the scores of query r at keys 4 kb .. 4 kb + 3 of both halves of the 32 keys,
+//   O^T = V^T P^T  which is the operand that the second product wants, if its contraction runs over the keys in that order:
+//                  lane (r, kb) loads channels 8 r .. 8 r + 7 of those eight keys, eight loads of which sixteen lanes cover a
+//                  row, and one v_perm_b32 a pair of values turns them into rows of V^T.  No value crosses a lane.
+//
+// A row's maximum and sum run along; the sum is that of the weights as they are rounded for the product (bf16: off by up to
+// 2^-9 of themselves, which then cancels where few keys carry the weight).  fp16 weights are scaled by 2^14, so that weights
+// down to 2^-38 of the largest still count.
+//
+// Values that no row of a block sees are replaced by zeros: their weight is zero, but zero times what an unused place of the
+// cache may hold need not be.  Within a window some rows see values that others do not.  Where one of those is infinite or NaN,
+// these values (at most 31, of two steps) are set aside and added row by row at the end of the run, to the rows that see them.
+//
+// Bound by HBM: 4 D bytes a key and head are needed once, for 4 D flops a row: a few dozen rows take a twentieth of what the
+// matrix cores can do at 6 TB/s.
+
+#include "decode_common.h"
+#include "mfma_bf16.h"
+#include "paged_schedule.h"
+
+namespace pla {
+
+struct PagedAttention {
+  const uint16_t* q; int64_t q_token, q_head;
+  const uint16_t *k, *v; int64_t kv_block, kv_token, kv_head;
+  const int32_t* table; int64_t table_row;
+  const void* mapping; int mapping_wide;
+  const void* offsets; int offsets_wide;          // NULL: token row n is request n
+  const void* lengths; int lengths_wide;
+  const uint16_t* gate; int64_t gate_token, gate_head;
+  uint16_t* out; int64_t out_token, out_head;
+  PagedShape shape;
+  int batch, blocks, block_size, table_rows;
+  float scale_log2;
+  int by_run, row_blocks;                         // descriptors: one a run, or one a worker; row blocks of the longest window
+  float* partial; float2* tops; int4* runs;
+
+  __device__ int64_t at(const void* base, int wide, int64_t i) const {
+    return wide ? static_cast<const int64_t*>(base)[i] : (int64_t) static_cast<const int32_t*>(base)[i];
+  }
+  __device__ PagedRequest request(int n) const {
+    const int64_t begin = offsets ? at(offsets, offsets_wide, n) : n, end = offsets ? at(offsets, offsets_wide, n + 1) : n + 1;
+    return paged_request(shape, begin, end, at(lengths, lengths_wide, n));
+  }
+};
+
+template <typename act_t> __device__ __forceinline__ f32x4_t mfma_act(bf16x8_t a, bf16x8_t b, f32x4_t c);
+template <> __device__ __forceinline__ f32x4_t mfma_act<bf16_t>(bf16x8_t a, bf16x8_t b, f32x4_t c) { return mfma16(a, b, c); }
+template <> __device__ __forceinline__ f32x4_t mfma_act<f16_t>(bf16x8_t a, bf16x8_t b, f32x4_t c) { return mfma16h(a, b, c); }
+
+template <typename act_t> constexpr float WEIGHT_SHIFT = 0.f;
+template <> constexpr float WEIGHT_SHIFT<f16_t> = 14.f;
+
+// Over the four lanes that hold a query's scores.
+__device__ __forceinline__ float query_max(float x) {
+  const LanePair a = swap_rows16(x);
+  const float y = fmaxf(a.lo, a.hi);
+  const LanePair b = swap_halves(y);
+  return fmaxf(b.lo, b.hi);
+}
+__device__ __forceinline__ float query_sum(float x) {
+  const LanePair a = swap_rows16(x);
+  const float y = a.lo + a.hi;
+  const LanePair b = swap_halves(y);
+  return b.lo + b.hi;
+}
+
+// The factor from maximum `m` to maximum `top` >= m; equal infinities are no step.
+__device__ __forceinline__ float rescale(float m, float top) { return m == top ? 1.f : __builtin_amdgcn_exp2f(m - top); }
+
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+template <int D> struct ValueWords { static constexpr int N = D == 64 ? 2 : 4; };      // 32-bit words of a lane's channels, a chunk
+
+// Keys in flight, values in flight and the state of the rows of one wavefront.
+template <typename act_t, int D, int RT>
+struct Wave {
+  static constexpr int STEPS = D / 32;                        // of the contraction of K Q^T
+  static constexpr int WORDS = ValueWords<D>::N, CHUNKS = D == 256 ? 2 : 1, TILES = 2 * WORDS;
+  static constexpr int LANE_CHANNELS = 2 * WORDS;             // channels of a value that a lane loads, a chunk of 16 times as many
+  u32x4_t k[2][STEPS];
+  uint32_t v[8][CHUNKS][WORDS];
+  // Large heads leave no registers for the queries: they are read from LDS, once a step.
+  static constexpr bool QUERIES_IN_LDS = D == 256;
+  u32x4_t q[RT][QUERIES_IN_LDS ? 1 : STEPS];
+  f32x4_t o[RT][CHUNKS][TILES];
+  float top[RT], sum[RT];
+  int limit[RT];
+  int set_aside;                                              // first key of the step whose partly seen values are added at the end, or -1
+};
+
+template <typename act_t, int D, int RT>
+__device__ __forceinline__ void load_keys(Wave<act_t, D, RT>& w, const uint16_t* base, const int64_t (&place)[2], uint32_t lane_offset) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const auto p = as_global(reinterpret_cast<const char*>(base + place[h]));
+#pragma unroll
+    for (int c = 0; c < Wave<act_t, D, RT>::STEPS; ++c) w.k[h][c] = *reinterpret_cast<global_ptr<const u32x4_t>>(p + lane_offset + 64 * c);
+  }
+}
+
+template <typename act_t, int D, int RT>
+__device__ __forceinline__ void load_values(Wave<act_t, D, RT>& w, const uint16_t* base, const int64_t (&place)[2], uint32_t lane_offset,
+                                            int64_t token_bytes) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const auto p = as_global(reinterpret_cast<const char*>(base + place[i / 4])) + (i & 3) * token_bytes;
+#pragma unroll
+    for (int c = 0; c < Wave<act_t, D, RT>::CHUNKS; ++c) {
+      if constexpr (Wave<act_t, D, RT>::WORDS == 4) {
+        const u32x4_t x = *reinterpret_cast<global_ptr<const u32x4_t>>(p + lane_offset + 256 * c);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) w.v[i][c][y] = x[y];
+      } else {
+        const u32x2_t x = *reinterpret_cast<global_ptr<const u32x2_t>>(p + lane_offset);
+        w.v[i][c][0] = x[0]; w.v[i][c][1] = x[1];
+      }
+    }
+  }
+}
+
+// For v_perm_b32 on the words of two keys that hold channels 2 j and 2 j + 1 of one each: channel 2 j (odd: 2 j + 1) of both,
+// zero where a key is left out.
+__device__ __forceinline__ uint32_t selection(int odd, bool first, bool second) {
+  return (first ? odd ? 0x0302u : 0x0100u : 0x0c0cu) | (second ? odd ? 0x07060000u : 0x05040000u : 0x0c0c0000u);
+}
+// Bit 15 or 31 is set if all bits of the exponent of that half are.
+template <typename act_t>
+__device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
+  return __is_same(act_t, bf16_t) ? (pair & 0x7f807f80u) + 0x00800080u : (pair & 0x7c007c00u) + 0x04000400u;
+}
+
+// One step of a wavefront: scores of 32 keys from key0 on, their weights, and the weighted values.  `next`: issues the loads of
+// the step after (keys once these are used, values once those are).
+template <typename act_t, int D, int RT, typename NextKeys, typename NextValues>
+__device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, const u32x4_t* queries, float scale_log2, const bool (&there)[2],
+                                       int key0, int least, int end, NextKeys next_keys, NextValues next_values) {
+  using W = Wave<act_t, D, RT>;
+  const int kb = (threadIdx.x & 63) >> 4;
+  f32x4_t s[RT][2];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[t][h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < W::STEPS; ++c)
+        s[t][h] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, w.k[h][c]),
+                                  __builtin_bit_cast(bf16x8_t, W::QUERIES_IN_LDS ? queries[(t * W::STEPS + c) * 64 + (threadIdx.x & 63)]
+                                                                                 : w.q[t][W::QUERIES_IN_LDS ? 0 : c]), s[t][h]);
+    }
+  next_keys();
+
+  const bool masked = key0 + 32 > least || !there[0] || !there[1];          // some row does not see some key
+  bf16x8_t packed[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = s[t][i / 4][i & 3] * scale_log2;
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = key0 + 16 * (i / 4) + 4 * kb + (i & 3);
+        x[i] = (key < w.limit[t]) & there[i / 4] ? x[i] : -INFINITY;
+      }
+    }
+    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    top = fmaxf(query_max(top), w.top[t]);
+    if (__ballot(top > w.top[t]) != 0) {
+      const float f = rescale(w.top[t], top);
+      w.sum[t] *= f;
+#pragma unroll
+      for (int c = 0; c < W::CHUNKS; ++c)
+#pragma unroll
+        for (int j = 0; j < W::TILES; ++j) w.o[t][c][j] *= f;
+      w.top[t] = top;
+    }
+    const float zero = (top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - zero);
+    const uint4 word = make_uint4(pack2<act_t>(x[0], x[1]), pack2<act_t>(x[2], x[3]), pack2<act_t>(x[4], x[5]), pack2<act_t>(x[6], x[7]));
+    const uint32_t u[4] = {word.x, word.y, word.z, word.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w.sum[t] += lo16<act_t>(u[i]) + hi16<act_t>(u[i]);
+    packed[t] = __builtin_bit_cast(bf16x8_t, word);
+  }
+
+  // Values of two keys are turned by one byte selection, which also puts zeros in the place of values that no row sees.
+  const int key = key0 + 4 * kb;
+  uint32_t select[2][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    select[0][i] = 0x05040100u;
+    select[1][i] = 0x07060302u;
+  }
+  if (masked) {
+    int stop = end;
+    if (least < end && key0 + 32 > least) {       // some rows see values that others do not
+      uint32_t odd = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = key + 16 * (i / 4) + (i & 3);
+        const bool partly = (at >= least) & (at < end) & there[i / 4];
+#pragma unroll
+        for (int c = 0; c < W::CHUNKS; ++c)
+#pragma unroll
+          for (int j = 0; j < W::WORDS; ++j) odd |= partly ? not_finite<act_t>(w.v[i][c][j]) : 0u;
+      }
+      if (__ballot((odd & 0x80008000u) != 0) != 0) {
+        stop = least;
+        w.set_aside = key0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = key + 16 * (i / 2) + 2 * (i & 1);
+      const bool first = (at < stop) & there[i / 2], second = (at + 1 < stop) & there[i / 2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) select[x][i] = selection(x, first, second);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < W::CHUNKS; ++c)
+#pragma unroll
+    for (int j = 0; j < W::TILES; ++j) {
+      u32x4_t a;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(w.v[2 * i + 1][c][j / 2], w.v[2 * i][c][j / 2], select[j & 1][i]);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) w.o[t][c][j] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, a), packed[t], w.o[t][c][j]);
+    }
+  next_values();
+}
+
+// The weighted values of keys [first, last) for one row, into the D / 16 channels of it that a thread has; the sixteen threads
+// of a row form its scores together.
+template <typename act_t, int D>
+__device__ __forceinline__ void add_set_aside(const PagedAttention& p, const PagedRequest& req, int kv_head, int row, int channel,
+                                              const int32_t* pages, int first, int last, float top, float (&o)[D / 16]) {
+  const int j = row / p.shape.group, head = kv_head * p.shape.group + row - j * p.shape.group;
+  const uint16_t* q = p.q + (req.begin + j) * p.q_token + head * p.q_head + channel;
+  last = min(last, paged_limit(p.shape, req, row));
+  for (int key = first; key < last; ++key) {
+    const int page = key / p.block_size, entry = pages[page];
+    if (entry < 0 || entry >= p.blocks) continue;
+    const int64_t at = entry * p.kv_block + (key - page * p.block_size) * p.kv_token + kv_head * p.kv_head + channel;
+    float score = 0.f;
+    for (int i = 0; i < D / 16; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
+    score = row16_allreduce(score) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
+    const float weight = to_float(from_float<act_t>(__builtin_amdgcn_exp2f(score)));
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[i] = fmaf(weight, to_float(act_t{p.v[at + i]}), o[i]);
+  }
+}
+
+// Workgroups a CU: as many as its registers hold.
+constexpr int residency(int D, int row_tiles) {
+  return D == 256 ? (row_tiles == 2 ? 1 : 2) : D == 128 ? (row_tiles == 2 ? 2 : 3) : row_tiles == 2 ? 3 : 4;
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
+}
+
+template <typename act_t, int D, int RT>
+__global__ __launch_bounds__(256, residency(D, RT)) void paged_attention_kernel(const PagedAttention p) {
+  using W = Wave<act_t, D, RT>;
+  constexpr int PITCH = D + 4;                    // floats of a row in LDS: rows of a quad of lanes start in different banks
+  __shared__ __align__(16) float outs[4][16][PITCH];
+  __shared__ __align__(16) u32x4_t queries[W::QUERIES_IN_LDS ? RT * W::STEPS * 64 : 1];
+  __shared__ float2 tops[4][16 * RT];
+  __shared__ int aside[4];
+  __shared__ int64_t sums[4];
+  __shared__ int64_t start_offset;
+  __shared__ int start_request;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, kb = lane >> 4;
+
+  // The line of work: all workgroups add up the whole batch, a thread a contiguous share of the requests.
+  const int share = (p.batch + 255) / 256, first = min(tid * share, p.batch), last = min(first + share, p.batch);
+  int64_t mine = 0;
+  for (int n = first; n < last; ++n) {
+    const PagedRequest req = p.request(n);
+    mine += paged_weight(p.shape, req);
+    if (p.by_run && p.runs && blockIdx.x == 0)    // runs that nobody has
+      for (int h = 0; h < p.shape.heads; ++h)
+        for (int b = req.blocks; b < p.row_blocks; ++b) p.runs[(n * p.shape.heads + h) * p.row_blocks + b] = int4{0, 0, 0, 0};
+  }
+  int64_t below = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t x = __shfl_up(below, d);
+    if (lane >= d) below += x;
+  }
+  if (lane == 63) sums[wave] = below;
+  __syncthreads();
+  int64_t total = 0;
+  below -= mine;
+  for (int i = 0; i < 4; ++i) {
+    if (i < wave) below += sums[i];
+    total += sums[i];
+  }
+  total = uniform64(total);
+  const int workers = paged_workers(gridDim.x, total);
+  // neighbours in the line on one XCD: row blocks of the same keys share its L2
+  const int worker = (int)blockIdx.x >= workers || workers < 8 ? (int)blockIdx.x
+                                                                : ((int)blockIdx.x & 7) * (workers / 8) + ((int)blockIdx.x >> 3);
+  if (!p.by_run && p.runs && tid == 0) p.runs[worker] = int4{0, 0, 0, 0};
+  if (worker >= workers) return;
+  int64_t unit = paged_stretch(worker, workers, total);
+  const int64_t stretch_end = paged_stretch(worker + 1, workers, total);
+  if (below <= unit && unit < below + mine) {
+    int64_t left = unit - below;
+    int n = first;
+    for (;; ++n) {
+      const int64_t weight = paged_weight(p.shape, p.request(n));
+      if (left < weight) break;
+      left -= weight;
+    }
+    start_request = n;
+    start_offset = left;
+  }
+  __syncthreads();
+  int n = __builtin_amdgcn_readfirstlane(start_request);
+  int64_t offset = uniform64(start_offset);
+
+  const uint32_t key_lane = (uint32_t)(r * p.kv_token + 8 * kb) * 2;
+  const uint32_t value_lane = (uint32_t)(4 * kb * p.kv_token + W::LANE_CHANNELS * r) * 2;
+  W w;
+
+  while (unit < stretch_end) {
+    const PagedRequest req = p.request(n);
+    if (offset >= paged_weight(p.shape, req)) {   // done with it (or passed over)
+      offset = 0;
+      ++n;
+      continue;
+    }
+    const PagedSegment seg = paged_segment(req, offset, unit, stretch_end, worker, workers, total);
+    unit += seg.tiles;
+    offset += seg.tiles;
+    const int row0 = seg.block * p.shape.rows, rows = min(req.window * p.shape.group - row0, p.shape.rows);
+    const int least = paged_limit(p.shape, req, row0), end = paged_limit(p.shape, req, row0 + rows - 1);
+    const int64_t table_row = p.mapping ? p.at(p.mapping, p.mapping_wide, n) : n;
+    const bool has_row = table_row >= 0 && table_row < p.table_rows;
+    const int32_t* pages = p.table + (has_row ? table_row : 0) * p.table_row;
+    const uint16_t* k_base = p.k + seg.head * p.kv_head;
+    const uint16_t* v_base = p.v + seg.head * p.kv_head;
+
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int row = 16 * t + r, j = (row0 + row) / p.shape.group, g = row0 + row - j * p.shape.group;
+      const bool real = row < rows;
+      const uint16_t* src = p.q + (req.begin + j) * p.q_token + (seg.head * p.shape.group + g) * p.q_head + 8 * kb;
+#pragma unroll
+      for (int c = 0; c < W::STEPS; ++c) {
+        const u32x4_t x = real ? *reinterpret_cast<const u32x4_t*>(src + 32 * c) : u32x4_t{0, 0, 0, 0};
+        if constexpr (!W::QUERIES_IN_LDS) w.q[t][c] = x;
+        else if (wave == 0) queries[(t * W::STEPS + c) * 64 + lane] = x;
+      }
+      w.limit[t] = real ? paged_limit(p.shape, req, row0 + row) : 0;
+      w.top[t] = -INFINITY;
+      w.sum[t] = 0.f;
+#pragma unroll
+      for (int c = 0; c < W::CHUNKS; ++c)
+#pragma unroll
+        for (int x = 0; x < W::TILES; ++x) w.o[t][c][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    if constexpr (W::QUERIES_IN_LDS) __syncthreads();
+
+    w.set_aside = -1;
+    // Steps of this wavefront: those of its keys that are below `end`.  Lane 2 i + h looks up where half h of step i lies,
+    // 32 steps ahead of their use.
+    const int key_first = seg.tile * PAGED_TILE + 32 * wave;
+    const int steps = end > key_first ? min((end - key_first - 1) / PAGED_TILE + 1, seg.tiles) : 0;
+    struct Places { int lo, hi; uint64_t there; };
+    auto look_up = [&](int step0) {
+      const int key = key_first + (step0 + (lane >> 1)) * PAGED_TILE + 16 * (lane & 1);
+      bool there = has_row && step0 + (lane >> 1) < steps && key < end;
+      int64_t place = 0;
+      if (there) {
+        const int page = key / p.block_size, entry = pages[page];
+        there = entry >= 0 && entry < p.blocks;
+        place = there ? entry * p.kv_block + (key - page * p.block_size) * p.kv_token : 0;
+      }
+      return Places{(int)place, (int)(place >> 32), __ballot(there)};
+    };
+    Places now = look_up(0), then = look_up(32);
+    auto place_of = [&](int step, int64_t (&place)[2], bool (&there)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = (step & 31) * 2 + h;
+        place[h] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(now.lo, at) |
+                             (uint64_t)(uint32_t)__builtin_amdgcn_readlane(now.hi, at) << 32);
+        there[h] = now.there >> at & 1;
+      }
+    };
+    if (steps > 0) {
+      int64_t place[2], next_place[2];
+      bool there[2], next_there[2];
+      place_of(0, place, there);
+      load_keys(w, k_base, place, key_lane);
+      load_values(w, v_base, place, value_lane, p.kv_token * 2);
+      for (int step = 0; step < steps; ++step) {
+        const bool more = step + 1 < steps;
+        if (more && (step + 1) % 32 == 0) {
+          now = then;
+          then = look_up(step + 1 + 32);
+        }
+        // the last step fetches its own keys once more, from the caches: a branch around the loads costs the compiler the registers
+        place_of(more ? step + 1 : step, next_place, next_there);
+        attend(w, queries, p.scale_log2, there, key_first + step * PAGED_TILE, least, end,
+               [&] { load_keys(w, k_base, next_place, key_lane); },
+               [&] { load_values(w, v_base, next_place, value_lane, p.kv_token * 2); });
+#pragma unroll
+        for (int h = 0; h < 2; ++h) { place[h] = next_place[h]; there[h] = next_there[h]; }
+      }
+    }
+
+    // The four wavefronts' rows together.
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const float sum = query_sum(w.sum[t]);
+      if (kb == 0) tops[wave][16 * t + r] = float2{w.top[t], sum};
+    }
+    if (lane == 0) aside[wave] = w.set_aside;
+    __syncthreads();
+    const int out_row = tid >> 4, out_channel = (tid & 15) * (D / 16);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if (16 * t >= rows) break;
+      float top = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) top = fmaxf(top, tops[x][16 * t + r].x);
+      const float f = rescale(w.top[t], top);
+#pragma unroll
+      for (int c = 0; c < W::CHUNKS; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int j = 0; j < W::TILES; j += 4) {
+            const int channel = 128 * c + W::LANE_CHANNELS * (4 * kb + e) + j;
+            *reinterpret_cast<float4*>(&outs[wave][r][channel]) =
+                float4{w.o[t][c][j][e] * f, w.o[t][c][j + 1][e] * f, w.o[t][c][j + 2][e] * f, w.o[t][c][j + 3][e] * f};
+          }
+      __syncthreads();
+      if (16 * t + out_row < rows) {
+        float row_top = -INFINITY, row_sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) row_top = fmaxf(row_top, tops[x][16 * t + out_row].x);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) row_sum += tops[x][16 * t + out_row].y * rescale(tops[x][16 * t + out_row].x, row_top);
+        float o[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 4) {
+          float4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float4 b = *reinterpret_cast<const float4*>(&outs[x][out_row][out_channel + i]);
+            a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+          }
+          o[i] = a.x; o[i + 1] = a.y; o[i + 2] = a.z; o[i + 3] = a.w;
+        }
+        for (int x = 0; x < 4; ++x)
+          if (aside[x] >= 0) add_set_aside<act_t, D>(p, req, seg.head, row0 + 16 * t + out_row, out_channel, pages, max(aside[x], least), min(aside[x] + 32, end), row_top, o);
+        if (seg.slot < 0) {
+          const int row = row0 + 16 * t + out_row, j = row / p.shape.group, head = seg.head * p.shape.group + row - j * p.shape.group;
+          const float norm = row_sum == 0.f ? 0.f : 1.0f / row_sum;         // no key: zeros
+          const int64_t token = req.begin + j;
+          uint32_t word[D / 32];
+#pragma unroll
+          for (int i = 0; i < D / 16; i += 2) {
+            float a = o[i] * norm, b = o[i + 1] * norm;
+            if (p.gate) {
+              const uint32_t g = *reinterpret_cast<const uint32_t*>(p.gate + token * p.gate_token + head * p.gate_head + out_channel + i);
+              a *= 1.0f / (1.0f + __expf(-lo16<act_t>(g)));
+              b *= 1.0f / (1.0f + __expf(-hi16<act_t>(g)));
+            }
+            word[i / 2] = pack2<act_t>(a, b);
+          }
+          uint16_t* dst = p.out + token * p.out_token + head * p.out_head + out_channel;
+          if constexpr (D == 64) {
+            *reinterpret_cast<uint2*>(dst) = uint2{word[0], word[1]};
+          } else {
+#pragma unroll
+            for (int i = 0; i < D / 128; ++i)
+              reinterpret_cast<uint4*>(dst)[i] = uint4{word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]};
+          }
+        } else {
+          const int64_t row = (int64_t)seg.slot * (16 * RT) + 16 * t + out_row;
+#pragma unroll
+          for (int i = 0; i < D / 16; i += 4)
+            *reinterpret_cast<float4*>(p.partial + row * D + out_channel + i) = float4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+          if ((tid & 15) == 0) p.tops[row] = float2{row_top, row_sum};
+        }
+      }
+      __syncthreads();
+    }
+    if (tid == 0 && p.runs && seg.pieces > 0) {
+      // who joins this run, if it is in pieces
+      const int run = (n * p.shape.heads + seg.head) * p.row_blocks + seg.block;
+      if (p.by_run) p.runs[run] = int4{n, run - n * p.shape.heads * p.row_blocks, worker, seg.slot < 0 ? 0 : seg.pieces};
+      else if (seg.slot >= 0) p.runs[worker] = int4{n, run - n * p.shape.heads * p.row_blocks, worker, seg.pieces};
+    }
+  }
+}
+
+// Pieces of a run to its output.  A workgroup a run and every gridDim.y-th of its rows; its wavefronts share the pieces, a
+// lane has D / 64 channels.
+template <typename act_t, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttention p) {
+  constexpr int LANE = D / 64;
+  __shared__ float outs[4][D];
+  const int4 run = p.runs[blockIdx.x];
+  const int pieces = run.w;
+  if (pieces < 2) return;
+  const int n = run.x, head = run.y / p.row_blocks, block = run.y - head * p.row_blocks, worker = run.z;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, R = p.shape.rows;
+  const PagedRequest req = p.request(n);
+  const int row0 = block * R, rows = min(req.window * p.shape.group - row0, R);
+  auto slot_row = [&](int piece, int row) { return (int64_t)(piece == 0 ? 2 * worker + 1 : 2 * (worker + piece)) * R + row; };
+  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+    float top = -INFINITY, sum = 0.f;
+    for (int i = lane; i < pieces; i += 64) top = fmaxf(top, p.tops[slot_row(i, row)].x);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    for (int i = lane; i < pieces; i += 64) {
+      const float2 x = p.tops[slot_row(i, row)];
+      sum += x.y * rescale(x.x, top);
+    }
+    sum = wave64_allreduce(sum);
+    float o[LANE] = {};
+    for (int i = wave; i < pieces; i += 4) {
+      const int64_t at = slot_row(i, row);
+      const float f = rescale(p.tops[at].x, top);
+#pragma unroll
+      for (int x = 0; x < LANE; ++x) o[x] = fmaf(p.partial[at * D + LANE * lane + x], f, o[x]);
+    }
+#pragma unroll
+    for (int x = 0; x < LANE; ++x) outs[wave][LANE * lane + x] = o[x];
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+      const int channel = 2 * threadIdx.x, j = (row0 + row) / p.shape.group, q_head = head * p.shape.group + row0 + row - j * p.shape.group;
+      const float norm = sum == 0.f ? 0.f : 1.0f / sum;
+      float a = 0.f, b = 0.f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) { a += outs[x][channel]; b += outs[x][channel + 1]; }
+      a *= norm;
+      b *= norm;
+      const int64_t token = req.begin + j;
+      if (p.gate) {
+        const uint32_t g = *reinterpret_cast<const uint32_t*>(p.gate + token * p.gate_token + q_head * p.gate_head + channel);
+        a *= 1.0f / (1.0f + __expf(-lo16<act_t>(g)));
+        b *= 1.0f / (1.0f + __expf(-hi16<act_t>(g)));
+      }
+      *reinterpret_cast<uint32_t*>(p.out + token * p.out_token + q_head * p.out_head + channel) = pack2<act_t>(a, b);
+    }
+    __syncthreads();
+  }
+}
+
+// How a call is launched: host arithmetic from what the host knows.
+struct PagedLaunch {
+  int row_tiles, rows, row_blocks, workers, by_run, join_rows;
+  bool split;                             // whether a run can be cut at all
+  int64_t runs, bytes, tops_at, runs_at;  // workspace: partial outputs, maxima and sums, runs
+};
+
+static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query, int64_t positions) {
+  PagedLaunch l{};
+  const int window_rows = max_query * (HQ / HKV);
+  l.row_tiles = window_rows <= 16 ? 1 : 2;
+  l.rows = 16 * l.row_tiles;
+  l.row_blocks = (window_rows + l.rows - 1) / l.rows;
+  l.runs = (int64_t)batch * HKV * l.row_blocks;
+  const int64_t tiles = positions > 0 ? (positions - 1) / PAGED_TILE + 1 : 1, most = 256 * residency(D, l.row_tiles);
+  l.workers = (int)(l.runs * tiles < most ? l.runs * tiles : most);
+  l.split = tiles > 1;
+  l.by_run = l.runs <= l.workers;
+  const int64_t groups = l.by_run ? l.runs : l.workers;
+  const int row_slices = (int)(2048 / (groups > 0 ? groups : 1)), used = window_rows < l.rows ? window_rows : l.rows;
+  l.join_rows = row_slices < 1 ? 1 : row_slices < used ? row_slices : used;
+  if (l.split) {
+    const int64_t slots = 2 * (int64_t)l.workers;
+    l.tops_at = slots * l.rows * D * 4;
+    l.runs_at = l.tops_at + slots * l.rows * 8;
+    l.bytes = (l.runs_at + l.workers * 16 + 255) / 256 * 256;
+  }
+  return l;
+}
+
+template <typename act_t, int D>
+static void launch_paged_attention(const PagedAttention& p, const PagedLaunch& l, hipStream_t s) {
+  if (l.row_tiles == 1) paged_attention_kernel<act_t, D, 1><<<l.workers, 256, 0, s>>>(p);
+  else paged_attention_kernel<act_t, D, 2><<<l.workers, 256, 0, s>>>(p);
+  if (l.split) paged_join_kernel<act_t, D><<<dim3((unsigned)(l.by_run ? l.runs : l.workers), l.join_rows), 256, 0, s>>>(p);
+}
+
+static int check_shape(int batch, int HQ, int HKV, int D, int max_query, int64_t positions) {
+  PLA_REQUIRE(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got %d", D);
+  PLA_REQUIRE(HKV > 0 && HQ >= HKV && HQ % HKV == 0, "query heads must be a positive multiple of key-value heads");
+  PLA_REQUIRE(max_query >= 1 && max_query <= 32, "max_query_len must be between 1 and 32");
+  PLA_REQUIRE(batch >= 0 && (int64_t)batch * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "too many requests");
+  PLA_REQUIRE(positions >= 0 && positions <= (1 << 30), "a row of the block table must hold at most 2^30 positions");
+  return 0;
+}
+
+}  // namespace pla
+
+extern "C" int64_t pla_paged_attention_workspace_bytes(int batch, int HQ, int HKV, int head_dim, int max_query_len, int64_t positions) {
+  using namespace pla;
+  if (check_shape(batch, HQ, HKV, head_dim, max_query_len, positions)) return -1;
+  return batch == 0 ? 0 : paged_launch(batch, HQ, HKV, head_dim, max_query_len, positions).bytes;
+}
+
+extern "C" int pla_paged_attention_segments(
+    const int32_t* offsets, const int32_t* seq_lens, int batch, int tokens, int HQ, int HKV, int head_dim, int max_query_len,
+    int64_t positions, int worker, int64_t* segments, int capacity) {
+  using namespace pla;
+  if (check_shape(batch, HQ, HKV, head_dim, max_query_len, positions) || batch == 0 || !offsets || !seq_lens) return -1;
+  const PagedLaunch l = paged_launch(batch, HQ, HKV, head_dim, max_query_len, positions);
+  const PagedShape shape{HKV, HQ / HKV, l.rows, max_query_len, tokens, positions};
+  auto request = [&](int n) { return paged_request(shape, offsets[n], offsets[n + 1], seq_lens[n]); };
+  int64_t total = 0;
+  for (int n = 0; n < batch; ++n) total += paged_weight(shape, request(n));
+  const int workers = paged_workers(l.workers, total);
+  if (worker < 0 || worker >= workers) return 0;
+  int64_t unit = paged_stretch(worker, workers, total), offset = unit;
+  const int64_t end = paged_stretch(worker + 1, workers, total);
+  int found = 0;
+  for (int n = 0; unit < end;) {
+    const PagedRequest r = request(n);
+    if (offset >= paged_weight(shape, r)) {
+      offset -= paged_weight(shape, r);
+      ++n;
+      continue;
+    }
+    const PagedSegment s = paged_segment(r, offset, unit, end, worker, workers, total);
+    if (found < capacity) {
+      const int64_t row[7] = {n, s.head, s.block, s.tile, s.tiles, s.slot, s.pieces};
+      for (int i = 0; i < 7; ++i) segments[7 * found + i] = row[i];
+    }
+    ++found;
+    unit += s.tiles;
+    offset += s.tiles;
+  }
+  return found;
+}
+
+extern "C" int pla_paged_attention_launch(
+    const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,
+    int64_t kv_block, int64_t kv_token, int64_t kv_head, int blocks, int block_size,
+    const int32_t* block_table, int64_t table_row_stride, int table_rows, int table_cols,
+    const void* mapping, int mapping_wide, const void* offsets, int offsets_wide, const void* seq_lens, int seq_lens_wide,
+    const void* gate, int64_t gate_token, int64_t gate_head, void* out, int64_t out_token, int64_t out_head,
+    float scale, int batch, int tokens, int max_query_len, int HQ, int HKV, int head_dim, int act_dtype,
+    void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace pla;
+  PLA_REQUIRE(block_size > 0 && block_size % 16 == 0, "block_size must be a multiple of 16");
+  const int64_t positions = (int64_t)table_cols * block_size;
+  if (const int bad = check_shape(batch, HQ, HKV, head_dim, max_query_len, positions)) return bad;
+  PLA_REQUIRE(act_dtype == PLA_BF16 || act_dtype == PLA_F16, "activations must be bf16 or fp16");
+  PLA_REQUIRE(tokens >= 0 && table_rows >= 0 && table_cols >= 0 && table_row_stride >= table_cols, "invalid dimensions");
+  PLA_REQUIRE(offsets || max_query_len >= 1, "invalid dimensions");
+  if (batch == 0 || tokens == 0) return 0;
+  PLA_REQUIRE(offsets || batch <= tokens, "more requests than token rows");
+  PLA_REQUIRE(mapping || batch <= table_rows, "more requests than rows of the block table");
+  PLA_REQUIRE(q && k_cache && v_cache && seq_lens && out, "null tensor pointer");
+  PLA_REQUIRE(block_table || table_rows == 0 || table_cols == 0, "null tensor pointer");
+  PLA_REQUIRE(blocks > 0, "the cache must hold a block");
+  for (const int64_t s : {q_token, q_head, kv_block, kv_token, kv_head, gate_token, gate_head, out_token, out_head})
+    PLA_REQUIRE(s % 8 == 0, "rows must be 16-byte aligned");
+  for (const void* x : {q, k_cache, v_cache, gate, (const void*)out})
+    PLA_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0, "rows must be 16-byte aligned");
+  PLA_REQUIRE(kv_token >= 0 && kv_token < (1 << 24), "the cache's token stride must be below 2^24");
+  const PagedLaunch l = paged_launch(batch, HQ, HKV, head_dim, max_query_len, positions);
+  PLA_REQUIRE(workspace_bytes >= l.bytes && (l.bytes == 0 || workspace), "workspace too small: %lld bytes needed", (long long)l.bytes);
+  PLA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be 16-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  const PagedAttention p{(const uint16_t*)q, q_token, q_head, (const uint16_t*)k_cache, (const uint16_t*)v_cache, kv_block, kv_token,
+                         kv_head, block_table, table_row_stride, mapping, mapping_wide, offsets, offsets_wide, seq_lens, seq_lens_wide,
+                         (const uint16_t*)gate, gate_token, gate_head, (uint16_t*)out, out_token, out_head,
+                         PagedShape{HKV, HQ / HKV, l.rows, max_query_len, tokens, positions},
+                         batch, blocks, block_size, table_rows, scale * 1.44269504088896341f, l.by_run, l.row_blocks,
+                         l.split ? reinterpret_cast<float*>(ws) : nullptr, l.split ? reinterpret_cast<float2*>(ws + l.tops_at) : nullptr,
+                         l.split ? reinterpret_cast<int4*>(ws + l.runs_at) : nullptr};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (act_dtype == PLA_BF16) {
+    if (head_dim == 64) launch_paged_attention<bf16_t, 64>(p, l, s);
+    else if (head_dim == 128) launch_paged_attention<bf16_t, 128>(p, l, s);
+    else launch_paged_attention<bf16_t, 256>(p, l, s);
+  } else {
+    if (head_dim == 64) launch_paged_attention<f16_t, 64>(p, l, s);
+    else if (head_dim == 128) launch_paged_attention<f16_t, 128>(p, l, s);
+    else launch_paged_attention<f16_t, 256>(p, l, s);
+  }
+  return check_launch("paged_attention_kernel");
+}

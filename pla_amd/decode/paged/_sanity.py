@@ -1,0 +1,70 @@
+"""Checks of values under ``PLA_SANITY_CHECK=1``: what the operators would pass over or leave out without a word.
+
+Every rejection raises ``RuntimeError("PLA_SANITY_CHECK [op]: ...")`` before anything is launched.  The checks read device memory
+and are skipped while a stream is being captured.
+"""
+
+import torch
+
+
+def _fail(op, msg):
+    raise RuntimeError(f"PLA_SANITY_CHECK [{op}]: {msg}")
+
+
+def _capturing():
+    return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+
+
+def check_plan(blocks, context_lens, query_lens, request_indices):
+    if _capturing():
+        return
+    op, (rows, cols) = "paged_kv_plan", blocks.block_table.shape
+    context, query = context_lens.tolist(), query_lens.tolist()
+    if any(x < 0 for x in context + query):
+        _fail(op, "lengths must not be negative")
+    if any(-(-(c + q) // blocks.block_size) > cols for c, q in zip(context, query)):
+        _fail(op, "a request's positions pass its row of the block table")
+    if request_indices is not None:
+        index = request_indices.tolist()
+        if len(set(index)) != len(index) or any(not 0 <= x < rows for x in index):
+            _fail(op, "request_indices must be different rows of the block table")
+    height, held = blocks.free_count.item(), blocks.held_blocks.tolist()
+    if not 0 <= height <= blocks.free_blocks.numel() or any(not 0 <= h <= cols for h in held):
+        _fail(op, "free_count and held_blocks must lie within their tables")
+    owned = blocks.free_blocks[:height].tolist()
+    for row, h in zip(blocks.block_table.tolist(), held):
+        owned += row[:h]
+    if len(set(owned)) != len(owned):
+        _fail(op, "a block is held twice")
+
+
+def check_slots(slot_mapping, k_cache):
+    if slot_mapping is None or k_cache is None or _capturing():
+        return
+    slots = [x for x in slot_mapping.tolist() if x >= 0]
+    if any(x >= k_cache.size(0) * k_cache.size(1) for x in slots):
+        _fail("fused_qk_norm_rope", "a slot is past the cache")
+    if len(set(slots)) != len(slots):
+        _fail("fused_qk_norm_rope", "two tokens name one slot")
+
+
+def check_attention(q, k_cache, block_table, seq_lens, query_start_loc, request_indices, max_query_len):
+    if _capturing():
+        return
+    op, (rows, cols) = "paged_attention_decode", block_table.shape
+    blocks, block_size = k_cache.shape[:2]
+    lengths = seq_lens.tolist()
+    offsets = list(range(len(lengths) + 1)) if query_start_loc is None else query_start_loc.tolist()
+    index = list(range(len(lengths))) if request_indices is None else request_indices.tolist()
+    if offsets[0] != 0 or any(b < a for a, b in zip(offsets, offsets[1:])) or offsets[-1] > q.size(0):
+        _fail(op, "query_start_loc must start at 0, not decrease and stay within q")
+    if any(b - a > max_query_len for a, b in zip(offsets, offsets[1:])):
+        _fail(op, "a window is longer than max_query_len")
+    if any(not 0 <= x < rows for x in index):
+        _fail(op, "request_indices must be rows of the block table")
+    table = block_table.tolist()
+    for row, length in zip(index, lengths):
+        if not 0 <= length <= cols * block_size:
+            _fail(op, "a sequence length is negative or passes the block table")
+        if any(not 0 <= b < blocks for b in table[row][:-(-length // block_size)]):
+            _fail(op, "a block of the table is not in the cache")
