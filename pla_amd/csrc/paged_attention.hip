@@ -31,6 +31,14 @@
 
 namespace pla {
 
+// A run in pieces, for the kernel that joins them.
+struct PagedRun {
+  int pieces;                                     // below 2: it is whole, or there is no such run
+  int worker;                                     // of the first piece
+  int begin, head, row0, rows;                    // first token row of the request, key-value head, rows of the run
+  int unused[2];
+};
+
 struct PagedAttention {
   const uint16_t* q; int64_t q_token, q_head;
   const uint16_t *k, *v; int64_t kv_block, kv_token, kv_head;
@@ -42,9 +50,10 @@ struct PagedAttention {
   uint16_t* out; int64_t out_token, out_head;
   PagedShape shape;
   int batch, blocks, block_size, table_rows;
+  PagedDivisor page_of;                           // position to page
   float scale_log2;
-  int by_run, row_blocks;                         // descriptors: one a run, or one a worker; row blocks of the longest window
-  float* partial; float2* tops; int4* runs;
+  int by_run, row_blocks;                         // runs in pieces are listed by run, or by worker; row blocks of the longest window
+  float* partial; float2* tops; PagedRun* runs;
 
   __device__ int64_t at(const void* base, int wide, int64_t i) const {
     return wide ? static_cast<const int64_t*>(base)[i] : (int64_t) static_cast<const int32_t*>(base)[i];
@@ -54,6 +63,19 @@ struct PagedAttention {
     return paged_request(shape, begin, end, at(lengths, lengths_wide, n));
   }
 };
+
+// Index vectors and block tables through the scalar cache, where the index is the same for a wavefront: nothing writes them while
+// the kernel runs, and a vector load would be waited for behind all keys and values in flight.
+__device__ __forceinline__ int32_t scalar_load(const int32_t* p) { return *(const __attribute__((address_space(4))) int32_t*)p; }
+__device__ __forceinline__ int64_t scalar_at(const void* base, int wide, int n) {
+  const int32_t* p = static_cast<const int32_t*>(base) + (wide ? 2 * (int64_t)n : n);
+  return wide ? (int64_t)((uint64_t)(uint32_t)scalar_load(p) | (uint64_t)(uint32_t)scalar_load(p + 1) << 32) : (int64_t)scalar_load(p);
+}
+__device__ __forceinline__ PagedRequest scalar_request(const PagedAttention& p, int n) {
+  const int64_t begin = p.offsets ? scalar_at(p.offsets, p.offsets_wide, n) : n;
+  const int64_t end = p.offsets ? scalar_at(p.offsets, p.offsets_wide, n + 1) : n + 1;
+  return paged_request(p.shape, begin, end, scalar_at(p.lengths, p.lengths_wide, n));
+}
 
 template <typename act_t> __device__ __forceinline__ f32x4_t mfma_act(bf16x8_t a, bf16x8_t b, f32x4_t c);
 template <> __device__ __forceinline__ f32x4_t mfma_act<bf16_t>(bf16x8_t a, bf16x8_t b, f32x4_t c) { return mfma16(a, b, c); }
@@ -90,9 +112,6 @@ struct Wave {
   static constexpr int LANE_CHANNELS = 2 * WORDS;             // channels of a value that a lane loads, a chunk of 16 times as many
   u32x4_t k[2][STEPS];
   uint32_t v[8][CHUNKS][WORDS];
-  // Large heads leave no registers for the queries: they are read from LDS, once a step.
-  static constexpr bool QUERIES_IN_LDS = D == 256;
-  u32x4_t q[RT][QUERIES_IN_LDS ? 1 : STEPS];
   f32x4_t o[RT][CHUNKS][TILES];
   float top[RT], sum[RT];
   int limit[RT];
@@ -118,11 +137,11 @@ __device__ __forceinline__ void load_values(Wave<act_t, D, RT>& w, const uint16_
 #pragma unroll
     for (int c = 0; c < Wave<act_t, D, RT>::CHUNKS; ++c) {
       if constexpr (Wave<act_t, D, RT>::WORDS == 4) {
-        const u32x4_t x = *reinterpret_cast<global_ptr<const u32x4_t>>(p + lane_offset + 256 * c);
+        const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<global_ptr<const u32x4_t>>(p + lane_offset + 256 * c));
 #pragma unroll
         for (int y = 0; y < 4; ++y) w.v[i][c][y] = x[y];
       } else {
-        const u32x2_t x = *reinterpret_cast<global_ptr<const u32x2_t>>(p + lane_offset);
+        const u32x2_t x = __builtin_nontemporal_load(reinterpret_cast<global_ptr<const u32x2_t>>(p + lane_offset));
         w.v[i][c][0] = x[0]; w.v[i][c][1] = x[1];
       }
     }
@@ -149,16 +168,17 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, const u32x4_t* que
   const int kb = (threadIdx.x & 63) >> 4;
   f32x4_t s[RT][2];
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+  for (int t = 0; t < RT; ++t) s[t][0] = s[t][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      s[t][h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < W::STEPS; ++c) {
 #pragma unroll
-      for (int c = 0; c < W::STEPS; ++c)
-        s[t][h] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, w.k[h][c]),
-                                  __builtin_bit_cast(bf16x8_t, W::QUERIES_IN_LDS ? queries[(t * W::STEPS + c) * 64 + (threadIdx.x & 63)]
-                                                                                 : w.q[t][W::QUERIES_IN_LDS ? 0 : c]), s[t][h]);
+    for (int t = 0; t < RT; ++t) {
+      const bf16x8_t q = __builtin_bit_cast(bf16x8_t, queries[(t * W::STEPS + c) * 64 + (threadIdx.x & 63)]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s[t][h] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, w.k[h][c]), q, s[t][h]);
     }
+    if (D == 256) __builtin_amdgcn_sched_barrier(0);          // queries of all steps at once would not fit the registers
+  }
   next_keys();
 
   const bool masked = key0 + 32 > least || !there[0] || !there[1];          // some row does not see some key
@@ -172,7 +192,7 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, const u32x4_t* que
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int key = key0 + 16 * (i / 4) + 4 * kb + (i & 3);
-        x[i] = (key < w.limit[t]) & there[i / 4] ? x[i] : -INFINITY;
+        x[i] = ((key < w.limit[t]) & there[i / 4]) ? x[i] : -INFINITY;
       }
     }
     float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
@@ -243,60 +263,78 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, const u32x4_t* que
   next_values();
 }
 
-// The weighted values of keys [first, last) for one row, into the D / 16 channels of it that a thread has; the sixteen threads
-// of a row form its scores together.
-template <typename act_t, int D>
+// The weighted values of keys [first, last) for one row, into the D / TEAM channels of it that a thread has; the TEAM threads of a
+// row form its scores together.
+template <typename act_t, int D, int TEAM>
 __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const PagedRequest& req, int kv_head, int row, int channel,
-                                              const int32_t* pages, int first, int last, float top, float (&o)[D / 16]) {
+                                              const int32_t* pages, int first, int last, float top, float (&o)[D / TEAM]) {
   const int j = row / p.shape.group, head = kv_head * p.shape.group + row - j * p.shape.group;
   const uint16_t* q = p.q + (req.begin + j) * p.q_token + head * p.q_head + channel;
   last = min(last, paged_limit(p.shape, req, row));
   for (int key = first; key < last; ++key) {
-    const int page = key / p.block_size, entry = pages[page];
-    if (entry < 0 || entry >= p.blocks) continue;
-    const int64_t at = entry * p.kv_block + (key - page * p.block_size) * p.kv_token + kv_head * p.kv_head + channel;
+    const int page = paged_page(p.page_of, key);
+    int64_t at = paged_place(pages[page], key - page * p.block_size, p.blocks, p.kv_block, p.kv_token);
+    if (at < 0) continue;
+    at += kv_head * p.kv_head + channel;
     float score = 0.f;
-    for (int i = 0; i < D / 16; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
-    score = row16_allreduce(score) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
+    for (int i = 0; i < D / TEAM; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
+    score = (TEAM == 16 ? row16_allreduce(score) : row32_allreduce(score)) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
     const float weight = to_float(from_float<act_t>(__builtin_amdgcn_exp2f(score)));
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[i] = fmaf(weight, to_float(act_t{p.v[at + i]}), o[i]);
+    for (int i = 0; i < D / TEAM; ++i) o[i] = fmaf(weight, to_float(act_t{p.v[at + i]}), o[i]);
   }
 }
 
-// Workgroups a CU: as many as its registers hold.
-constexpr int residency(int D, int row_tiles) {
-  return D == 256 ? (row_tiles == 2 ? 1 : 2) : D == 128 ? (row_tiles == 2 ? 2 : 3) : row_tiles == 2 ? 3 : 4;
-}
+// Workgroups a CU.  More waves than these want more of the memory system than it has: one request after the other of 8000 keys
+// (D 128, 1.64 GB) takes 264 us with two, 290 with three and 422 with four.
+constexpr int residency(int D, int row_tiles) { return D == 256 ? 1 : D == 128 ? 2 : row_tiles == 2 ? 3 : 4; }
+
+// Wavefronts a workgroup.
+constexpr int waves(int D, int row_tiles) { return 4; }
 
 __device__ __forceinline__ int64_t uniform64(int64_t x) {
   return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
                    (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
 }
 
+// A segment as a wavefront takes it.
+struct Part {
+  PagedRequest req;
+  PagedSegment seg;
+  int row0, rows;                         // of the window
+  int least, end;                         // keys that all rows see, that any row sees
+  int key, steps;                         // first key and steps of this wavefront
+  int index;                              // of the request
+  const int32_t* pages;
+};
+
 template <typename act_t, int D, int RT>
-__global__ __launch_bounds__(256, residency(D, RT)) void paged_attention_kernel(const PagedAttention p) {
+__global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) / 4) void paged_attention_kernel(const PagedAttention p) {
   using W = Wave<act_t, D, RT>;
+  constexpr int WAVES = waves(D, RT), THREADS = 64 * WAVES, TILE = 32 * WAVES;
+  constexpr int TEAM = THREADS / 16, CHANNELS = D / TEAM;       // threads that put a row's outputs together, and channels of each
   constexpr int PITCH = D + 4;                    // floats of a row in LDS: rows of a quad of lanes start in different banks
-  __shared__ __align__(16) float outs[4][16][PITCH];
-  __shared__ __align__(16) u32x4_t queries[W::QUERIES_IN_LDS ? RT * W::STEPS * 64 : 1];
-  __shared__ float2 tops[4][16 * RT];
-  __shared__ int aside[4];
-  __shared__ int64_t sums[4];
-  __shared__ int64_t start_offset;
-  __shared__ int start_request;
+  constexpr int PIECES = 16 * RT * D / 8, MINE = (PIECES + THREADS - 1) / THREADS;          // 16-byte pieces of the queries, and of a thread
+  __shared__ __align__(16) float outs[WAVES][16][PITCH];
+  __shared__ __align__(16) u32x4_t queries[PIECES];
+  __shared__ float2 tops[WAVES][16 * RT];
+  __shared__ int aside[WAVES];
+  __shared__ int64_t sums[WAVES];
+  __shared__ PagedRequest start_request;
+  __shared__ int start_index, start_offset;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, kb = lane >> 4;
 
   // The line of work: all workgroups add up the whole batch, a thread a contiguous share of the requests.
-  const int share = (p.batch + 255) / 256, first = min(tid * share, p.batch), last = min(first + share, p.batch);
+  const int share = (p.batch + THREADS - 1) / THREADS, first = min(tid * share, p.batch), last = min(first + share, p.batch);
   int64_t mine = 0;
+  PagedRequest own{};
   for (int n = first; n < last; ++n) {
-    const PagedRequest req = p.request(n);
-    mine += paged_weight(p.shape, req);
+    own = p.request(n);
+    mine += paged_weight(p.shape, own);
     if (p.by_run && p.runs && blockIdx.x == 0)    // runs that nobody has
       for (int h = 0; h < p.shape.heads; ++h)
-        for (int b = req.blocks; b < p.row_blocks; ++b) p.runs[(n * p.shape.heads + h) * p.row_blocks + b] = int4{0, 0, 0, 0};
+        for (int b = own.blocks; b < p.row_blocks; ++b) p.runs[(n * p.shape.heads + h) * p.row_blocks + b].pieces = 0;
   }
   int64_t below = mine;
 #pragma unroll
@@ -308,68 +346,131 @@ __global__ __launch_bounds__(256, residency(D, RT)) void paged_attention_kernel(
   __syncthreads();
   int64_t total = 0;
   below -= mine;
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < WAVES; ++i) {
     if (i < wave) below += sums[i];
     total += sums[i];
   }
-  total = uniform64(total);
-  const int workers = paged_workers(gridDim.x, total);
+  const PagedLine line = paged_line(gridDim.x, uniform64(total));
   // neighbours in the line on one XCD: row blocks of the same keys share its L2
-  const int worker = (int)blockIdx.x >= workers || workers < 8 ? (int)blockIdx.x
-                                                                : ((int)blockIdx.x & 7) * (workers / 8) + ((int)blockIdx.x >> 3);
-  if (!p.by_run && p.runs && tid == 0) p.runs[worker] = int4{0, 0, 0, 0};
-  if (worker >= workers) return;
-  int64_t unit = paged_stretch(worker, workers, total);
-  const int64_t stretch_end = paged_stretch(worker + 1, workers, total);
+  const int block = blockIdx.x, worker = block >= line.workers || line.workers % 8 ? block : (block & 7) * (line.workers / 8) + (block >> 3);
+  if (!p.by_run && p.runs && tid == 0) p.runs[worker].pieces = 0;
+  if (worker >= line.workers) return;
+  int64_t unit = paged_stretch(line, worker);
+  const int64_t stretch_end = paged_stretch(line, worker + 1);
   if (below <= unit && unit < below + mine) {
     int64_t left = unit - below;
     int n = first;
-    for (;; ++n) {
-      const int64_t weight = paged_weight(p.shape, p.request(n));
-      if (left < weight) break;
-      left -= weight;
-    }
-    start_request = n;
-    start_offset = left;
+    if (share > 1)
+      for (;; ++n) {
+        own = p.request(n);
+        if (left < paged_weight(p.shape, own)) break;
+        left -= paged_weight(p.shape, own);
+      }
+    start_request = own;
+    start_index = n;
+    start_offset = (int)left;
   }
   __syncthreads();
-  int n = __builtin_amdgcn_readfirstlane(start_request);
-  int64_t offset = uniform64(start_offset);
+  int n = __builtin_amdgcn_readfirstlane(start_index), offset = __builtin_amdgcn_readfirstlane(start_offset);
 
   const uint32_t key_lane = (uint32_t)(r * p.kv_token + 8 * kb) * 2;
   const uint32_t value_lane = (uint32_t)(4 * kb * p.kv_token + W::LANE_CHANNELS * r) * 2;
-  W w;
 
-  while (unit < stretch_end) {
-    const PagedRequest req = p.request(n);
-    if (offset >= paged_weight(p.shape, req)) {   // done with it (or passed over)
+  // The next part of the stretch (there is one), from request n on, `offset` units into it; `req`: that request.
+  auto next_part = [&](PagedRequest req) {
+    Part a;
+    while (offset >= paged_weight(p.shape, req)) {        // done with it, or passed over
       offset = 0;
-      ++n;
-      continue;
+      req = scalar_request(p, ++n);
     }
-    const PagedSegment seg = paged_segment(req, offset, unit, stretch_end, worker, workers, total);
-    unit += seg.tiles;
-    offset += seg.tiles;
-    const int row0 = seg.block * p.shape.rows, rows = min(req.window * p.shape.group - row0, p.shape.rows);
-    const int least = paged_limit(p.shape, req, row0), end = paged_limit(p.shape, req, row0 + rows - 1);
-    const int64_t table_row = p.mapping ? p.at(p.mapping, p.mapping_wide, n) : n;
+    a.req = req;
+    a.index = n;
+    a.seg = paged_segment(line, req, offset, unit, stretch_end, worker);
+    unit += a.seg.tiles;
+    offset += a.seg.tiles;
+    a.row0 = a.seg.block * p.shape.rows;
+    a.rows = min(req.window * p.shape.group - a.row0, p.shape.rows);
+    a.least = paged_limit(p.shape, req, a.row0);
+    a.end = paged_limit(p.shape, req, a.row0 + a.rows - 1);
+    const int64_t table_row = p.mapping ? scalar_at(p.mapping, p.mapping_wide, n) : n;
     const bool has_row = table_row >= 0 && table_row < p.table_rows;
-    const int32_t* pages = p.table + (has_row ? table_row : 0) * p.table_row;
-    const uint16_t* k_base = p.k + seg.head * p.kv_head;
-    const uint16_t* v_base = p.v + seg.head * p.kv_head;
+    a.pages = p.table + (has_row ? table_row : 0) * p.table_row;
+    // steps of this wavefront: those of its keys that are below `end`
+    a.key = a.seg.tile * TILE + 32 * wave;
+    a.steps = has_row && a.end > a.key ? min((a.end - a.key - 1) / TILE + 1, a.seg.tiles) : 0;
+    return a;
+  };
+  // Where the two halves of a step's keys lie: the table's entries first (always two loads, of anything where there is no such
+  // step: a branch would wait for them), then, when they are there, the places.  Place 0, some block's first keys, serves loads
+  // whose results do not count.
+  struct Entries { int block[2]; };
+  auto look_up = [&](const Part& a, int step) {
+    Entries x;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = min(a.key + step * TILE + 16 * h, a.end - 1);
+      x.block[h] = scalar_load(a.steps > 0 ? a.pages + paged_page(p.page_of, key) : static_cast<const int32_t*>(p.lengths));
+    }
+    return x;
+  };
+  auto place_of = [&](const Part& a, int step, const Entries& x, int64_t (&place)[2], bool (&there)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = a.key + step * TILE + 16 * h;
+      place[h] = paged_place(x.block[h], key - paged_page(p.page_of, key) * p.block_size, p.blocks, p.kv_block, p.kv_token);
+      there[h] = a.steps > 0 && key < a.end && place[h] >= 0;
+      if (!there[h]) place[h] = 0;
+    }
+  };
+  // This thread's pieces of the queries: 16 bytes each, to where lane 16 kb + r of step c of row tile t reads its operand.
+  auto load_queries = [&](const Part& a, u32x4_t (&x)[MINE]) {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const int piece = tid + THREADS * i, row = piece / (D / 8), channel = piece % (D / 8) * 8;
+      x[i] = u32x4_t{0, 0, 0, 0};
+      if (row < a.rows) {
+        const int j = (a.row0 + row) / p.shape.group, g = a.row0 + row - j * p.shape.group;
+        x[i] = *reinterpret_cast<const u32x4_t*>(p.q + (a.req.begin + j) * p.q_token + (a.seg.head * p.shape.group + g) * p.q_head + channel);
+      }
+    }
+  };
+  auto store_queries = [&](const u32x4_t (&x)[MINE]) {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const int piece = tid + THREADS * i, row = piece / (D / 8), chunk = piece % (D / 8);
+      if (piece < PIECES) queries[((row >> 4) * W::STEPS + (chunk >> 2)) * 64 + 16 * (chunk & 3) + (row & 15)] = x[i];
+    }
+  };
 
+  W w;
+  u32x4_t q_words[MINE];
+  int64_t place[2], next_place[2];
+  bool there[2], next_there[2];
+  Part a = next_part(start_request);
+  load_queries(a, q_words);
+  if (a.steps > 0) {
+    place_of(a, 0, look_up(a, 0), place, there);
+    load_keys(w, p.k + a.seg.head * p.kv_head, place, key_lane);
+    load_values(w, p.v + a.seg.head * p.kv_head, place, value_lane, p.kv_token * 2);
+  }
+  store_queries(q_words);
+  __syncthreads();
+
+  for (;;) {
+    // The part after this one is worked out now, and its first keys and values are fetched by this part's last step.
+    const bool more_parts = unit < stretch_end;
+    Part b = a;
+    if (more_parts) {
+      b = next_part(a.req);
+      load_queries(b, q_words);
+    }
+    // entries of the step after the one in flight
+    Entries coming = a.steps > 1 ? look_up(a, 1) : look_up(b, 0);
+    w.set_aside = -1;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int row = 16 * t + r, j = (row0 + row) / p.shape.group, g = row0 + row - j * p.shape.group;
-      const bool real = row < rows;
-      const uint16_t* src = p.q + (req.begin + j) * p.q_token + (seg.head * p.shape.group + g) * p.q_head + 8 * kb;
-#pragma unroll
-      for (int c = 0; c < W::STEPS; ++c) {
-        const u32x4_t x = real ? *reinterpret_cast<const u32x4_t*>(src + 32 * c) : u32x4_t{0, 0, 0, 0};
-        if constexpr (!W::QUERIES_IN_LDS) w.q[t][c] = x;
-        else if (wave == 0) queries[(t * W::STEPS + c) * 64 + lane] = x;
-      }
-      w.limit[t] = real ? paged_limit(p.shape, req, row0 + row) : 0;
+      const int row = 16 * t + r;
+      w.limit[t] = row < a.rows ? paged_limit(p.shape, a.req, a.row0 + row) : 0;
       w.top[t] = -INFINITY;
       w.sum[t] = 0.f;
 #pragma unroll
@@ -377,56 +478,25 @@ __global__ __launch_bounds__(256, residency(D, RT)) void paged_attention_kernel(
 #pragma unroll
         for (int x = 0; x < W::TILES; ++x) w.o[t][c][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-
-    if constexpr (W::QUERIES_IN_LDS) __syncthreads();
-
-    w.set_aside = -1;
-    // Steps of this wavefront: those of its keys that are below `end`.  Lane 2 i + h looks up where half h of step i lies,
-    // 32 steps ahead of their use.
-    const int key_first = seg.tile * PAGED_TILE + 32 * wave;
-    const int steps = end > key_first ? min((end - key_first - 1) / PAGED_TILE + 1, seg.tiles) : 0;
-    struct Places { int lo, hi; uint64_t there; };
-    auto look_up = [&](int step0) {
-      const int key = key_first + (step0 + (lane >> 1)) * PAGED_TILE + 16 * (lane & 1);
-      bool there = has_row && step0 + (lane >> 1) < steps && key < end;
-      int64_t place = 0;
-      if (there) {
-        const int page = key / p.block_size, entry = pages[page];
-        there = entry >= 0 && entry < p.blocks;
-        place = there ? entry * p.kv_block + (key - page * p.block_size) * p.kv_token : 0;
-      }
-      return Places{(int)place, (int)(place >> 32), __ballot(there)};
-    };
-    Places now = look_up(0), then = look_up(32);
-    auto place_of = [&](int step, int64_t (&place)[2], bool (&there)[2]) {
+    for (int step = 0; step < a.steps; ++step) {
+      const bool more = step + 1 < a.steps;
+      // The very last step fetches something once more, from the caches: a branch around the loads costs the compiler the registers.
+      // The entries for the step after next are asked for behind the keys of the next: a wait for queries in LDS is one for them too.
+      const int64_t head = (more ? a.seg.head : b.seg.head) * p.kv_head;
+      attend(w, queries, p.scale_log2, there, a.key + step * TILE, a.least, a.end,
+             [&] {
+               place_of(more ? a : b, more ? step + 1 : 0, coming, next_place, next_there);
+               load_keys(w, p.k + head, next_place, key_lane);
+               coming = step + 2 < a.steps ? look_up(a, step + 2) : look_up(b, 0);
+             },
+             [&] { load_values(w, p.v + head, next_place, value_lane, p.kv_token * 2); });
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int at = (step & 31) * 2 + h;
-        place[h] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(now.lo, at) |
-                             (uint64_t)(uint32_t)__builtin_amdgcn_readlane(now.hi, at) << 32);
-        there[h] = now.there >> at & 1;
-      }
-    };
-    if (steps > 0) {
-      int64_t place[2], next_place[2];
-      bool there[2], next_there[2];
-      place_of(0, place, there);
-      load_keys(w, k_base, place, key_lane);
-      load_values(w, v_base, place, value_lane, p.kv_token * 2);
-      for (int step = 0; step < steps; ++step) {
-        const bool more = step + 1 < steps;
-        if (more && (step + 1) % 32 == 0) {
-          now = then;
-          then = look_up(step + 1 + 32);
-        }
-        // the last step fetches its own keys once more, from the caches: a branch around the loads costs the compiler the registers
-        place_of(more ? step + 1 : step, next_place, next_there);
-        attend(w, queries, p.scale_log2, there, key_first + step * PAGED_TILE, least, end,
-               [&] { load_keys(w, k_base, next_place, key_lane); },
-               [&] { load_values(w, v_base, next_place, value_lane, p.kv_token * 2); });
-#pragma unroll
-        for (int h = 0; h < 2; ++h) { place[h] = next_place[h]; there[h] = next_there[h]; }
-      }
+      for (int h = 0; h < 2; ++h) { place[h] = next_place[h]; there[h] = next_there[h]; }
+    }
+    if (a.steps == 0 && b.steps > 0) {
+      place_of(b, 0, coming, place, there);
+      load_keys(w, p.k + b.seg.head * p.kv_head, place, key_lane);
+      load_values(w, p.v + b.seg.head * p.kv_head, place, value_lane, p.kv_token * 2);
     }
 
     // The four wavefronts' rows together.
@@ -437,13 +507,14 @@ __global__ __launch_bounds__(256, residency(D, RT)) void paged_attention_kernel(
     }
     if (lane == 0) aside[wave] = w.set_aside;
     __syncthreads();
-    const int out_row = tid >> 4, out_channel = (tid & 15) * (D / 16);
+    if (more_parts) store_queries(q_words);
+    const int out_row = tid / TEAM, out_channel = tid % TEAM * CHANNELS;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      if (16 * t >= rows) break;
+      if (16 * t >= a.rows) break;
       float top = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) top = fmaxf(top, tops[x][16 * t + r].x);
+      for (int x = 0; x < WAVES; ++x) top = fmaxf(top, tops[x][16 * t + r].x);
       const float f = rescale(w.top[t], top);
 #pragma unroll
       for (int c = 0; c < W::CHUNKS; ++c)
@@ -456,124 +527,148 @@ __global__ __launch_bounds__(256, residency(D, RT)) void paged_attention_kernel(
                 float4{w.o[t][c][j][e] * f, w.o[t][c][j + 1][e] * f, w.o[t][c][j + 2][e] * f, w.o[t][c][j + 3][e] * f};
           }
       __syncthreads();
-      if (16 * t + out_row < rows) {
+      if (16 * t + out_row < a.rows) {
         float row_top = -INFINITY, row_sum = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) row_top = fmaxf(row_top, tops[x][16 * t + out_row].x);
+        for (int x = 0; x < WAVES; ++x) row_top = fmaxf(row_top, tops[x][16 * t + out_row].x);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) row_sum += tops[x][16 * t + out_row].y * rescale(tops[x][16 * t + out_row].x, row_top);
-        float o[D / 16];
+        for (int x = 0; x < WAVES; ++x) row_sum += tops[x][16 * t + out_row].y * rescale(tops[x][16 * t + out_row].x, row_top);
+        float o[CHANNELS];
 #pragma unroll
-        for (int i = 0; i < D / 16; i += 4) {
-          float4 a = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < CHANNELS; ++i) {
+          o[i] = 0.f;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float4 b = *reinterpret_cast<const float4*>(&outs[x][out_row][out_channel + i]);
-            a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-          }
-          o[i] = a.x; o[i + 1] = a.y; o[i + 2] = a.z; o[i + 3] = a.w;
+          for (int x = 0; x < WAVES; ++x) o[i] += outs[x][out_row][out_channel + i];
         }
-        for (int x = 0; x < 4; ++x)
-          if (aside[x] >= 0) add_set_aside<act_t, D>(p, req, seg.head, row0 + 16 * t + out_row, out_channel, pages, max(aside[x], least), min(aside[x] + 32, end), row_top, o);
-        if (seg.slot < 0) {
-          const int row = row0 + 16 * t + out_row, j = row / p.shape.group, head = seg.head * p.shape.group + row - j * p.shape.group;
+        const int row = a.row0 + 16 * t + out_row;
+        for (int x = 0; x < WAVES; ++x)
+          if (aside[x] >= 0)
+            add_set_aside<act_t, D, TEAM>(p, a.req, a.seg.head, row, out_channel, a.pages, max(aside[x], a.least), min(aside[x] + 32, a.end), row_top, o);
+        if (a.seg.slot < 0) {
+          const int j = row / p.shape.group, head = a.seg.head * p.shape.group + row - j * p.shape.group;
           const float norm = row_sum == 0.f ? 0.f : 1.0f / row_sum;         // no key: zeros
-          const int64_t token = req.begin + j;
-          uint32_t word[D / 32];
+          const int64_t token = a.req.begin + j;
+          uint32_t word[CHANNELS / 2];
 #pragma unroll
-          for (int i = 0; i < D / 16; i += 2) {
-            float a = o[i] * norm, b = o[i + 1] * norm;
+          for (int i = 0; i < CHANNELS; i += 2) {
+            float x = o[i] * norm, y = o[i + 1] * norm;
             if (p.gate) {
               const uint32_t g = *reinterpret_cast<const uint32_t*>(p.gate + token * p.gate_token + head * p.gate_head + out_channel + i);
-              a *= 1.0f / (1.0f + __expf(-lo16<act_t>(g)));
-              b *= 1.0f / (1.0f + __expf(-hi16<act_t>(g)));
+              x *= 1.0f / (1.0f + __expf(-lo16<act_t>(g)));
+              y *= 1.0f / (1.0f + __expf(-hi16<act_t>(g)));
             }
-            word[i / 2] = pack2<act_t>(a, b);
+            word[i / 2] = pack2<act_t>(x, y);
           }
           uint16_t* dst = p.out + token * p.out_token + head * p.out_head + out_channel;
-          if constexpr (D == 64) {
-            *reinterpret_cast<uint2*>(dst) = uint2{word[0], word[1]};
-          } else {
 #pragma unroll
-            for (int i = 0; i < D / 128; ++i)
-              reinterpret_cast<uint4*>(dst)[i] = uint4{word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]};
-          }
+          for (int i = 0; i < CHANNELS / 2; ++i) reinterpret_cast<uint32_t*>(dst)[i] = word[i];
         } else {
-          const int64_t row = (int64_t)seg.slot * (16 * RT) + 16 * t + out_row;
+          const int64_t at = (int64_t)a.seg.slot * (16 * RT) + 16 * t + out_row;
 #pragma unroll
-          for (int i = 0; i < D / 16; i += 4)
-            *reinterpret_cast<float4*>(p.partial + row * D + out_channel + i) = float4{o[i], o[i + 1], o[i + 2], o[i + 3]};
-          if ((tid & 15) == 0) p.tops[row] = float2{row_top, row_sum};
+          for (int i = 0; i < CHANNELS; ++i) p.partial[at * D + out_channel + i] = o[i];
+          if (tid % TEAM == 0) p.tops[at] = float2{row_top, row_sum};
         }
       }
       __syncthreads();
     }
-    if (tid == 0 && p.runs && seg.pieces > 0) {
-      // who joins this run, if it is in pieces
-      const int run = (n * p.shape.heads + seg.head) * p.row_blocks + seg.block;
-      if (p.by_run) p.runs[run] = int4{n, run - n * p.shape.heads * p.row_blocks, worker, seg.slot < 0 ? 0 : seg.pieces};
-      else if (seg.slot >= 0) p.runs[worker] = int4{n, run - n * p.shape.heads * p.row_blocks, worker, seg.pieces};
+    if (tid == 0 && p.runs && a.seg.tile == 0 && (p.by_run || a.seg.pieces > 1)) {
+      // in pieces or not: with a list by run somebody has to say
+      PagedRun* run = p.runs + (p.by_run ? (a.index * p.shape.heads + a.seg.head) * p.row_blocks + a.seg.block : worker);
+      *run = PagedRun{a.seg.pieces, worker, (int)a.req.begin, a.seg.head, a.row0, a.rows, {0, 0}};
     }
+    if (!more_parts) break;
+    a = b;
   }
 }
 
-// Pieces of a run to its output.  A workgroup a run and every gridDim.y-th of its rows; its wavefronts share the pieces, a
-// lane has D / 64 channels.
-template <typename act_t, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttention p) {
-  constexpr int LANE = D / 64;
-  __shared__ float outs[4][D];
-  const int4 run = p.runs[blockIdx.x];
-  const int pieces = run.w;
+// Pieces of a run to its output: a workgroup a run and every gridDim.y-th of its rows.  The wavefronts share the rows, or
+// (PER_ROW; many pieces) the pieces of a row; a lane has D / 64 channels.  Everything that a row takes is asked for at once, as
+// far as it is no more than eight pieces a wavefront.
+template <typename act_t, int D, bool PER_ROW, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void paged_join_kernel(const PagedAttention p) {
+  constexpr int LANE = D / 64, AHEAD = 8;
+  typedef float lane_t __attribute__((ext_vector_type(LANE)));
+  __shared__ float outs[PER_ROW ? WAVES : 1][D];
+  __shared__ float2 parts[PER_ROW ? WAVES : 1];
+  const PagedRun run = p.runs[blockIdx.x];
+  const int pieces = run.pieces;
   if (pieces < 2) return;
-  const int n = run.x, head = run.y / p.row_blocks, block = run.y - head * p.row_blocks, worker = run.z;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, R = p.shape.rows;
-  const PagedRequest req = p.request(n);
-  const int row0 = block * R, rows = min(req.window * p.shape.group - row0, R);
-  auto slot_row = [&](int piece, int row) { return (int64_t)(piece == 0 ? 2 * worker + 1 : 2 * (worker + piece)) * R + row; };
-  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), R = p.shape.rows;
+  const int first = PER_ROW ? wave : 0, stride = PER_ROW ? WAVES : 1;
+  for (int row = PER_ROW ? blockIdx.y : blockIdx.y * WAVES + wave; row < run.rows; row += PER_ROW ? gridDim.y : gridDim.y * WAVES) {
+    const int j = (run.row0 + row) / p.shape.group, head = run.head * p.shape.group + run.row0 + row - j * p.shape.group;
+    const int64_t token = run.begin + j;
+    uint16_t gate[LANE] = {};
+    if (p.gate) {
+#pragma unroll
+      for (int c = 0; c < LANE; ++c) gate[c] = p.gate[token * p.gate_token + head * p.gate_head + LANE * lane + c];
+    }
+    // the wavefront's pieces: eight at a time, with a maximum and a sum that run along
     float top = -INFINITY, sum = 0.f;
-    for (int i = lane; i < pieces; i += 64) top = fmaxf(top, p.tops[slot_row(i, row)].x);
+    lane_t o = {};
+    for (int i = first; i < pieces; i += AHEAD * stride) {
+      lane_t x[AHEAD];
+      float2 y[AHEAD];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    for (int i = lane; i < pieces; i += 64) {
-      const float2 x = p.tops[slot_row(i, row)];
-      sum += x.y * rescale(x.x, top);
-    }
-    sum = wave64_allreduce(sum);
-    float o[LANE] = {};
-    for (int i = wave; i < pieces; i += 4) {
-      const int64_t at = slot_row(i, row);
-      const float f = rescale(p.tops[at].x, top);
-#pragma unroll
-      for (int x = 0; x < LANE; ++x) o[x] = fmaf(p.partial[at * D + LANE * lane + x], f, o[x]);
-    }
-#pragma unroll
-    for (int x = 0; x < LANE; ++x) outs[wave][LANE * lane + x] = o[x];
-    __syncthreads();
-    if (threadIdx.x < D / 2) {
-      const int channel = 2 * threadIdx.x, j = (row0 + row) / p.shape.group, q_head = head * p.shape.group + row0 + row - j * p.shape.group;
-      const float norm = sum == 0.f ? 0.f : 1.0f / sum;
-      float a = 0.f, b = 0.f;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) { a += outs[x][channel]; b += outs[x][channel + 1]; }
-      a *= norm;
-      b *= norm;
-      const int64_t token = req.begin + j;
-      if (p.gate) {
-        const uint32_t g = *reinterpret_cast<const uint32_t*>(p.gate + token * p.gate_token + q_head * p.gate_head + channel);
-        a *= 1.0f / (1.0f + __expf(-lo16<act_t>(g)));
-        b *= 1.0f / (1.0f + __expf(-hi16<act_t>(g)));
+      for (int a = 0; a < AHEAD; ++a) {
+        const int piece = min(i + a * stride, pieces - 1);
+        const int64_t at = (int64_t)(piece == 0 ? 2 * run.worker + 1 : 2 * (run.worker + piece)) * R + row;
+        x[a] = *reinterpret_cast<const lane_t*>(p.partial + at * D + LANE * lane);
+        y[a] = p.tops[at];
       }
-      *reinterpret_cast<uint32_t*>(p.out + token * p.out_token + q_head * p.out_head + channel) = pack2<act_t>(a, b);
+      float high = top;
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) high = fmaxf(high, y[a].x);          // one piece twice does no harm here
+      const float back = rescale(top, high);
+      sum *= back;
+      o *= back;
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const bool counts = i + a * stride < pieces;
+        const float f = rescale(y[a].x, high);
+        sum = counts ? fmaf(y[a].y, f, sum) : sum;
+#pragma unroll
+        for (int c = 0; c < LANE; ++c) o[c] = counts ? fmaf(x[a][c], f, o[c]) : o[c];
+      }
+      top = high;
     }
-    __syncthreads();
+    if constexpr (PER_ROW) {
+      *reinterpret_cast<lane_t*>(&outs[wave][LANE * lane]) = o;
+      if (lane == 0) parts[wave] = float2{top, sum};
+      __syncthreads();
+      if (wave == 0) {
+        for (int x = 0; x < WAVES; ++x) top = fmaxf(top, parts[x].x);
+        sum = 0.f;
+        o = lane_t{};
+        for (int x = 0; x < WAVES; ++x) {
+          const float f = rescale(parts[x].x, top);
+          sum = fmaf(parts[x].y, f, sum);
+          const lane_t y = *reinterpret_cast<const lane_t*>(&outs[x][LANE * lane]);
+#pragma unroll
+          for (int c = 0; c < LANE; ++c) o[c] = fmaf(y[c], f, o[c]);
+        }
+      }
+    }
+    if (!PER_ROW || wave == 0) {
+      const float norm = sum == 0.f ? 0.f : 1.0f / sum;
+      float x[LANE];
+#pragma unroll
+      for (int c = 0; c < LANE; ++c) {
+        x[c] = o[c] * norm;
+        if (p.gate) x[c] *= 1.0f / (1.0f + __expf(-to_float(act_t{gate[c]})));
+      }
+      uint16_t* dst = p.out + token * p.out_token + head * p.out_head + LANE * lane;
+      if constexpr (LANE == 1) *dst = from_float<act_t>(x[0]).bits;
+      else if constexpr (LANE == 2) *reinterpret_cast<uint32_t*>(dst) = pack2<act_t>(x[0], x[1]);
+      else *reinterpret_cast<uint2*>(dst) = uint2{pack2<act_t>(x[0], x[1]), pack2<act_t>(x[2], x[3])};
+    }
+    if constexpr (PER_ROW) __syncthreads();
   }
 }
 
 // How a call is launched: host arithmetic from what the host knows.
 struct PagedLaunch {
-  int row_tiles, rows, row_blocks, workers, by_run, join_rows;
+  int row_tiles, rows, tile, row_blocks, workers, by_run, per_row, join_rows;
   bool split;                             // whether a run can be cut at all
   int64_t runs, bytes, tops_at, runs_at;  // workspace: partial outputs, maxima and sums, runs
 };
@@ -583,29 +678,34 @@ static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query
   const int window_rows = max_query * (HQ / HKV);
   l.row_tiles = window_rows <= 16 ? 1 : 2;
   l.rows = 16 * l.row_tiles;
+  l.tile = 32 * waves(D, l.row_tiles);
   l.row_blocks = (window_rows + l.rows - 1) / l.rows;
   l.runs = (int64_t)batch * HKV * l.row_blocks;
-  const int64_t tiles = positions > 0 ? (positions - 1) / PAGED_TILE + 1 : 1, most = 256 * residency(D, l.row_tiles);
+  const int64_t tiles = positions > 0 ? (positions - 1) / l.tile + 1 : 1, most = 256 * residency(D, l.row_tiles);
   l.workers = (int)(l.runs * tiles < most ? l.runs * tiles : most);
   l.split = tiles > 1;
   l.by_run = l.runs <= l.workers;
-  const int64_t groups = l.by_run ? l.runs : l.workers;
-  const int row_slices = (int)(2048 / (groups > 0 ? groups : 1)), used = window_rows < l.rows ? window_rows : l.rows;
-  l.join_rows = row_slices < 1 ? 1 : row_slices < used ? row_slices : used;
+  // Join: where few runs share all workers each is in many pieces, and a workgroup takes one row of one run; else a wavefront does.
+  const int used = window_rows < l.rows ? window_rows : l.rows;
+  l.per_row = l.runs * 16 <= l.workers;
+  l.join_rows = l.per_row ? used : (used + 3) / 4;
   if (l.split) {
     const int64_t slots = 2 * (int64_t)l.workers;
     l.tops_at = slots * l.rows * D * 4;
     l.runs_at = l.tops_at + slots * l.rows * 8;
-    l.bytes = (l.runs_at + l.workers * 16 + 255) / 256 * 256;
+    l.bytes = (l.runs_at + l.workers * (int64_t)sizeof(PagedRun) + 255) / 256 * 256;
   }
   return l;
 }
 
 template <typename act_t, int D>
 static void launch_paged_attention(const PagedAttention& p, const PagedLaunch& l, hipStream_t s) {
-  if (l.row_tiles == 1) paged_attention_kernel<act_t, D, 1><<<l.workers, 256, 0, s>>>(p);
-  else paged_attention_kernel<act_t, D, 2><<<l.workers, 256, 0, s>>>(p);
-  if (l.split) paged_join_kernel<act_t, D><<<dim3((unsigned)(l.by_run ? l.runs : l.workers), l.join_rows), 256, 0, s>>>(p);
+  if (l.row_tiles == 1) paged_attention_kernel<act_t, D, 1><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
+  else paged_attention_kernel<act_t, D, 2><<<l.workers, 64 * waves(D, 2), 0, s>>>(p);
+  if (!l.split) return;
+  const dim3 grid((unsigned)(l.by_run ? l.runs : l.workers), l.join_rows);
+  if (l.per_row) paged_join_kernel<act_t, D, true, 16><<<grid, 1024, 0, s>>>(p);
+  else paged_join_kernel<act_t, D, false, 4><<<grid, 256, 0, s>>>(p);
 }
 
 static int check_shape(int batch, int HQ, int HKV, int D, int max_query, int64_t positions) {
@@ -614,6 +714,7 @@ static int check_shape(int batch, int HQ, int HKV, int D, int max_query, int64_t
   PLA_REQUIRE(max_query >= 1 && max_query <= 32, "max_query_len must be between 1 and 32");
   PLA_REQUIRE(batch >= 0 && (int64_t)batch * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "too many requests");
   PLA_REQUIRE(positions >= 0 && positions <= (1 << 30), "a row of the block table must hold at most 2^30 positions");
+  PLA_REQUIRE((positions / 128 + 1) * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "a request with too many heads for its positions");
   return 0;
 }
 
@@ -631,14 +732,14 @@ extern "C" int pla_paged_attention_segments(
   using namespace pla;
   if (check_shape(batch, HQ, HKV, head_dim, max_query_len, positions) || batch == 0 || !offsets || !seq_lens) return -1;
   const PagedLaunch l = paged_launch(batch, HQ, HKV, head_dim, max_query_len, positions);
-  const PagedShape shape{HKV, HQ / HKV, l.rows, max_query_len, tokens, positions};
+  const PagedShape shape{HKV, HQ / HKV, l.rows, l.tile, max_query_len, tokens, positions};
   auto request = [&](int n) { return paged_request(shape, offsets[n], offsets[n + 1], seq_lens[n]); };
   int64_t total = 0;
   for (int n = 0; n < batch; ++n) total += paged_weight(shape, request(n));
-  const int workers = paged_workers(l.workers, total);
-  if (worker < 0 || worker >= workers) return 0;
-  int64_t unit = paged_stretch(worker, workers, total), offset = unit;
-  const int64_t end = paged_stretch(worker + 1, workers, total);
+  const PagedLine line = paged_line(l.workers, total);
+  if (worker < 0 || worker >= line.workers) return 0;
+  int64_t unit = paged_stretch(line, worker), offset = unit;
+  const int64_t end = paged_stretch(line, worker + 1);
   int found = 0;
   for (int n = 0; unit < end;) {
     const PagedRequest r = request(n);
@@ -647,7 +748,7 @@ extern "C" int pla_paged_attention_segments(
       ++n;
       continue;
     }
-    const PagedSegment s = paged_segment(r, offset, unit, end, worker, workers, total);
+    const PagedSegment s = paged_segment(line, r, (int)offset, unit, end, worker);
     if (found < capacity) {
       const int64_t row[7] = {n, s.head, s.block, s.tile, s.tiles, s.slot, s.pieces};
       for (int i = 0; i < 7; ++i) segments[7 * found + i] = row[i];
@@ -692,10 +793,10 @@ extern "C" int pla_paged_attention_launch(
   const PagedAttention p{(const uint16_t*)q, q_token, q_head, (const uint16_t*)k_cache, (const uint16_t*)v_cache, kv_block, kv_token,
                          kv_head, block_table, table_row_stride, mapping, mapping_wide, offsets, offsets_wide, seq_lens, seq_lens_wide,
                          (const uint16_t*)gate, gate_token, gate_head, (uint16_t*)out, out_token, out_head,
-                         PagedShape{HKV, HQ / HKV, l.rows, max_query_len, tokens, positions},
-                         batch, blocks, block_size, table_rows, scale * 1.44269504088896341f, l.by_run, l.row_blocks,
+                         PagedShape{HKV, HQ / HKV, l.rows, l.tile, max_query_len, tokens, positions},
+                         batch, blocks, block_size, table_rows, paged_divisor(block_size), scale * 1.44269504088896341f, l.by_run, l.row_blocks,
                          l.split ? reinterpret_cast<float*>(ws) : nullptr, l.split ? reinterpret_cast<float2*>(ws + l.tops_at) : nullptr,
-                         l.split ? reinterpret_cast<int4*>(ws + l.runs_at) : nullptr};
+                         l.split ? reinterpret_cast<PagedRun*>(ws + l.runs_at) : nullptr};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (act_dtype == PLA_BF16) {
     if (head_dim == 64) launch_paged_attention<bf16_t, 64>(p, l, s);

@@ -1,7 +1,7 @@
 // How the attention over a paged cache is dealt out.  Host and device use the same functions: the host's side is arithmetic
 // for tests and logs.
 //
-// The unit of work is a tile of TILE keys for one (request, key-value head, block of query rows).  All units of a call stand
+// The unit of work is a tile of keys, 32 for each wavefront of a workgroup, for one (request, key-value head, block of query rows).  All units of a call stand
 // in one line - requests, within them heads, within them row blocks, within them tiles - and every worker (workgroup) takes
 // an equal stretch of it.  So a batch of very different lengths keeps the whole chip busy to the end, and one long request is
 // split as finely as there are workers, with no number of splits to choose and no length read back by the host.  A run of
@@ -21,11 +21,9 @@
 
 namespace pla {
 
-constexpr int PAGED_TILE = 128;           // keys a workgroup takes at a time, 32 a wavefront
-
 struct PagedShape {
   int heads, group;                       // key-value heads, query heads of each
-  int rows;                               // query rows of a block
+  int rows, tile;                         // query rows of a block, keys of a tile
   int max_query, tokens;                  // longest window, rows of q
   int64_t positions;                      // that a row of the block table has pages for
 };
@@ -46,10 +44,10 @@ PLA_HD PagedRequest paged_request(const PagedShape& s, int64_t begin, int64_t en
   r.length = (int)(length < 0 ? 0 : length > INT32_MAX ? INT32_MAX : length);
   r.keys = (int)(r.length < s.positions ? r.length : s.positions);
   r.blocks = (r.window * s.group + s.rows - 1) / s.rows;
-  r.tiles = r.keys > 0 ? (r.keys - 1) / PAGED_TILE + 1 : 1;
+  r.tiles = r.keys > 0 ? (r.keys - 1) / s.tile + 1 : 1;
   return r;
 }
-PLA_HD int64_t paged_weight(const PagedShape& s, const PagedRequest& r) { return (int64_t)r.tiles * r.blocks * s.heads; }
+PLA_HD int paged_weight(const PagedShape& s, const PagedRequest& r) { return r.tiles * r.blocks * s.heads; }     // fits: the host checks
 
 // Keys that the token row `row / group` of a request sees (they are the first ones).
 PLA_HD int paged_limit(const PagedShape& s, const PagedRequest& r, int row) {
@@ -57,35 +55,61 @@ PLA_HD int paged_limit(const PagedShape& s, const PagedRequest& r, int row) {
   return (int)(limit < 0 ? 0 : limit < r.keys ? limit : r.keys);
 }
 
-// Every worker has a unit, and from eight on their number divides by the XCDs.
-PLA_HD int paged_workers(int grid, int64_t total) {
-  const int n = total < grid ? (int)total : grid;
-  return n >= 8 ? n & ~7 : n;
+// Division by a number known ahead: with 2^(b - 1) < d <= 2^b the factor ceil(2^(31 + b) / d) has 32 bits and is off by less than
+// one part in 2^31, so the quotient of a number below 2^31 is exact.
+struct PagedDivisor { uint32_t factor; int shift; };
+inline PagedDivisor paged_divisor(int d) {
+  int bits = 0;
+  while ((1ll << bits) < d) ++bits;
+  return {(uint32_t)(((1ull << (31 + bits)) + d - 1) / d), bits + 31};
 }
-PLA_HD int64_t paged_stretch(int worker, int workers, int64_t total) { return worker * total / workers; }
-PLA_HD int paged_worker_of(int64_t unit, int workers, int64_t total) {
-  return (int)(((unit + 1) * workers + total - 1) / total - 1);
+PLA_HD int paged_page(const PagedDivisor& d, int n) { return (int)((uint64_t)(uint32_t)n * d.factor >> d.shift); }
+
+// Where the keys of half a step lie, in elements from the cache's start: place `place` of block `entry` of the table; -1: nowhere.
+PLA_HD int64_t paged_place(int entry, int place, int blocks, int64_t block_stride, int64_t token_stride) {
+  return entry >= 0 && entry < blocks ? entry * block_stride + place * token_stride : -1;
+}
+
+// The line of `total` units and its workers: every worker has a unit, and the first `rest` of them have one more than the others.
+struct PagedLine {
+  int64_t total, each;
+  int workers, rest;
+};
+PLA_HD int64_t paged_divide(int64_t a, int64_t b) {        // of numbers that are not negative; short where they are
+  return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+PLA_HD PagedLine paged_line(int grid, int64_t total) {
+  PagedLine l{total, 0, 0, 0};
+  if (total <= 0) return l;
+  l.workers = total < grid ? (int)total : grid;
+  l.each = paged_divide(total, l.workers);
+  l.rest = (int)(total - l.each * l.workers);
+  return l;
+}
+PLA_HD int64_t paged_stretch(const PagedLine& l, int worker) { return l.each * worker + (worker < l.rest ? worker : l.rest); }
+PLA_HD int paged_worker_of(const PagedLine& l, int64_t unit) {
+  const int64_t longer = (l.each + 1) * l.rest;
+  return (int)(unit < longer ? paged_divide(unit, l.each + 1) : l.rest + paged_divide(unit - longer, l.each));
 }
 
 struct PagedSegment {
   int head, block, tile, tiles;           // tiles [tile, tile + tiles) of a run
   int slot;                               // of the workspace, -1: the run is whole
-  int pieces;                             // of the run, where this is its first piece
+  int pieces;                             // of the run (1: it is whole) where this is its first, else 0
 };
 
 // The segment that starts `offset` units into the request `r`, which is unit `unit` of the line; `end`: of the stretch.
-PLA_HD PagedSegment paged_segment(const PagedRequest& r, int64_t offset, int64_t unit, int64_t end, int worker, int workers,
-                                  int64_t total) {
+PLA_HD PagedSegment paged_segment(const PagedLine& l, const PagedRequest& r, int offset, int64_t unit, int64_t end, int worker) {
   PagedSegment s;
-  const int64_t run = offset / r.tiles;
-  s.tile = (int)(offset - run * r.tiles);
-  s.head = (int)(run / r.blocks);
-  s.block = (int)(run - (int64_t)s.head * r.blocks);
+  const int run = (uint32_t)offset / (uint32_t)r.tiles;
+  s.tile = offset - run * r.tiles;
+  s.head = (uint32_t)run / (uint32_t)r.blocks;
+  s.block = run - s.head * r.blocks;
   const int64_t left = end - unit;
   s.tiles = r.tiles - s.tile < left ? r.tiles - s.tile : (int)left;
-  const bool first = s.tile == 0;
-  s.slot = first && s.tiles == r.tiles ? -1 : 2 * worker + (first ? 1 : 0);
-  s.pieces = first ? paged_worker_of(unit + r.tiles - 1, workers, total) - worker + 1 : 0;
+  const bool whole = s.tiles == r.tiles;
+  s.slot = whole ? -1 : 2 * worker + (s.tile == 0 ? 1 : 0);
+  s.pieces = s.tile != 0 ? 0 : whole ? 1 : paged_worker_of(l, unit + r.tiles - 1) - worker + 1;
   return s;
 }
 
