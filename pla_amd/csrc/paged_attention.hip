@@ -285,12 +285,13 @@ __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const Pag
   }
 }
 
-// Workgroups a CU.  More waves than these want more of the memory system than it has: one request after the other of 8000 keys
-// (D 128, 1.64 GB) takes 264 us with two, 290 with three and 422 with four.
-constexpr int residency(int D, int row_tiles) { return D == 256 ? 1 : D == 128 ? 2 : row_tiles == 2 ? 3 : 4; }
-
-// Wavefronts a workgroup.
-constexpr int waves(int D, int row_tiles) { return 4; }
+// Wavefronts a workgroup and workgroups a CU, so that 96 to 128 KiB of keys and values are in flight there.  More want more of the
+// memory system than it has: 50 requests of 8000 keys (D 128, 1.64 GB) take 264 us with two workgroups of four wavefronts, 290 with
+// three and 422 with four.  D 64: 37 windows of up to 9000 keys (167 MB) take 32.8 us as two workgroups of eight wavefronts and 36.2 as
+// four of four; 32 rows do not fit the registers of that (64 windows of eight over 1000 to 16 000 keys, 8 heads, 214 us), and take 171
+// as one workgroup of eight and 162 as three of four.
+constexpr int waves(int D, int row_tiles) { return D == 64 && row_tiles == 1 ? 8 : 4; }
+constexpr int residency(int D, int row_tiles) { return D == 256 ? 1 : D == 64 && row_tiles == 2 ? 3 : 2; }
 
 __device__ __forceinline__ int64_t uniform64(int64_t x) {
   return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
@@ -447,12 +448,13 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
   int64_t place[2], next_place[2];
   bool there[2], next_there[2];
   Part a = next_part(start_request);
-  load_queries(a, q_words);
+  const Entries entries = look_up(a, 0);
   if (a.steps > 0) {
-    place_of(a, 0, look_up(a, 0), place, there);
+    place_of(a, 0, entries, place, there);
     load_keys(w, p.k + a.seg.head * p.kv_head, place, key_lane);
-    load_values(w, p.v + a.seg.head * p.kv_head, place, value_lane, p.kv_token * 2);
   }
+  load_queries(a, q_words);
+  if (a.steps > 0) load_values(w, p.v + a.seg.head * p.kv_head, place, value_lane, p.kv_token * 2);
   store_queries(q_words);
   __syncthreads();
 
@@ -479,6 +481,10 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
         for (int x = 0; x < W::TILES; ++x) w.o[t][c][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
     for (int step = 0; step < a.steps; ++step) {
+      // The wavefronts of a CU's workgroups take turns: the older ones would always go first, end early and leave the others alone
+      // with half of the requests in flight (D 64, 64 windows over 4000 keys 123.7 -> 118.0 us, 50 requests of 8000 269.5 -> 266.3).
+      if ((step + (blockIdx.x >> 8)) & 1) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
       const bool more = step + 1 < a.steps;
       // The very last step fetches something once more, from the caches: a branch around the loads costs the compiler the registers.
       // The entries for the step after next are asked for behind the keys of the next: a wait for queries in LDS is one for them too.
@@ -583,10 +589,10 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
 
 // Pieces of a run to its output: a workgroup a run and every gridDim.y-th of its rows.  The wavefronts share the rows, or
 // (PER_ROW; many pieces) the pieces of a row; a lane has D / 64 channels.  Everything that a row takes is asked for at once, as
-// far as it is no more than eight pieces a wavefront.
+// far as it is no more than AHEAD pieces a wavefront.
 template <typename act_t, int D, bool PER_ROW, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void paged_join_kernel(const PagedAttention p) {
-  constexpr int LANE = D / 64, AHEAD = 8;
+  constexpr int LANE = D / 64, AHEAD = !PER_ROW ? 8 : D == 256 ? 10 : 18;
   typedef float lane_t __attribute__((ext_vector_type(LANE)));
   __shared__ float outs[PER_ROW ? WAVES : 1][D];
   __shared__ float2 parts[PER_ROW ? WAVES : 1];

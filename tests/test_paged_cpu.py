@@ -10,7 +10,6 @@ from pla.decode.paged import (PagedKVBlocks, PagedKVPlan, fused_qk_norm_rope, pa
                               rotary_frequencies)
 
 BF16 = torch.bfloat16
-TILE = 128
 
 
 # ---- schedule ---------------------------------------------------------------------------------------------------
@@ -41,6 +40,10 @@ def _rows_of_a_block(max_query, group):
     return 16 if max_query * group <= 16 else 32
 
 
+def _keys_of_a_tile(D, rows):
+    return 256 if D == 64 and rows == 16 else 128
+
+
 @pytest.mark.parametrize("seed", range(12))
 def test_every_tile_of_every_run_is_taken_once_and_its_pieces_are_found(seed):
     rng = random.Random(seed)
@@ -53,9 +56,10 @@ def test_every_tile_of_every_run_is_taken_once_and_its_pieces_are_found(seed):
     lengths = [rng.choice((0, -3, 1, 127, 128, 129, positions, positions + 500, rng.randint(0, positions))) for _ in range(n)]
     got = _segments(windows, lengths, HKV * group, HKV, D, max_query, positions)
     rows = _rows_of_a_block(max_query, group)
+    tile_keys = _keys_of_a_tile(D, rows)
     expected = {}
     for i, (w, length) in enumerate(zip(windows, lengths)):
-        tiles = max(1, -(-min(max(length, 0), positions) // TILE))
+        tiles = max(1, -(-min(max(length, 0), positions) // tile_keys))
         for h in range(HKV):
             for b in range(-(-w * group // rows)):
                 expected[i, h, b] = tiles
