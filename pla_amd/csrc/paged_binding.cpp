@@ -105,7 +105,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> paged_kv_plan(
   dense_ints(held_blocks, "held_blocks", at::kInt, rows);
   TORCH_CHECK(free_blocks.dim() == 1 && free_blocks.scalar_type() == at::kInt && free_blocks.is_contiguous(), "free_blocks must be a contiguous Int vector");
   dense_ints(free_count, "free_count", at::kInt, 1);
-  TORCH_CHECK(block_size > 0 && cols * block_size <= (1 << 30), "block_size must be positive and a row's positions at most 2^30");
+  TORCH_CHECK(block_size > 0 && block_size <= (1 << 30) && cols * block_size <= (1 << 30), "block_size must be positive and a row's positions at most 2^30");
   TORCH_CHECK(token_capacity >= 0 && token_capacity <= (1 << 30), "token_capacity must be between 0 and 2^30");
   TORCH_CHECK(mapping || batch <= rows, "more batch entries than rows of the block table");
   if (out_offsets) {

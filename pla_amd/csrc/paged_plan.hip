@@ -10,17 +10,18 @@
 //             (0: unsound or refused, such an entry keeps its blocks), and for every token row its position and slot
 //             block * block_size + position % block_size (0 and -1 for rows of refused entries and behind the batch).
 //
-// Bound by latency: lengths, held counts, stack and table are four dependent trips to memory, the scans between them run in
-// one workgroup, an entry per thread.  Everything whose number depends on the values (blocks moved, token rows) is dealt out
-// flat: thread i finds its entry by bisection of the running sums in LDS, so that one long prompt costs no more than many
-// short ones.  Steps of many token rows leave these to a second launch over the whole chip.
+// Bound by latency: lengths and rows, held counts, then table and stack are dependent trips to memory, the two scans between them
+// run in one workgroup, up to four entries a thread.  Everything whose number depends on the values (blocks moved, token rows) is
+// dealt out flat: thread i finds its entry by bisection of the running sums in LDS, so that one long prompt costs no more than many
+// short ones.  Token rows take a new block's number from the stack and do not wait for the table; steps of many token rows leave
+// these to a second launch over the whole chip.
 
 #include "decode_common.h"
 
 namespace pla {
 
-constexpr int PAGED_PLAN_THREADS = 1024;
-// Token rows up to which the workgroup that makes the plan writes them as well.
+// Token rows up to which the workgroup that makes the plan writes them as well: two steps of 40 requests with 4000 rows take 18.2 us
+// with one launch each and 21.6 with two, with 8000 rows 24.9 and 21.6.
 constexpr int PAGED_PLAN_INLINE_ROWS = 4096;
 constexpr int PAGED_PLAN_MAPPED_ROWS = 8192;      // rows whose first entry is looked up in LDS: 32 KB
 constexpr int32_t PAGED_SATURATED = INT32_MAX;    // of running sums: more than any capacity
@@ -43,26 +44,32 @@ __device__ __forceinline__ int add_saturated(int a, int b) {      // of numbers 
   return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)PAGED_SATURATED);
 }
 
-// Running sum over the workgroup's threads, own value included; `total` gets the sum of all.  Sums saturate, which keeps
+// Running sums over the workgroup's entries, E a thread, own value included; returns the sum of all.  Sums saturate, which keeps
 // them monotone.  `scratch`: one word a wavefront, free again after the caller's next barrier.
-__device__ __forceinline__ int running_sum(int x, int* scratch, int& total) {
+template <int THREADS, int E>
+__device__ __forceinline__ int running_sums(int (&x)[E], int* scratch) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int below = __shfl_up(x, d);
-    if (lane >= d) x = add_saturated(x, below);
-  }
-  if (lane == 63) scratch[wave] = x;
-  __syncthreads();
-  int before = 0;
-  total = 0;
+  for (int i = 1; i < E; ++i) x[i] = add_saturated(x[i - 1], x[i]);
+  int sum = x[E - 1];
 #pragma unroll
-  for (int w = 0; w < PAGED_PLAN_THREADS / 64; ++w) {
+  for (int d = 1; d < 64; d <<= 1) {
+    const int below = __shfl_up(sum, d);
+    if (lane >= d) sum = add_saturated(sum, below);
+  }
+  if (lane == 63) scratch[wave] = sum;
+  const int below = __shfl_up(sum, 1);
+  __syncthreads();
+  int before = lane ? below : 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
     const int s = scratch[w];
     if (w < wave) before = add_saturated(before, s);
     total = add_saturated(total, s);
   }
-  return add_saturated(before, x);
+#pragma unroll
+  for (int i = 0; i < E; ++i) x[i] = add_saturated(before, x[i]);
+  return total;
 }
 
 // The entry whose share of a running sum holds item i: the first of `ends` above i (there is one).
@@ -76,69 +83,74 @@ __device__ __forceinline__ int entry_of(const int* ends, int n, int i) {
 }
 
 struct PagedEntry {
-  int64_t row, context;
-  int query;              // token rows it stands for: its q, or 0 where q is no count
-  int end;                // running sum of these
+  int64_t row, context, query;
+  int end;                // running sum of the token rows
   int held, want;         // equal unless the entry is sound
-  bool sound;
+  bool counted, sound;    // counted: its q is a number of token rows
 };
 
-// Entry `n` (of one thread each; n >= batch: nothing).  `carry`: token rows of the chunks before.
-__device__ __forceinline__ PagedEntry load_entry(const PagedPlan& p, const int* owner, int n, int& carry, int* scratch) {
-  PagedEntry e{0, 0, 0, 0, 0, 0, false};
-  int64_t query = -1;
-  bool inside = false;
-  if (n < p.batch) {
-    e.context = p.at(p.context, p.context_wide, n);
-    query = p.at(p.query, p.query_wide, n);
-    e.row = p.row_of(n);
-    inside = e.row >= 0 && e.row < p.rows;
-    if (inside) e.held = min(max(p.held[e.row], 0), p.cols);
+// A thread's entries n .. n + E - 1 (from the batch's end on: nothing).  `carry`: token rows of the chunks before.
+template <int THREADS, int E>
+__device__ __forceinline__ void load_entries(const PagedPlan& p, const int* owner, int n, int& carry, int* scratch, PagedEntry (&e)[E]) {
+  bool inside[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    e[i] = PagedEntry{0, 0, -1, 0, 0, 0, false, false};
+    if (n + i < p.batch) {
+      e[i].context = p.at(p.context, p.context_wide, n + i);
+      e[i].query = p.at(p.query, p.query_wide, n + i);
+      e[i].row = p.row_of(n + i);
+    }
+    inside[i] = n + i < p.batch && e[i].row >= 0 && e[i].row < p.rows;
+    if (inside[i]) e[i].held = p.held[e[i].row];
   }
-  const bool counted = query >= 0 && query <= p.capacity;
-  e.query = counted ? (int)query : 0;
-  int total;
-  e.end = add_saturated(carry, running_sum(e.query, scratch, total));
+  int rows[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    e[i].counted = e[i].query >= 0 && e[i].query <= p.capacity;
+    rows[i] = e[i].counted ? (int)e[i].query : 0;
+  }
+  const int total = running_sums<THREADS>(rows, scratch);
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    e[i].end = add_saturated(carry, rows[i]);
+    e[i].held = min(max(e[i].held, 0), p.cols);
+    e[i].want = e[i].held;
+    if (inside[i] && e[i].counted && e[i].context >= 0 && e[i].context <= (int64_t)p.cols * p.block && e[i].end <= p.capacity &&
+        (owner == nullptr || owner[e[i].row] == n + i)) {
+      const int want = (int)(((uint32_t)e[i].context + (uint32_t)e[i].query + (uint32_t)p.block - 1) / (uint32_t)p.block);
+      e[i].sound = want <= p.cols;
+      if (e[i].sound) e[i].want = want;
+    }
+  }
   carry = add_saturated(carry, total);
-  e.want = e.held;
-  if (inside && counted && e.context >= 0 && e.context <= (int64_t)p.cols * p.block && e.end <= p.capacity &&
-      (owner == nullptr || owner[e.row] == n)) {
-    const int64_t want = (e.context + query + p.block - 1) / p.block;
-    e.sound = want <= p.cols;
-    if (e.sound) e.want = (int)want;
-  }
-  return e;
 }
 
-// Position and slot of token row t: the plan's results so far say all that is needed.
-__device__ __forceinline__ void write_token_row(const PagedPlan& p, int t, int n, int begin, int length, int end) {
-  // length: of the entry's sequence, 0 if it was refused; its token rows are [begin, end)
-  const bool live = t < end && length > 0;
-  const int position = live ? length - (end - begin) + (t - begin) : 0;
-  int64_t slot = -1;
-  if (live) {
-    const int page = position / p.block;
-    slot = (int64_t)p.table[p.row_of(n) * p.table_stride + page] * p.block + (position - page * p.block);
-  }
-  p.positions[t] = position;
-  p.slots[t] = slot;
+// Position of token row t of an entry whose token rows are [begin, end), and whose sequence has `length` tokens (0: refused);
+// -1: it has none.
+__device__ __forceinline__ int position_of(int t, int begin, int end, int length) {
+  return t < end && length > 0 ? length - (end - begin) + (t - begin) : -1;
+}
+__device__ __forceinline__ void write_token_row(const PagedPlan& p, int t, int position, int block) {
+  p.positions[t] = max(position, 0);
+  p.slots[t] = position < 0 ? -1 : (int64_t)block * p.block + position % p.block;
 }
 
-template <bool TOKEN_ROWS>
-__global__ __launch_bounds__(PAGED_PLAN_THREADS) void paged_plan_kernel(const PagedPlan p) {
+template <int THREADS, int E, bool TOKEN_ROWS>
+__global__ __launch_bounds__(THREADS) void paged_plan_kernel(const PagedPlan p) {
+  constexpr int CHUNK = THREADS * E;
   extern __shared__ int32_t owner_lds[];
-  __shared__ int ends[2][PAGED_PLAN_THREADS];        // of blocks returned or taken | of token rows
-  __shared__ int first[PAGED_PLAN_THREADS];          // page of an entry's first block that moves
-  __shared__ int64_t line[PAGED_PLAN_THREADS];       // its row's start in the table
-  __shared__ int length[PAGED_PLAN_THREADS];
-  __shared__ int scratch[3][PAGED_PLAN_THREADS / 64];
-  const int tid = threadIdx.x, chunks = (p.batch + PAGED_PLAN_THREADS - 1) / PAGED_PLAN_THREADS;
+  __shared__ int token_ends[CHUNK], back_ends[CHUNK], take_ends[CHUNK];   // running sums: token rows, blocks returned, blocks asked for
+  __shared__ int first[CHUNK];                       // page of an entry's first block that moves, or its number of pages
+  __shared__ int length[CHUNK];
+  __shared__ int scratch[3][THREADS / 64], granted_end;
+  const int tid = threadIdx.x, chunks = (p.batch + CHUNK - 1) / CHUNK;
   const int* owner = nullptr;
   if (p.mapping) {
     // the first entry of a row is the row's
-    for (int r = tid; r < p.rows; r += PAGED_PLAN_THREADS) owner_lds[r] = INT32_MAX;
+    for (int r = tid; r < p.rows; r += THREADS) owner_lds[r] = INT32_MAX;
     __syncthreads();
-    for (int n = tid; n < p.batch; n += PAGED_PLAN_THREADS) {
+    for (int n = tid; n < p.batch; n += THREADS) {
       const int64_t row = p.row_of(n);
       if (row >= 0 && row < p.rows) atomicMin(&owner_lds[row], n);
     }
@@ -146,86 +158,105 @@ __global__ __launch_bounds__(PAGED_PLAN_THREADS) void paged_plan_kernel(const Pa
     owner = owner_lds;
   }
 
-  int height = min(max(*p.height, 0), p.stack_size), carry = 0;
-  PagedEntry e{};
-  for (int c = 0; c < chunks; ++c) {                 // blocks that go back
-    const int base = c * PAGED_PLAN_THREADS, count = min(p.batch - base, PAGED_PLAN_THREADS);
-    e = load_entry(p, owner, base + tid, carry, scratch[0]);
-    int total;
-    ends[0][tid] = running_sum(max(e.held - e.want, 0), scratch[1], total);
-    first[tid] = e.want;
-    line[tid] = e.row * p.table_stride;
-    __syncthreads();
-    for (int i = tid; i < total; i += PAGED_PLAN_THREADS) {
-      const int n = entry_of(ends[0], count, i), before = n ? ends[0][n - 1] : 0;
-      if (i < p.stack_size - height) p.stack[height + i] = p.table[line[n] + first[n] + (i - before)];
+  int height = min(max(*p.height, 0), p.stack_size), carry = 0, asked_all = 0;
+  PagedEntry e[E];
+  int take[E];
+  // Running sums of a chunk; returns the blocks it gives back.
+  auto load_chunk = [&](int base, int& asked) {
+    load_entries<THREADS, E>(p, owner, base + tid * E, carry, scratch[0], e);
+    int back[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      back[i] = max(e[i].held - e[i].want, 0);
+      take[i] = max(e[i].want - e[i].held, 0);
     }
-    height = (int)min((int64_t)height + total, (int64_t)p.stack_size);
+    const int returned = running_sums<THREADS>(back, scratch[1]);
+    asked = running_sums<THREADS>(take, scratch[2]);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      back_ends[tid * E + i] = back[i];
+      take_ends[tid * E + i] = take[i];
+      token_ends[tid * E + i] = e[i].end;
+      first[tid * E + i] = min(e[i].held, e[i].want);
+    }
+    if (tid == 0) granted_end = 0;
     __syncthreads();
+    return returned;
+  };
+  int asked = 0;
+  for (int c = 0; c < chunks; ++c) {                 // blocks that go back
+    const int base = c * CHUNK, count = min(p.batch - base, CHUNK), returned = load_chunk(base, asked);
+    for (int i = tid; i < min(returned, p.stack_size - height); i += THREADS) {
+      const int m = entry_of(back_ends, count, i), before = m ? back_ends[m - 1] : 0;
+      p.stack[height + i] = p.table[p.row_of(base + m) * p.table_stride + first[m] + (i - before)];
+    }
+    height = (int)min((int64_t)height + returned, (int64_t)p.stack_size);
+    if (chunks > 1) __syncthreads();
   }
 
   carry = 0;
-  int asked = 0, taken = 0;
+  int taken = 0, first_row = 0;                      // of the chunk's token rows
   for (int c = 0; c < chunks; ++c) {                 // blocks that are taken, and the results
-    const int base = c * PAGED_PLAN_THREADS, count = min(p.batch - base, PAGED_PLAN_THREADS), n = base + tid;
-    if (chunks > 1) e = load_entry(p, owner, n, carry, scratch[0]);
-    const int need = max(e.want - e.held, 0);
-    int total, granted_total;
-    const int sum = add_saturated(asked, running_sum(need, scratch[1], total));
-    asked = add_saturated(asked, total);
-    const bool granted = e.sound && (need == 0 || sum <= height);
-    ends[0][tid] = running_sum(granted ? need : 0, scratch[2], granted_total);
-    ends[1][tid] = e.end;
-    first[tid] = e.held;
-    line[tid] = e.row * p.table_stride;
-    length[tid] = granted ? (int)(e.context + e.query) : 0;
-    if (n < p.batch) {
-      p.offsets[n + 1] = min(e.end, p.capacity);
-      p.seq_lens[n] = length[tid];
-      if (granted) p.held[e.row] = e.want;
+    const int base = c * CHUNK, count = min(p.batch - base, CHUNK);
+    if (chunks > 1) load_chunk(base, asked);
+    // Who is granted blocks: those up to whose own the sum fits.  They come before all that are not, so the sum is also the place.
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int n = base + tid * E + i;
+      const bool needs = e[i].want > e[i].held, granted = e[i].sound && (!needs || add_saturated(asked_all, take[i]) <= height);
+      if (needs && granted) atomicMax(&granted_end, take[i]);
+      const int tokens = granted ? (int)(e[i].context + e[i].query) : 0;
+      length[tid * E + i] = tokens;
+      if (n < p.batch) {
+        p.offsets[n + 1] = min(e[i].end, p.capacity);
+        p.seq_lens[n] = tokens;
+        if (granted) p.held[e[i].row] = e[i].want;
+      }
+      if (n == 0) p.offsets[0] = 0;
     }
-    if (n == 0) p.offsets[0] = 0;
     __syncthreads();
-    for (int i = tid; i < granted_total; i += PAGED_PLAN_THREADS) {
-      const int m = entry_of(ends[0], count, i), before = m ? ends[0][m - 1] : 0;
-      p.table[line[m] + first[m] + (i - before)] = p.stack[height - 1 - (taken + i)];
+    const int granted_total = granted_end;
+    const int top = height - 1 - taken;              // of the stack, for this chunk's first block
+    for (int i = tid; i < granted_total; i += THREADS) {
+      const int m = entry_of(take_ends, count, i), before = m ? take_ends[m - 1] : 0;
+      p.table[p.row_of(base + m) * p.table_stride + first[m] + (i - before)] = p.stack[top - i];
+    }
+    if (TOKEN_ROWS) {
+      const int end = min(token_ends[count - 1], p.capacity);
+      for (int t = first_row + tid; t < end; t += THREADS) {
+        const int m = entry_of(token_ends, count, t), position = position_of(t, m ? token_ends[m - 1] : first_row, token_ends[m], length[m]);
+        const int page = max(position, 0) / p.block;
+        int block = 0;
+        if (position >= 0)
+          block = page < first[m] ? p.table[p.row_of(base + m) * p.table_stride + page]
+                                  : p.stack[top - ((m ? take_ends[m - 1] : 0) + page - first[m])];
+        write_token_row(p, t, position, block);
+      }
+      first_row = end;
     }
     taken += granted_total;
-    __syncthreads();
-    if (TOKEN_ROWS) {
-      const int begin = base ? p.offsets[base] : 0, end = min(ends[1][count - 1], p.capacity);
-      for (int t = begin + tid; t < end; t += PAGED_PLAN_THREADS) {
-        const int m = entry_of(ends[1], count, t);
-        write_token_row(p, t, base + m, m ? ends[1][m - 1] : begin, length[m], ends[1][m]);
-      }
-      __syncthreads();
-    }
+    asked_all = add_saturated(asked_all, asked);
+    if (chunks > 1) __syncthreads();
   }
   if (tid == 0) {
     *p.height = height - taken;
     if (p.batch == 0) p.offsets[0] = 0;
   }
-  if (TOKEN_ROWS) {
-    const int used = p.batch ? p.offsets[p.batch] : 0;
-    for (int t = used + tid; t < p.capacity; t += PAGED_PLAN_THREADS) {
-      p.positions[t] = 0;
-      p.slots[t] = -1;
-    }
-  }
+  if (TOKEN_ROWS)
+    for (int t = first_row + tid; t < p.capacity; t += THREADS) write_token_row(p, t, -1, 0);
 }
 
 // Token rows of a step that has many: one a thread.
 __global__ __launch_bounds__(256) void paged_token_rows_kernel(const PagedPlan p) {
   const int t = blockIdx.x * 256 + threadIdx.x;
   if (t >= p.capacity) return;
-  int n = 0, begin = 0, end = 0, length = 0;
+  int position = -1, block = 0;
   if (p.batch > 0 && t < p.offsets[p.batch]) {
-    n = entry_of(p.offsets + 1, p.batch, t);
-    begin = p.offsets[n];
-    end = p.offsets[n + 1];
-    length = p.seq_lens[n];
+    const int n = entry_of(p.offsets + 1, p.batch, t);
+    position = position_of(t, p.offsets[n], p.offsets[n + 1], p.seq_lens[n]);
+    if (position >= 0) block = p.table[p.row_of(n) * p.table_stride + position / p.block];
   }
-  write_token_row(p, t, n, begin, length, end);
+  write_token_row(p, t, position, block);
 }
 
 }  // namespace pla
@@ -238,7 +269,8 @@ extern "C" int pla_paged_kv_plan_launch(
   using namespace pla;
   PLA_REQUIRE(batch >= 0 && token_capacity >= 0 && token_capacity <= (1 << 30), "batch and token_capacity must be between 0 and 2^30");
   PLA_REQUIRE(table_rows >= 0 && table_cols >= 0 && table_row_stride >= table_cols, "invalid block table dimensions");
-  PLA_REQUIRE(block_size > 0 && (int64_t)table_cols * block_size <= INT32_MAX, "block_size must be positive and a row's positions must fit 32 bits");
+  PLA_REQUIRE(block_size > 0 && block_size <= (1 << 30) && (int64_t)table_cols * block_size <= (1 << 30),
+              "block_size must be positive and a row's positions at most 2^30");
   PLA_REQUIRE(free_capacity >= 0 && free_capacity <= (1 << 30), "invalid free stack size");
   PLA_REQUIRE(mapping != nullptr || batch <= table_rows, "more batch entries than rows of the block table");
   PLA_REQUIRE(mapping == nullptr || table_rows <= PAGED_PLAN_MAPPED_ROWS, "request_indices take at most %d rows", PAGED_PLAN_MAPPED_ROWS);
@@ -252,11 +284,12 @@ extern "C" int pla_paged_kv_plan_launch(
                     offsets, seq_lens, positions, slots};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const size_t lds = mapping ? (size_t)table_rows * sizeof(int32_t) : 0;
-  if (token_capacity <= PAGED_PLAN_INLINE_ROWS) {
-    paged_plan_kernel<true><<<1, PAGED_PLAN_THREADS, lds, s>>>(p);
-  } else {
-    paged_plan_kernel<false><<<1, PAGED_PLAN_THREADS, lds, s>>>(p);
-    paged_token_rows_kernel<<<(token_capacity + 255) / 256, 256, 0, s>>>(p);
-  }
+  const bool rows_inline = token_capacity <= PAGED_PLAN_INLINE_ROWS;
+  if (batch <= 256 && token_capacity <= 1024) paged_plan_kernel<256, 1, true><<<1, 256, lds, s>>>(p);
+  else if (batch <= 1024 && rows_inline) paged_plan_kernel<1024, 1, true><<<1, 1024, lds, s>>>(p);
+  else if (batch <= 1024) paged_plan_kernel<1024, 1, false><<<1, 1024, lds, s>>>(p);
+  else if (rows_inline) paged_plan_kernel<1024, 4, true><<<1, 1024, lds, s>>>(p);
+  else paged_plan_kernel<1024, 4, false><<<1, 1024, lds, s>>>(p);
+  if (!rows_inline) paged_token_rows_kernel<<<(token_capacity + 255) / 256, 256, 0, s>>>(p);
   return check_launch("paged_plan_kernel");
 }
