@@ -7,11 +7,18 @@
 // to k_out and / or the cache row of the token's slot, values to the cache as they are.  FP32 throughout, one rounding at the end.
 //
 // Angles: at position 10^6 a product in FP32 is off by 0.06 radians.  Position and frequency are multiplied in FP64, as
-// revolutions, and only the part below one revolution is narrowed: sine and cosine are then good to FP32's own rounding.  A
-// workgroup works out the rot/2 pairs of its token once and leaves them in LDS for all of its heads.
+// revolutions, and only the part below one revolution is narrowed, for v_sin_f32 and v_cos_f32, which take revolutions and are off by
+// at most 1.3e-7 between minus and plus a half (measured at 2^20 places).
 //
-// Bound by HBM: every row is read once and written once, 16 bytes a lane.  D / 8 lanes hold a row, so its sum of squares is a
-// few DPP steps, and the partner channels of the split layout sit in another lane of the same wavefront.
+// Bound by HBM, if the instructions stay out of its way: every row is read once and written once, 16 bytes a lane, D / 8 lanes a row.
+// A wavefront takes a step of 64 / (D / 8) heads of one kind (q, k or v) at a time, so pointers, strides and kind are scalars, and
+// all of a token's steps in a large call: a lane works out an angle, the pairs go through LDS of the wavefront's own without a
+// barrier, and weight, cosine and sine become two factors a channel once for all rows of a kind.  The sum of squares is a few DPP
+// steps, the partner channels of the split layout sit in another lane of the row.  16 384 tokens of 32 + 8 heads (D 128, 336 MB) take
+// 63.5 us (5.3 TB/s; a large copy runs at 4.75), with norms 68, with norms and both caches (403 MB) 80; a workgroup a token, whose
+// wavefronts each worked out the factors for two or three rows, took 65, 85 and 100.  Without the hint that rows go past the caches
+// 82, 82 and 96.
+// Small calls take a step a wavefront, for the shortest chain: 8 tokens 5.6 us a call, launch bound (kernel 4.6).
 
 #include "decode_common.h"
 
@@ -29,7 +36,9 @@ struct QkNormRope {
   uint16_t *k_cache, *v_cache;
   int64_t kc_block, kc_token, kc_head, vc_block, vc_token, vc_head;
   const void* slots; int slots_wide; int block, cache_slots;
-  int tokens, HQ, HKV, chunks;        // chunks: workgroups a token
+  int tokens, HQ, HKV;
+  int q_steps, k_steps, steps;        // of a token: for queries, for keys, and with those for values
+  int chunk, chunks;                  // steps a wavefront, wavefronts a token
 };
 
 template <int LANES>
@@ -64,133 +73,171 @@ __device__ __forceinline__ void weights8(const void* weight, int f32, int channe
   for (int i = 0; i < 8; ++i) w[i] += offset;
 }
 
-// ROWS rows a group of D / 8 lanes, all of one token; their loads go out together, before the angles are worked out.
-template <typename act_t, int D, int ROWS>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
-  constexpr int LANES = D / 8, GROUPS = 256 / LANES;
-  __shared__ __align__(16) float cosines[D / 2], sines[D / 2];
-  const int token = blockIdx.x / p.chunks, chunk = blockIdx.x - token * p.chunks;
-  const int group = threadIdx.x / LANES, lane = threadIdx.x & (LANES - 1), channel = 8 * lane;
-  const int heads = p.HQ + (p.v_cache ? 2 : 1) * p.HKV;
-  const int first = chunk * GROUPS * ROWS + group;
+// Through the scalar cache, where the address is one for the wavefront.
+__device__ __forceinline__ int64_t scalar_index(const void* base, int wide, int i) {
+  typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+  const int32_t* p = static_cast<const int32_t*>(base) + (wide ? 2 * (int64_t)i : i);
+  const int32_t low = *(scalar_ptr)p;
+  return wide ? (int64_t)((uint64_t)(uint32_t)low | (uint64_t)(uint32_t)*(scalar_ptr)(p + 1) << 32) : (int64_t)low;
+}
 
-  // the token's cache row, -1: nowhere
-  int64_t slot = -1;
-  if (p.slots) {
-    slot = p.slots_wide ? static_cast<const int64_t*>(p.slots)[token] : (int64_t) static_cast<const int32_t*>(p.slots)[token];
-    if (slot >= p.cache_slots) slot = -1;
-  }
-  uint4 raw[ROWS] = {};
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const int h = first + r * GROUPS;
-    if (h >= heads) continue;
-    const uint16_t* row = h < p.HQ ? p.q + token * p.q_token + h * p.q_head
-                        : h < p.HQ + p.HKV ? p.k + token * p.k_token + (h - p.HQ) * p.k_head
-                                           : p.v + token * p.v_token + (h - p.HQ - p.HKV) * p.v_head;
-    raw[r] = *reinterpret_cast<const uint4*>(row + channel);
-  }
-  if (p.rot) {
-    const int half = p.rot / 2;
-    for (int i = threadIdx.x; i < half; i += 256) {
-      const int64_t position = p.positions_wide ? static_cast<const int64_t*>(p.positions)[token]
-                                                : (int64_t) static_cast<const int32_t*>(p.positions)[token];
-      const double turns = (double)position * ((double)p.inv_freq[i] * 0.15915494309189533577);     // 1 / (2 pi)
-      float s, c;
-      sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-      cosines[i] = c * p.attention_factor;
-      sines[i] = s * p.attention_factor;
+// Bytes of rows from which on a call's rows go past the caches; below, whoever reads them next finds them there.
+constexpr int64_t PAST_CACHES = 48ll << 20;
+constexpr int WAVES_RESIDENT = 8192;  // on the chip, about
+
+template <typename act_t, int D, bool PAST>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
+  constexpr int LANES = D / 8, HEADS = 64 / LANES, AHEAD = 2;            // heads of a step, steps whose rows are asked for together
+  __shared__ __align__(16) float turn[4][2][D / 2];                      // cosines and sines of a wavefront's token
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), item = blockIdx.x * 4 + wave;
+  const int token = item / p.chunks, begin = (item - token * p.chunks) * p.chunk, end = min(begin + p.chunk, p.steps);
+  if (token >= p.tokens) return;
+  const int here = threadIdx.x & 63, lane = here & (LANES - 1), channel = 8 * lane, head = here / LANES;
+
+  // Kind of a step (0 q, 1 k, 2 v) and the head that this lane has of it.
+  auto kind_of = [&](int step) { return step < p.q_steps ? 0 : step < p.q_steps + p.k_steps ? 1 : 2; };
+  auto head_of = [&](int step, int kind) { return (step - (kind == 0 ? 0 : kind == 1 ? p.q_steps : p.q_steps + p.k_steps)) * HEADS + head; };
+  auto load_row = [&](int step) {
+    uint4 x = {0, 0, 0, 0};
+    if (step >= end) return x;
+    const int kind = kind_of(step), h = head_of(step, kind);
+    const uint16_t* base = kind == 0 ? p.q + token * p.q_token : kind == 1 ? p.k + token * p.k_token : p.v + token * p.v_token;
+    const int64_t stride = kind == 0 ? p.q_head : kind == 1 ? p.k_head : p.v_head;
+    if (h < (kind == 0 ? p.HQ : p.HKV)) {
+      const uint16_t* row = base + h * stride + channel;
+      x = PAST ? __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const v4i_t*>(row))) : *reinterpret_cast<const uint4*>(row);
     }
-    __syncthreads();
+    return x;
+  };
+  auto store_row = [&](uint16_t* row, uint4 x) {
+    if (PAST) __builtin_nontemporal_store(__builtin_bit_cast(v4i_t, x), reinterpret_cast<v4i_t*>(row + channel));
+    else *reinterpret_cast<uint4*>(row + channel) = x;
+  };
+  // The longest chain first: position, angle, LDS, factors.  Then the rows, then where they go.
+  constexpr int FREQUENCIES = D > 128 ? D / 128 : 1;
+  float frequency[FREQUENCIES];
+  int64_t position = 0;
+  if (p.rot) {
+    position = scalar_index(p.positions, p.positions_wide, token);
+#pragma unroll
+    for (int i = 0; i < FREQUENCIES; ++i) frequency[i] = p.inv_freq[min(here + 64 * i, p.rot / 2 - 1)];
   }
-  // this lane's part of the rotation: out = x * cos + partner * sin, sin with the sign of its side
+  uint4 raw[AHEAD];
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a) raw[a] = load_row(begin + a);
+  // the token's cache row; negative: nowhere
+  int64_t slot = p.slots ? scalar_index(p.slots, p.slots_wide, token) : -1;
+  if (slot >= p.cache_slots) slot = -1;
+  const int block = slot >= 0 ? (int)slot / p.block : 0, place = slot >= 0 ? (int)slot - block * p.block : 0;
+  if (p.rot) {
+#pragma unroll
+    for (int i = 0; i < FREQUENCIES; ++i) {
+      const double turns = (double)position * ((double)frequency[i] * 0.15915494309189533577);        // 1 / (2 pi)
+      const float part = (float)(turns - rint(turns));
+      if (here + 64 * i < p.rot / 2) {
+        turn[wave][0][here + 64 * i] = __builtin_amdgcn_cosf(part) * p.attention_factor;
+        turn[wave][1][here + 64 * i] = __builtin_amdgcn_sinf(part) * p.attention_factor;
+      }
+    }
+  }
+  // out = rstd (x straight + partner cross)
   const bool turns = channel < p.rot;
-  const int half = p.rot / 2, side = p.interleaved ? 0 : half / 8;          // lanes to the partner
-  const bool upper = !p.interleaved && channel >= half;
-  float cosine[8], sine[8];
-  if (turns) {
-    const int i0 = p.interleaved ? channel / 2 : upper ? channel - half : channel;
+  const int half = p.rot / 2;
+  const bool split = p.rot && !p.interleaved, upper = split && channel >= half;
+  const int partner = !turns || !split ? here : upper ? here - half / 8 : here + half / 8;
+  float straight[8], cross[8];
+  auto prepare = [&](int kind) {
+    const void* weight = kind ? p.k_weight : p.q_weight;
+    float w[8], v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = v[i] = 1.f;
+    if (weight) {
+      weights8<act_t>(weight, p.weights_f32, channel, p.weight_offset, w);
+      if (split) weights8<act_t>(weight, p.weights_f32, channel + 8 * (partner - here), p.weight_offset, v);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int f = p.interleaved ? i0 + i / 2 : i0 + i;
-      cosine[i] = cosines[f];
-      sine[i] = (p.interleaved ? (i & 1) != 0 : upper) ? sines[f] : -sines[f];
-    }
-  }
-  const int here = threadIdx.x & 63, partner_lane = !turns || p.interleaved ? here : upper ? here - side : here + side;
-  const int partner_channel = channel + 8 * (partner_lane - here);
-
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const int h = first + r * GROUPS;
-    // all lanes of a wavefront take part in the exchange
-    uint4 other;
-    other.x = __shfl(raw[r].x, partner_lane); other.y = __shfl(raw[r].y, partner_lane);
-    other.z = __shfl(raw[r].z, partner_lane); other.w = __shfl(raw[r].w, partner_lane);
-    float x[8], y[8];
-    widen8<act_t>(raw[r], x);
-    widen8<act_t>(other, y);
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-    sum = lanes_allreduce<LANES>(sum);
-    if (h >= heads) continue;
-    const bool is_q = h < p.HQ, is_v = h >= p.HQ + p.HKV;
-    uint4 result = raw[r];
-    if (!is_v) {
-      const void* weight = is_q ? p.q_weight : p.k_weight;
-      if (weight) {
-        const float rstd = 1.0f / sqrtf(sum * (1.0f / D) + p.eps);
-        float w[8];
-        weights8<act_t>(weight, p.weights_f32, channel, p.weight_offset, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= rstd * w[i];
-        if (turns && !p.interleaved) {
-          weights8<act_t>(weight, p.weights_f32, partner_channel, p.weight_offset, w);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] *= rstd * w[i];
-        }
-      }
+      straight[i] = w[i];
+      cross[i] = 0.f;
       if (turns) {
-        if (p.interleaved) {
+        const int f = split ? channel + i - (upper ? half : 0) : (channel + i) / 2;
+        const float s = (split ? upper : (i & 1) != 0) ? turn[wave][1][f] : -turn[wave][1][f];
+        straight[i] = w[i] * turn[wave][0][f];
+        cross[i] = (split ? v[i] : w[i ^ 1]) * s;
+      }
+    }
+  };
+
+  int prepared = -1;
+  for (int step0 = begin; step0 < end; step0 += AHEAD) {
+    uint4 now[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) now[a] = raw[a];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) raw[a] = load_row(step0 + AHEAD + a);
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int step = step0 + a;
+      if (step >= end) break;
+      const int kind = kind_of(step), h = head_of(step, kind);
+      uint4 result = now[a];
+      if (kind < 2) {
+        if (kind != prepared) {
+          prepare(kind);
+          prepared = kind;
+        }
+        float x[8], y[8];
+        widen8<act_t>(now[a], x);
+        if (split) {
+          uint4 other;
+          other.x = __shfl(now[a].x, partner); other.y = __shfl(now[a].y, partner);
+          other.z = __shfl(now[a].z, partner); other.w = __shfl(now[a].w, partner);
+          widen8<act_t>(other, y);
+        } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
         }
+        float rstd = 1.f;
+        if (kind ? p.k_weight : p.q_weight) {
+          float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], cosine[i], y[i] * sine[i]);
+          for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+          rstd = fast_rsqrt(lanes_allreduce<LANES>(sum) * (1.0f / D) + p.eps);
+        }
+        // (a channel that does not turn has no partner: what stands in its place must not meet the factor of zero)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float along = x[i] * straight[i];
+          x[i] = (turns ? fmaf(y[i], cross[i], along) : along) * rstd;
+        }
+        result = make_uint4(pack2<act_t>(x[0], x[1]), pack2<act_t>(x[2], x[3]), pack2<act_t>(x[4], x[5]), pack2<act_t>(x[6], x[7]));
       }
-      result = make_uint4(pack2<act_t>(x[0], x[1]), pack2<act_t>(x[2], x[3]), pack2<act_t>(x[4], x[5]), pack2<act_t>(x[6], x[7]));
-    }
-    const int kv = is_v ? h - p.HQ - p.HKV : h - p.HQ;
-    if (is_q) {
-      *reinterpret_cast<uint4*>(p.q_out + token * p.qo_token + h * p.qo_head + channel) = result;
-    } else if (!is_v && p.k_out) {
-      *reinterpret_cast<uint4*>(p.k_out + token * p.ko_token + kv * p.ko_head + channel) = result;
-    }
-    if (!is_q && slot >= 0) {
-      const int block = (int)slot / p.block, place = (int)slot - block * p.block;
-      uint16_t* row = is_v ? p.v_cache + block * p.vc_block + place * p.vc_token + kv * p.vc_head
-                           : p.k_cache + block * p.kc_block + place * p.kc_token + kv * p.kc_head;
-      *reinterpret_cast<uint4*>(row + channel) = result;
+      if (h >= (kind == 0 ? p.HQ : p.HKV)) continue;
+      if (kind == 0) {
+        store_row(p.q_out + token * p.qo_token + h * p.qo_head, result);
+      } else {
+        if (kind == 1 && p.k_out) store_row(p.k_out + token * p.ko_token + h * p.ko_head, result);
+        if (slot >= 0)
+          store_row(kind == 1 ? p.k_cache + block * p.kc_block + place * p.kc_token + h * p.kc_head
+                              : p.v_cache + block * p.vc_block + place * p.vc_token + h * p.vc_head, result);
+      }
     }
   }
 }
 
 template <typename act_t, int D>
 static void launch_qk_norm_rope(QkNormRope p, hipStream_t s) {
-  constexpr int GROUPS = 256 / (D / 8);
-  const int heads = p.HQ + (p.v_cache ? 2 : 1) * p.HKV;
-  // Few rows: one a group, for the shortest chain.  Many: up to four a group share the token's angles.
-  const int per_token = (heads + GROUPS - 1) / GROUPS;
-  const int rows = (int64_t)p.tokens * per_token <= 1024 ? 1 : per_token < 4 ? per_token : 4;
-  p.chunks = (per_token + rows - 1) / rows;
-  const dim3 grid((unsigned)p.tokens * p.chunks);
-  switch (rows) {
-    case 1: qk_norm_rope_kernel<act_t, D, 1><<<grid, 256, 0, s>>>(p); break;
-    case 2: qk_norm_rope_kernel<act_t, D, 2><<<grid, 256, 0, s>>>(p); break;
-    case 3: qk_norm_rope_kernel<act_t, D, 3><<<grid, 256, 0, s>>>(p); break;
-    default: qk_norm_rope_kernel<act_t, D, 4><<<grid, 256, 0, s>>>(p); break;
-  }
+  constexpr int HEADS = 64 / (D / 8);
+  p.q_steps = (p.HQ + HEADS - 1) / HEADS;
+  p.k_steps = (p.HKV + HEADS - 1) / HEADS;
+  p.steps = p.q_steps + (p.v_cache ? 2 : 1) * p.k_steps;
+  // As many steps a wavefront as leave the chip its wavefronts; a token's angles are worked out by each of its wavefronts.
+  const int64_t share = ((int64_t)p.tokens * p.steps + WAVES_RESIDENT - 1) / WAVES_RESIDENT;
+  p.chunk = (int)(share < p.steps ? share : p.steps);
+  p.chunks = (p.steps + p.chunk - 1) / p.chunk;
+  const dim3 grid((unsigned)(((int64_t)p.tokens * p.chunks + 3) / 4));
+  if ((int64_t)p.tokens * (p.HQ + p.HKV) * D * 2 > PAST_CACHES) qk_norm_rope_kernel<act_t, D, true><<<grid, 256, 0, s>>>(p);
+  else qk_norm_rope_kernel<act_t, D, false><<<grid, 256, 0, s>>>(p);
 }
 
 template <typename act_t>
@@ -231,7 +278,7 @@ extern "C" int pla_qk_norm_rope_launch(
                      positions, positions_wide, q_weight, k_weight, weights_f32, eps, weight_offset, inv_freq, rotary_dim,
                      attention_factor, interleaved, (uint16_t*)q_out, (uint16_t*)k_out, t[6], t[7], t[8], t[9],
                      (uint16_t*)k_cache, (uint16_t*)v_cache, t[10], t[11], t[12], t[13], t[14], t[15],
-                     slots, slots_wide, block_size, k_cache ? blocks * block_size : 0, tokens, HQ, HKV, 1};
+                     slots, slots_wide, block_size, k_cache ? blocks * block_size : 0, tokens, HQ, HKV, 0, 0, 0, 0, 0};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (act_dtype == PLA_BF16) launch_qk_norm_rope<bf16_t>(p, D, s);
   else launch_qk_norm_rope<f16_t>(p, D, s);
