@@ -240,6 +240,16 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, const u32x4_t* que
       if (__ballot((odd & 0x80008000u) != 0) != 0) {
         stop = least;
         w.set_aside = key0;
+        // their weights come back into the sum with their values, rounded alike
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const u32x4_t u = __builtin_bit_cast(u32x4_t, packed[t]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float weight = i & 1 ? hi16<act_t>(u[i / 2]) : lo16<act_t>(u[i / 2]);
+            if (key + 16 * (i / 4) + (i & 3) >= least) w.sum[t] -= weight;
+          }
+        }
       }
     }
 #pragma unroll
@@ -263,11 +273,11 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, const u32x4_t* que
   next_values();
 }
 
-// The weighted values of keys [first, last) for one row, into the D / TEAM channels of it that a thread has; the TEAM threads of a
-// row form its scores together.
+// The weights of keys [first, last) for one row into its sum, and their values into the D / TEAM channels of it that a thread has;
+// the TEAM threads of a row form its scores together.
 template <typename act_t, int D, int TEAM>
 __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const PagedRequest& req, int kv_head, int row, int channel,
-                                              const int32_t* pages, int first, int last, float top, float (&o)[D / TEAM]) {
+                                              const int32_t* pages, int first, int last, float top, float& sum, float (&o)[D / TEAM]) {
   const int j = row / p.shape.group, head = kv_head * p.shape.group + row - j * p.shape.group;
   const uint16_t* q = p.q + (req.begin + j) * p.q_token + head * p.q_head + channel;
   last = min(last, paged_limit(p.shape, req, row));
@@ -280,8 +290,13 @@ __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const Pag
     for (int i = 0; i < D / TEAM; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
     score = (TEAM == 16 ? row16_allreduce(score) : row32_allreduce(score)) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
     const float weight = to_float(from_float<act_t>(__builtin_amdgcn_exp2f(score)));
+    sum += weight;
 #pragma unroll
-    for (int i = 0; i < D / TEAM; ++i) o[i] = fmaf(weight, to_float(act_t{p.v[at + i]}), o[i]);
+    for (int i = 0; i < D / TEAM; ++i) {
+      const float x = to_float(act_t{p.v[at + i]});
+      // a weight below the smallest is no weight, but an infinite value has some
+      o[i] = fmaf(weight == 0.f && !(fabsf(x) < INFINITY) ? 0x1p-126f : weight, x, o[i]);
+    }
   }
 }
 
@@ -549,7 +564,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
         const int row = a.row0 + 16 * t + out_row;
         for (int x = 0; x < WAVES; ++x)
           if (aside[x] >= 0)
-            add_set_aside<act_t, D, TEAM>(p, a.req, a.seg.head, row, out_channel, a.pages, max(aside[x], a.least), min(aside[x] + 32, a.end), row_top, o);
+            add_set_aside<act_t, D, TEAM>(p, a.req, a.seg.head, row, out_channel, a.pages, max(aside[x], a.least), min(aside[x] + 32, a.end), row_top, row_sum, o);
         if (a.seg.slot < 0) {
           const int j = row / p.shape.group, head = a.seg.head * p.shape.group + row - j * p.shape.group;
           const float norm = row_sum == 0.f ? 0.f : 1.0f / row_sum;         // no key: zeros

@@ -9,11 +9,13 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <initializer_list>
 #include <optional>
 #include <tuple>
+#include <vector>
 
 #include "../../include/pla_gfx950.h"
 
@@ -58,23 +60,35 @@ void on_one_gpu(const Tensor& ref, const char* name, std::initializer_list<std::
   TORCH_CHECK(ref.is_cuda(), name, " must be a CUDA tensor");
 }
 
-// Whether two tensors may share memory: extents apart, or rows of one pitch (dimension 0) that lie apart within it.
-std::pair<uintptr_t, uintptr_t> extent(const Tensor& t, int from) {
-  int64_t n = 1;
-  for (int64_t d = from; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
-  const auto base = reinterpret_cast<uintptr_t>(t.data_ptr());
-  return {base, base + n * t.element_size()};
+// Whether two tensors may share memory.  Views of one buffer interleave (q, k and v of a projection row; K and V of a block): where
+// both step by the same stride, what counts is where one lies within a step of the other, dimension by dimension.
+struct Dims { int64_t size, stride; };         // bytes
+int64_t extent(const std::vector<Dims>& d, size_t from, int64_t element) {
+  int64_t n = element;
+  for (size_t i = from; i < d.size(); ++i) n += (d[i].size - 1) * d[i].stride;
+  return n;
+}
+bool lap(const std::vector<Dims>& a, const std::vector<Dims>& b, size_t i, size_t j, int64_t ahead, int64_t ea, int64_t eb) {
+  // `ahead`: of b's first byte to a's
+  if (ahead >= extent(a, i, ea) || -ahead >= extent(b, j, eb)) return false;
+  if (i == a.size() || j == b.size() || a[i].stride != b[j].stride) return true;
+  const int64_t step = a[i].stride, rest = ((ahead % step) + step) % step;
+  return lap(a, b, i + 1, j + 1, rest, ea, eb) || lap(a, b, i + 1, j + 1, rest - step, ea, eb);
+}
+std::vector<Dims> dims_of(const Tensor& t) {
+  std::vector<Dims> d;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) > 0) d.push_back({t.size(i), t.stride(i) * (int64_t)t.element_size()});
+  std::stable_sort(d.begin(), d.end(), [](const Dims& x, const Dims& y) { return x.stride > y.stride; });
+  return d;
 }
 bool may_overlap(const Tensor& a, const Tensor& b) {
   if (a.numel() == 0 || b.numel() == 0) return false;
-  const auto [a0, a1] = extent(a, 0);
-  const auto [b0, b1] = extent(b, 0);
-  if (a1 <= b0 || b1 <= a0) return false;
-  const uintptr_t pitch = a.dim() > 1 ? a.stride(0) * a.element_size() : 0;
-  if (pitch == 0 || b.dim() < 2 || (uintptr_t)(b.stride(0) * b.element_size()) != pitch) return true;
-  const uintptr_t row_a = extent(a, 1).second - a0, row_b = extent(b, 1).second - b0;
-  const uintptr_t ahead = b0 >= a0 ? (b0 - a0) % pitch : (pitch - (a0 - b0) % pitch) % pitch;
-  return !(ahead >= row_a && ahead + row_b <= pitch);
+  const auto base_a = reinterpret_cast<intptr_t>(a.data_ptr()), base_b = reinterpret_cast<intptr_t>(b.data_ptr());
+  const int64_t ahead = base_b - base_a;
+  if (a.is_contiguous() && ahead >= (int64_t)(a.numel() * a.element_size())) return false;        // the usual case, quickly
+  if (b.is_contiguous() && -ahead >= (int64_t)(b.numel() * b.element_size())) return false;
+  return lap(dims_of(a), dims_of(b), 0, 0, ahead, a.element_size(), b.element_size());
 }
 bool same_rows(const Tensor& a, const Tensor& b) { return a.data_ptr() == b.data_ptr() && a.strides() == b.strides(); }
 void apart(std::initializer_list<std::pair<const char*, const OptTensor*>> written,
@@ -141,18 +155,22 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> paged_kv_plan(
 
 // ---- caches ------------------------------------------------------------------------------------------------------
 
+// A dimension of one entry steps nowhere, whatever its stride says.
+int64_t step(const Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+int64_t step(const OptTensor& t, int64_t d) { return t ? step(*t, d) : 0; }
+
 void head_rows(const Tensor& t, const char* name, int64_t tokens, int64_t heads, int64_t D, at::ScalarType act) {
   TORCH_CHECK(t.dim() == 3 && t.size(0) == tokens && t.size(1) == heads && t.size(2) == D, name, " must be [", tokens, ", ", heads, ", ", D,
               "], got ", t.sizes());
   TORCH_CHECK(t.scalar_type() == act, name, " must be ", act, ", got ", t.scalar_type());
-  TORCH_CHECK(t.numel() == 0 || (t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0),
+  TORCH_CHECK(t.numel() == 0 || (t.stride(2) == 1 && step(t, 0) % 8 == 0 && step(t, 1) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0),
               name, " must have dense channels and 16-byte aligned rows");
 }
 void cache_form(const Tensor& t, const char* name, int64_t heads, int64_t D, at::ScalarType act) {
   TORCH_CHECK(t.dim() == 4 && t.size(2) == heads && t.size(3) == D, name, " must be [blocks, block_size, ", heads, ", ", D, "], got ", t.sizes());
   TORCH_CHECK(t.scalar_type() == act, name, " must be ", act, ", got ", t.scalar_type());
   TORCH_CHECK(t.size(0) > 0 && t.size(1) > 0, name, " must hold at least one block");
-  TORCH_CHECK(t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
+  TORCH_CHECK(t.stride(3) == 1 && step(t, 0) % 8 == 0 && step(t, 1) % 8 == 0 && step(t, 2) % 8 == 0 &&
                   reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
               name, " must have dense channels and 16-byte aligned rows");
   TORCH_CHECK(t.size(0) * t.size(1) <= INT32_MAX, name, " must have at most 2^31 - 1 slots");
@@ -224,11 +242,9 @@ std::tuple<Tensor, OptTensor> fused_qk_norm_rope(
   OptTensor k_out = k_out_in;
   if (!k_out && !k_cache) k_out = at::empty({T, HKV, D}, q.options());
   if (bypass() || T == 0) return {q_out, k_out};
-  const int64_t strides[16] = {
-      q.stride(0), q.stride(1), k.stride(0), k.stride(1), v ? v->stride(0) : 0, v ? v->stride(1) : 0, q_out.stride(0), q_out.stride(1),
-      k_out ? k_out->stride(0) : 0, k_out ? k_out->stride(1) : 0,
-      k_cache ? k_cache->stride(0) : 0, k_cache ? k_cache->stride(1) : 0, k_cache ? k_cache->stride(2) : 0,
-      v_cache ? v_cache->stride(0) : 0, v_cache ? v_cache->stride(1) : 0, v_cache ? v_cache->stride(2) : 0};
+  const int64_t strides[16] = {step(q, 0), step(q, 1), step(k, 0), step(k, 1), step(v, 0), step(v, 1), step(q_out, 0), step(q_out, 1),
+                               step(k_out, 0), step(k_out, 1), step(k_cache, 0), step(k_cache, 1), step(k_cache, 2),
+                               step(v_cache, 0), step(v_cache, 1), step(v_cache, 2)};
   const bool f32 = (q_weight && q_weight->scalar_type() == at::kFloat) || (k_weight && k_weight->scalar_type() == at::kFloat);
   launched(pla_qk_norm_rope_launch(
       q.data_ptr(), k.data_ptr(), ptr(v), strides, ptr(positions), wide(positions), ptr(q_weight), ptr(k_weight), f32 ? 1 : 0, (float)eps,
@@ -256,9 +272,11 @@ Tensor paged_attention_decode(
   TORCH_CHECK(HKV > 0 && HQ >= HKV && HQ % HKV == 0, "query heads must be a positive multiple of key-value heads, got ", HQ, " and ", HKV);
   cache_form(k_cache, "k_cache", HKV, D, type);
   cache_form(v_cache, "v_cache", HKV, D, type);
-  TORCH_CHECK(v_cache.sizes() == k_cache.sizes() && v_cache.strides() == k_cache.strides(), "k_cache and v_cache must have the same shape and strides");
+  TORCH_CHECK(v_cache.sizes() == k_cache.sizes() && step(v_cache, 0) == step(k_cache, 0) && step(v_cache, 1) == step(k_cache, 1) &&
+                  step(v_cache, 2) == step(k_cache, 2),
+              "k_cache and v_cache must have the same shape and strides");
   TORCH_CHECK(block_size % 16 == 0, "block_size must be a multiple of 16, got ", block_size);
-  TORCH_CHECK(k_cache.stride(1) >= 0 && k_cache.stride(1) < (1 << 24), "the caches' token stride must be below 2^24");
+  TORCH_CHECK(step(k_cache, 1) < (1 << 24), "the caches' token stride must be below 2^24");
   block_table_form(block_table);
   const int64_t rows = block_table.size(0), cols = block_table.size(1);
   TORCH_CHECK(cols * block_size <= (1 << 30), "a row of the block table must hold at most 2^30 positions");
@@ -288,10 +306,10 @@ Tensor paged_attention_decode(
   Tensor workspace;
   if (bytes > 0) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
   launched(pla_paged_attention_launch(
-      q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
-      k_cache.stride(2), (int)k_cache.size(0), (int)block_size, block_table.data_ptr<int32_t>(), table_pitch(block_table), (int)rows,
+      q.data_ptr(), step(q, 0), step(q, 1), k_cache.data_ptr(), v_cache.data_ptr(), step(k_cache, 0), step(k_cache, 1),
+      step(k_cache, 2), (int)k_cache.size(0), (int)block_size, block_table.data_ptr<int32_t>(), table_pitch(block_table), (int)rows,
       (int)cols, ptr(mapping), wide(mapping), ptr(offsets), wide(offsets), seq_lens.data_ptr(), wide(seq_lens), ptr(output_gate),
-      output_gate ? output_gate->stride(0) : 0, output_gate ? output_gate->stride(1) : 0, out.data_ptr(), out.stride(0), out.stride(1),
+      step(output_gate, 0), step(output_gate, 1), out.data_ptr(), step(out, 0), step(out, 1),
       (float)scale.value_or(1.0 / std::sqrt((double)D)), (int)batch, (int)T, (int)max_query_len, (int)HQ, (int)HKV, (int)D, act,
       bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(q)));
   return out;

@@ -172,8 +172,10 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, query_
     Without ``query_start_loc`` row n is the one new token of request n.  With it (int32 or int64 [N+1]) rows
     query_start_loc[n] .. query_start_loc[n+1] - 1 are request n's window, at most ``max_query_len`` (up to 32) tokens; token j of
     a window of m sees the first seq_lens[n] - m + j + 1 positions.  A request whose window is empty, longer or not within q is
-    passed over, and rows of no request are left as they are.  A row that sees nothing is zeros.  Positions whose block is no
-    block of the cache, or past the table, are left out; what the cache holds behind a request's end never counts.
+    passed over, and rows of no request are left as they are (anything, where ``out`` is made here); no two windows may share a row.
+    A row that sees nothing is zeros.  Positions whose block is no block of the cache, or past the table, are left out; what the
+    cache holds behind a request's end never counts, and a draft token's key or value that is infinite or NaN reaches no token
+    before it.
     ``request_indices`` [N]: rows of the block table, n without it.
 
     scale (default D^-0.5) applies to the scores; output_gate [T, HQ, D] multiplies the result by its sigmoid.  Scores, their

@@ -118,6 +118,35 @@ def test_workspace_is_host_arithmetic():
         assert size(*bad) == -1
 
 
+def test_places_of_pages_good_and_bad(tmp_path):
+    """The kernel's own arithmetic from position to page to place in the cache, compiled for the host: entries that are no block of
+    the cache lie nowhere, whatever they are, and the division by the block size is exact."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    source, library = tmp_path / "places.cpp", tmp_path / "places.so"
+    source.write_text('#include "%s"\n' % os.path.join(root, "pla_amd", "csrc", "paged_schedule.h") + """
+        extern "C" long long place(int entry, int at, int blocks, long long block, long long token) {
+          return pla::paged_place(entry, at, blocks, block, token);
+        }
+        extern "C" int page(int n, int d) { return pla::paged_page(pla::paged_divisor(d), n); }
+    """)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", str(library), str(source)], check=True)
+    lib = ctypes.CDLL(str(library))
+    lib.place.restype = ctypes.c_longlong
+    lib.place.argtypes = [ctypes.c_int] * 3 + [ctypes.c_longlong] * 2
+    far = 2 ** 33 + 8
+    assert [lib.place(e, 5, 7, far, 128) for e in (0, 3, 6)] == [640, 3 * far + 640, 6 * far + 640]
+    for bad in (-1, 7, 8, 2 ** 31 - 1, -2 ** 31):
+        assert lib.place(bad, 5, 7, far, 128) == -1
+    rng = random.Random(1)
+    for d in list(range(1, 70)) + [528, 784, 1000, 4096, 65520, 2 ** 30 - 1, 2 ** 30]:
+        edges = [k * d + e for k in (0, 1, 2, 1000, (2 ** 31 - 1) // d) for e in (-1, 0, 1)]
+        for n in edges + [2 ** 31 - 1] + [rng.randrange(2 ** 31) for _ in range(200)]:
+            if 0 <= n < 2 ** 31:
+                assert lib.page(n, d) == n // d, (n, d)
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------------
 
 def _rope_args(**change):

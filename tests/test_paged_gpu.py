@@ -545,6 +545,48 @@ def test_draft_tokens_that_are_not_finite_do_not_reach_the_ones_before(D, act, H
     _close(got[8:], ref[8:], slack[8:], "other request")
 
 
+@pytest.mark.parametrize("act, length", [("bf16", 70), ("fp16", 1500)])
+def test_values_set_aside_weigh_as_much_as_the_others(act, length):
+    """Scores so far apart that the draft tokens' own keys carry most of the weight, with one value among them that is not finite:
+    the rows that do not see it, and the other channels of those that do, are what they are without it."""
+    D, windows, lengths = 128, [8], [length]
+    cache = _Cache(lengths, 1, D, 16, act, seed=41)
+    q = _randn(torch.Generator().manual_seed(42), 8, 4, D, dtype=DTYPES[act])
+    k = cache.k[0]
+    # every query is near the key of its own token
+    for j in range(8):
+        at = length - 8 + j
+        k[at] = (q[j, 0].cpu().float() * 0.7).to(DTYPES[act])
+        cache.store[cache.table[0, at // 16].item(), 0, at % 16, 0] = k[at, 0].to(DEV)
+    cache.store[cache.table[0, (length - 2) // 16].item(), 1, (length - 2) % 16, 0, 9] = math.inf
+    ref, slack = _attention_reference(q, cache, lengths, windows, 0.5)
+    got = _attend(cache, q, lengths, windows, scale=0.5)
+    assert (got[6:, :, 9] == math.inf).all()
+    got[6:, :, 9] = ref[6:, :, 9].to(got)
+    _close(got, ref, slack, "set aside")
+
+
+def test_caches_side_by_side_in_one_buffer_and_strides_of_single_rows():
+    """K and V of a token next to each other, one head with a stride of its own, one token whose stride means nothing."""
+    from pla.decode.paged import fused_qk_norm_rope, paged_attention_decode
+    D, bs = 64, 16
+    g = torch.Generator().manual_seed(61)
+    both = torch.zeros(4, bs, 1, 2 * D, dtype=torch.bfloat16, device=DEV)
+    k_cache, v_cache = both[..., :D], both[..., D:]
+    odd = torch.as_strided(both, (4, bs, 1, D), (bs * 2 * D, 2 * D, 3, 1))           # the head stride of one head
+    row = _randn(g, 20, 3 * D, dtype=torch.bfloat16)
+    q, k, v = (row[:, i * D:(i + 1) * D].view(20, 1, D) for i in range(3))
+    slots = torch.arange(20, device=DEV) + bs
+    table = _ints([[1, 2]])
+    fused_qk_norm_rope(q, k, q_weight=_randn(g, D, dtype=torch.bfloat16), v=v, k_cache=k_cache, v_cache=v_cache, slot_mapping=slots, q_out=q)
+    assert torch.equal(both.view(-1, 2 * D)[bs:bs + 20, :D], k[:, 0]) and torch.equal(both.view(-1, 2 * D)[bs:bs + 20, D:], v[:, 0])
+    last = torch.as_strided(q, (1, 1, D), (5, 7, 1), q[19:].storage_offset())
+    expect = paged_attention_decode(q[19:].contiguous(), k_cache.contiguous(), v_cache.contiguous(), table, _ints([20]))
+    assert torch.equal(paged_attention_decode(last, odd, v_cache, table, _ints([20])), expect)
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        fused_qk_norm_rope(q, k, v=v, k_cache=k_cache, v_cache=both[..., D // 2:D // 2 + D], slot_mapping=slots)
+
+
 def test_offsets_past_32_bits():
     """Blocks 2^32 bytes and more apart."""
     D, HKV, pitch = 128, 1, 2 ** 31 + 1024
