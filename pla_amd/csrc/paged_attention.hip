@@ -278,11 +278,11 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, const u32x4_t* que
 template <typename act_t, int D, int TEAM>
 __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const PagedRequest& req, int kv_head, int row, int channel,
                                               const int32_t* pages, int first, int last, float top, float& sum, float (&o)[D / TEAM]) {
-  const int j = row / p.shape.group, head = kv_head * p.shape.group + row - j * p.shape.group;
+  const int j = paged_quotient(p.shape.by_group, row), head = kv_head * p.shape.group + row - j * p.shape.group;
   const uint16_t* q = p.q + (req.begin + j) * p.q_token + head * p.q_head + channel;
   last = min(last, paged_limit(p.shape, req, row));
   for (int key = first; key < last; ++key) {
-    const int page = paged_page(p.page_of, key);
+    const int page = paged_quotient(p.page_of, key);
     int64_t at = paged_place(pages[page], key - page * p.block_size, p.blocks, p.kv_block, p.kv_token);
     if (at < 0) continue;
     at += kv_head * p.kv_head + channel;
@@ -311,6 +311,11 @@ constexpr int residency(int D, int row_tiles) { return D == 256 ? 1 : D == 64 &&
 __device__ __forceinline__ int64_t uniform64(int64_t x) {
   return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
                    (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
+}
+
+__device__ __forceinline__ PagedRequest uniform(const PagedRequest& r) {
+  return PagedRequest{uniform64(r.begin), __builtin_amdgcn_readfirstlane(r.window), __builtin_amdgcn_readfirstlane(r.length),
+                      __builtin_amdgcn_readfirstlane(r.keys), __builtin_amdgcn_readfirstlane(r.blocks), __builtin_amdgcn_readfirstlane(r.tiles)};
 }
 
 // A segment as a wavefront takes it.
@@ -387,25 +392,20 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     start_offset = (int)left;
   }
   __syncthreads();
-  int n = __builtin_amdgcn_readfirstlane(start_index), offset = __builtin_amdgcn_readfirstlane(start_offset);
+  int n = __builtin_amdgcn_readfirstlane(start_index);
 
   const uint32_t key_lane = (uint32_t)(r * p.kv_token + 8 * kb) * 2;
   const uint32_t value_lane = (uint32_t)(4 * kb * p.kv_token + W::LANE_CHANNELS * r) * 2;
 
-  // The next part of the stretch (there is one), from request n on, `offset` units into it; `req`: that request.
-  auto next_part = [&](PagedRequest req) {
+  // The part of the stretch at `at` in request n, `req`.
+  auto part_at = [&](const PagedRequest& req, const PagedStart& at) {
     Part a;
-    while (offset >= paged_weight(p.shape, req)) {        // done with it, or passed over
-      offset = 0;
-      req = scalar_request(p, ++n);
-    }
     a.req = req;
     a.index = n;
-    a.seg = paged_segment(line, req, offset, unit, stretch_end, worker);
+    a.seg = paged_segment(line, req, at, unit, stretch_end, worker);
     unit += a.seg.tiles;
-    offset += a.seg.tiles;
-    a.row0 = a.seg.block * p.shape.rows;
-    a.rows = min(req.window * p.shape.group - a.row0, p.shape.rows);
+    a.row0 = a.seg.block << p.shape.row_bits;
+    a.rows = min(req.window * p.shape.group - a.row0, 16 * RT);
     a.least = paged_limit(p.shape, req, a.row0);
     a.end = paged_limit(p.shape, req, a.row0 + a.rows - 1);
     const int64_t table_row = p.mapping ? scalar_at(p.mapping, p.mapping_wide, n) : n;
@@ -416,6 +416,21 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     a.steps = has_row && a.end > a.key ? min((a.end - a.key - 1) / TILE + 1, a.seg.tiles) : 0;
     return a;
   };
+  // The one after it: the next run, of the next request that has any where this one has no more.
+  auto part_after = [&](const Part& a) {
+    PagedStart at{a.seg.head, a.seg.block + 1, 0};
+    PagedRequest req = a.req;
+    if (at.block == req.blocks) {
+      at.block = 0;
+      ++at.head;
+    }
+    if (at.head == p.shape.heads) {
+      at.head = 0;
+      do req = scalar_request(p, ++n);
+      while (req.blocks == 0);
+    }
+    return part_at(req, at);
+  };
   // Where the two halves of a step's keys lie: the table's entries first (always two loads, of anything where there is no such
   // step: a branch would wait for them), then, when they are there, the places.  Place 0, some block's first keys, serves loads
   // whose results do not count.
@@ -425,7 +440,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int key = min(a.key + step * TILE + 16 * h, a.end - 1);
-      x.block[h] = scalar_load(a.steps > 0 ? a.pages + paged_page(p.page_of, key) : static_cast<const int32_t*>(p.lengths));
+      x.block[h] = scalar_load(a.steps > 0 ? a.pages + paged_quotient(p.page_of, key) : static_cast<const int32_t*>(p.lengths));
     }
     return x;
   };
@@ -433,7 +448,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int key = a.key + step * TILE + 16 * h;
-      place[h] = paged_place(x.block[h], key - paged_page(p.page_of, key) * p.block_size, p.blocks, p.kv_block, p.kv_token);
+      place[h] = paged_place(x.block[h], key - paged_quotient(p.page_of, key) * p.block_size, p.blocks, p.kv_block, p.kv_token);
       there[h] = a.steps > 0 && key < a.end && place[h] >= 0;
       if (!there[h]) place[h] = 0;
     }
@@ -445,7 +460,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       const int piece = tid + THREADS * i, row = piece / (D / 8), channel = piece % (D / 8) * 8;
       x[i] = u32x4_t{0, 0, 0, 0};
       if (row < a.rows) {
-        const int j = (a.row0 + row) / p.shape.group, g = a.row0 + row - j * p.shape.group;
+        const int j = paged_quotient(p.shape.by_group, a.row0 + row), g = a.row0 + row - j * p.shape.group;
         x[i] = *reinterpret_cast<const u32x4_t*>(p.q + (a.req.begin + j) * p.q_token + (a.seg.head * p.shape.group + g) * p.q_head + channel);
       }
     }
@@ -462,7 +477,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
   u32x4_t q_words[MINE];
   int64_t place[2], next_place[2];
   bool there[2], next_there[2];
-  Part a = next_part(start_request);
+  Part a = part_at(uniform(start_request), paged_start(uniform(start_request), __builtin_amdgcn_readfirstlane(start_offset)));
   const Entries entries = look_up(a, 0);
   if (a.steps > 0) {
     place_of(a, 0, entries, place, there);
@@ -478,7 +493,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     const bool more_parts = unit < stretch_end;
     Part b = a;
     if (more_parts) {
-      b = next_part(a.req);
+      b = part_after(a);
       load_queries(b, q_words);
     }
     // entries of the step after the one in flight
@@ -566,7 +581,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
           if (aside[x] >= 0)
             add_set_aside<act_t, D, TEAM>(p, a.req, a.seg.head, row, out_channel, a.pages, max(aside[x], a.least), min(aside[x] + 32, a.end), row_top, row_sum, o);
         if (a.seg.slot < 0) {
-          const int j = row / p.shape.group, head = a.seg.head * p.shape.group + row - j * p.shape.group;
+          const int j = paged_quotient(p.shape.by_group, row), head = a.seg.head * p.shape.group + row - j * p.shape.group;
           const float norm = row_sum == 0.f ? 0.f : 1.0f / row_sum;         // no key: zeros
           const int64_t token = a.req.begin + j;
           uint32_t word[CHANNELS / 2];
@@ -614,10 +629,10 @@ __global__ __launch_bounds__(64 * WAVES) void paged_join_kernel(const PagedAtten
   const PagedRun run = p.runs[blockIdx.x];
   const int pieces = run.pieces;
   if (pieces < 2) return;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), R = p.shape.rows;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), R = 1 << p.shape.row_bits;
   const int first = PER_ROW ? wave : 0, stride = PER_ROW ? WAVES : 1;
   for (int row = PER_ROW ? blockIdx.y : blockIdx.y * WAVES + wave; row < run.rows; row += PER_ROW ? gridDim.y : gridDim.y * WAVES) {
-    const int j = (run.row0 + row) / p.shape.group, head = run.head * p.shape.group + run.row0 + row - j * p.shape.group;
+    const int j = paged_quotient(p.shape.by_group, run.row0 + row), head = run.head * p.shape.group + run.row0 + row - j * p.shape.group;
     const int64_t token = run.begin + j;
     uint16_t gate[LANE] = {};
     if (p.gate) {
@@ -694,6 +709,12 @@ struct PagedLaunch {
   int64_t runs, bytes, tops_at, runs_at;  // workspace: partial outputs, maxima and sums, runs
 };
 
+static int bits_of(int power) {
+  int bits = 0;
+  while (1 << bits < power) ++bits;
+  return bits;
+}
+
 static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query, int64_t positions) {
   PagedLaunch l{};
   const int window_rows = max_query * (HQ / HKV);
@@ -753,7 +774,7 @@ extern "C" int pla_paged_attention_segments(
   using namespace pla;
   if (check_shape(batch, HQ, HKV, head_dim, max_query_len, positions) || batch == 0 || !offsets || !seq_lens) return -1;
   const PagedLaunch l = paged_launch(batch, HQ, HKV, head_dim, max_query_len, positions);
-  const PagedShape shape{HKV, HQ / HKV, l.rows, l.tile, max_query_len, tokens, positions};
+  const PagedShape shape{HKV, HQ / HKV, paged_divisor(HQ / HKV), bits_of(l.rows), bits_of(l.tile), max_query_len, tokens, positions};
   auto request = [&](int n) { return paged_request(shape, offsets[n], offsets[n + 1], seq_lens[n]); };
   int64_t total = 0;
   for (int n = 0; n < batch; ++n) total += paged_weight(shape, request(n));
@@ -769,7 +790,7 @@ extern "C" int pla_paged_attention_segments(
       ++n;
       continue;
     }
-    const PagedSegment s = paged_segment(line, r, (int)offset, unit, end, worker);
+    const PagedSegment s = paged_segment(line, r, paged_start(r, (int)offset), unit, end, worker);
     if (found < capacity) {
       const int64_t row[7] = {n, s.head, s.block, s.tile, s.tiles, s.slot, s.pieces};
       for (int i = 0; i < 7; ++i) segments[7 * found + i] = row[i];
@@ -814,7 +835,7 @@ extern "C" int pla_paged_attention_launch(
   const PagedAttention p{(const uint16_t*)q, q_token, q_head, (const uint16_t*)k_cache, (const uint16_t*)v_cache, kv_block, kv_token,
                          kv_head, block_table, table_row_stride, mapping, mapping_wide, offsets, offsets_wide, seq_lens, seq_lens_wide,
                          (const uint16_t*)gate, gate_token, gate_head, (uint16_t*)out, out_token, out_head,
-                         PagedShape{HKV, HQ / HKV, l.rows, l.tile, max_query_len, tokens, positions},
+                         PagedShape{HKV, HQ / HKV, paged_divisor(HQ / HKV), bits_of(l.rows), bits_of(l.tile), max_query_len, tokens, positions},
                          batch, blocks, block_size, table_rows, paged_divisor(block_size), scale * 1.44269504088896341f, l.by_run, l.row_blocks,
                          l.split ? reinterpret_cast<float*>(ws) : nullptr, l.split ? reinterpret_cast<float2*>(ws + l.tops_at) : nullptr,
                          l.split ? reinterpret_cast<PagedRun*>(ws + l.runs_at) : nullptr};

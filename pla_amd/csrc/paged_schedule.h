@@ -21,9 +21,20 @@
 
 namespace pla {
 
+// Division by a number known ahead: with 2^(b - 1) < d <= 2^b the factor ceil(2^(31 + b) / d) has 32 bits and is off by less than
+// one part in 2^31, so the quotient of a number below 2^31 is exact.
+struct PagedDivisor { uint32_t factor; int shift; };
+inline PagedDivisor paged_divisor(int d) {
+  int bits = 0;
+  while ((1ll << bits) < d) ++bits;
+  return {(uint32_t)(((1ull << (31 + bits)) + d - 1) / d), bits + 31};
+}
+PLA_HD int paged_quotient(const PagedDivisor& d, int n) { return (int)((uint64_t)(uint32_t)n * d.factor >> d.shift); }
+
 struct PagedShape {
   int heads, group;                       // key-value heads, query heads of each
-  int rows, tile;                         // query rows of a block, keys of a tile
+  PagedDivisor by_group;
+  int row_bits, tile_bits;                // query rows of a block and keys of a tile are 2 to these
   int max_query, tokens;                  // longest window, rows of q
   int64_t positions;                      // that a row of the block table has pages for
 };
@@ -43,27 +54,17 @@ PLA_HD PagedRequest paged_request(const PagedShape& s, int64_t begin, int64_t en
   r.window = (int)(end - begin);
   r.length = (int)(length < 0 ? 0 : length > INT32_MAX ? INT32_MAX : length);
   r.keys = (int)(r.length < s.positions ? r.length : s.positions);
-  r.blocks = (r.window * s.group + s.rows - 1) / s.rows;
-  r.tiles = r.keys > 0 ? (r.keys - 1) / s.tile + 1 : 1;
+  r.blocks = (r.window * s.group + (1 << s.row_bits) - 1) >> s.row_bits;
+  r.tiles = r.keys > 0 ? ((r.keys - 1) >> s.tile_bits) + 1 : 1;
   return r;
 }
 PLA_HD int paged_weight(const PagedShape& s, const PagedRequest& r) { return r.tiles * r.blocks * s.heads; }     // fits: the host checks
 
 // Keys that the token row `row / group` of a request sees (they are the first ones).
 PLA_HD int paged_limit(const PagedShape& s, const PagedRequest& r, int row) {
-  const int64_t limit = (int64_t)r.length - r.window + row / s.group + 1;
+  const int64_t limit = (int64_t)r.length - r.window + paged_quotient(s.by_group, row) + 1;
   return (int)(limit < 0 ? 0 : limit < r.keys ? limit : r.keys);
 }
-
-// Division by a number known ahead: with 2^(b - 1) < d <= 2^b the factor ceil(2^(31 + b) / d) has 32 bits and is off by less than
-// one part in 2^31, so the quotient of a number below 2^31 is exact.
-struct PagedDivisor { uint32_t factor; int shift; };
-inline PagedDivisor paged_divisor(int d) {
-  int bits = 0;
-  while ((1ll << bits) < d) ++bits;
-  return {(uint32_t)(((1ull << (31 + bits)) + d - 1) / d), bits + 31};
-}
-PLA_HD int paged_page(const PagedDivisor& d, int n) { return (int)((uint64_t)(uint32_t)n * d.factor >> d.shift); }
 
 // Where the keys of half a step lie, in elements from the cache's start: place `place` of block `entry` of the table; -1: nowhere.
 PLA_HD int64_t paged_place(int entry, int place, int blocks, int64_t block_stride, int64_t token_stride) {
@@ -92,19 +93,22 @@ PLA_HD int paged_worker_of(const PagedLine& l, int64_t unit) {
   return (int)(unit < longer ? paged_divide(unit, l.each + 1) : l.rest + paged_divide(unit - longer, l.each));
 }
 
+// Where in a request's part of the line its unit `offset` lies.
+struct PagedStart { int head, block, tile; };
+PLA_HD PagedStart paged_start(const PagedRequest& r, int offset) {
+  const int run = (uint32_t)offset / (uint32_t)r.tiles, head = (uint32_t)run / (uint32_t)r.blocks;
+  return {head, run - head * r.blocks, offset - run * r.tiles};
+}
+
 struct PagedSegment {
   int head, block, tile, tiles;           // tiles [tile, tile + tiles) of a run
   int slot;                               // of the workspace, -1: the run is whole
   int pieces;                             // of the run (1: it is whole) where this is its first, else 0
 };
 
-// The segment that starts `offset` units into the request `r`, which is unit `unit` of the line; `end`: of the stretch.
-PLA_HD PagedSegment paged_segment(const PagedLine& l, const PagedRequest& r, int offset, int64_t unit, int64_t end, int worker) {
-  PagedSegment s;
-  const int run = (uint32_t)offset / (uint32_t)r.tiles;
-  s.tile = offset - run * r.tiles;
-  s.head = (uint32_t)run / (uint32_t)r.blocks;
-  s.block = run - s.head * r.blocks;
+// The segment that starts at `at` in the request `r`, unit `unit` of the line; `end`: of the stretch.
+PLA_HD PagedSegment paged_segment(const PagedLine& l, const PagedRequest& r, const PagedStart& at, int64_t unit, int64_t end, int worker) {
+  PagedSegment s{at.head, at.block, at.tile, 0, 0, 0};
   const int64_t left = end - unit;
   s.tiles = r.tiles - s.tile < left ? r.tiles - s.tile : (int)left;
   const bool whole = s.tiles == r.tiles;

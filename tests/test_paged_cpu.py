@@ -129,7 +129,7 @@ def test_places_of_pages_good_and_bad(tmp_path):
         extern "C" long long place(int entry, int at, int blocks, long long block, long long token) {
           return pla::paged_place(entry, at, blocks, block, token);
         }
-        extern "C" int page(int n, int d) { return pla::paged_page(pla::paged_divisor(d), n); }
+        extern "C" int page(int n, int d) { return pla::paged_quotient(pla::paged_divisor(d), n); }
     """)
     subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", str(library), str(source)], check=True)
     lib = ctypes.CDLL(str(library))
