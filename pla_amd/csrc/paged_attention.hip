@@ -495,6 +495,8 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     if (more_parts) {
       b = part_after(a);
       load_queries(b, q_words);
+    } else {
+      b.steps = 0;
     }
     // entries of the step after the one in flight
     Entries coming = a.steps > 1 ? look_up(a, 1) : look_up(b, 0);
@@ -516,7 +518,8 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       if ((step + (blockIdx.x >> 8)) & 1) __builtin_amdgcn_s_setprio(1);
       else __builtin_amdgcn_s_setprio(0);
       const bool more = step + 1 < a.steps;
-      // The very last step fetches something once more, from the caches: a branch around the loads costs the compiler the registers.
+      // The very last step fetches some block's first keys, the same for all, from the caches: a branch around the loads costs the
+      // compiler the registers.
       // The entries for the step after next are asked for behind the keys of the next: a wait for queries in LDS is one for them too.
       const int64_t head = (more ? a.seg.head : b.seg.head) * p.kv_head;
       attend(w, queries, p.scale_log2, there, a.key + step * TILE, a.least, a.end,
