@@ -3,7 +3,8 @@
 //   o = sum_p softmax_p(scale q.k_p) v_p  [* sigmoid(gate)]      over the keys p that the token sees: p < length - window + j + 1
 //
 // for token j of a request's window.  The query heads of a key-value head and the tokens of the window are the rows of one
-// product, so keys and values are read once for all of them (blocks of 16 or 32 rows).
+// product, so keys and values are read once for all of them, in blocks of 16, 32 or (D 64 and 128) 64 rows: 16 windows of eight over
+// 8000 keys, 64 rows a head of 128, take 85.5 us as blocks of 32 and 72.5 as one of 64; 64 rows of 256 channels do not fit the registers.
 //
 // Each wavefront takes 32 keys at a time, alone: keys and values go from memory to the registers in which the matrix
 // instructions want them, through no LDS, and nothing waits for another wavefront until the end of a run.
@@ -304,9 +305,11 @@ __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const Pag
 // memory system than it has: 50 requests of 8000 keys (D 128, 1.64 GB) take 264 us with two workgroups of four wavefronts, 290 with
 // three and 422 with four.  D 64: 37 windows of up to 9000 keys (167 MB) take 32.8 us as two workgroups of eight wavefronts and 36.2 as
 // four of four; 32 rows do not fit the registers of that (64 windows of eight over 1000 to 16 000 keys, 8 heads, 214 us), and take 171
-// as one workgroup of eight and 162 as three of four.
+// as one workgroup of eight and 162 as three of four.  64 rows of 128 channels need 450 registers: one workgroup.
 constexpr int waves(int D, int row_tiles) { return D == 64 && row_tiles == 1 ? 8 : 4; }
-constexpr int residency(int D, int row_tiles) { return D == 256 ? 1 : D == 64 && row_tiles == 2 ? 3 : 2; }
+constexpr int residency(int D, int row_tiles) {
+  return D == 256 || (D == 128 && row_tiles == 4) ? 1 : D == 64 && row_tiles == 2 ? 3 : 2;
+}
 
 __device__ __forceinline__ int64_t uniform64(int64_t x) {
   return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
@@ -721,7 +724,7 @@ static int bits_of(int power) {
 static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query, int64_t positions) {
   PagedLaunch l{};
   const int window_rows = max_query * (HQ / HKV);
-  l.row_tiles = window_rows <= 16 ? 1 : 2;
+  l.row_tiles = window_rows <= 16 ? 1 : window_rows <= 32 || D == 256 ? 2 : 4;
   l.rows = 16 * l.row_tiles;
   l.tile = 32 * waves(D, l.row_tiles);
   l.row_blocks = (window_rows + l.rows - 1) / l.rows;
@@ -746,7 +749,8 @@ static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query
 template <typename act_t, int D>
 static void launch_paged_attention(const PagedAttention& p, const PagedLaunch& l, hipStream_t s) {
   if (l.row_tiles == 1) paged_attention_kernel<act_t, D, 1><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
-  else paged_attention_kernel<act_t, D, 2><<<l.workers, 64 * waves(D, 2), 0, s>>>(p);
+  else if (l.row_tiles == 2) paged_attention_kernel<act_t, D, 2><<<l.workers, 64 * waves(D, 2), 0, s>>>(p);
+  else if constexpr (D != 256) paged_attention_kernel<act_t, D, 4><<<l.workers, 64 * waves(D, 4), 0, s>>>(p);
   if (!l.split) return;
   const dim3 grid((unsigned)(l.by_run ? l.runs : l.workers), l.join_rows);
   if (l.per_row) paged_join_kernel<act_t, D, true, 16><<<grid, 1024, 0, s>>>(p);

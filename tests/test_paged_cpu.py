@@ -36,8 +36,8 @@ def _segments(windows, lengths, HQ, HKV, D, max_query, positions, tokens=None):
     return out
 
 
-def _rows_of_a_block(max_query, group):
-    return 16 if max_query * group <= 16 else 32
+def _rows_of_a_block(D, max_query, group):
+    return 16 if max_query * group <= 16 else 32 if max_query * group <= 32 or D == 256 else 64
 
 
 def _keys_of_a_tile(D, rows):
@@ -55,7 +55,7 @@ def test_every_tile_of_every_run_is_taken_once_and_its_pieces_are_found(seed):
     windows[rng.randrange(n)] = max_query
     lengths = [rng.choice((0, -3, 1, 127, 128, 129, positions, positions + 500, rng.randint(0, positions))) for _ in range(n)]
     got = _segments(windows, lengths, HKV * group, HKV, D, max_query, positions)
-    rows = _rows_of_a_block(max_query, group)
+    rows = _rows_of_a_block(D, max_query, group)
     tile_keys = _keys_of_a_tile(D, rows)
     expected = {}
     for i, (w, length) in enumerate(zip(windows, lengths)):
