@@ -303,7 +303,7 @@ __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const Pag
 
 // Wavefronts a workgroup and workgroups a CU, so that 96 to 128 KiB of keys and values are in flight there.  More want more of the
 // memory system than it has: 50 requests of 8000 keys (D 128, 1.64 GB) take 264 us with two workgroups of four wavefronts, 290 with
-// three and 422 with four.  D 64: 37 windows of up to 9000 keys (167 MB) take 32.8 us as two workgroups of eight wavefronts and 36.2 as
+// three and 422 with four.  D 64: 37 windows of up to 9000 keys (10 heads, 104 MB) take 32.8 us as two workgroups of eight wavefronts and 36.2 as
 // four of four; 32 rows do not fit the registers of that (64 windows of eight over 1000 to 16 000 keys, 8 heads, 214 us), and take 171
 // as one workgroup of eight and 162 as three of four.  64 rows of 128 channels need 450 registers: one workgroup.
 constexpr int waves(int D, int row_tiles) { return D == 64 && row_tiles == 1 ? 8 : 4; }
@@ -761,6 +761,7 @@ static int check_shape(int batch, int HQ, int HKV, int D, int max_query, int64_t
   PLA_REQUIRE(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got %d", D);
   PLA_REQUIRE(HKV > 0 && HQ >= HKV && HQ % HKV == 0, "query heads must be a positive multiple of key-value heads");
   PLA_REQUIRE(max_query >= 1 && max_query <= 32, "max_query_len must be between 1 and 32");
+  PLA_REQUIRE(max_query * (int64_t)(HQ / HKV) <= (1 << 30), "too many query heads");
   PLA_REQUIRE(batch >= 0 && (int64_t)batch * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "too many requests");
   PLA_REQUIRE(positions >= 0 && positions <= (1 << 30), "a row of the block table must hold at most 2^30 positions");
   PLA_REQUIRE((positions / 128 + 1) * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "a request with too many heads for its positions");

@@ -5,7 +5,6 @@
 // judged before devices.
 
 #include <torch/extension.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -15,7 +14,6 @@
 #include <initializer_list>
 #include <optional>
 #include <tuple>
-#include <vector>
 
 #include "../../include/pla_gfx950.h"
 
@@ -33,6 +31,11 @@ bool bypass() {                                   // read once, as in the other 
 int wide(const Tensor& t) { return t.scalar_type() == at::kLong ? 1 : 0; }
 int wide(const OptTensor& t) { return t ? wide(*t) : 0; }
 const void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
+int count(int64_t n, const char* what) {
+  TORCH_CHECK(n <= INT32_MAX, "too many ", what, ": ", n);
+  return (int)n;
+}
+bool finite(double x) { return std::isfinite((float)x); }
 int act_code(const Tensor& t, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, name, " must be bf16 or fp16, got ", t.scalar_type());
   return t.scalar_type() == at::kHalf ? PLA_F16 : PLA_BF16;
@@ -62,25 +65,31 @@ void on_one_gpu(const Tensor& ref, const char* name, std::initializer_list<std::
 
 // Whether two tensors may share memory.  Views of one buffer interleave (q, k and v of a projection row; K and V of a block): where
 // both step by the same stride, what counts is where one lies within a step of the other, dimension by dimension.
-struct Dims { int64_t size, stride; };         // bytes
-int64_t extent(const std::vector<Dims>& d, size_t from, int64_t element) {
+struct Dim { int64_t size, stride; };          // bytes
+struct Dims { Dim d[8]; int n; };              // of a tensor, largest stride first, without those of one entry or stride 0
+int64_t extent(const Dims& t, int from, int64_t element) {
   int64_t n = element;
-  for (size_t i = from; i < d.size(); ++i) n += (d[i].size - 1) * d[i].stride;
+  for (int i = from; i < t.n; ++i) n += (t.d[i].size - 1) * t.d[i].stride;
   return n;
 }
-bool lap(const std::vector<Dims>& a, const std::vector<Dims>& b, size_t i, size_t j, int64_t ahead, int64_t ea, int64_t eb) {
+bool lap(const Dims& a, const Dims& b, int i, int j, int64_t ahead, int64_t ea, int64_t eb) {
   // `ahead`: of b's first byte to a's
   if (ahead >= extent(a, i, ea) || -ahead >= extent(b, j, eb)) return false;
-  if (i == a.size() || j == b.size() || a[i].stride != b[j].stride) return true;
-  const int64_t step = a[i].stride, rest = ((ahead % step) + step) % step;
+  if (i == a.n || j == b.n || a.d[i].stride != b.d[j].stride) return true;
+  const int64_t step = a.d[i].stride, rest = ((ahead % step) + step) % step;
   return lap(a, b, i + 1, j + 1, rest, ea, eb) || lap(a, b, i + 1, j + 1, rest - step, ea, eb);
 }
-std::vector<Dims> dims_of(const Tensor& t) {
-  std::vector<Dims> d;
-  for (int64_t i = 0; i < t.dim(); ++i)
-    if (t.size(i) > 1 && t.stride(i) > 0) d.push_back({t.size(i), t.stride(i) * (int64_t)t.element_size()});
-  std::stable_sort(d.begin(), d.end(), [](const Dims& x, const Dims& y) { return x.stride > y.stride; });
-  return d;
+Dims dims_of(const Tensor& t) {
+  Dims r{{}, 0};
+  TORCH_CHECK(t.dim() <= 8, "too many dimensions");
+  const int64_t element = t.element_size();
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) <= 1 || t.stride(i) <= 0) continue;
+    int at = r.n++;
+    for (; at > 0 && r.d[at - 1].stride < t.stride(i) * element; --at) r.d[at] = r.d[at - 1];
+    r.d[at] = {t.size(i), t.stride(i) * element};
+  }
+  return r;
 }
 bool may_overlap(const Tensor& a, const Tensor& b) {
   if (a.numel() == 0 || b.numel() == 0) return false;
@@ -90,12 +99,22 @@ bool may_overlap(const Tensor& a, const Tensor& b) {
   if (b.is_contiguous() && -ahead >= (int64_t)(b.numel() * b.element_size())) return false;
   return lap(dims_of(a), dims_of(b), 0, 0, ahead, a.element_size(), b.element_size());
 }
+// A step of a dimension leaves the smaller ones behind.
+bool overlaps_itself(const Tensor& t) {
+  if (t.numel() == 0 || t.is_contiguous()) return false;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) return true;
+  const Dims d = dims_of(t);
+  for (int i = 0; i < d.n; ++i)
+    if (d.d[i].stride < extent(d, i + 1, t.element_size())) return true;
+  return false;
+}
 bool same_rows(const Tensor& a, const Tensor& b) { return a.data_ptr() == b.data_ptr() && a.strides() == b.strides(); }
 void apart(std::initializer_list<std::pair<const char*, const OptTensor*>> written,
            std::initializer_list<std::pair<const char*, const OptTensor*>> read) {
   for (auto w = written.begin(); w != written.end(); ++w) {
     if (!*w->second) continue;
-    at::assert_no_internal_overlap(**w->second);
+    TORCH_CHECK(!overlaps_itself(**w->second), w->first, " must not share memory with itself");
     for (auto o = written.begin(); o != w; ++o)
       TORCH_CHECK(!*o->second || !may_overlap(**w->second, **o->second), w->first, " must not share memory with ", o->first);
     for (const auto& [what, t] : read)
@@ -122,6 +141,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> paged_kv_plan(
   TORCH_CHECK(block_size > 0 && block_size <= (1 << 30) && cols * block_size <= (1 << 30), "block_size must be positive and a row's positions at most 2^30");
   TORCH_CHECK(token_capacity >= 0 && token_capacity <= (1 << 30), "token_capacity must be between 0 and 2^30");
   TORCH_CHECK(mapping || batch <= rows, "more batch entries than rows of the block table");
+  const int table_rows = count(rows, "rows of the block table"), entries = count(batch, "batch entries"),
+            stack_size = count(free_blocks.numel(), "places for free blocks");
   if (out_offsets) {
     TORCH_CHECK(out_seq_lens && out_positions && out_slots, "the four outputs come together");
     dense_ints(*out_offsets, "query_start_loc", at::kInt, batch + 1);
@@ -146,8 +167,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> paged_kv_plan(
   if (!bypass())
     launched(pla_paged_kv_plan_launch(
         context.data_ptr(), wide(context), query.data_ptr(), wide(query), ptr(mapping), wide(mapping), block_table.data_ptr<int32_t>(),
-        table_pitch(block_table), (int)rows, (int)cols, held_blocks.data_ptr<int32_t>(), free_blocks.data_ptr<int32_t>(),
-        free_count.data_ptr<int32_t>(), (int)free_blocks.numel(), (int)batch, (int)block_size, (int)token_capacity,
+        table_pitch(block_table), table_rows, (int)cols, held_blocks.data_ptr<int32_t>(), free_blocks.data_ptr<int32_t>(),
+        free_count.data_ptr<int32_t>(), stack_size, entries, (int)block_size, (int)token_capacity,
         offsets.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
         stream_of(block_table)));
   return {offsets, seq_lens, positions, slots};
@@ -199,7 +220,7 @@ std::tuple<Tensor, OptTensor> fused_qk_norm_rope(
                 name, " must be ", D, " contiguous values of q's type or float32, 16-byte aligned");
   }
   TORCH_CHECK(!q_weight || !k_weight || q_weight->scalar_type() == k_weight->scalar_type(), "q_weight and k_weight must be of one type");
-  TORCH_CHECK(std::isfinite(eps) && eps >= 0 && std::isfinite(weight_offset) && std::isfinite(attention_factor),
+  TORCH_CHECK(finite(eps) && eps >= 0 && finite(weight_offset) && finite(attention_factor),
               "eps, weight_offset and attention_factor must be finite, eps not negative");
   int64_t rot = 0;
   OptTensor positions;
@@ -289,7 +310,8 @@ Tensor paged_attention_decode(
   else TORCH_CHECK(T == batch, "without query_start_loc every request has one token row: ", batch, " requests, ", T, " rows");
   if (request_indices) mapping = index_vector(*request_indices, "request_indices", batch);
   else TORCH_CHECK(batch <= rows, "more requests than rows of the block table");
-  TORCH_CHECK(!scale || std::isfinite(*scale), "scale must be finite");
+  const int requests = count(batch, "requests"), tokens = count(T, "token rows"), heads = count(HQ, "heads"), table_rows = count(rows, "rows of the block table");
+  TORCH_CHECK(!scale || finite(*scale), "scale must be finite");
   if (output_gate) head_rows(*output_gate, "output_gate", T, HQ, D, type);
   if (out_in) head_rows(*out_in, "out", T, HQ, D, type);
   const OptTensor qt(q), kt(k_cache), vt(v_cache), table(block_table), lens(seq_lens);
@@ -301,16 +323,16 @@ Tensor paged_attention_decode(
   const c10::DeviceGuard guard(q.device());
   Tensor out = out_in ? *out_in : at::empty({T, HQ, D}, q.options());
   if (bypass() || T == 0 || batch == 0) return out;
-  const int64_t bytes = pla_paged_attention_workspace_bytes((int)batch, (int)HQ, (int)HKV, (int)D, (int)max_query_len, cols * block_size);
+  const int64_t bytes = pla_paged_attention_workspace_bytes(requests, heads, (int)HKV, (int)D, (int)max_query_len, cols * block_size);
   TORCH_CHECK(bytes >= 0, pla_last_error());
   Tensor workspace;
   if (bytes > 0) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
   launched(pla_paged_attention_launch(
       q.data_ptr(), step(q, 0), step(q, 1), k_cache.data_ptr(), v_cache.data_ptr(), step(k_cache, 0), step(k_cache, 1),
-      step(k_cache, 2), (int)k_cache.size(0), (int)block_size, block_table.data_ptr<int32_t>(), table_pitch(block_table), (int)rows,
+      step(k_cache, 2), (int)k_cache.size(0), (int)block_size, block_table.data_ptr<int32_t>(), table_pitch(block_table), table_rows,
       (int)cols, ptr(mapping), wide(mapping), ptr(offsets), wide(offsets), seq_lens.data_ptr(), wide(seq_lens), ptr(output_gate),
       step(output_gate, 0), step(output_gate, 1), out.data_ptr(), step(out, 0), step(out, 1),
-      (float)scale.value_or(1.0 / std::sqrt((double)D)), (int)batch, (int)T, (int)max_query_len, (int)HQ, (int)HKV, (int)D, act,
+      (float)scale.value_or(1.0 / std::sqrt((double)D)), requests, tokens, (int)max_query_len, heads, (int)HKV, (int)D, act,
       bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(q)));
   return out;
 }

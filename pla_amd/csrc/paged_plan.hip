@@ -267,7 +267,7 @@ extern "C" int pla_paged_kv_plan_launch(
     int32_t* free_blocks, int32_t* free_count, int free_capacity, int batch, int block_size, int token_capacity,
     int32_t* offsets, int32_t* seq_lens, int32_t* positions, int64_t* slots, void* stream) {
   using namespace pla;
-  PLA_REQUIRE(batch >= 0 && token_capacity >= 0 && token_capacity <= (1 << 30), "batch and token_capacity must be between 0 and 2^30");
+  PLA_REQUIRE(batch >= 0 && batch <= (1 << 30) && token_capacity >= 0 && token_capacity <= (1 << 30), "batch and token_capacity must be between 0 and 2^30");
   PLA_REQUIRE(table_rows >= 0 && table_cols >= 0 && table_row_stride >= table_cols, "invalid block table dimensions");
   PLA_REQUIRE(block_size > 0 && block_size <= (1 << 30) && (int64_t)table_cols * block_size <= (1 << 30),
               "block_size must be positive and a row's positions at most 2^30");

@@ -139,6 +139,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
         turn[wave][1][here + 64 * i] = __builtin_amdgcn_sinf(part) * p.attention_factor;
       }
     }
+    // other lanes read them: the LDS serves a wavefront in order, the compiler has to keep it
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
   // out = rstd (x straight + partner cross)
   const bool turns = channel < p.rot;

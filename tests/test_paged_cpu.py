@@ -114,7 +114,7 @@ def test_workspace_is_host_arithmetic():
     one, many = size(1, 16, 2, 128, 1, 4096), size(64, 16, 2, 128, 1, 4096)
     assert 0 < one < many and one % 256 == 0 and many == size(1000, 16, 2, 128, 1, 4096)      # bounded by the chip
     for bad in ((1, 16, 3, 128, 1, 99), (1, 16, 2, 96, 1, 99), (1, 16, 2, 128, 33, 99), (1, 16, 2, 128, 0, 99), (-1, 16, 2, 128, 1, 99),
-                (1, 16, 2, 128, 1, 2 ** 30 + 1)):
+                (1, 16, 2, 128, 1, 2 ** 30 + 1), (1, 2 ** 26, 1, 128, 32, 99)):
         assert size(*bad) == -1
 
 
@@ -184,6 +184,7 @@ def _rope_args(**change):
     (dict(eps=-1.0), "eps not negative"),
     (dict(eps=float("nan")), "must be finite"),
     (dict(attention_factor=float("inf")), "must be finite"),
+    (dict(weight_offset=1e300), "must be finite"),           # not in float32
     (dict(q_out=torch.zeros(5, 3, 64, dtype=BF16)), "q_out must be"),
     (dict(slot_mapping=torch.zeros(5, dtype=torch.int64, device="meta")), "slot_mapping must be on the device of q"),
     (dict(), "q must be a CUDA tensor"),
@@ -221,6 +222,7 @@ def _attention_args(**change):
     (dict(max_query_len=33), "between 1 and 32"),
     (dict(request_indices=torch.zeros(2, dtype=torch.int32)), "request_indices must have 3 entries"),
     (dict(scale=float("nan")), "scale must be finite"),
+    (dict(scale=1e39), "scale must be finite"),              # not in float32
     (dict(output_gate=torch.zeros(6, 4, 64, dtype=BF16)), "output_gate must be"),
     (dict(out=torch.zeros(5, 4, 128, dtype=BF16)), "out must be"),
     (dict(out=torch.zeros(6, 4, 128, dtype=torch.float16)), "out must be"),

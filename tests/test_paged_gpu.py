@@ -319,6 +319,28 @@ def test_norm_refuses_shared_memory():
             fused_qk_norm_rope(**args)
 
 
+def test_written_tensors_that_overlap_themselves_are_refused():
+    """Rows or blocks a step apart that is smaller than they are: two workgroups would write one place."""
+    from pla.decode.paged import fused_qk_norm_rope, paged_attention_decode
+    x = torch.zeros(8, 4, 64, dtype=torch.bfloat16, device=DEV)
+    store = torch.zeros(4096, dtype=torch.bfloat16, device=DEV)
+    rows, slots = store.as_strided((8, 4, 64), (128, 64, 1)), torch.arange(8, device=DEV)
+    cache = torch.zeros(2, 16, 4, 64, dtype=torch.bfloat16, device=DEV)
+    close = torch.zeros(8192, dtype=torch.bfloat16, device=DEV).as_strided((2, 16, 4, 64), (2048, 256, 64, 1))
+    for args in (dict(q_out=rows), dict(k_out=rows), dict(k_cache=close, slot_mapping=slots),
+                 dict(k_cache=cache, v_cache=close, v=x, slot_mapping=slots)):
+        with pytest.raises(RuntimeError, match="must not share memory with itself"):
+            fused_qk_norm_rope(x, x, **args)
+    with pytest.raises(RuntimeError, match="must not share memory with itself"):
+        paged_attention_decode(x, cache, cache, _ints([[0]] * 8), _ints([1] * 8), out=rows)
+    # read only: a cache whose blocks lie half on each other is what it is
+    got = paged_attention_decode(x, close, close, _ints([[0]] * 8), _ints([1] * 8))
+    assert torch.equal(got, torch.zeros_like(got))
+    # rows far enough apart in any order of the dimensions
+    out = torch.zeros(64 * 4 * 9, dtype=torch.bfloat16, device=DEV).as_strided((8, 4, 64), (64, 64 * 9, 1))
+    assert torch.equal(paged_attention_decode(x, cache, cache, _ints([[0]] * 8), _ints([1] * 8), out=out), got)
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------
 
 class _Cache:
