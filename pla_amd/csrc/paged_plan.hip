@@ -86,29 +86,37 @@ struct PagedEntry {
   int64_t row, context, query;
   int end;                // running sum of the token rows
   int held, want;         // equal unless the entry is sound
-  bool counted, sound;    // counted: its q is a number of token rows
+  bool inside;            // its row is one of the table's
+  bool sound;
 };
 
-// A thread's entries n .. n + E - 1 (from the batch's end on: nothing).  `carry`: token rows of the chunks before.
-template <int THREADS, int E>
-__device__ __forceinline__ void load_entries(const PagedPlan& p, const int* owner, int n, int& carry, int* scratch, PagedEntry (&e)[E]) {
-  bool inside[E];
+// What memory has of a thread's entries n .. n + E - 1 (from the batch's end on: nothing).
+template <int E>
+__device__ __forceinline__ void fetch_entries(const PagedPlan& p, int n, PagedEntry (&e)[E]) {
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     e[i] = PagedEntry{0, 0, -1, 0, 0, 0, false, false};
     if (n + i < p.batch) {
+      e[i].row = p.row_of(n + i);
       e[i].context = p.at(p.context, p.context_wide, n + i);
       e[i].query = p.at(p.query, p.query_wide, n + i);
-      e[i].row = p.row_of(n + i);
     }
-    inside[i] = n + i < p.batch && e[i].row >= 0 && e[i].row < p.rows;
-    if (inside[i]) e[i].held = p.held[e[i].row];
+    e[i].inside = n + i < p.batch && e[i].row >= 0 && e[i].row < p.rows;
   }
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    if (e[i].inside) e[i].held = p.held[e[i].row];
+}
+
+// What they ask for.  `carry`: token rows of the chunks before.
+template <int THREADS, int E>
+__device__ __forceinline__ void judge_entries(const PagedPlan& p, const int* owner, int n, int& carry, int* scratch, PagedEntry (&e)[E]) {
+  bool counted[E];        // its q is a number of token rows
   int rows[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    e[i].counted = e[i].query >= 0 && e[i].query <= p.capacity;
-    rows[i] = e[i].counted ? (int)e[i].query : 0;
+    counted[i] = e[i].query >= 0 && e[i].query <= p.capacity;
+    rows[i] = counted[i] ? (int)e[i].query : 0;
   }
   const int total = running_sums<THREADS>(rows, scratch);
 #pragma unroll
@@ -116,7 +124,7 @@ __device__ __forceinline__ void load_entries(const PagedPlan& p, const int* owne
     e[i].end = add_saturated(carry, rows[i]);
     e[i].held = min(max(e[i].held, 0), p.cols);
     e[i].want = e[i].held;
-    if (inside[i] && e[i].counted && e[i].context >= 0 && e[i].context <= (int64_t)p.cols * p.block && e[i].end <= p.capacity &&
+    if (e[i].inside && counted[i] && e[i].context >= 0 && e[i].context <= (int64_t)p.cols * p.block && e[i].end <= p.capacity &&
         (owner == nullptr || owner[e[i].row] == n + i)) {
       const int want = (int)(((uint32_t)e[i].context + (uint32_t)e[i].query + (uint32_t)p.block - 1) / (uint32_t)p.block);
       e[i].sound = want <= p.cols;
@@ -142,15 +150,21 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(const PagedPlan p) 
   extern __shared__ int32_t owner_lds[];
   __shared__ int token_ends[CHUNK], back_ends[CHUNK], take_ends[CHUNK];   // running sums: token rows, blocks returned, blocks asked for
   __shared__ int first[CHUNK];                       // page of an entry's first block that moves, or its number of pages
-  __shared__ int length[CHUNK];
+  __shared__ int length[CHUNK], table_row[CHUNK];
   __shared__ int scratch[3][THREADS / 64], granted_end;
   const int tid = threadIdx.x, chunks = (p.batch + CHUNK - 1) / CHUNK;
+  PagedEntry e[E];
+  fetch_entries<E>(p, tid * E, e);
+  int height = min(max(*p.height, 0), p.stack_size), carry = 0, asked_all = 0;
   const int* owner = nullptr;
   if (p.mapping) {
     // the first entry of a row is the row's
     for (int r = tid; r < p.rows; r += THREADS) owner_lds[r] = INT32_MAX;
     __syncthreads();
-    for (int n = tid; n < p.batch; n += THREADS) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (e[i].inside) atomicMin(&owner_lds[e[i].row], tid * E + i);
+    for (int n = CHUNK + tid; n < p.batch; n += THREADS) {
       const int64_t row = p.row_of(n);
       if (row >= 0 && row < p.rows) atomicMin(&owner_lds[row], n);
     }
@@ -158,12 +172,11 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(const PagedPlan p) 
     owner = owner_lds;
   }
 
-  int height = min(max(*p.height, 0), p.stack_size), carry = 0, asked_all = 0;
-  PagedEntry e[E];
   int take[E];
   // Running sums of a chunk; returns the blocks it gives back.
   auto load_chunk = [&](int base, int& asked) {
-    load_entries<THREADS, E>(p, owner, base + tid * E, carry, scratch[0], e);
+    if (chunks > 1) fetch_entries<E>(p, base + tid * E, e);
+    judge_entries<THREADS, E>(p, owner, base + tid * E, carry, scratch[0], e);
     int back[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -178,6 +191,7 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(const PagedPlan p) 
       take_ends[tid * E + i] = take[i];
       token_ends[tid * E + i] = e[i].end;
       first[tid * E + i] = min(e[i].held, e[i].want);
+      table_row[tid * E + i] = (int)e[i].row;
     }
     if (tid == 0) granted_end = 0;
     __syncthreads();
@@ -188,7 +202,7 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(const PagedPlan p) 
     const int base = c * CHUNK, count = min(p.batch - base, CHUNK), returned = load_chunk(base, asked);
     for (int i = tid; i < min(returned, p.stack_size - height); i += THREADS) {
       const int m = entry_of(back_ends, count, i), before = m ? back_ends[m - 1] : 0;
-      p.stack[height + i] = p.table[p.row_of(base + m) * p.table_stride + first[m] + (i - before)];
+      p.stack[height + i] = p.table[table_row[m] * p.table_stride + first[m] + (i - before)];
     }
     height = (int)min((int64_t)height + returned, (int64_t)p.stack_size);
     if (chunks > 1) __syncthreads();
@@ -218,8 +232,8 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(const PagedPlan p) 
     const int granted_total = granted_end;
     const int top = height - 1 - taken;              // of the stack, for this chunk's first block
     for (int i = tid; i < granted_total; i += THREADS) {
-      const int m = entry_of(take_ends, count, i), before = m ? take_ends[m - 1] : 0;
-      p.table[p.row_of(base + m) * p.table_stride + first[m] + (i - before)] = p.stack[top - i];
+      const int block = p.stack[top - i], m = entry_of(take_ends, count, i), before = m ? take_ends[m - 1] : 0;
+      p.table[table_row[m] * p.table_stride + first[m] + (i - before)] = block;
     }
     if (TOKEN_ROWS) {
       const int end = min(token_ends[count - 1], p.capacity);
@@ -228,7 +242,7 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(const PagedPlan p) 
         const int page = max(position, 0) / p.block;
         int block = 0;
         if (position >= 0)
-          block = page < first[m] ? p.table[p.row_of(base + m) * p.table_stride + page]
+          block = page < first[m] ? p.table[table_row[m] * p.table_stride + page]
                                   : p.stack[top - ((m ? take_ends[m - 1] : 0) + page - first[m])];
         write_token_row(p, t, position, block);
       }
@@ -246,17 +260,35 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(const PagedPlan p) 
     for (int t = first_row + tid; t < p.capacity; t += THREADS) write_token_row(p, t, -1, 0);
 }
 
-// Token rows of a step that has many: one a thread.
+// Token rows of a step that has many: one a thread.  A wavefront looks for the entry of its first row with 64 probes at a time, two
+// trips to memory for 4096 entries; those of the other rows are, but for runs of empty entries, among the next 64.
 __global__ __launch_bounds__(256) void paged_token_rows_kernel(const PagedPlan p) {
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t >= p.capacity) return;
+  const int t = blockIdx.x * 256 + threadIdx.x, lane = threadIdx.x & 63, t0 = __builtin_amdgcn_readfirstlane(t);
+  if (t0 >= p.capacity) return;
+  const int32_t* ends = p.offsets + 1;
+  const int total = p.batch > 0 ? p.offsets[p.batch] : 0;
   int position = -1, block = 0;
-  if (p.batch > 0 && t < p.offsets[p.batch]) {
-    const int n = entry_of(p.offsets + 1, p.batch, t);
-    position = position_of(t, p.offsets[n], p.offsets[n + 1], p.seq_lens[n]);
-    if (position >= 0) block = p.table[p.row_of(n) * p.table_stride + position / p.block];
+  if (t0 < total) {
+    int from = 0;
+    for (int span = p.batch; span > 64;) {
+      const int step = (span + 63) / 64;
+      const uint64_t above = __ballot(ends[from + min((lane + 1) * step, span) - 1] > t0);         // the last lane's is
+      const int skip = (__ffsll((unsigned long long)above) - 1) * step;
+      from += skip;
+      span = min(step, span - skip);
+    }
+    const int end = ends[min(from + lane, p.batch - 1)];
+    int below = 0;                          // of these 64 ends, those up to t
+#pragma unroll
+    for (int d = 32; d; d >>= 1) below += __shfl(end, below + d - 1) <= t ? d : 0;
+    below += __shfl(end, below) <= t ? 1 : 0;
+    if (t < total) {
+      const int n = from + below + (below == 64 ? entry_of(ends + from + 64, p.batch - from - 64, t) : 0);
+      position = position_of(t, p.offsets[n], ends[n], p.seq_lens[n]);
+      if (position >= 0) block = p.table[p.row_of(n) * p.table_stride + position / p.block];
+    }
   }
-  write_token_row(p, t, position, block);
+  if (t < p.capacity) write_token_row(p, t, position, block);
 }
 
 }  // namespace pla

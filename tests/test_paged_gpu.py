@@ -159,6 +159,40 @@ def test_plan_writes_into_given_outputs_and_many_token_rows():
     _check_plan(pool, lists, [3001, 90, 3, 0, 2006], [1, 8, 0, 0, 1], None, 4097)
 
 
+@pytest.mark.parametrize("batch, mapped, capacity, blocks", [(9001, False, 4000, 14000), (9001, False, 13000, 11000), (5000, True, 12000, 12000),
+                                                             (8192, True, 3000, 9000), (4097, False, 9000, 20000)])
+def test_plan_of_more_entries_than_a_workgroup_holds_at_once(batch, mapped, capacity, blocks):
+    """Several passes over the entries: sums, blocks and refusals (of a stack too small, of a capacity too small) go on over their ends."""
+    rng = random.Random(batch + capacity)
+    rows, cols, bs = 8192 if mapped else batch + 3, 5, 4
+    pool, lists = _pool(blocks, bs, rows, cols)
+    index = rng.sample(range(rows), batch) if mapped else None
+    context = [rng.randint(0, 5) for _ in range(batch)]
+    for step in range(3):
+        query = [rng.choice((0, 0, 1, 1, 2, 3)) for _ in range(batch)]
+        used = index
+        if mapped and step == 1:                             # the same row in two passes, twice in one
+            used = list(index)
+            used[-1], used[-2], used[-3] = used[0], used[-4], rows
+        _, lists = _check_plan(pool, lists, context, query, used, capacity)
+        context = [rng.choice((0, max(0, c - 3), min(cols * bs - 3, c + q))) for c, q in zip(context, query)]
+
+
+@pytest.mark.parametrize("batch", [1, 63, 64, 65, 700, 4096, 4200])
+def test_token_rows_between_runs_of_empty_entries(batch):
+    """More token rows than the planning workgroup writes: entries without any between long and short ones, at the ends and in runs
+    of more than 64, rows without an entry behind them."""
+    rng = random.Random(batch)
+    cols, bs = 40, 16
+    pool, lists = _pool(4000, bs, batch, cols)
+    query = [0] * batch
+    for n in rng.sample(range(batch), min(batch, 40)):
+        query[n] = rng.choice((1, 2, 7, 64, 65, 300, 600))
+    for step in range(2):
+        _, lists = _check_plan(pool, lists, [rng.randint(0, 9) for _ in range(batch)], query, None, max(sum(query), 4097) + 70 * step)
+        query = query[::-1] if step else [0] * (batch // 2) + [1] * (batch - batch // 2)
+
+
 def test_plan_refuses_shared_memory():
     from pla.decode.paged import PagedKVPlan, paged_kv_plan
     pool, _ = _pool(9, 16, 3, 4)
