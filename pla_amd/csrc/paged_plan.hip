@@ -20,9 +20,10 @@
 
 namespace pla {
 
-// Token rows up to which the workgroup that makes the plan writes them as well: two steps of 40 requests with 4000 rows take 18.2 us
-// with one launch each and 21.6 with two, with 8000 rows 24.9 and 21.6.
-constexpr int PAGED_PLAN_INLINE_ROWS = 4096;
+// Token rows up to which the workgroup that makes the plan writes them as well: a step of 1000 requests takes 8.8 us on the device
+// with 2000 rows by one launch and 9.8 by two, with 4000 rows 10.9 and 9.8; one of 40 requests with 1920 rows 7.5 and 8.7, with 4000
+// rows 9.0 and 8.7.
+constexpr int PAGED_PLAN_INLINE_ROWS = 2048;
 constexpr int PAGED_PLAN_MAPPED_ROWS = 8192;      // rows whose first entry is looked up in LDS: 32 KB
 constexpr int32_t PAGED_SATURATED = INT32_MAX;    // of running sums: more than any capacity
 
