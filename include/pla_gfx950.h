@@ -550,7 +550,8 @@ int pla_paged_attention_launch(
 /*
  * How pla_paged_attention_launch deals a batch out, from HOST copies of its offsets and lengths (host arithmetic only, for tests
  * and for callers who log the plan): the segments of workgroup `worker`, up to `capacity` rows of (request, key-value head, block
- * of query rows, first tile (128 keys, 256 for head_dim 64 and 16 rows), tiles, workspace slot or -1 for a whole run, pieces of the run if this is its first).
+ * of query rows, first tile, tiles, workspace slot or -1 for a whole run, pieces of the run if this is its first).  A tile is 128
+ * keys, 256 for head_dim 64 and 16 rows; where wavefronts work alone it is 32, and a run counts one more than it has.
  * Returns their number, 0 for a worker without work, -1 for an invalid shape.
  */
 int pla_paged_attention_segments(

@@ -6,8 +6,13 @@
 // product, so keys and values are read once for all of them, in blocks of 16, 32 or (D 64 and 128) 64 rows: 16 windows of eight over
 // 8000 keys, 64 rows a head of 128, take 85.5 us as blocks of 32 and 72.5 as one of 64; 64 rows of 256 channels do not fit the registers.
 //
-// Each wavefront takes 32 keys at a time, alone: keys and values go from memory to the registers in which the matrix
-// instructions want them, through no LDS, and nothing waits for another wavefront until the end of a run.
+// Each wavefront takes 32 keys at a time: keys and values go from memory to the registers in which the matrix instructions want them,
+// through no LDS.  The wavefronts of a workgroup work together, one 32 keys after the other's, and put their rows together at the
+// end of a run.  Or (ALONE; 16 rows, many runs) each has runs of its own, with the queries in registers, and writes what it has whole
+// from registers: nothing waits for another wavefront before the end of the kernel, where what they share is put together.  256
+// requests of 300 to 4000 keys (D 128, 8 heads) take 250 us together and 245 alone, 1000 of 50 keys 79.0 and 68.1 (D 64: 72.2
+// and 39.9), 64 of 200 to 4000 (D 256, 2 heads) 43.3 and 39.1.  Few runs, which wavefronts would have to share all the same, lose
+// by it (8 requests of 180 to 700 keys, 2 heads, 12.1 and 13.0), so they stay together.
 //
 //   S^T = K Q^T    keys are the rows: lane (r, kb) loads 16 bytes of key r a step, any channels, as Q holds the same ones.
 //                  It gets the scores of query r at keys 4 kb .. 4 kb + 3 of both halves of the 32 keys,
@@ -116,7 +121,8 @@ struct Wave {
   f32x4_t o[RT][CHUNKS][TILES];
   float top[RT], sum[RT];
   int limit[RT];
-  int set_aside;                                              // first key of the step whose partly seen values are added at the end, or -1
+  int set_aside;                                              // first key of the step whose partly seen values are added at the end, + 1 if those
+                                                              // of the next are too (a wavefront alone may have both), or -1
 };
 
 template <typename act_t, int D, int RT>
@@ -162,8 +168,8 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
 
 // One step of a wavefront: scores of 32 keys from key0 on, their weights, and the weighted values.  `next`: issues the loads of
 // the step after (keys once these are used, values once those are).
-template <typename act_t, int D, int RT, typename NextKeys, typename NextValues>
-__device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, const u32x4_t* queries, float scale_log2, const bool (&there)[2],
+template <typename act_t, int D, int RT, typename Queries, typename NextKeys, typename NextValues>
+__device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, float scale_log2, const bool (&there)[2],
                                        int key0, int least, int end, NextKeys next_keys, NextValues next_values) {
   using W = Wave<act_t, D, RT>;
   const int kb = (threadIdx.x & 63) >> 4;
@@ -174,7 +180,7 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, const u32x4_t* que
   for (int c = 0; c < W::STEPS; ++c) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const bf16x8_t q = __builtin_bit_cast(bf16x8_t, queries[(t * W::STEPS + c) * 64 + (threadIdx.x & 63)]);
+      const bf16x8_t q = __builtin_bit_cast(bf16x8_t, queries(t, c));
 #pragma unroll
       for (int h = 0; h < 2; ++h) s[t][h] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, w.k[h][c]), q, s[t][h]);
     }
@@ -240,7 +246,7 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, const u32x4_t* que
       }
       if (__ballot((odd & 0x80008000u) != 0) != 0) {
         stop = least;
-        w.set_aside = key0;
+        w.set_aside = w.set_aside < 0 ? key0 : w.set_aside | 1;
         // their weights come back into the sum with their values, rounded alike
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
@@ -301,7 +307,7 @@ __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const Pag
   }
 }
 
-// Wavefronts a workgroup and workgroups a CU, so that 96 to 128 KiB of keys and values are in flight there.  More want more of the
+// (Measured with wavefronts together.)  Wavefronts a workgroup and workgroups a CU, so that 96 to 128 KiB of keys and values are in flight there.  More want more of the
 // memory system than it has: 50 requests of 8000 keys (D 128, 1.64 GB) take 264 us with two workgroups of four wavefronts, 290 with
 // three and 422 with four.  D 64: 37 windows of up to 9000 keys (10 heads, 104 MB) take 32.8 us as two workgroups of eight wavefronts and 36.2 as
 // four of four; 32 rows do not fit the registers of that (64 windows of eight over 1000 to 16 000 keys, 8 heads, 214 us), and take 171
@@ -328,28 +334,85 @@ struct Part {
   int row0, rows;                         // of the window
   int least, end;                         // keys that all rows see, that any row sees
   int key, steps;                         // first key and steps of this wavefront
+  int64_t last;                           // unit of the run
   int index;                              // of the request
   const int32_t* pages;
 };
 
-template <typename act_t, int D, int RT>
-__global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) / 4) void paged_attention_kernel(const PagedAttention p) {
-  using W = Wave<act_t, D, RT>;
-  constexpr int WAVES = waves(D, RT), THREADS = 64 * WAVES, TILE = 32 * WAVES;
-  constexpr int TEAM = THREADS / 16, CHANNELS = D / TEAM;       // threads that put a row's outputs together, and channels of each
-  constexpr int PITCH = D + 4;                    // floats of a row in LDS: rows of a quad of lanes start in different banks
-  constexpr int PIECES = 16 * RT * D / 8, MINE = (PIECES + THREADS - 1) / THREADS;          // 16-byte pieces of the queries, and of a thread
-  __shared__ __align__(16) float outs[WAVES][16][PITCH];
-  __shared__ __align__(16) u32x4_t queries[PIECES];
-  __shared__ float2 tops[WAVES][16 * RT];
-  __shared__ int aside[WAVES];
-  __shared__ int64_t sums[WAVES];
-  __shared__ PagedRequest start_request;
-  __shared__ int start_index, start_offset;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 15, kb = lane >> 4;
+// CHANNELS channels of a row's output from their sums.
+template <typename act_t, int CHANNELS>
+__device__ __forceinline__ void write_row(const PagedAttention& p, int64_t token, int head, int channel, float sum, const float (&o)[CHANNELS]) {
+  const float norm = sum == 0.f ? 0.f : 1.0f / sum;         // no key: zeros
+  uint32_t word[CHANNELS / 2];
+#pragma unroll
+  for (int i = 0; i < CHANNELS; i += 2) {
+    float x = o[i] * norm, y = o[i + 1] * norm;
+    if (p.gate) {
+      const uint32_t g = *reinterpret_cast<const uint32_t*>(p.gate + token * p.gate_token + head * p.gate_head + channel + i);
+      x *= 1.0f / (1.0f + __expf(-lo16<act_t>(g)));
+      y *= 1.0f / (1.0f + __expf(-hi16<act_t>(g)));
+    }
+    word[i / 2] = pack2<act_t>(x, y);
+  }
+  uint16_t* dst = p.out + token * p.out_token + head * p.out_head + channel;
+#pragma unroll
+  for (int i = 0; i < CHANNELS / 2; ++i) reinterpret_cast<uint32_t*>(dst)[i] = word[i];
+}
 
-  // The line of work: all workgroups add up the whole batch, a thread a contiguous share of the requests.
+// The same as add_set_aside for all 16 rows at once, by a wavefront alone: lane (r, kb) has a quarter of row r's channels, from
+// `o` on in LDS.  row < 0: none.
+template <typename act_t, int D>
+__device__ __forceinline__ void add_set_aside_alone(const PagedAttention& p, const PagedRequest& req, int kv_head, int row, int kb,
+                                                    const int32_t* pages, int first, int last, float top, float& sum, float* o) {
+  const int j = row < 0 ? 0 : paged_quotient(p.shape.by_group, row), head = kv_head * p.shape.group + (row < 0 ? 0 : row - j * p.shape.group);
+  const uint16_t* q = p.q + (req.begin + j) * p.q_token + head * p.q_head + kb * (D / 4);
+  const int limit = row < 0 ? 0 : paged_limit(p.shape, req, row);
+  for (int key = first; key < last; ++key) {
+    const int page = paged_quotient(p.page_of, key);
+    int64_t at = paged_place(pages[page], key - page * p.block_size, p.blocks, p.kv_block, p.kv_token);
+    if (at < 0) continue;
+    at += kv_head * p.kv_head + kb * (D / 4);
+    float score = 0.f;
+#pragma nounroll
+    for (int i = 0; i < D / 4; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
+    score = query_sum(score) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
+    if (key >= limit) continue;
+    const float weight = to_float(from_float<act_t>(__builtin_amdgcn_exp2f(score)));
+    sum += weight;
+#pragma nounroll
+    for (int i = 0; i < D / 4; ++i) {
+      const float x = to_float(act_t{p.v[at + i]});
+      // a weight below the smallest is no weight, but an infinite value has some
+      o[kb * (D / 4) + i] = fmaf(weight == 0.f && !(fabsf(x) < INFINITY) ? 0x1p-126f : weight, x, o[kb * (D / 4) + i]);
+    }
+  }
+}
+
+// Order of this wavefront's own LDS accesses: the LDS serves one wavefront in order, the compiler has to keep it.
+__device__ __forceinline__ void own_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Where the stretch of a workgroup starts, or (STARTS > 1) the shares of its wavefronts.
+template <int WAVES, int STARTS>
+struct StartRoom {
+  int64_t sums[WAVES];
+  PagedRequest request[STARTS];
+  int index[STARTS], offset[STARTS];
+};
+__device__ __forceinline__ int64_t share_of(int64_t length, int parts, int i) {
+  const int64_t each = (int64_t)((uint64_t)length / (uint32_t)parts);
+  return each * i + min(i, (int)(length - each * parts));
+}
+
+// The line of work, and this workgroup's place in it: all workgroups add up the whole batch, a thread a contiguous share of the
+// requests.  Returns the worker, -1 if there is nothing for it.
+template <int WAVES, int STARTS>
+__device__ __forceinline__ int take_stretch(const PagedAttention& p, StartRoom<WAVES, STARTS>& room, PagedLine& line) {
+  constexpr int THREADS = 64 * WAVES;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int share = (p.batch + THREADS - 1) / THREADS, first = min(tid * share, p.batch), last = min(first + share, p.batch);
   int64_t mine = 0;
   PagedRequest own{};
@@ -366,36 +429,76 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     const int64_t x = __shfl_up(below, d);
     if (lane >= d) below += x;
   }
-  if (lane == 63) sums[wave] = below;
+  if (lane == 63) room.sums[wave] = below;
   __syncthreads();
   int64_t total = 0;
   below -= mine;
   for (int i = 0; i < WAVES; ++i) {
-    if (i < wave) below += sums[i];
-    total += sums[i];
+    if (i < wave) below += room.sums[i];
+    total += room.sums[i];
   }
-  const PagedLine line = paged_line(gridDim.x, uniform64(total));
+  line = paged_line(p.shape, gridDim.x, uniform64(total));
   // neighbours in the line on one XCD: row blocks of the same keys share its L2
   const int block = blockIdx.x, worker = block >= line.workers || line.workers % 8 ? block : (block & 7) * (line.workers / 8) + (block >> 3);
   if (!p.by_run && p.runs && tid == 0) p.runs[worker].pieces = 0;
-  if (worker >= line.workers) return;
-  int64_t unit = paged_stretch(line, worker);
-  const int64_t stretch_end = paged_stretch(line, worker + 1);
-  if (below <= unit && unit < below + mine) {
-    int64_t left = unit - below;
-    int n = first;
-    if (share > 1)
-      for (;; ++n) {
-        own = p.request(n);
-        if (left < paged_weight(p.shape, own)) break;
-        left -= paged_weight(p.shape, own);
-      }
-    start_request = own;
-    start_index = n;
-    start_offset = (int)left;
+  if (worker >= line.workers) return -1;
+  const int64_t begin = paged_stretch(line, worker), end = paged_stretch(line, worker + 1);
+  if (below < end && below + mine > begin) {      // these requests have some of it
+    const int64_t length = end - begin;
+#pragma nounroll
+    for (int i = 0; i < STARTS; ++i) {
+      int64_t left = begin + share_of(length, STARTS, i) - below;
+      if (left < 0 || left >= mine) continue;
+      int n = first;
+      if (share > 1)
+        for (;; ++n) {
+          own = p.request(n);
+          if (left < paged_weight(p.shape, own)) break;
+          left -= paged_weight(p.shape, own);
+        }
+      room.request[i] = own;
+      room.index[i] = n;
+      room.offset[i] = (int)left;
+    }
   }
   __syncthreads();
-  int n = __builtin_amdgcn_readfirstlane(start_index);
+  return worker;
+}
+
+// What a wavefront leaves of a run that it did not have alone.
+struct PieceOfRun {
+  int there, open;                        // open: the run goes on behind this wavefront's keys
+  int begin, index, head, block, rows;    // first token row of its request, the request, ...
+  int64_t last;                           // unit of the line
+};
+
+template <typename act_t, int D, int RT, bool ALONE>
+__global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) / 4) void paged_attention_kernel(const PagedAttention p) {
+  using W = Wave<act_t, D, RT>;
+  constexpr int WAVES = waves(D, RT), THREADS = 64 * WAVES, TILE = 32 * WAVES;
+  constexpr int TEAM = THREADS / 16, CHANNELS = D / TEAM;       // threads that put a row's outputs together, and channels of each
+  constexpr int PITCH = D + 4;                    // floats of a row in LDS: rows of a quad of lanes start in different banks
+  constexpr int PIECES = 16 * RT * D / 8, MINE = ALONE ? D / 32 : (PIECES + THREADS - 1) / THREADS;          // 16-byte pieces of the queries, and of a thread
+  constexpr int STRIDE = ALONE ? 32 : TILE;       // keys from a wavefront's step to its next
+  __shared__ __align__(16) float outs[ALONE ? 2 : 1][WAVES][16][PITCH];
+  __shared__ __align__(16) u32x4_t queries[ALONE ? 1 : PIECES];
+  __shared__ float2 tops[ALONE ? 2 : 1][WAVES][16 * RT];
+  __shared__ int aside[WAVES];
+  __shared__ PieceOfRun left[2][ALONE ? WAVES : 1];
+  __shared__ StartRoom<WAVES, ALONE ? WAVES : 1> room;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, kb = lane >> 4;
+  PagedLine line;
+  const int worker = take_stretch(p, room, line);
+  if (worker < 0) return;
+  int64_t unit = paged_stretch(line, worker), stretch_end = paged_stretch(line, worker + 1);
+  if (ALONE) {
+    const int64_t length = stretch_end - unit;
+    stretch_end = unit + share_of(length, WAVES, wave + 1);
+    unit += share_of(length, WAVES, wave);
+  }
+  const int start = ALONE ? wave : 0;
+  int n = __builtin_amdgcn_readfirstlane(room.index[start]);
 
   const uint32_t key_lane = (uint32_t)(r * p.kv_token + 8 * kb) * 2;
   const uint32_t value_lane = (uint32_t)(4 * kb * p.kv_token + W::LANE_CHANNELS * r) * 2;
@@ -406,6 +509,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     a.req = req;
     a.index = n;
     a.seg = paged_segment(line, req, at, unit, stretch_end, worker);
+    a.last = unit - at.tile + req.tiles - 1;
     unit += a.seg.tiles;
     a.row0 = a.seg.block << p.shape.row_bits;
     a.rows = min(req.window * p.shape.group - a.row0, 16 * RT);
@@ -415,8 +519,9 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     const bool has_row = table_row >= 0 && table_row < p.table_rows;
     a.pages = p.table + (has_row ? table_row : 0) * p.table_row;
     // steps of this wavefront: those of its keys that are below `end`
-    a.key = a.seg.tile * TILE + 32 * wave;
-    a.steps = has_row && a.end > a.key ? min((a.end - a.key - 1) / TILE + 1, a.seg.tiles) : 0;
+    a.key = (a.seg.tile << p.shape.tile_bits) + (ALONE ? 0 : 32 * wave);
+    const int stop = min(a.end, (a.seg.tile + a.seg.tiles) << p.shape.tile_bits);
+    a.steps = has_row && stop > a.key ? (stop - a.key - 1) / STRIDE + 1 : 0;
     return a;
   };
   // The one after it: the next run, of the next request that has any where this one has no more.
@@ -442,7 +547,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     Entries x;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int key = min(a.key + step * TILE + 16 * h, a.end - 1);
+      const int key = min(a.key + step * STRIDE + 16 * h, a.end - 1);
       x.block[h] = scalar_load(a.steps > 0 ? a.pages + paged_quotient(p.page_of, key) : static_cast<const int32_t*>(p.lengths));
     }
     return x;
@@ -450,17 +555,18 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
   auto place_of = [&](const Part& a, int step, const Entries& x, int64_t (&place)[2], bool (&there)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int key = a.key + step * TILE + 16 * h;
+      const int key = a.key + step * STRIDE + 16 * h;
       place[h] = paged_place(x.block[h], key - paged_quotient(p.page_of, key) * p.block_size, p.blocks, p.kv_block, p.kv_token);
       there[h] = a.steps > 0 && key < a.end && place[h] >= 0;
       if (!there[h]) place[h] = 0;
     }
   };
-  // This thread's pieces of the queries: 16 bytes each, to where lane 16 kb + r of step c of row tile t reads its operand.
+  // The queries: a wavefront alone keeps its operands, row r at channels 32 c + 8 kb, in registers.  Together a thread has pieces of
+  // 16 bytes, which go to where lane 16 kb + r of step c of row tile t reads its operand.
   auto load_queries = [&](const Part& a, u32x4_t (&x)[MINE]) {
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
-      const int piece = tid + THREADS * i, row = piece / (D / 8), channel = piece % (D / 8) * 8;
+      const int piece = tid + THREADS * i, row = ALONE ? r : piece / (D / 8), channel = ALONE ? 32 * i + 8 * kb : piece % (D / 8) * 8;
       x[i] = u32x4_t{0, 0, 0, 0};
       if (row < a.rows) {
         const int j = paged_quotient(p.shape.by_group, a.row0 + row), g = a.row0 + row - j * p.shape.group;
@@ -480,7 +586,10 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
   u32x4_t q_words[MINE];
   int64_t place[2], next_place[2];
   bool there[2], next_there[2];
-  Part a = part_at(uniform(start_request), paged_start(uniform(start_request), __builtin_amdgcn_readfirstlane(start_offset)));
+  if (ALONE && lane < 2) left[lane][wave] = PieceOfRun{};
+  if (!ALONE || unit < stretch_end) {
+  const PagedRequest first_request = uniform(room.request[start]);
+  Part a = part_at(first_request, paged_start(first_request, __builtin_amdgcn_readfirstlane(room.offset[start])));
   const Entries entries = look_up(a, 0);
   if (a.steps > 0) {
     place_of(a, 0, entries, place, there);
@@ -488,8 +597,15 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
   }
   load_queries(a, q_words);
   if (a.steps > 0) load_values(w, p.v + a.seg.head * p.kv_head, place, value_lane, p.kv_token * 2);
-  store_queries(q_words);
-  __syncthreads();
+  u32x4_t q_now[ALONE ? MINE : 1];
+  if constexpr (ALONE) {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) q_now[i] = q_words[i];
+  } else {
+    store_queries(q_words);
+    __syncthreads();
+  }
+  auto query = [&](int t, int c) { return ALONE ? q_now[ALONE ? c : 0] : queries[ALONE ? 0 : (t * W::STEPS + c) * 64 + lane]; };
 
   for (;;) {
     // The part after this one is worked out now, and its first keys and values are fetched by this part's last step.
@@ -525,7 +641,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       // compiler the registers.
       // The entries for the step after next are asked for behind the keys of the next: a wait for queries in LDS is one for them too.
       const int64_t head = (more ? a.seg.head : b.seg.head) * p.kv_head;
-      attend(w, queries, p.scale_log2, there, a.key + step * TILE, a.least, a.end,
+      attend(w, query, p.scale_log2, there, a.key + step * STRIDE, a.least, a.end,
              [&] {
                place_of(more ? a : b, more ? step + 1 : 0, coming, next_place, next_there);
                load_keys(w, p.k + head, next_place, key_lane);
@@ -541,11 +657,74 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       load_values(w, p.v + b.seg.head * p.kv_head, place, value_lane, p.kv_token * 2);
     }
 
+    if constexpr (ALONE) {
+      const int row = a.row0 + r, j = paged_quotient(p.shape.by_group, row), head = a.seg.head * p.shape.group + row - j * p.shape.group;
+      float sum = query_sum(w.sum[0]);
+      // this lane's channels of row r: LANE_CHANNELS at a time from these on
+      auto channel_of = [&](int c, int e) { return 128 * c + W::LANE_CHANNELS * (4 * kb + e); };
+      auto park = [&](float* to) {
+#pragma unroll
+        for (int c = 0; c < W::CHUNKS; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int x = 0; x < W::TILES; x += 4)
+              *reinterpret_cast<float4*>(to + channel_of(c, e) + x) =
+                  float4{w.o[0][c][x][e], w.o[0][c][x + 1][e], w.o[0][c][x + 2][e], w.o[0][c][x + 3][e]};
+      };
+      if (w.set_aside >= 0) {
+        float* mine = &outs[1][wave][r][0];               // not in use before the wavefront's last run
+        park(mine);
+        own_lds_order();
+        add_set_aside_alone<act_t, D>(p, a.req, a.seg.head, r < a.rows ? row : -1, kb, a.pages, max(w.set_aside & ~31, a.least),
+                                      min((w.set_aside & ~31) + (w.set_aside & 1 ? 64 : 32), a.end), w.top[0], sum, mine);
+        own_lds_order();
+#pragma unroll
+        for (int c = 0; c < W::CHUNKS; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int x = 0; x < W::TILES; ++x) w.o[0][c][x][e] = mine[channel_of(c, e) + x];
+        own_lds_order();
+      }
+      if (a.seg.tiles == a.req.tiles) {
+        if (r < a.rows) {
+          const float norm = sum == 0.f ? 0.f : 1.0f / sum;         // no key: zeros
+          const int64_t token = a.req.begin + j;
+#pragma unroll
+          for (int c = 0; c < W::CHUNKS; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t word[W::WORDS];
+#pragma unroll
+              for (int x = 0; x < W::WORDS; ++x) {
+                float y0 = w.o[0][c][2 * x][e] * norm, y1 = w.o[0][c][2 * x + 1][e] * norm;
+                if (p.gate) {
+                  const uint32_t g = *reinterpret_cast<const uint32_t*>(p.gate + token * p.gate_token + head * p.gate_head + channel_of(c, e) + 2 * x);
+                  y0 *= 1.0f / (1.0f + __expf(-lo16<act_t>(g)));
+                  y1 *= 1.0f / (1.0f + __expf(-hi16<act_t>(g)));
+                }
+                word[x] = pack2<act_t>(y0, y1);
+              }
+              uint16_t* dst = p.out + token * p.out_token + head * p.out_head + channel_of(c, e);
+              if constexpr (W::WORDS == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
+              else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
+            }
+        }
+        if (p.by_run && p.runs && lane == 0) p.runs[(a.index * p.shape.heads + a.seg.head) * p.row_blocks + a.seg.block].pieces = 1;
+      } else {
+        const int kind = a.seg.tile == 0;
+        park(&outs[kind][wave][r][0]);
+        if (kb == 0) tops[kind][wave][r] = float2{w.top[0], sum};
+        if (lane == 0)
+          left[kind][wave] = PieceOfRun{1, a.seg.tile + a.seg.tiles < a.req.tiles, (int)a.req.begin, a.index, a.seg.head, a.seg.block, a.rows, a.last};
+      }
+    } else {
     // The four wavefronts' rows together.
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const float sum = query_sum(w.sum[t]);
-      if (kb == 0) tops[wave][16 * t + r] = float2{w.top[t], sum};
+      if (kb == 0) tops[0][wave][16 * t + r] = float2{w.top[t], sum};
     }
     if (lane == 0) aside[wave] = w.set_aside;
     __syncthreads();
@@ -556,7 +735,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       if (16 * t >= a.rows) break;
       float top = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < WAVES; ++x) top = fmaxf(top, tops[x][16 * t + r].x);
+      for (int x = 0; x < WAVES; ++x) top = fmaxf(top, tops[0][x][16 * t + r].x);
       const float f = rescale(w.top[t], top);
 #pragma unroll
       for (int c = 0; c < W::CHUNKS; ++c)
@@ -565,22 +744,22 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
 #pragma unroll
           for (int j = 0; j < W::TILES; j += 4) {
             const int channel = 128 * c + W::LANE_CHANNELS * (4 * kb + e) + j;
-            *reinterpret_cast<float4*>(&outs[wave][r][channel]) =
+            *reinterpret_cast<float4*>(&outs[0][wave][r][channel]) =
                 float4{w.o[t][c][j][e] * f, w.o[t][c][j + 1][e] * f, w.o[t][c][j + 2][e] * f, w.o[t][c][j + 3][e] * f};
           }
       __syncthreads();
       if (16 * t + out_row < a.rows) {
         float row_top = -INFINITY, row_sum = 0.f;
 #pragma unroll
-        for (int x = 0; x < WAVES; ++x) row_top = fmaxf(row_top, tops[x][16 * t + out_row].x);
+        for (int x = 0; x < WAVES; ++x) row_top = fmaxf(row_top, tops[0][x][16 * t + out_row].x);
 #pragma unroll
-        for (int x = 0; x < WAVES; ++x) row_sum += tops[x][16 * t + out_row].y * rescale(tops[x][16 * t + out_row].x, row_top);
+        for (int x = 0; x < WAVES; ++x) row_sum += tops[0][x][16 * t + out_row].y * rescale(tops[0][x][16 * t + out_row].x, row_top);
         float o[CHANNELS];
 #pragma unroll
         for (int i = 0; i < CHANNELS; ++i) {
           o[i] = 0.f;
 #pragma unroll
-          for (int x = 0; x < WAVES; ++x) o[i] += outs[x][out_row][out_channel + i];
+          for (int x = 0; x < WAVES; ++x) o[i] += outs[0][x][out_row][out_channel + i];
         }
         const int row = a.row0 + 16 * t + out_row;
         for (int x = 0; x < WAVES; ++x)
@@ -588,22 +767,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
             add_set_aside<act_t, D, TEAM>(p, a.req, a.seg.head, row, out_channel, a.pages, max(aside[x], a.least), min(aside[x] + 32, a.end), row_top, row_sum, o);
         if (a.seg.slot < 0) {
           const int j = paged_quotient(p.shape.by_group, row), head = a.seg.head * p.shape.group + row - j * p.shape.group;
-          const float norm = row_sum == 0.f ? 0.f : 1.0f / row_sum;         // no key: zeros
-          const int64_t token = a.req.begin + j;
-          uint32_t word[CHANNELS / 2];
-#pragma unroll
-          for (int i = 0; i < CHANNELS; i += 2) {
-            float x = o[i] * norm, y = o[i + 1] * norm;
-            if (p.gate) {
-              const uint32_t g = *reinterpret_cast<const uint32_t*>(p.gate + token * p.gate_token + head * p.gate_head + out_channel + i);
-              x *= 1.0f / (1.0f + __expf(-lo16<act_t>(g)));
-              y *= 1.0f / (1.0f + __expf(-hi16<act_t>(g)));
-            }
-            word[i / 2] = pack2<act_t>(x, y);
-          }
-          uint16_t* dst = p.out + token * p.out_token + head * p.out_head + out_channel;
-#pragma unroll
-          for (int i = 0; i < CHANNELS / 2; ++i) reinterpret_cast<uint32_t*>(dst)[i] = word[i];
+          write_row<act_t, CHANNELS>(p, a.req.begin + j, head, out_channel, row_sum, o);
         } else {
           const int64_t at = (int64_t)a.seg.slot * (16 * RT) + 16 * t + out_row;
 #pragma unroll
@@ -618,8 +782,73 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       PagedRun* run = p.runs + (p.by_run ? (a.index * p.shape.heads + a.seg.head) * p.row_blocks + a.seg.block : worker);
       *run = PagedRun{a.seg.pieces, worker, (int)a.req.begin, a.seg.head, a.row0, a.rows, {0, 0}};
     }
+    }
     if (!more_parts) break;
     a = b;
+    if constexpr (ALONE) {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) q_now[i] = q_words[i];
+    }
+  }
+  }
+  if constexpr (ALONE) {
+    // Runs that wavefronts of this workgroup share, and what it has of runs that it shares with others: one begun before its stretch
+    // (g < 0), and those begun by wavefront g, each with the pieces of the wavefronts behind, which share its rows.
+    __syncthreads();
+    const bool has = lane < WAVES;
+    const bool from_before = has && left[0][lane].there != 0, to_behind = from_before && left[0][lane].open != 0;
+    const uint32_t goes_on = (uint32_t)__ballot(from_before), closed = (uint32_t)__ballot(from_before && !to_behind);
+    const uint32_t begins = (uint32_t)__ballot(has && left[1][lane].there != 0);
+    constexpr int LANES = D / 8, ROWS = 64 / LANES;           // lanes a row, rows at a time
+    for (int kind = 0; kind < 2; ++kind) {        // the run that this wavefront's keys begin in, the one that they end in
+      if (!((kind ? begins : goes_on) >> wave & 1)) continue;
+      const uint32_t before = begins & ((1u << wave) - 1);
+      const int g = kind ? wave : before ? 31 - __clz(before) : -1, first = max(g, 0), from = wave + kind;
+      const bool more = kind == 0 || (goes_on >> from & 1);
+      const uint32_t close = more ? closed >> from : 0;
+      const bool open = close == 0;
+      const int last = !open ? from + __ffs(close) - 1 : more ? 31 - __clz(goes_on) : wave;
+      const PieceOfRun& run = left[g >= 0][first];
+      const int rows = run.rows, row0 = run.block << p.shape.row_bits;
+      for (int base = (wave - first) * ROWS; base < rows; base += (last - first + 1) * ROWS) {
+        const int mine = base + lane / LANES, channel = lane % LANES * 8;
+        if (mine >= rows) continue;
+        float2 y[WAVES];
+        float row_top = -INFINITY, row_sum = 0.f, o[8];
+#pragma unroll
+        for (int x = 0; x < WAVES; ++x) {
+          y[x] = tops[x == g][x][mine];
+          if (x < first || x > last) y[x] = float2{-INFINITY, 0.f};
+          row_top = fmaxf(row_top, y[x].x);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = 0.f;
+#pragma unroll
+        for (int x = 0; x < WAVES; ++x) {
+          if (x < first || x > last) continue;
+          const float f = rescale(y[x].x, row_top);
+          row_sum = fmaf(y[x].y, f, row_sum);
+          const float4* part = reinterpret_cast<const float4*>(&outs[x == g][x][mine][channel]);
+          const float4 low = part[0], high = part[1];
+          o[0] = fmaf(low.x, f, o[0]); o[1] = fmaf(low.y, f, o[1]); o[2] = fmaf(low.z, f, o[2]); o[3] = fmaf(low.w, f, o[3]);
+          o[4] = fmaf(high.x, f, o[4]); o[5] = fmaf(high.y, f, o[5]); o[6] = fmaf(high.z, f, o[6]); o[7] = fmaf(high.w, f, o[7]);
+        }
+        if (g >= 0 && !open) {
+          const int row = row0 + mine, j = paged_quotient(p.shape.by_group, row), head = run.head * p.shape.group + row - j * p.shape.group;
+          write_row<act_t, 8>(p, run.begin + j, head, channel, row_sum, o);
+        } else {
+          const int64_t at = (int64_t)(2 * worker + (g >= 0)) * 16 + mine;
+          float4* dst = reinterpret_cast<float4*>(p.partial + at * D + channel);
+          dst[0] = float4{o[0], o[1], o[2], o[3]};
+          dst[1] = float4{o[4], o[5], o[6], o[7]};
+          if (channel == 0) p.tops[at] = float2{row_top, row_sum};
+        }
+      }
+      if (kind && lane == 0 && p.runs && (p.by_run || open)) {
+        PagedRun* list = p.runs + (p.by_run ? (run.index * p.shape.heads + run.head) * p.row_blocks + run.block : worker);
+        *list = PagedRun{open ? paged_worker_of(line, run.last) - worker + 1 : 1, worker, run.begin, run.head, row0, run.rows, {0, 0}};
+      }
+    }
   }
 }
 
@@ -710,7 +939,8 @@ __global__ __launch_bounds__(64 * WAVES) void paged_join_kernel(const PagedAtten
 
 // How a call is launched: host arithmetic from what the host knows.
 struct PagedLaunch {
-  int row_tiles, rows, tile, row_blocks, workers, by_run, per_row, join_rows;
+  int row_tiles, rows, tile, units, extra, row_blocks, workers, by_run, per_row, join_rows;
+  bool alone;                             // wavefronts have stretches of their own
   bool split;                             // whether a run can be cut at all
   int64_t runs, bytes, tops_at, runs_at;  // workspace: partial outputs, maxima and sums, runs
 };
@@ -726,11 +956,21 @@ static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query
   const int window_rows = max_query * (HQ / HKV);
   l.row_tiles = window_rows <= 16 ? 1 : window_rows <= 32 || D == 256 ? 2 : 4;
   l.rows = 16 * l.row_tiles;
-  l.tile = 32 * waves(D, l.row_tiles);
   l.row_blocks = (window_rows + l.rows - 1) / l.rows;
   l.runs = (int64_t)batch * HKV * l.row_blocks;
-  const int64_t tiles = positions > 0 ? (positions - 1) / l.tile + 1 : 1, most = 256 * residency(D, l.row_tiles);
-  l.workers = (int)(l.runs * tiles < most ? l.runs * tiles : most);
+  // Wavefronts alone from a run for every 32 of them on: D 128 with 64 runs 21.3 us together and 21.5 alone, with 32 19.2 and 20.5; D 64
+  // with 128 runs 22.4 and 21.9, with 64 16.5 and 18.2; D 256 with 32 runs 26.8 and 22.7, with 16 19.0 and 19.4.  But not where every
+  // run is one tile and gets a workgroup: then no run is cut, and no join runs (64 requests of one head, D 128, 12.9 and 8.1).
+  // A run counts a unit more than it has: without it 200 ragged windows (4 heads, D 64) take 56.4 us, with it 50.5, with two 48.6
+  // (but the 256 requests above 251 in place of 247).
+  const int64_t most = 256 * residency(D, l.row_tiles);
+  const int waves_of = waves(D, l.row_tiles);
+  l.alone = l.row_tiles == 1 && l.runs >= most * waves_of / 32 && !(positions <= 32 * waves_of && l.runs <= most);
+  l.tile = l.alone ? 32 : 32 * waves_of;
+  l.units = l.alone ? waves_of : 1;
+  l.extra = l.alone ? 1 : 0;
+  const int64_t tiles = (positions > 0 ? (positions - 1) / l.tile + 1 : 1) + l.extra;
+  l.workers = (int)(l.runs * tiles < most * l.units ? (l.runs * tiles + l.units - 1) / l.units : most);
   l.split = tiles > 1;
   l.by_run = l.runs <= l.workers;
   // Join: where few runs share all workers each is in many pieces, and a workgroup takes one row of one run; else a wavefront does.
@@ -748,9 +988,10 @@ static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query
 
 template <typename act_t, int D>
 static void launch_paged_attention(const PagedAttention& p, const PagedLaunch& l, hipStream_t s) {
-  if (l.row_tiles == 1) paged_attention_kernel<act_t, D, 1><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
-  else if (l.row_tiles == 2) paged_attention_kernel<act_t, D, 2><<<l.workers, 64 * waves(D, 2), 0, s>>>(p);
-  else if constexpr (D != 256) paged_attention_kernel<act_t, D, 4><<<l.workers, 64 * waves(D, 4), 0, s>>>(p);
+  if (l.alone) paged_attention_kernel<act_t, D, 1, true><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
+  else if (l.row_tiles == 1) paged_attention_kernel<act_t, D, 1, false><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
+  else if (l.row_tiles == 2) paged_attention_kernel<act_t, D, 2, false><<<l.workers, 64 * waves(D, 2), 0, s>>>(p);
+  else if constexpr (D != 256) paged_attention_kernel<act_t, D, 4, false><<<l.workers, 64 * waves(D, 4), 0, s>>>(p);
   if (!l.split) return;
   const dim3 grid((unsigned)(l.by_run ? l.runs : l.workers), l.join_rows);
   if (l.per_row) paged_join_kernel<act_t, D, true, 16><<<grid, 1024, 0, s>>>(p);
@@ -764,7 +1005,7 @@ static int check_shape(int batch, int HQ, int HKV, int D, int max_query, int64_t
   PLA_REQUIRE(max_query * (int64_t)(HQ / HKV) <= (1 << 30), "too many query heads");
   PLA_REQUIRE(batch >= 0 && (int64_t)batch * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "too many requests");
   PLA_REQUIRE(positions >= 0 && positions <= (1 << 30), "a row of the block table must hold at most 2^30 positions");
-  PLA_REQUIRE((positions / 128 + 1) * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "a request with too many heads for its positions");
+  PLA_REQUIRE((positions / 32 + 1) * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "a request with too many heads for its positions");
   return 0;
 }
 
@@ -782,11 +1023,11 @@ extern "C" int pla_paged_attention_segments(
   using namespace pla;
   if (check_shape(batch, HQ, HKV, head_dim, max_query_len, positions) || batch == 0 || !offsets || !seq_lens) return -1;
   const PagedLaunch l = paged_launch(batch, HQ, HKV, head_dim, max_query_len, positions);
-  const PagedShape shape{HKV, HQ / HKV, paged_divisor(HQ / HKV), bits_of(l.rows), bits_of(l.tile), max_query_len, tokens, positions};
+  const PagedShape shape{HKV, HQ / HKV, paged_divisor(HQ / HKV), bits_of(l.rows), bits_of(l.tile), l.units, l.extra, max_query_len, tokens, positions};
   auto request = [&](int n) { return paged_request(shape, offsets[n], offsets[n + 1], seq_lens[n]); };
   int64_t total = 0;
   for (int n = 0; n < batch; ++n) total += paged_weight(shape, request(n));
-  const PagedLine line = paged_line(l.workers, total);
+  const PagedLine line = paged_line(shape, l.workers, total);
   if (worker < 0 || worker >= line.workers) return 0;
   int64_t unit = paged_stretch(line, worker), offset = unit;
   const int64_t end = paged_stretch(line, worker + 1);
@@ -843,7 +1084,7 @@ extern "C" int pla_paged_attention_launch(
   const PagedAttention p{(const uint16_t*)q, q_token, q_head, (const uint16_t*)k_cache, (const uint16_t*)v_cache, kv_block, kv_token,
                          kv_head, block_table, table_row_stride, mapping, mapping_wide, offsets, offsets_wide, seq_lens, seq_lens_wide,
                          (const uint16_t*)gate, gate_token, gate_head, (uint16_t*)out, out_token, out_head,
-                         PagedShape{HKV, HQ / HKV, paged_divisor(HQ / HKV), bits_of(l.rows), bits_of(l.tile), max_query_len, tokens, positions},
+                         PagedShape{HKV, HQ / HKV, paged_divisor(HQ / HKV), bits_of(l.rows), bits_of(l.tile), l.units, l.extra, max_query_len, tokens, positions},
                          batch, blocks, block_size, table_rows, paged_divisor(block_size), scale * 1.44269504088896341f, l.by_run, l.row_blocks,
                          l.split ? reinterpret_cast<float*>(ws) : nullptr, l.split ? reinterpret_cast<float2*>(ws + l.tops_at) : nullptr,
                          l.split ? reinterpret_cast<PagedRun*>(ws + l.runs_at) : nullptr};

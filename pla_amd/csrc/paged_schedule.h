@@ -1,13 +1,14 @@
 // How the attention over a paged cache is dealt out.  Host and device use the same functions: the host's side is arithmetic
 // for tests and logs.
 //
-// The unit of work is a tile of keys, 32 for each wavefront of a workgroup, for one (request, key-value head, block of query rows).  All units of a call stand
-// in one line - requests, within them heads, within them row blocks, within them tiles - and every worker (workgroup) takes
-// an equal stretch of it.  So a batch of very different lengths keeps the whole chip busy to the end, and one long request is
-// split as finely as there are workers, with no number of splits to choose and no length read back by the host.  A run of
-// tiles that a stretch cuts is summed up in pieces: every piece leaves its rows' maxima, sums and unnormalised outputs in the
-// workspace, in slot 2 w + 1 of worker w if it is the first of its run (at most one a worker: the last run it begins), in
-// slot 2 w otherwise (at most one: the run its stretch begins in).
+// The unit of work is a tile of keys, 32 for each wavefront of a workgroup that works together, 32 where wavefronts work alone, for
+// one (request, key-value head, block of query rows).  All units of a call stand in one line - requests, within them heads, within them
+// row blocks, within them tiles - and every worker (workgroup) takes an equal stretch of it, which wavefronts that work alone share
+// out in the same way.  So a batch of very different lengths keeps the whole chip busy to the end, and one long request is split as
+// finely as there are workers, with no number of splits to choose and no length read back by the host.  A run of tiles that a
+// stretch cuts is summed up in pieces: every piece leaves its rows' maxima, sums and unnormalised outputs in the workspace, in slot
+// 2 w + 1 of worker w if it is the first of its run (at most one a worker: the last run it begins), in slot 2 w otherwise (at most
+// one: the run its stretch begins in).
 #pragma once
 
 #include <stdint.h>
@@ -35,6 +36,7 @@ struct PagedShape {
   int heads, group;                       // key-value heads, query heads of each
   PagedDivisor by_group;
   int row_bits, tile_bits;                // query rows of a block and keys of a tile are 2 to these
+  int units, extra;                       // that a worker has at least, but for the last; that a run takes on top of its tiles
   int max_query, tokens;                  // longest window, rows of q
   int64_t positions;                      // that a row of the block table has pages for
 };
@@ -55,7 +57,7 @@ PLA_HD PagedRequest paged_request(const PagedShape& s, int64_t begin, int64_t en
   r.length = (int)(length < 0 ? 0 : length > INT32_MAX ? INT32_MAX : length);
   r.keys = (int)(r.length < s.positions ? r.length : s.positions);
   r.blocks = (r.window * s.group + (1 << s.row_bits) - 1) >> s.row_bits;
-  r.tiles = r.keys > 0 ? ((r.keys - 1) >> s.tile_bits) + 1 : 1;
+  r.tiles = (r.keys > 0 ? ((r.keys - 1) >> s.tile_bits) + 1 : 1) + s.extra;
   return r;
 }
 PLA_HD int paged_weight(const PagedShape& s, const PagedRequest& r) { return r.tiles * r.blocks * s.heads; }     // fits: the host checks
@@ -79,10 +81,10 @@ struct PagedLine {
 PLA_HD int64_t paged_divide(int64_t a, int64_t b) {        // of numbers that are not negative; short where they are
   return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
-PLA_HD PagedLine paged_line(int grid, int64_t total) {
+PLA_HD PagedLine paged_line(const PagedShape& s, int grid, int64_t total) {
   PagedLine l{total, 0, 0, 0};
   if (total <= 0) return l;
-  l.workers = total < grid ? (int)total : grid;
+  l.workers = total < (int64_t)grid * s.units ? ((int)total + s.units - 1) / s.units : grid;
   l.each = paged_divide(total, l.workers);
   l.rest = (int)(total - l.each * l.workers);
   return l;

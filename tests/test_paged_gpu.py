@@ -448,6 +448,15 @@ def _attention_reference(q, cache, lengths, windows, scale, gate=None, visible=N
     return out, slack
 
 
+CROWD = 0                                                    # requests without a window behind those of a call
+
+
+@pytest.fixture(params=[0, 160], ids=["together", "alone"])
+def crowd(request, monkeypatch):
+    """Calls of few runs, whose workgroups work together, and of many, whose wavefronts have runs of their own."""
+    monkeypatch.setitem(globals(), "CROWD", request.param)
+
+
 def _attend(cache, q, lengths, windows, *, max_query=None, index_dtype=torch.int32, gate=None, scale=None, rows=None, out=None, offsets=None):
     from pla.decode.paged import paged_attention_decode
     if offsets is None:
@@ -455,10 +464,14 @@ def _attend(cache, q, lengths, windows, *, max_query=None, index_dtype=torch.int
         for w in windows:
             offsets.append(offsets[-1] + w)
     single = max_query is None and all(w == 1 for w in windows)
+    max_query = 1 if single else max_query or max(windows)
+    if CROWD:
+        rows = (list(range(len(lengths))) if rows is None else list(rows)) + [0] * CROWD
+        lengths, offsets, single = list(lengths) + [9] * CROWD, list(offsets) + [offsets[-1]] * CROWD, False
     return paged_attention_decode(q, cache.k_cache, cache.v_cache, cache.table, _ints(lengths, index_dtype),
                                   query_start_loc=None if single else _ints(offsets, index_dtype),
                                   request_indices=None if rows is None else _ints(rows, index_dtype),
-                                  max_query_len=1 if single else max_query or max(windows), scale=scale, output_gate=gate, out=out)
+                                  max_query_len=max_query, scale=scale, output_gate=gate, out=out)
 
 
 EDGES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 64, 127, 128, 129, 130, 255, 257, 500]
@@ -468,6 +481,7 @@ EDGES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 64, 127, 128, 129, 130, 255, 257, 500]
 @pytest.mark.parametrize("act", ["bf16", "fp16"])
 @pytest.mark.parametrize("HQ, HKV, bs, heads_first, gated", [(1, 1, 16, False, False), (8, 2, 32, True, True), (7, 1, 48, False, False),
                                                              (16, 1, 528, False, True), (40, 2, 16, True, False)])
+@pytest.mark.usefixtures("crowd")
 def test_one_new_token_at_the_edges_of_pages_and_tiles(D, act, HQ, HKV, bs, heads_first, gated):
     cache = _Cache(EDGES, HKV, D, bs, act, seed=D + HQ, heads_first=heads_first)
     g = torch.Generator().manual_seed(HQ)
@@ -481,6 +495,7 @@ def test_one_new_token_at_the_edges_of_pages_and_tiles(D, act, HQ, HKV, bs, head
 
 @pytest.mark.parametrize("D, act, HQ, HKV, max_query", [(64, "fp16", 4, 4, 8), (128, "bf16", 16, 2, 4), (128, "fp16", 6, 2, 32), (256, "bf16", 8, 1, 32),
                                                         (256, "fp16", 3, 1, 5), (64, "bf16", 16, 1, 17), (128, "bf16", 12, 1, 3)])
+@pytest.mark.usefixtures("crowd")
 def test_windows_of_draft_tokens(D, act, HQ, HKV, max_query):
     """Windows of every size against lengths that are shorter, equal, at a page's or a tile's edge; the longest split into pieces."""
     rng = random.Random(D + max_query)
@@ -498,6 +513,7 @@ def test_windows_of_draft_tokens(D, act, HQ, HKV, max_query):
 
 
 @pytest.mark.parametrize("D, act, HQ, HKV, bs", [(128, "bf16", 16, 2, 16), (64, "fp16", 2, 2, 64), (256, "bf16", 16, 1, 528)])
+@pytest.mark.usefixtures("crowd")
 def test_one_long_request_among_short_ones_is_split_and_joined(D, act, HQ, HKV, bs):
     lengths = [40000, 3, 700, 0, 129]
     cache = _Cache(lengths, HKV, D, bs, act, seed=1)
@@ -519,6 +535,7 @@ def test_more_runs_than_workgroups():
     _close(out, ref, slack, "many")
 
 
+@pytest.mark.usefixtures("crowd")
 def test_peaked_and_flat_scores_and_other_scales():
     lengths = [1000, 1000, 1000]
     for act in ("bf16", "fp16"):
@@ -531,6 +548,7 @@ def test_peaked_and_flat_scores_and_other_scales():
             _close(out, ref, slack, scale)
 
 
+@pytest.mark.usefixtures("crowd")
 def test_requests_that_are_passed_over_leave_their_rows():
     """Windows that are empty, longer than declared or not within q; rows of the block table by index, in any order."""
     lengths, rows = [50, 60, 70, 80, 20], [4, 0, 7, 2, 9]
@@ -551,6 +569,7 @@ def test_requests_that_are_passed_over_leave_their_rows():
     _close(out, ref, slack, "rows")
 
 
+@pytest.mark.usefixtures("crowd")
 def test_positions_without_a_block_are_left_out():
     lengths = [300, 90, 40, 1000]
     cache = _Cache(lengths, 2, 64, 16, "fp16", seed=12)
@@ -575,6 +594,7 @@ def test_positions_without_a_block_are_left_out():
 
 @pytest.mark.parametrize("D, act, HQ, HKV, length", [(128, "bf16", 8, 2, 133), (64, "fp16", 4, 4, 640), (256, "bf16", 8, 1, 46), (128, "fp16", 16, 1, 5000)])
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.usefixtures("crowd")
 def test_draft_tokens_that_are_not_finite_do_not_reach_the_ones_before(D, act, HQ, HKV, length, value):
     """The keys and values of draft token 5 of 8: tokens 0 to 4 do not see them and equal a call without them."""
     windows, lengths = [8, 8], [length, length + 3]
@@ -601,7 +621,30 @@ def test_draft_tokens_that_are_not_finite_do_not_reach_the_ones_before(D, act, H
     _close(got[8:], ref[8:], slack[8:], "other request")
 
 
+@pytest.mark.parametrize("places", [(4,), (13,), (4, 13), (1, 2, 14, 15)])
+def test_values_set_aside_in_two_steps_of_one_wavefront(places):
+    """Windows that lie in two groups of 32 keys, long requests enough that a wavefront has several groups of a run: values that are
+    infinite in the first, the second or both reach the tokens that see them, and every other channel is as without them."""
+    D, HKV = 256, 4
+    lengths = [1000, 1064, 1032] + [1000 + 7 * i for i in range(27)]           # the windows from 985, 1049 and 1017 on
+    windows = [16] * 3 + [1] * 27
+    cache = _Cache(lengths, HKV, D, 16, "bf16", seed=71)
+    q = _randn(torch.Generator().manual_seed(72), sum(windows), HKV, D, dtype=torch.bfloat16)
+    ref, slack = _attention_reference(q, cache, lengths, windows, D ** -0.5)
+    for n in range(3):
+        for place in places:
+            at = lengths[n] - 16 + place
+            cache.store[cache.table[n, at // 16].item(), 1, at % 16, :, 5] = math.inf
+    got = _attend(cache, q, lengths, windows)
+    for n in range(3):
+        rows = got[16 * n:16 * n + 16, :, 5]
+        assert rows[:places[0]].isfinite().all() and (rows[places[0]:] == math.inf).all()
+        rows[places[0]:] = ref[16 * n + places[0]:16 * n + 16, :, 5].to(rows)
+    _close(got, ref, slack, "set aside")
+
+
 @pytest.mark.parametrize("act, length", [("bf16", 70), ("fp16", 1500)])
+@pytest.mark.usefixtures("crowd")
 def test_values_set_aside_weigh_as_much_as_the_others(act, length):
     """Scores so far apart that the draft tokens' own keys carry most of the weight, with one value among them that is not finite:
     the rows that do not see it, and the other channels of those that do, are what they are without it."""
@@ -643,6 +686,7 @@ def test_caches_side_by_side_in_one_buffer_and_strides_of_single_rows():
         fused_qk_norm_rope(q, k, v=v, k_cache=k_cache, v_cache=both[..., D // 2:D // 2 + D], slot_mapping=slots)
 
 
+@pytest.mark.usefixtures("crowd")
 def test_offsets_past_32_bits():
     """Blocks 2^32 bytes and more apart."""
     D, HKV, pitch = 128, 1, 2 ** 31 + 1024
@@ -666,6 +710,7 @@ def test_offsets_past_32_bits():
     assert torch.equal(k_cache[2, 15], k[0]) and torch.equal(v_cache[2, 15], v[0]) and torch.equal(k_cache[0, 0], k[1])
 
 
+@pytest.mark.usefixtures("crowd")
 def test_strided_rows_of_q_gate_and_out():
     lengths = [100, 7, 300]
     cache = _Cache(lengths, 2, 128, 16, "bf16", seed=31)
