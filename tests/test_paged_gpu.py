@@ -842,6 +842,41 @@ def test_a_captured_step_replays_over_other_lengths():
         assert (s.out[sum(query):] == 9).all()
 
 
+@pytest.mark.parametrize("D, HKV, batch", [(64, 2, 90), (128, 4, 30), (256, 1, 300)])
+def test_captured_calls_of_many_runs_replay_over_other_lengths(D, HKV, batch):
+    """Wavefronts that have runs of their own: what is cut, and where, follows the lengths at the time of the replay."""
+    from pla.decode.paged import paged_attention_decode
+    g = torch.Generator().manual_seed(D)
+    bs, pages = 32, 12
+    cache = _randn(g, batch * pages // 2, 2, bs, HKV, D, dtype=torch.bfloat16)
+    table = torch.randint(0, cache.size(0), (batch, pages), generator=g).to(torch.int32).to(DEV)
+    q = _randn(g, batch, 4 * HKV, D, dtype=torch.bfloat16)
+    lengths, out = _ints([1] * batch), torch.zeros_like(q)
+    call = lambda to: paged_attention_decode(q, cache[:, 0], cache[:, 1], table, lengths, out=to)
+    call(out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for high in (0, 1, 40, 384, 3, 200):
+        lengths.copy_(torch.randint(0, high + 1, (batch,), generator=g).to(torch.int32))
+        q.copy_(_randn(g, *q.shape, dtype=torch.bfloat16))
+        expect = call(torch.empty_like(q))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, expect)
+        k = cache[:, 0][table.long()].reshape(batch, pages * bs, HKV, D).double()
+        v = cache[:, 1][table.long()].reshape(batch, pages * bs, HKV, D).double()
+        score = (q.double().view(batch, HKV, 4, 1, D) * k.transpose(1, 2)[:, :, None]).sum(-1) * D ** -0.5
+        score = score.masked_fill(torch.arange(pages * bs, device=DEV) >= lengths[:, None, None, None], -math.inf)
+        weight = torch.softmax(score, -1).nan_to_num(0.0)
+        plain = (weight[..., None] * v.transpose(1, 2)[:, :, None]).sum(-2).view_as(q)
+        # weights are rounded by 2^-8 at most, and the outputs; scores in 32 bits are far below that
+        slack = 1.1 * 2.0 ** -8 * ((weight[..., None] * (v.transpose(1, 2)[:, :, None] - plain.view(batch, HKV, 4, 1, D)).abs()).sum(-2).view_as(q) + plain.abs()) + 1e-6
+        assert ((out.double() - plain).abs() <= slack).all()
+
+
 def test_two_captured_graphs_and_two_streams_do_not_share_anything():
     lengths = [3000, 50, 900, 0, 131]
     cases = []
