@@ -20,9 +20,9 @@
 //                  lane (r, kb) loads channels 8 r .. 8 r + 7 of those eight keys, eight loads of which sixteen lanes cover a
 //                  row, and one v_perm_b32 a pair of values turns them into rows of V^T.  No value crosses a lane.
 //
-// A row's maximum and sum run along; the sum is that of the weights as they are rounded for the product (bf16: off by up to
-// 2^-9 of themselves, which then cancels where few keys carry the weight).  fp16 weights are scaled by 2^14, so that weights
-// down to 2^-38 of the largest still count.
+// A row's maximum and sum run along, in FP32.  For the product a weight goes in two parts of the cache's type, what remains of it
+// in the second: off by up to 2^-16 of itself (fp16 2^-22; weights scaled by 2^14, so that those down to 2^-38 of the largest still
+// count).  One part alone would be off by 2^-8, as much as the output's own rounding where values cancel.
 //
 // Values that no row of a block sees are replaced by zeros: their weight is zero, but zero times what an unused place of the
 // cache may hold need not be.  Within a window some rows see values that others do not.  Where one of those is infinite or NaN,
@@ -107,6 +107,19 @@ __device__ __forceinline__ float query_sum(float x) {
 // The factor from maximum `m` to maximum `top` >= m; equal infinities are no step.
 __device__ __forceinline__ float rescale(float m, float top) { return m == top ? 1.f : __builtin_amdgcn_exp2f(m - top); }
 
+// Two weights as packed pairs of a first part, cut off, and of what remains, rounded; the cut keeps the second from being negative.
+// A weight that counts has a positive second part: an infinite value stays what it is when both parts are summed.
+template <typename act_t> constexpr float LEAST_PART = 0x1p-126f;
+template <> constexpr float LEAST_PART<f16_t> = 0x1p-24f;
+template <typename act_t>
+__device__ __forceinline__ void weight_parts(float x, float y, uint32_t& high, uint32_t& low) {
+  high = __is_same(act_t, bf16_t) ? __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u)
+                                  : pack2_rtz(x, y);
+  // between the least part and the weight itself: a weight of zero has none
+  low = pack2<act_t>(__builtin_amdgcn_fmed3f(x - lo16<act_t>(high), LEAST_PART<act_t>, x),
+                     __builtin_amdgcn_fmed3f(y - hi16<act_t>(high), LEAST_PART<act_t>, y));
+}
+
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 template <int D> struct ValueWords { static constexpr int N = D == 64 ? 2 : 4; };      // 32-bit words of a lane's channels, a chunk
 
@@ -189,7 +202,7 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
   next_keys();
 
   const bool masked = key0 + 32 > least || !there[0] || !there[1];          // some row does not see some key
-  bf16x8_t packed[RT];
+  bf16x8_t high[RT], low[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     float x[8];
@@ -216,11 +229,17 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
     const float zero = (top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - zero);
-    const uint4 word = make_uint4(pack2<act_t>(x[0], x[1]), pack2<act_t>(x[2], x[3]), pack2<act_t>(x[4], x[5]), pack2<act_t>(x[6], x[7]));
-    const uint32_t u[4] = {word.x, word.y, word.z, word.w};
+    u32x4_t a, b;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w.sum[t] += lo16<act_t>(u[i]) + hi16<act_t>(u[i]);
-    packed[t] = __builtin_bit_cast(bf16x8_t, word);
+    for (int i = 0; i < 4; ++i) {
+      w.sum[t] += x[2 * i] + x[2 * i + 1];
+      uint32_t first, second;
+      weight_parts<act_t>(x[2 * i], x[2 * i + 1], first, second);
+      a[i] = first;
+      b[i] = second;
+    }
+    high[t] = __builtin_bit_cast(bf16x8_t, a);
+    low[t] = __builtin_bit_cast(bf16x8_t, b);
   }
 
   // Values of two keys are turned by one byte selection, which also puts zeros in the place of values that no row sees.
@@ -247,16 +266,6 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
       if (__ballot((odd & 0x80008000u) != 0) != 0) {
         stop = least;
         w.set_aside = w.set_aside < 0 ? key0 : w.set_aside | 1;
-        // their weights come back into the sum with their values, rounded alike
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const u32x4_t u = __builtin_bit_cast(u32x4_t, packed[t]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float weight = i & 1 ? hi16<act_t>(u[i / 2]) : lo16<act_t>(u[i / 2]);
-            if (key + 16 * (i / 4) + (i & 3) >= least) w.sum[t] -= weight;
-          }
-        }
       }
     }
 #pragma unroll
@@ -275,16 +284,19 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(w.v[2 * i + 1][c][j / 2], w.v[2 * i][c][j / 2], select[j & 1][i]);
 #pragma unroll
-      for (int t = 0; t < RT; ++t) w.o[t][c][j] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, a), packed[t], w.o[t][c][j]);
+      for (int t = 0; t < RT; ++t) {
+        w.o[t][c][j] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, a), high[t], w.o[t][c][j]);
+        w.o[t][c][j] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, a), low[t], w.o[t][c][j]);
+      }
     }
   next_values();
 }
 
-// The weights of keys [first, last) for one row into its sum, and their values into the D / TEAM channels of it that a thread has;
+// The weighted values of keys [first, last) into the D / TEAM channels of a row that a thread has (the sum has the weights already);
 // the TEAM threads of a row form its scores together.
 template <typename act_t, int D, int TEAM>
 __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const PagedRequest& req, int kv_head, int row, int channel,
-                                              const int32_t* pages, int first, int last, float top, float& sum, float (&o)[D / TEAM]) {
+                                              const int32_t* pages, int first, int last, float top, float (&o)[D / TEAM]) {
   const int j = paged_quotient(p.shape.by_group, row), head = kv_head * p.shape.group + row - j * p.shape.group;
   const uint16_t* q = p.q + (req.begin + j) * p.q_token + head * p.q_head + channel;
   last = min(last, paged_limit(p.shape, req, row));
@@ -296,8 +308,7 @@ __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const Pag
     float score = 0.f;
     for (int i = 0; i < D / TEAM; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
     score = (TEAM == 16 ? row16_allreduce(score) : row32_allreduce(score)) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
-    const float weight = to_float(from_float<act_t>(__builtin_amdgcn_exp2f(score)));
-    sum += weight;
+    const float weight = __builtin_amdgcn_exp2f(score);
 #pragma unroll
     for (int i = 0; i < D / TEAM; ++i) {
       const float x = to_float(act_t{p.v[at + i]});
@@ -363,7 +374,7 @@ __device__ __forceinline__ void write_row(const PagedAttention& p, int64_t token
 // `o` on in LDS.  row < 0: none.
 template <typename act_t, int D>
 __device__ __forceinline__ void add_set_aside_alone(const PagedAttention& p, const PagedRequest& req, int kv_head, int row, int kb,
-                                                    const int32_t* pages, int first, int last, float top, float& sum, float* o) {
+                                                    const int32_t* pages, int first, int last, float top, float* o) {
   const int j = row < 0 ? 0 : paged_quotient(p.shape.by_group, row), head = kv_head * p.shape.group + (row < 0 ? 0 : row - j * p.shape.group);
   const uint16_t* q = p.q + (req.begin + j) * p.q_token + head * p.q_head + kb * (D / 4);
   const int limit = row < 0 ? 0 : paged_limit(p.shape, req, row);
@@ -377,8 +388,7 @@ __device__ __forceinline__ void add_set_aside_alone(const PagedAttention& p, con
     for (int i = 0; i < D / 4; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
     score = query_sum(score) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
     if (key >= limit) continue;
-    const float weight = to_float(from_float<act_t>(__builtin_amdgcn_exp2f(score)));
-    sum += weight;
+    const float weight = __builtin_amdgcn_exp2f(score);
 #pragma nounroll
     for (int i = 0; i < D / 4; ++i) {
       const float x = to_float(act_t{p.v[at + i]});
@@ -677,7 +687,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
         park(mine);
         own_lds_order();
         add_set_aside_alone<act_t, D>(p, a.req, a.seg.head, r < a.rows ? row : -1, kb, a.pages, max(w.set_aside & ~31, a.least),
-                                      min((w.set_aside & ~31) + (w.set_aside & 1 ? 64 : 32), a.end), w.top[0], sum, mine);
+                                      min((w.set_aside & ~31) + (w.set_aside & 1 ? 64 : 32), a.end), w.top[0], mine);
         own_lds_order();
 #pragma unroll
         for (int c = 0; c < W::CHUNKS; ++c)
@@ -764,7 +774,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
         const int row = a.row0 + 16 * t + out_row;
         for (int x = 0; x < WAVES; ++x)
           if (aside[x] >= 0)
-            add_set_aside<act_t, D, TEAM>(p, a.req, a.seg.head, row, out_channel, a.pages, max(aside[x], a.least), min(aside[x] + 32, a.end), row_top, row_sum, o);
+            add_set_aside<act_t, D, TEAM>(p, a.req, a.seg.head, row, out_channel, a.pages, max(aside[x], a.least), min(aside[x] + 32, a.end), row_top, o);
         if (a.seg.slot < 0) {
           const int j = paged_quotient(p.shape.by_group, row), head = a.seg.head * p.shape.group + row - j * p.shape.group;
           write_row<act_t, CHANNELS>(p, a.req.begin + j, head, out_channel, row_sum, o);

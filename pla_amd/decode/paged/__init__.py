@@ -179,8 +179,9 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, query_
     ``request_indices`` [N]: rows of the block table, n without it.
 
     scale (default D^-0.5) applies to the scores; output_gate [T, HQ, D] multiplies the result by its sigmoid.  Scores, their
-    maxima and sums and the outputs are float32; weights are rounded to q's type for the product with the values (and summed as
-    rounded), outputs once.  Returns ``out`` [T, HQ, D], which shares memory with no input.  Results do not depend on timing.
+    maxima and sums and the outputs are float32; weights meet the values in two parts of q's type (off by 2^-16 of themselves at most,
+    fp16 2^-22), outputs are rounded once.  Returns ``out`` [T, HQ, D], which shares memory with no input.  Results do not depend on
+    timing.
     """
     if _sanity_enabled():
         from ._sanity import check_attention

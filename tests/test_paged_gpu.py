@@ -951,3 +951,47 @@ def test_calls_on_another_stream_than_the_tensors_own():
         got = [_attend(cache, q, [700, 20], [1, 1]) for _ in range(3)]
     s.synchronize()
     assert all(torch.equal(x, expect) for x in got)
+
+
+# ---- weights ------------------------------------------------------------------------------------------------------
+
+def _attention_reference_32(q, cache, lengths, windows, scale):
+    """As _attention_reference, with the error of weights that are as good as 32-bit arithmetic makes the rest, against outputs that
+    values of both signs make small.
+
+    The two parts of a weight are off by 2^-16 of it at most (bf16: eight bits cut off, eight more rounded; fp16 2^-22), in the
+    product alone, and by the least fp16, 2^-24 where the largest weight is 2^14; scores, sums and division as there."""
+    T, HQ, D = q.shape
+    G = HQ // cache.k_cache.size(2)
+    part = 2.0 ** -16 if q.dtype == torch.bfloat16 else 2.0 ** -22
+    out, slack = torch.zeros(T, HQ, D, dtype=torch.float64), torch.zeros(T, HQ, D, dtype=torch.float64)
+    qd, token = q.double().cpu(), 0
+    for n, (length, window) in enumerate(zip(lengths, windows)):
+        for j in range(window):
+            sees = min(max(length - window + j + 1, 0), max(length, 0))
+            if sees:
+                k, v = cache.k[n][:sees].double().repeat_interleave(G, 1), cache.v[n][:sees].double().repeat_interleave(G, 1)
+                terms = qd[token][None] * k
+                score = terms.sum(-1) * scale
+                wrong = (terms.abs().sum(-1) * abs(scale) * D + 3 * score.abs()) * 2.0 ** -24 + 2.0 ** -22
+                w = torch.softmax(score, 0)[:, :, None]
+                out[token] = (w * v).sum(0)
+                size = (w * v.abs()).sum(0)
+                slack[token] = (w * (2 * wrong[:, :, None]) * (v - out[token]).abs()).sum(0) + (part + (sees + 16) * 2.0 ** -24) * size + sees * 2.0 ** -37 * v.abs().amax()
+            token += 1
+    return out, slack
+
+
+@pytest.mark.parametrize("D, act, HQ, HKV, max_query", [(64, "bf16", 4, 2, 3), (64, "fp16", 8, 1, 4), (64, "bf16", 8, 1, 8), (128, "bf16", 8, 2, 2),
+                                                        (128, "fp16", 7, 1, 3), (128, "fp16", 16, 2, 8), (256, "bf16", 8, 1, 2), (256, "fp16", 4, 1, 8)])
+@pytest.mark.usefixtures("crowd")
+def test_weights_are_as_good_as_the_sums(D, act, HQ, HKV, max_query):
+    """Few keys, whose values partly cancel: an output's own rounding is then small, and a weight in 16 bits would show."""
+    rng = random.Random(D + HQ)
+    lengths = [1, 2, 3, 4, 5, 8, 15, 16, 17, 33, 40, 64, 100, 130, 300, 700]
+    windows = [min(n, rng.randint(1, max_query)) for n in lengths]
+    cache = _Cache(lengths, HKV, D, 16, act, seed=D + max_query)
+    q = _randn(torch.Generator().manual_seed(HQ), sum(windows), HQ, D, dtype=DTYPES[act])
+    out = _attend(cache, q, lengths, windows, max_query=max_query)
+    ref, slack = _attention_reference_32(q, cache, lengths, windows, D ** -0.5)
+    _close(out, ref, slack, "weights")
