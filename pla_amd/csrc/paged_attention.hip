@@ -21,8 +21,8 @@
 //                  row, and one v_perm_b32 a pair of values turns them into rows of V^T.  No value crosses a lane.
 //
 // A row's maximum and sum run along, in FP32.  For the product a weight goes in two parts of the cache's type, what remains of it
-// in the second: off by up to 2^-16 of itself (fp16 2^-22; weights scaled by 2^14, so that those down to 2^-38 of the largest still
-// count).  One part alone would be off by 2^-8, as much as the output's own rounding where values cancel.
+// in the second: off by up to 2^-16 of itself (fp16 2^-22; weights are scaled by 2^14 there), and by up to two least parts, 2^-37 of
+// the largest weight in fp16.  One part alone would be off by 2^-8, as much as the output's own rounding where values cancel.
 //
 // Values that no row of a block sees are replaced by zeros: their weight is zero, but zero times what an unused place of the
 // cache may hold need not be.  Within a window some rows see values that others do not.  Where one of those is infinite or NaN,
@@ -104,20 +104,26 @@ __device__ __forceinline__ float query_sum(float x) {
   return b.lo + b.hi;
 }
 
-// The factor from maximum `m` to maximum `top` >= m; equal infinities are no step.
-__device__ __forceinline__ float rescale(float m, float top) { return m == top ? 1.f : __builtin_amdgcn_exp2f(m - top); }
+// The factor from maximum `m` to maximum `top` >= m; equal infinities are no step.  Never zero: an infinite output stays one.
+__device__ __forceinline__ float rescale(float m, float top) { return m == top ? 1.f : fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-126f); }
 
-// Two weights as packed pairs of a first part, cut off, and of what remains, rounded; the cut keeps the second from being negative.
-// A weight that counts has a positive second part: an infinite value stays what it is when both parts are summed.
+// Two weights as packed pairs of a first part, cut off, and of what remains, rounded.  Neither part is negative (the cut sees to it)
+// nor zero: a key that a row sees has some weight, so that an infinite value there makes the output infinite, as in the formula, by
+// whichever way it comes into the sum.
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 template <typename act_t> constexpr float LEAST_PART = 0x1p-126f;
 template <> constexpr float LEAST_PART<f16_t> = 0x1p-24f;
+template <typename act_t>
+__device__ __forceinline__ uint32_t at_least_least(uint32_t pair) {         // of numbers that are not negative: they are ordered as their bits
+  const uint16_t least = __is_same(act_t, bf16_t) ? 0x0080 : 0x0001;
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, pair), u16x2_t{least, least}));
+}
 template <typename act_t>
 __device__ __forceinline__ void weight_parts(float x, float y, uint32_t& high, uint32_t& low) {
   high = __is_same(act_t, bf16_t) ? __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u)
                                   : pack2_rtz(x, y);
-  // between the least part and the weight itself: a weight of zero has none
-  low = pack2<act_t>(__builtin_amdgcn_fmed3f(x - lo16<act_t>(high), LEAST_PART<act_t>, x),
-                     __builtin_amdgcn_fmed3f(y - hi16<act_t>(high), LEAST_PART<act_t>, y));
+  low = at_least_least<act_t>(pack2<act_t>(x - lo16<act_t>(high), y - hi16<act_t>(high)));
+  high = at_least_least<act_t>(high);
 }
 
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -202,6 +208,7 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
   next_keys();
 
   const bool masked = key0 + 32 > least || !there[0] || !there[1];          // some row does not see some key
+  auto sees = [&](int t, int i) { return (key0 + 16 * (i / 4) + 4 * kb + (i & 3) < w.limit[t]) & there[i / 4]; };
   bf16x8_t high[RT], low[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
@@ -210,10 +217,7 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
     for (int i = 0; i < 8; ++i) x[i] = s[t][i / 4][i & 3] * scale_log2;
     if (masked) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = key0 + 16 * (i / 4) + 4 * kb + (i & 3);
-        x[i] = ((key < w.limit[t]) & there[i / 4]) ? x[i] : -INFINITY;
-      }
+      for (int i = 0; i < 8; ++i) x[i] = sees(t, i) ? x[i] : -INFINITY;
     }
     float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     top = fmaxf(query_max(top), w.top[t]);
@@ -237,6 +241,14 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
       weight_parts<act_t>(x[2 * i], x[2 * i + 1], first, second);
       a[i] = first;
       b[i] = second;
+    }
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t seen = (sees(t, 2 * i) ? 0xffffu : 0u) | (sees(t, 2 * i + 1) ? 0xffff0000u : 0u);
+        a[i] &= seen;
+        b[i] &= seen;
+      }
     }
     high[t] = __builtin_bit_cast(bf16x8_t, a);
     low[t] = __builtin_bit_cast(bf16x8_t, b);
@@ -308,13 +320,9 @@ __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const Pag
     float score = 0.f;
     for (int i = 0; i < D / TEAM; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
     score = (TEAM == 16 ? row16_allreduce(score) : row32_allreduce(score)) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
-    const float weight = __builtin_amdgcn_exp2f(score);
+    const float weight = fmaxf(__builtin_amdgcn_exp2f(score), LEAST_PART<act_t>);
 #pragma unroll
-    for (int i = 0; i < D / TEAM; ++i) {
-      const float x = to_float(act_t{p.v[at + i]});
-      // a weight below the smallest is no weight, but an infinite value has some
-      o[i] = fmaf(weight == 0.f && !(fabsf(x) < INFINITY) ? 0x1p-126f : weight, x, o[i]);
-    }
+    for (int i = 0; i < D / TEAM; ++i) o[i] = fmaf(weight, to_float(act_t{p.v[at + i]}), o[i]);
   }
 }
 
@@ -388,13 +396,9 @@ __device__ __forceinline__ void add_set_aside_alone(const PagedAttention& p, con
     for (int i = 0; i < D / 4; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
     score = query_sum(score) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
     if (key >= limit) continue;
-    const float weight = __builtin_amdgcn_exp2f(score);
+    const float weight = fmaxf(__builtin_amdgcn_exp2f(score), LEAST_PART<act_t>);
 #pragma nounroll
-    for (int i = 0; i < D / 4; ++i) {
-      const float x = to_float(act_t{p.v[at + i]});
-      // a weight below the smallest is no weight, but an infinite value has some
-      o[kb * (D / 4) + i] = fmaf(weight == 0.f && !(fabsf(x) < INFINITY) ? 0x1p-126f : weight, x, o[kb * (D / 4) + i]);
-    }
+    for (int i = 0; i < D / 4; ++i) o[kb * (D / 4) + i] = fmaf(weight, to_float(act_t{p.v[at + i]}), o[kb * (D / 4) + i]);
   }
 }
 

@@ -995,3 +995,27 @@ def test_weights_are_as_good_as_the_sums(D, act, HQ, HKV, max_query):
     out = _attend(cache, q, lengths, windows, max_query=max_query)
     ref, slack = _attention_reference_32(q, cache, lengths, windows, D ** -0.5)
     _close(out, ref, slack, "weights")
+
+
+@pytest.mark.parametrize("D, act, HQ, HKV", [(64, "fp16", 4, 4), (64, "bf16", 12, 1), (128, "fp16", 8, 2), (128, "bf16", 16, 1), (256, "fp16", 2, 1), (256, "bf16", 8, 1)])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.usefixtures("crowd")
+def test_an_infinite_value_counts_however_small_its_weight(D, act, HQ, HKV, sign):
+    """Keys that weigh e^-60 and less of the others, in any place of a sequence, whose value is infinite in one channel: every token that
+    sees them is infinite there, tokens before them and other channels are what they are."""
+    for window, length, places in ((1, 50, (3,)), (1, 900, (600,)), (4, 700, (0, 698)), (4, 7000, (6500, 6998)), (4, 70, (68, 69))):
+        cache = _Cache([length, length], HKV, D, 16, act, seed=length)
+        q = _randn(torch.Generator().manual_seed(5), 2 * window, HQ, D, dtype=DTYPES[act])
+        q[:, :, 0] = 8.0
+        clean = _attend(cache, q, [length] * 2, [window] * 2, scale=1.0)
+        for at in places:
+            block, place = cache.table[0, at // 16].item(), at % 16
+            cache.store[block, 0, place, :, 0] = -200.0      # the score falls by more than a thousand
+            cache.store[block, 1, place, :, 7] = sign * math.inf
+        before = _attend(cache, q, [length] * 2, [window] * 2, scale=1.0)
+        for j in range(window):
+            sees = any(at < length - window + j + 1 for at in places)
+            assert (before[j, :, 7] == sign * math.inf).all() if sees else torch.equal(before[j], clean[j]), (window, length, j)
+        before[:, :, 7] = 0
+        assert before.isfinite().all()
+        assert torch.equal(before[window:, :, 8:], clean[window:, :, 8:])
