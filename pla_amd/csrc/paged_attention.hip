@@ -1019,7 +1019,9 @@ static int check_shape(int batch, int HQ, int HKV, int D, int max_query, int64_t
   PLA_REQUIRE(max_query * (int64_t)(HQ / HKV) <= (1 << 30), "too many query heads");
   PLA_REQUIRE(batch >= 0 && (int64_t)batch * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "too many requests");
   PLA_REQUIRE(positions >= 0 && positions <= (1 << 30), "a row of the block table must hold at most 2^30 positions");
-  PLA_REQUIRE((positions / 32 + 1) * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "a request with too many heads for its positions");
+  // the most units that a request can have: a run's tiles of 32 keys and the one more that it counts where wavefronts work alone
+  const int64_t units = (positions > 0 ? (positions - 1) / 32 + 1 : 1) + 1;
+  PLA_REQUIRE(units * HKV * ((max_query * (int64_t)(HQ / HKV) + 15) / 16) <= INT32_MAX, "a request with too many heads for its positions");
   return 0;
 }
 

@@ -367,3 +367,26 @@ def test_the_namespace_is_the_same_module_under_both_names():
     assert pla.decode.paged is pla_amd.decode.paged
     assert set(pla.decode.paged.__all__) == {"PagedKVBlocks", "PagedKVPlan", "paged_kv_plan", "rotary_frequencies", "fused_qk_norm_rope",
                                              "paged_attention_decode"}
+
+
+@pytest.mark.parametrize("HKV, D, positions", [(128, 128, 536870864), (1000, 128, 68719440), (2 ** 30, 64, 16)])
+def test_a_request_of_more_units_than_32_bits_count_is_refused(HKV, D, positions):
+    """A run takes one unit more than it has tiles of 32 keys where wavefronts work alone; the largest number of positions that fits is
+    dealt out, and one block more is refused."""
+    from pla_amd import _lib
+    lib = _lib.load()
+    size = lib.pla_paged_attention_workspace_bytes
+    units = lambda p: (-(-max(p, 1) // 32) + 1) * HKV
+    assert units(positions) > 2 ** 31 - 1 and size(1, HKV, HKV, D, 1, positions) == -1
+    assert b"too many heads" in lib.pla_last_error()
+    fits = positions - 16
+    if units(fits) > 2 ** 31 - 1:
+        return
+    assert size(1, HKV, HKV, D, 1, fits) > 0
+    offsets, lengths, buf = (ctypes.c_int32 * 2)(0, 1), (ctypes.c_int32 * 1)(fits), (ctypes.c_int64 * (7 * 4096))()
+    taken = 0
+    for worker in range(1025):
+        found = lib.pla_paged_attention_segments(offsets, lengths, 1, 1, HKV, HKV, D, 1, fits, worker, buf, 4096)
+        assert 0 <= found <= 4096
+        taken += sum(buf[7 * i + 4] for i in range(found))
+    assert taken == units(fits)
