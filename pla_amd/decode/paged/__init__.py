@@ -105,7 +105,7 @@ def paged_kv_plan(blocks, context_lens, query_lens, request_indices=None, *, tok
     """
     if _sanity_enabled():
         from ._sanity import check_plan
-        check_plan(blocks, context_lens, query_lens, request_indices)
+        check_plan(blocks, context_lens, query_lens, request_indices, token_capacity)
     outs = (None,) * 4 if out is None else (out.query_start_loc, out.seq_lens, out.positions, out.slot_mapping)
     made = _compiled().paged_kv_plan(blocks.block_table, blocks.held_blocks, blocks.free_blocks, blocks.free_count, blocks.block_size,
                                      context_lens, query_lens, request_indices, token_capacity, *outs)

@@ -1,7 +1,8 @@
 """Checks of values under ``PLA_SANITY_CHECK=1``: what the operators would pass over or leave out without a word.
 
 Every rejection raises ``RuntimeError("PLA_SANITY_CHECK [op]: ...")`` before anything is launched.  The checks read device memory
-and are skipped while a stream is being captured.
+and are skipped while a stream is being captured.  A plan's entry that the free blocks do not suffice for is no mistake: its sequence
+length of 0 is the answer that a scheduler waits for.
 """
 
 import torch
@@ -15,13 +16,15 @@ def _capturing():
     return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
 
 
-def check_plan(blocks, context_lens, query_lens, request_indices):
+def check_plan(blocks, context_lens, query_lens, request_indices, token_capacity=None):
     if _capturing():
         return
     op, (rows, cols) = "paged_kv_plan", blocks.block_table.shape
     context, query = context_lens.tolist(), query_lens.tolist()
     if any(x < 0 for x in context + query):
         _fail(op, "lengths must not be negative")
+    if token_capacity is not None and sum(query) > token_capacity:
+        _fail(op, "the batch's token rows pass token_capacity")
     if any(-(-(c + q) // blocks.block_size) > cols for c, q in zip(context, query)):
         _fail(op, "a request's positions pass its row of the block table")
     if request_indices is not None:

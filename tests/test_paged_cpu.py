@@ -390,3 +390,15 @@ def test_a_request_of_more_units_than_32_bits_count_is_refused(HKV, D, positions
         assert 0 <= found <= 4096
         taken += sum(buf[7 * i + 4] for i in range(found))
     assert taken == units(fits)
+
+
+def test_sanity_mode_names_token_rows_that_pass_the_capacity(monkeypatch):
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32)
+    monkeypatch.setenv("PLA_SANITY_CHECK", "1")
+    for query, capacity in ((ints(4, 5), 8), (ints(0, 9), 8), (ints(1, 0), 0)):
+        with pytest.raises(RuntimeError, match=r"PLA_SANITY_CHECK \[paged_kv_plan\]: .*token rows pass token_capacity"):
+            paged_kv_plan(PagedKVBlocks.allocate(10, 16, 3, 4, "cpu"), ints(1, 2), query, token_capacity=capacity)
+    # a batch that fits goes on to the compiled checks, and so does one that asks for more blocks than are free
+    for context, query in ((ints(1, 2), ints(4, 4)), (ints(50, 50, 50), ints(4, 4, 0))):
+        with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+            paged_kv_plan(PagedKVBlocks.allocate(5, 16, 3, 4, "cpu"), context, query, token_capacity=8)
