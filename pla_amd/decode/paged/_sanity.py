@@ -16,8 +16,15 @@ def _capturing():
     return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
 
 
+def _formed(table, *vectors):
+    """Whether a call's tables and vectors have values to look at; what is not of its form the compiled layer refuses."""
+    return ((table is None or (table.dim() == 2 and not table.is_meta)) and
+            all(v is None or (v.dim() == 1 and v.dtype in (torch.int32, torch.int64) and not v.is_meta) for v in vectors))
+
+
 def check_plan(blocks, context_lens, query_lens, request_indices, token_capacity=None):
-    if _capturing():
+    if _capturing() or not _formed(blocks.block_table, blocks.held_blocks, blocks.free_blocks, blocks.free_count, context_lens, query_lens,
+                                   request_indices) or blocks.block_size < 1 or blocks.free_count.numel() != 1:
         return
     op, (rows, cols) = "paged_kv_plan", blocks.block_table.shape
     context, query = context_lens.tolist(), query_lens.tolist()
@@ -42,7 +49,7 @@ def check_plan(blocks, context_lens, query_lens, request_indices, token_capacity
 
 
 def check_slots(slot_mapping, k_cache):
-    if slot_mapping is None or k_cache is None or _capturing():
+    if slot_mapping is None or k_cache is None or _capturing() or not _formed(None, slot_mapping) or k_cache.dim() < 2:
         return
     slots = [x for x in slot_mapping.tolist() if x >= 0]
     if any(x >= k_cache.size(0) * k_cache.size(1) for x in slots):
@@ -52,7 +59,8 @@ def check_slots(slot_mapping, k_cache):
 
 
 def check_attention(q, k_cache, block_table, seq_lens, query_start_loc, request_indices, max_query_len):
-    if _capturing():
+    if (_capturing() or not _formed(block_table, seq_lens, query_start_loc, request_indices) or k_cache.dim() < 2 or q.dim() < 1 or
+            k_cache.size(1) < 1 or (query_start_loc is not None and query_start_loc.numel() != seq_lens.numel() + 1)):
         return
     op, (rows, cols) = "paged_attention_decode", block_table.shape
     blocks, block_size = k_cache.shape[:2]

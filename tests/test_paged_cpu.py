@@ -402,3 +402,22 @@ def test_sanity_mode_names_token_rows_that_pass_the_capacity(monkeypatch):
     for context, query in ((ints(1, 2), ints(4, 4)), (ints(50, 50, 50), ints(4, 4, 0))):
         with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
             paged_kv_plan(PagedKVBlocks.allocate(5, 16, 3, 4, "cpu"), context, query, token_capacity=8)
+
+
+@pytest.mark.parametrize("call, message", [
+    (lambda: paged_kv_plan(_blocks(block_size=0), torch.zeros(3, **_INTS), torch.zeros(3, **_INTS), token_capacity=8), "block_size must be positive"),
+    (lambda: paged_kv_plan(_blocks(free_count=torch.zeros(2, **_INTS)), torch.zeros(3, **_INTS), torch.zeros(3, **_INTS), token_capacity=8), "free_count must have 1"),
+    (lambda: paged_kv_plan(_blocks(block_table=torch.zeros(4, **_INTS)), torch.zeros(3, **_INTS), torch.zeros(3, **_INTS), token_capacity=8), "block_table must be int32"),
+    (lambda: paged_kv_plan(_blocks(), torch.zeros(3, 1, **_INTS), torch.zeros(3, **_INTS), token_capacity=8), "context_lens must be an int32"),
+    (lambda: paged_kv_plan(_blocks(), torch.zeros(3, **_INTS), torch.zeros(3, device="meta", **_INTS), token_capacity=8), "query_lens must be on the device"),
+    (lambda: fused_qk_norm_rope(**_rope_args(slot_mapping=torch.zeros(5, dtype=torch.int64, device="meta"))), "slot_mapping must be on the device of q"),
+    (lambda: fused_qk_norm_rope(**_rope_args(slot_mapping=torch.zeros(5, 1, dtype=torch.int64))), "slot_mapping must be an int32 or int64 vector"),
+    (lambda: paged_attention_decode(**_attention_args(seq_lens=torch.zeros(3))), "seq_lens must be an int32 or int64 vector"),
+    (lambda: paged_attention_decode(**_attention_args(query_start_loc=torch.zeros(0, **_INTS))), "query_start_loc must have 4 entries"),
+    (lambda: paged_attention_decode(**_attention_args(block_table=torch.zeros(3, 4, 1, **_INTS))), "block_table must be int32"),
+    (lambda: paged_attention_decode(**_attention_args(seq_lens=torch.zeros(3, device="meta", **_INTS))), "seq_lens must be on the device of q"),
+])
+def test_sanity_mode_leaves_what_is_not_of_its_form_to_the_compiled_checks(call, message, monkeypatch):
+    monkeypatch.setenv("PLA_SANITY_CHECK", "1")
+    with pytest.raises(RuntimeError, match=message):
+        call()
