@@ -131,7 +131,9 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, factor=1.0, original_length=
     def index_of(turns):                         # i whose frequency turns that often within the original length
         return rotary_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
     low, high = max(math.floor(index_of(beta_fast)), 0), min(math.ceil(index_of(beta_slow)), rotary_dim - 1)
-    ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    ramp = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
+    ramp[i >= index_of(beta_slow)] = 1           # also where that is below the first
     inv_freq = inv_freq * (1 - ramp) + inv_freq / factor * ramp
     return inv_freq.to(torch.float32).to(device), 0.1 * math.log(factor) + 1.0
 

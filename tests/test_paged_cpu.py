@@ -421,3 +421,14 @@ def test_sanity_mode_leaves_what_is_not_of_its_form_to_the_compiled_checks(call,
     monkeypatch.setenv("PLA_SANITY_CHECK", "1")
     with pytest.raises(RuntimeError, match=message):
         call()
+
+
+@pytest.mark.parametrize("original_length, beta_slow", [(1, 1.0), (6, 1.0), (25, 4.0), (7, 1.0), (4096, 1.0)])
+def test_frequencies_that_hardly_turn_within_the_original_length_are_divided(original_length, beta_slow):
+    """All that turn at most beta_slow times, also where that is every one of them."""
+    inv, _ = rotary_frequencies(64, 10000.0)
+    scaled, _ = rotary_frequencies(64, 10000.0, factor=4.0, original_length=original_length, beta_slow=beta_slow)
+    turns, ratio = inv.double() * original_length / (2 * math.pi), (scaled / inv).double()
+    few, many = turns <= beta_slow * (1 - 1e-6), turns >= 32.0 * (1 + 1e-6)
+    assert few.any() and torch.allclose(ratio[few], torch.full((1,), 0.25, dtype=torch.float64), atol=1e-6)
+    assert torch.allclose(ratio[many], torch.ones(1, dtype=torch.float64), atol=1e-6)
