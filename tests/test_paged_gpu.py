@@ -1019,3 +1019,37 @@ def test_an_infinite_value_counts_however_small_its_weight(D, act, HQ, HKV, sign
         before[:, :, 7] = 0
         assert before.isfinite().all()
         assert torch.equal(before[window:, :, 8:], clean[window:, :, 8:])
+
+
+# ---- plans of every size ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("capacity", [40, 300, 1024, 1025, 1500, 1920, 2048, 2049, 3000])
+@pytest.mark.parametrize("batch", [1, 40, 256, 257, 700, 1024, 1025, 2500, 4096, 4097, 8192, 9001])
+@pytest.mark.parametrize("mapped", [False, True])
+def test_plans_of_every_size(batch, capacity, mapped):
+    """Batches and token rows on both sides of each size from which a plan is made in another way (256 and 1024 entries, passes of 4096,
+    1024 and 2048 token rows).  Steps whose rows just fit, run out among the last entries and fall back, over a stack that runs out too."""
+    rng, bs = random.Random(batch * 4099 + capacity + mapped), 8
+    rows = min(8192, batch + 50) if mapped else batch + 3
+    longest = 2 * capacity // batch + 3
+    cols = -(-(longest + 24) // bs) + 1
+    pool, lists = _pool(2 + int(0.9 * batch * (8 + capacity / batch) / bs + 0.6 * batch), bs, rows, cols)
+    # more entries than rows that a mapping may name: the last ones name rows of earlier ones
+    index = rng.sample(range(rows), min(batch, rows)) + [rng.randrange(rows) for _ in range(batch - rows)] if mapped else None
+    context, refused = [rng.randint(0, 9) for _ in range(batch)], 0
+    for step, total in enumerate((capacity - 1, capacity + batch // 20 + 3, capacity)):
+        query = [0] * batch
+        for _ in range(total):
+            n = rng.randrange(batch)
+            query[n] = min(query[n] + 1, longest)
+        if step == 2:
+            query[-1] = 0
+            query[batch // 2] = -1                           # an entry in the middle that is none, rows of nobody at the end
+        used = index
+        if mapped and step == 1 and batch > 4:
+            used = list(index)
+            used[-1], used[-3] = used[0], rows
+        plan, lists = _check_plan(pool, lists, context, query, used, capacity)
+        refused += sum(s == 0 and c + q > 0 for s, c, q in zip(plan.seq_lens.tolist(), context, query))
+        context = [rng.choice((0, max(0, c - 3), min(cols * bs - longest, c + max(q, 0)))) for c, q in zip(context, query)]
+    assert refused > 0
