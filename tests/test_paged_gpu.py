@@ -1053,3 +1053,55 @@ def test_plans_of_every_size(batch, capacity, mapped):
         refused += sum(s == 0 and c + q > 0 for s, c, q in zip(plan.seq_lens.tolist(), context, query))
         context = [rng.choice((0, max(0, c - 3), min(cols * bs - longest, c + max(q, 0)))) for c, q in zip(context, query)]
     assert refused > 0
+
+
+# ---- rows of a prompt ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T, HQ, HKV, D, rot, interleaved, norm, act, stored", [
+    (7300, 24, 6, 128, 128, False, True, "bf16", True), (16500, 20, 4, 64, 32, True, True, "fp16", False), (3500, 20, 10, 256, 64, False, True, "bf16", True),
+    (2600, 40, 40, 128, 96, False, True, "fp16", True), (6100, 33, 1, 128, 128, True, False, "bf16", False), (4096, 16, 2, 256, 256, False, True, "fp16", True),
+    (9001, 9, 3, 128, 128, False, True, "bf16", True)])
+def test_norm_rotation_and_store_of_a_prompt(T, HQ, HKV, D, rot, interleaved, norm, act, stored):
+    """Wavefronts that have many steps of a token's heads, with weights, stored and unstored, at sizes whose rows stay in the caches and
+    at such whose do not.  Every row against 64 bits on the GPU."""
+    from pla.decode.paged import fused_qk_norm_rope
+    dtype = DTYPES[act]
+    g = torch.Generator(device=DEV).manual_seed(T)
+    row = torch.empty(T, (HQ + 2 * HKV) * D + 8, dtype=dtype, device=DEV).normal_(generator=g)
+    q, k, v = (row[:, a * D:b * D].view(T, b - a, D) for a, b in ((0, HQ), (HQ, HQ + HKV), (HQ + HKV, HQ + 2 * HKV)))
+    before = row.clone()
+    positions = torch.randint(0, 1 << 20, (T,), generator=g, device=DEV, dtype=torch.int32)
+    inv_freq = (10000.0 ** -(torch.arange(0, rot, 2).double() / rot)).float().to(DEV)
+    q_weight, k_weight = (torch.empty(D, dtype=dtype, device=DEV).normal_(0, 0.2, generator=g) if norm else None for _ in range(2))
+    bs, blocks = 16, -(-T // 16) + 3
+    caches = [torch.full((blocks, bs, HKV, D), 7.0, dtype=dtype, device=DEV) for _ in range(2)] if stored else None
+    slots = torch.randperm(blocks * bs, generator=g, device=DEV)[:T]
+    slots[T - 40:] = -1
+    store = dict(v=v, k_cache=caches[0], v_cache=caches[1], slot_mapping=slots) if stored else {}
+    k_out = torch.zeros(T, HKV, D, dtype=dtype, device=DEV)
+    q_out, _ = fused_qk_norm_rope(q, k, positions, q_weight=q_weight, k_weight=k_weight, weight_offset=1.0, inv_freq=inv_freq,
+                                  attention_factor=1.25, interleaved=interleaved, k_out=k_out, **store)
+    assert torch.equal(row, before)
+    angle = positions.double()[:, None, None] * inv_freq.double()
+    cos, sin = angle.cos() * 1.25, angle.sin() * 1.25
+    first = torch.arange(0, rot, 2, device=DEV) if interleaved else torch.arange(rot // 2, device=DEV)
+    second = first + (1 if interleaved else rot // 2)
+    info = torch.finfo(dtype)
+    for got, x, weight in ((q_out, q, q_weight), (k_out, k, k_weight)):
+        for part in range(0, T, 2000):
+            y = x[part:part + 2000].double()
+            if weight is not None:
+                y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + 1e-6) * (weight.double() + 1.0)
+            size = y.abs()
+            a, b, c, s = y[..., first], y[..., second], cos[part:part + 2000], sin[part:part + 2000]
+            y[..., first], y[..., second] = a * c - b * s, b * c + a * s
+            size[..., first] = size[..., second] = (a.abs() + b.abs()) * 1.25
+            slack = size * 2.0 ** -20                        # as in _rope_reference
+            bound = (y.abs() + slack) * (info.eps / 2) + slack + info.tiny * info.eps / 2
+            assert ((got[part:part + 2000].double() - y).abs() <= bound).all(), part
+    if stored:
+        flat, kept = [c.view(-1, HKV, D) for c in caches], slots >= 0
+        assert torch.equal(flat[0][slots[kept]], k_out[kept]) and torch.equal(flat[1][slots[kept]], v[kept])
+        rest = torch.ones(blocks * bs, dtype=torch.bool, device=DEV)
+        rest[slots[kept]] = False
+        assert (flat[0][rest] == 7).all() and (flat[1][rest] == 7).all()
