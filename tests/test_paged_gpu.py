@@ -1105,3 +1105,30 @@ def test_norm_rotation_and_store_of_a_prompt(T, HQ, HKV, D, rot, interleaved, no
         rest = torch.ones(blocks * bs, dtype=torch.bool, device=DEV)
         rest[slots[kept]] = False
         assert (flat[0][rest] == 7).all() and (flat[1][rest] == 7).all()
+
+
+# ---- wavefronts alone ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("places", [(4,), (13,), (4, 13), (1, 2, 14, 15)])
+@pytest.mark.parametrize("D, HKV, act", [(64, 8, "bf16"), (64, 8, "fp16"), (128, 4, "bf16"), (128, 4, "fp16"), (256, 4, "fp16")])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_values_set_aside_in_two_steps_of_every_form(places, D, HKV, act, value):
+    """As above for every head size and type: a wavefront has at least three groups of 32 keys of the long runs."""
+    lengths = [1000, 1064, 1032] + [2000 + 7 * i for i in range(37)]
+    windows = [16] * 3 + [1] * 37
+    cache = _Cache(lengths, HKV, D, 16, act, seed=73)
+    q = _randn(torch.Generator().manual_seed(74), sum(windows), HKV, D, dtype=DTYPES[act])
+    clean = _attend(cache, q, lengths, windows)
+    for n in range(3):
+        for place in places:
+            at = lengths[n] - 16 + place
+            cache.store[cache.table[n, at // 16].item(), 1, at % 16, :, 5] = value
+    got = _attend(cache, q, lengths, windows)
+    for n in range(3):
+        rows = got[16 * n:16 * n + 16, :, 5]
+        assert rows[:places[0]].isfinite().all()
+        assert rows[places[0]:].isnan().all() if math.isnan(value) else (rows[places[0]:] == value).all()
+        rows[places[0]:] = clean[16 * n + places[0]:16 * n + 16, :, 5]
+    assert torch.equal(got[48:], clean[48:])
+    ref, slack = _attention_reference_32(q[:48], cache, lengths[:3], windows[:3], D ** -0.5)
+    _close(got[:48], ref, slack, "set aside")
