@@ -1132,3 +1132,43 @@ def test_values_set_aside_in_two_steps_of_every_form(places, D, HKV, act, value)
     assert torch.equal(got[48:], clean[48:])
     ref, slack = _attention_reference_32(q[:48], cache, lengths[:3], windows[:3], D ** -0.5)
     _close(got[:48], ref, slack, "set aside")
+
+
+@pytest.mark.parametrize("D, HKV, batch, window", [(64, 2, 90, 1), (128, 4, 300, 1), (256, 1, 300, 4), (128, 2, 40, 8), (64, 1, 600, 2)])
+def test_calls_of_many_runs_side_by_side(D, HKV, batch, window):
+    """Two captured graphs and two streams over batches whose wavefronts have runs of their own (and one whose workgroups work together),
+    with fewer and with more runs than workgroups: none reads what another leaves."""
+    from pla.decode.paged import paged_attention_decode
+    bs, pages, cases = 16, 80, []
+    for seed in (1, 2):
+        g = torch.Generator().manual_seed(seed + D)
+        cache = _randn(g, 500, 2, bs, HKV, D, dtype=torch.bfloat16)
+        table = torch.randint(0, 500, (batch, pages), generator=g).to(torch.int32).to(DEV)
+        lengths = torch.randint(window, pages * bs + 1, (batch,), generator=g).to(torch.int32).to(DEV)
+        q = _randn(g, batch * window, 2 * HKV, D, dtype=torch.bfloat16)
+        offsets = torch.arange(0, batch * window + 1, window, dtype=torch.int32, device=DEV)
+        cases.append((q, cache[:, 0], cache[:, 1], table, lengths, offsets, torch.zeros_like(q)))
+
+    def call(q, k, v, table, lengths, offsets, out):
+        return paged_attention_decode(q, k, v, table, lengths, query_start_loc=offsets, max_query_len=window, out=out)
+    expects = [call(*case[:6], torch.empty_like(case[0])) for case in cases]
+    torch.cuda.synchronize()
+    graphs, streams = [], [torch.cuda.Stream() for _ in cases]
+    for case in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(*case)
+        graphs.append(graph)
+    for turn in range(6):
+        for case in cases:
+            case[-1].fill_(-1.0)
+        torch.cuda.synchronize()
+        for graph, stream, case in zip(graphs, streams, cases):
+            with torch.cuda.stream(stream):
+                if turn % 2:
+                    graph.replay()
+                else:
+                    call(*case)
+        torch.cuda.synchronize()
+        for case, expect in zip(cases, expects):
+            assert torch.equal(case[-1], expect), turn
