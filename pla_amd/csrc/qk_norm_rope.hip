@@ -6,9 +6,10 @@
 // for the pairs (i, i + rot/2) or (2i, 2i + 1) of the first `rot` channels; the other channels pass.  Queries go to q_out, keys
 // to k_out and / or the cache row of the token's slot, values to the cache as they are.  FP32 throughout, one rounding at the end.
 //
-// Angles: at position 10^6 a product in FP32 is off by 0.06 radians.  Position and frequency are multiplied in FP64, as
-// revolutions, and only the part below one revolution is narrowed, for v_sin_f32 and v_cos_f32, which take revolutions and are off by
-// at most 1.3e-7 between minus and plus a half (measured at 2^20 places).
+// Angles: at position 10^6 a product in FP32 is off by 0.06 radians, and at 2^40 one in FP64 by 0.001.  Position and frequency are
+// multiplied in two FP64 words, as revolutions, and only the part below one revolution is narrowed, for v_sin_f32 and v_cos_f32, which
+// take revolutions and are off by at most 1.3e-7 between minus and plus a half (measured at 2^20 places).  So an angle is as exact at
+// any position up to 2^53, which FP64 holds, as at the first.
 //
 // Bound by HBM, if the instructions stay out of its way: every row is read once and written once, 16 bytes a lane, D / 8 lanes a row.
 // A wavefront takes a step of 64 / (D / 8) heads of one kind (q, k or v) at a time, so pointers, strides and kind are scalars, and
@@ -81,6 +82,16 @@ __device__ __forceinline__ int64_t scalar_index(const void* base, int wide, int 
   return wide ? (int64_t)((uint64_t)(uint32_t)low | (uint64_t)(uint32_t)*(scalar_ptr)(p + 1) << 32) : (int64_t)low;
 }
 
+// position * frequency / (2 pi) without its whole revolutions: what the first word of each product leaves goes on in the second.
+__device__ __forceinline__ float part_of_turn(int64_t position, float frequency) {
+#pragma clang fp contract(off)
+  constexpr double INVERSE_TURN = 0x1.45f306dc9c883p-3, INVERSE_TURN_REST = -0x1.6b01ec5417056p-57;      // of 1 / (2 pi)
+  const double p = (double)position, f = (double)frequency;
+  const double rate = f * INVERSE_TURN, rate_rest = fma(f, INVERSE_TURN_REST, fma(f, INVERSE_TURN, -rate));
+  const double turns = p * rate, turns_rest = fma(p, rate_rest, fma(p, rate, -turns));
+  return (float)((turns - rint(turns)) + turns_rest);
+}
+
 // Bytes of rows from which on a call's rows go past the caches; below, whoever reads them next finds them there.
 constexpr int64_t PAST_CACHES = 48ll << 20;
 constexpr int WAVES_RESIDENT = 8192;  // on the chip, about
@@ -132,8 +143,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
   if (p.rot) {
 #pragma unroll
     for (int i = 0; i < FREQUENCIES; ++i) {
-      const double turns = (double)position * ((double)frequency[i] * 0.15915494309189533577);        // 1 / (2 pi)
-      const float part = (float)(turns - rint(turns));
+      const float part = part_of_turn(position, frequency[i]);
       if (here + 64 * i < p.rot / 2) {
         turn[wave][0][here + 64 * i] = __builtin_amdgcn_cosf(part) * p.attention_factor;
         turn[wave][1][here + 64 * i] = __builtin_amdgcn_sinf(part) * p.attention_factor;

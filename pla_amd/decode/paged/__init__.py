@@ -148,7 +148,7 @@ def fused_qk_norm_rope(q, k, positions=None, *, q_weight=None, k_weight=None, ep
     norm      x rsqrt(mean(x^2) + eps) (weight + weight_offset) where a weight [D] (of q's type or float32) is given.
     rotation  of the first ``2 * inv_freq.numel()`` channels (a multiple of 16) by positions [T] (int32 or int64) times inv_freq
               float32, cosine and sine times ``attention_factor``; pairs are (i, i + half) or, ``interleaved``, (2i, 2i + 1).
-              Angles are exact to float32 at any position.  No inv_freq: no rotation.
+              Angles are exact to float32 at any position up to 2^53.  No inv_freq: no rotation.
     store     with k_cache (and v, v_cache) [blocks, block_size, HKV, D] and slot_mapping [T] (int32 or int64), token t goes to
               slot ``block * block_size + place``; a slot that is negative or past the cache is nowhere.  No two tokens may
               name one slot.

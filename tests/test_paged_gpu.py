@@ -1172,3 +1172,38 @@ def test_calls_of_many_runs_side_by_side(D, HKV, batch, window):
         torch.cuda.synchronize()
         for case, expect in zip(cases, expects):
             assert torch.equal(case[-1], expect), turn
+
+
+# ---- far positions ------------------------------------------------------------------------------------------------
+
+def _exact_turns(positions, inv_freq):
+    """Cosine and sine of position * inv_freq with the product, and its part of a revolution, in 70 digits."""
+    from decimal import Decimal, getcontext
+    getcontext().prec = 70
+
+    def arctan_of_inverse(n):
+        term = total = Decimal(1) / n
+        k = 1
+        while abs(term) > Decimal(10) ** -68:
+            term, k = -term / (n * n), k + 2
+            total += term / k
+        return total
+    turn = 8 * (4 * arctan_of_inverse(5) - arctan_of_inverse(239))
+    rest = [[math.fmod(float(Decimal(p) * Decimal(f) % turn), 2 * math.pi) for f in inv_freq.tolist()] for p in positions]
+    rest = torch.tensor(rest, dtype=torch.float64)
+    return rest.cos(), rest.sin()
+
+
+@pytest.mark.parametrize("act", ["bf16", "fp16"])
+def test_angles_are_as_exact_at_far_positions_as_at_near_ones(act):
+    from pla.decode.paged import fused_qk_norm_rope
+    D = 128
+    far = [3, 2 ** 31 - 1, -2 ** 31, 2 ** 36 + 12345, -2 ** 40 - 1, 2 ** 45 + 7, 2 ** 50 - 3, 2 ** 52 + 1, -2 ** 53 + 1, 2 ** 53 - 1]
+    g, _, q, k, _, _ = _rope_case(6, len(far), 4, 2, D, act)
+    inv_freq = (1000000.0 ** -(torch.arange(0, D, 2).double() / D)).float().to(DEV)
+    q_out, k_out = fused_qk_norm_rope(q, k, torch.tensor(far, dtype=torch.int64, device=DEV), inv_freq=inv_freq)
+    cos, sin = (x[:, None, :] for x in _exact_turns(far, inv_freq))
+    for got, x in ((q_out, q), (k_out, k)):
+        a, b = x.double().cpu().split(D // 2, -1)
+        size = (a.abs() + b.abs()) * 2.0 ** -20              # as in _rope_reference
+        _close(got, torch.cat([a * cos - b * sin, b * cos + a * sin], -1), torch.cat([size, size], -1), "far")
