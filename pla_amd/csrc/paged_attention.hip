@@ -3,16 +3,17 @@
 //   o = sum_p softmax_p(scale q.k_p) v_p  [* sigmoid(gate)]      over the keys p that the token sees: p < length - window + j + 1
 //
 // for token j of a request's window.  The query heads of a key-value head and the tokens of the window are the rows of one
-// product, so keys and values are read once for all of them, in blocks of 16, 32 or (D 64 and 128) 64 rows: 16 windows of eight over
-// 8000 keys, 64 rows a head of 128, take 85.5 us as blocks of 32 and 72.5 as one of 64; 64 rows of 256 channels do not fit the registers.
+// product, in blocks of 16, 32 or (D 64 and 128) 64 rows; keys and values are read once for a block.  16 windows of eight over 8000
+// keys, 64 rows a head of 128, take 88.5 us as blocks of 32 and 79.8 as one of 64, windows of sixteen (two blocks) 129; 64 rows of 256
+// channels do not fit the registers.
 //
 // Each wavefront takes 32 keys at a time: keys and values go from memory to the registers in which the matrix instructions want them,
 // through no LDS.  The wavefronts of a workgroup work together, one 32 keys after the other's, and put their rows together at the
 // end of a run.  Or (ALONE; 16 rows, many runs) each has runs of its own, with the queries in registers, and writes what it has whole
 // from registers: nothing waits for another wavefront before the end of the kernel, where what they share is put together.  256
-// requests of 300 to 4000 keys (D 128, 8 heads) take 250 us together and 245 alone, 1000 of 50 keys 79.0 and 68.1 (D 64: 72.2
-// and 39.9), 64 of 200 to 4000 (D 256, 2 heads) 43.3 and 39.1.  Few runs, which wavefronts would have to share all the same, lose
-// by it (8 requests of 180 to 700 keys, 2 heads, 12.1 and 13.0), so they stay together.
+// requests of 300 to 4000 keys (D 128, 8 heads) take 251 us together and 245 alone, 1000 of 50 keys 82.6 and 67.3 (D 64: 74.7
+// and 40.1), 64 of 200 to 4000 (D 256, 2 heads) 43.2 and 38.8.  Few runs, which wavefronts would have to share all the same, lose
+// by it (one request of 60 000 keys, D 64, 2 heads, 20.1 and 22.0), so they stay together.
 //
 //   S^T = K Q^T    keys are the rows: lane (r, kb) loads 16 bytes of key r a step, any channels, as Q holds the same ones.
 //                  It gets the scores of query r at keys 4 kb .. 4 kb + 3 of both halves of the 32 keys,
@@ -28,8 +29,9 @@
 // cache may hold need not be.  Within a window some rows see values that others do not.  Where one of those is infinite or NaN,
 // these values (at most 31, of two steps) are set aside and added row by row at the end of the run, to the rows that see them.
 //
-// Bound by HBM: 4 D bytes a key and head are needed once, for 4 D flops a row: a few dozen rows take a twentieth of what the
-// matrix cores can do at 6 TB/s.
+// Bound by HBM: 4 D bytes a key and head are needed once, for 4 D flops a row and 2 D for the weights' second part.  32 rows at
+// 6 TB/s are 290 TFLOP/s of products, a quarter of what a large product reaches here; blocks of 64 rows, of which a SIMD has one
+// wavefront, wait for the products and the exponentials too.
 
 #include "decode_common.h"
 #include "mfma_bf16.h"
@@ -326,11 +328,12 @@ __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const Pag
   }
 }
 
-// (Measured with wavefronts together.)  Wavefronts a workgroup and workgroups a CU, so that 96 to 128 KiB of keys and values are in flight there.  More want more of the
-// memory system than it has: 50 requests of 8000 keys (D 128, 1.64 GB) take 264 us with two workgroups of four wavefronts, 290 with
-// three and 422 with four.  D 64: 37 windows of up to 9000 keys (10 heads, 104 MB) take 32.8 us as two workgroups of eight wavefronts and 36.2 as
-// four of four; 32 rows do not fit the registers of that (64 windows of eight over 1000 to 16 000 keys, 8 heads, 214 us), and take 171
-// as one workgroup of eight and 162 as three of four.  64 rows of 128 channels need 450 registers: one workgroup.
+// Wavefronts a workgroup and workgroups a CU, so that 96 to 128 KiB of keys and values are in flight there (64 with blocks of 64
+// rows).  More want more of the memory system than it has: 50 requests of 8000 keys (D 128, 1.64 GB) take 265 us with two workgroups of
+// four wavefronts, 285 with three and 447 with four (all working together; two working alone 262).  D 64: 37 windows of up to 9000 keys
+// (10 heads, 104 MB) take 31.2 us as two workgroups of eight wavefronts and 34.5 as four of four (together; alone 29.9); 32 rows do not
+// fit the registers of that (64 windows of eight over 1000 to 16 000 keys, 8 heads, 208 us), and take 147 as one workgroup of eight and
+// 150 as three of four.  64 rows of 128 channels need 450 registers: one workgroup.
 constexpr int waves(int D, int row_tiles) { return D == 64 && row_tiles == 1 ? 8 : 4; }
 constexpr int residency(int D, int row_tiles) {
   return D == 256 || (D == 128 && row_tiles == 4) ? 1 : D == 64 && row_tiles == 2 ? 3 : 2;
@@ -647,7 +650,8 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     }
     for (int step = 0; step < a.steps; ++step) {
       // The wavefronts of a CU's workgroups take turns: the older ones would always go first, end early and leave the others alone
-      // with half of the requests in flight (D 64, 64 windows over 4000 keys 123.7 -> 118.0 us, 50 requests of 8000 269.5 -> 266.3).
+      // with half of the requests in flight (D 64, 64 windows of four over 4000 keys 124.8 -> 121.2 us, of eight over 1000 to 16 000
+      // 167 -> 150).
       if ((step + (blockIdx.x >> 8)) & 1) __builtin_amdgcn_s_setprio(1);
       else __builtin_amdgcn_s_setprio(0);
       const bool more = step + 1 < a.steps;
@@ -734,7 +738,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
           left[kind][wave] = PieceOfRun{1, a.seg.tile + a.seg.tiles < a.req.tiles, (int)a.req.begin, a.index, a.seg.head, a.seg.block, a.rows, a.last};
       }
     } else {
-    // The four wavefronts' rows together.
+    // The wavefronts' rows together.
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const float sum = query_sum(w.sum[t]);
@@ -888,7 +892,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_join_kernel(const PagedAtten
 #pragma unroll
       for (int c = 0; c < LANE; ++c) gate[c] = p.gate[token * p.gate_token + head * p.gate_head + LANE * lane + c];
     }
-    // the wavefront's pieces: eight at a time, with a maximum and a sum that run along
+    // the wavefront's pieces, AHEAD at a time, with a maximum and a sum that run along
     float top = -INFINITY, sum = 0.f;
     lane_t o = {};
     for (int i = first; i < pieces; i += AHEAD * stride) {
@@ -972,11 +976,11 @@ static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query
   l.rows = 16 * l.row_tiles;
   l.row_blocks = (window_rows + l.rows - 1) / l.rows;
   l.runs = (int64_t)batch * HKV * l.row_blocks;
-  // Wavefronts alone from a run for every 32 of them on: D 128 with 64 runs 21.3 us together and 21.5 alone, with 32 19.2 and 20.5; D 64
-  // with 128 runs 22.4 and 21.9, with 64 16.5 and 18.2; D 256 with 32 runs 26.8 and 22.7, with 16 19.0 and 19.4.  But not where every
-  // run is one tile and gets a workgroup: then no run is cut, and no join runs (64 requests of one head, D 128, 12.9 and 8.1).
-  // A run counts a unit more than it has: without it 200 ragged windows (4 heads, D 64) take 56.4 us, with it 50.5, with two 48.6
-  // (but the 256 requests above 251 in place of 247).
+  // Wavefronts alone from a run for every 32 of them on: D 128 with 64 runs 21.8 us together and 21.1 alone, with 32 19.8 and 20.7; D 64
+  // with 128 runs 22.3 and 22.3, with 64 17.0 and 18.6; D 256 with 32 runs 26.6 and 22.6, with 16 18.9 and 19.0.  But not where every
+  // run is one tile and gets a workgroup: then no run is cut, and no join runs (64 requests of one head, D 128, up to 112 keys, 13.3 and 9.1).
+  // A run counts a unit more than it has: without it 200 ragged windows (4 heads, D 64) take 60.2 us, with it 53.0, with two 52.4
+  // (but the 256 requests above 249 in place of 245).
   const int64_t most = 256 * residency(D, l.row_tiles);
   const int waves_of = waves(D, l.row_tiles);
   l.alone = l.row_tiles == 1 && l.runs >= most * waves_of / 32 && !(positions <= 32 * waves_of && l.runs <= most);

@@ -10,19 +10,20 @@
 //             (0: unsound or refused, such an entry keeps its blocks), and for every token row its position and slot
 //             block * block_size + position % block_size (0 and -1 for rows of refused entries and behind the batch).
 //
-// Bound by latency: lengths and rows, held counts, then table and stack are dependent trips to memory, the two scans between them
-// run in one workgroup, up to four entries a thread.  Everything whose number depends on the values (blocks moved, token rows) is
-// dealt out flat: thread i finds its entry by bisection of the running sums in LDS, so that one long prompt costs no more than many
-// short ones.  Token rows take a new block's number from the stack and do not wait for the table; steps of many token rows leave
-// these to a second launch over the whole chip.
+// Bound by latency in small steps: lengths and rows, held counts, then table and stack are dependent trips to memory, the two scans
+// between them run in one workgroup, up to four entries a thread.  Large ones are bound by that workgroup's rate: it moves a thousand
+// blocks in 0.8 to 0.9 us, 4 of the 15 us of a plan of 1500 entries that returns or takes 4600.  Everything whose number depends on
+// the values (blocks moved, token rows) is dealt out flat: thread i finds its entry by bisection of the running sums in LDS, so that
+// one long prompt costs no more than many short ones.  Token rows take a new block's number from the stack and do not wait for the
+// table; steps of many token rows leave these to a second launch over the whole chip.
 
 #include "decode_common.h"
 
 namespace pla {
 
 // Token rows up to which the workgroup that makes the plan writes them as well: a step of 1000 requests takes 8.8 us on the device
-// with 2000 rows by one launch and 9.8 by two, with 4000 rows 10.9 and 9.8; one of 40 requests with 1920 rows 7.5 and 8.7, with 4000
-// rows 9.0 and 8.7.
+// with 2000 rows by one launch and 9.5 by two, with 4000 rows 10.9 and 9.4; one of 40 requests with 1920 rows 7.5 and 8.7, with 4000
+// rows 9.0 and 8.6.
 constexpr int PAGED_PLAN_INLINE_ROWS = 2048;
 constexpr int PAGED_PLAN_MAPPED_ROWS = 8192;      // rows whose first entry is looked up in LDS: 32 KB
 constexpr int32_t PAGED_SATURATED = INT32_MAX;    // of running sums: more than any capacity

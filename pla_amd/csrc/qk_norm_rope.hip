@@ -16,10 +16,10 @@
 // all of a token's steps in a large call: a lane works out an angle, the pairs go through LDS of the wavefront's own without a
 // barrier, and weight, cosine and sine become two factors a channel once for all rows of a kind.  The sum of squares is a few DPP
 // steps, the partner channels of the split layout sit in another lane of the row.  16 384 tokens of 32 + 8 heads (D 128, 336 MB) take
-// 63.5 us (5.3 TB/s; a large copy runs at 4.75), with norms 68, with norms and both caches (403 MB) 80; a workgroup a token, whose
+// 64 us (5.3 TB/s; a large copy runs at 4.75), with norms 65.5, with norms and both caches (403 MB) 78; a workgroup a token, whose
 // wavefronts each worked out the factors for two or three rows, took 65, 85 and 100.  Without the hint that rows go past the caches
-// 82, 82 and 96.
-// Small calls take a step a wavefront, for the shortest chain: 8 tokens 5.6 us a call, launch bound (kernel 4.6).
+// 84, 81 and 97.
+// Small calls take a step a wavefront, for the shortest chain: 8 tokens 5.8 us a call, launch bound (kernel 4.6).
 
 #include "decode_common.h"
 
@@ -92,7 +92,10 @@ __device__ __forceinline__ float part_of_turn(int64_t position, float frequency)
   return (float)((turns - rint(turns)) + turns_rest);
 }
 
-// Bytes of rows from which on a call's rows go past the caches; below, whoever reads them next finds them there.
+// Bytes of q and k from which on a call's rows go past the caches; below, whoever reads them next finds them there, which is not in
+// these figures.  Through the caches and past them, 32 + 8 heads of 128 channels (us, inputs that change): 1024 tokens 8.4 and 7.1,
+// 2048 12.7 and 12.3, 4096 (42 MB) 20.3 and 20.3, 6000 (61 MB) 35.0 and 27.6, 8192 52.5 and 38.1; with norms and both caches, whose
+// values and copies are not counted, 1024 10.6 and 9.3, 2048 16.4 and 15.6, 4096 29.2 and 23.9, 6000 44.4 and 35.7.
 constexpr int64_t PAST_CACHES = 48ll << 20;
 constexpr int WAVES_RESIDENT = 8192;  // on the chip, about
 

@@ -1,6 +1,6 @@
 """Paged softmax attention next to the linear-attention layers (``pla.decode.paged``).
 
-The models that the rest of this package serves put softmax-attention layers between their linear-attention layers.  Both see the
+Many of the models that the rest of this package serves put softmax-attention layers between their linear-attention layers.  Both see the
 same serving step: the same requests, windows of draft tokens and ``query_start_loc``.  This namespace holds what such a step
 needs besides the linear-attention operators; it has no counterpart in the reference.
 
@@ -52,7 +52,8 @@ def _sanity_enabled():
 class PagedKVBlocks:
     """Which blocks of a paged cache belong to which request: block_table [requests, blocks a request] int32, of whose rows the
     first held_blocks [requests] int32 entries count, and the other blocks as a stack, free_blocks [capacity] int32 of height
-    free_count [1] int32.  ``paged_kv_plan`` updates all four in place."""
+    free_count [1] int32, with places for all blocks (one that comes back to a full stack is nobody's from then on).
+    ``paged_kv_plan`` updates all four in place."""
     block_table: torch.Tensor
     held_blocks: torch.Tensor
     free_blocks: torch.Tensor
