@@ -91,23 +91,29 @@ Dims dims_of(const Tensor& t) {
   }
   return r;
 }
+// A step of a dimension leaves the smaller ones behind, or not.
+bool folds(const Dims& d, int64_t element) {
+  for (int i = 0; i < d.n; ++i)
+    if (d.d[i].stride < extent(d, i + 1, element)) return true;
+  return false;
+}
 bool may_overlap(const Tensor& a, const Tensor& b) {
   if (a.numel() == 0 || b.numel() == 0) return false;
   const auto base_a = reinterpret_cast<intptr_t>(a.data_ptr()), base_b = reinterpret_cast<intptr_t>(b.data_ptr());
   const int64_t ahead = base_b - base_a;
   if (a.is_contiguous() && ahead >= (int64_t)(a.numel() * a.element_size())) return false;        // the usual case, quickly
   if (b.is_contiguous() && -ahead >= (int64_t)(b.numel() * b.element_size())) return false;
-  return lap(dims_of(a), dims_of(b), 0, 0, ahead, a.element_size(), b.element_size());
+  const Dims x = dims_of(a), y = dims_of(b);
+  const int64_t ex = a.element_size(), ey = b.element_size();
+  // of rows that lie on each other there may be another one anywhere within a step: what counts is the whole extent
+  if (folds(x, ex) || folds(y, ey)) return ahead < extent(x, 0, ex) && -ahead < extent(y, 0, ey);
+  return lap(x, y, 0, 0, ahead, ex, ey);
 }
-// A step of a dimension leaves the smaller ones behind.
 bool overlaps_itself(const Tensor& t) {
   if (t.numel() == 0 || t.is_contiguous()) return false;
   for (int64_t i = 0; i < t.dim(); ++i)
     if (t.size(i) > 1 && t.stride(i) == 0) return true;
-  const Dims d = dims_of(t);
-  for (int i = 0; i < d.n; ++i)
-    if (d.d[i].stride < extent(d, i + 1, t.element_size())) return true;
-  return false;
+  return folds(dims_of(t), t.element_size());
 }
 bool same_rows(const Tensor& a, const Tensor& b) { return a.data_ptr() == b.data_ptr() && a.strides() == b.strides(); }
 void apart(std::initializer_list<std::pair<const char*, const OptTensor*>> written,

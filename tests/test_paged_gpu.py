@@ -1207,3 +1207,24 @@ def test_angles_are_as_exact_at_far_positions_as_at_near_ones(act):
         a, b = x.double().cpu().split(D // 2, -1)
         size = (a.abs() + b.abs()) * 2.0 ** -20              # as in _rope_reference
         _close(got, torch.cat([a * cos - b * sin, b * cos + a * sin], -1), torch.cat([size, size], -1), "far")
+
+
+# ---- shared memory ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens, token_stride, head_stride, ahead", [(5, 432, 248, -72), (4, 480, 408, 800), (2, 408, 296, 184), (2, 464, 280, 400)])
+def test_written_rows_among_rows_that_lie_on_each_other_are_refused(tokens, token_stride, head_stride, ahead):
+    """q's rows lie on each other, as it may be where they are only read; some place of k_out is one of q's."""
+    from pla.decode.paged import fused_qk_norm_rope
+    buffer = torch.zeros(8192, dtype=torch.bfloat16, device=DEV)
+    q = buffer.as_strided((tokens, 4, 64), (token_stride, head_stride, 1), 1024)
+    k_out = buffer.as_strided((tokens, 2, 64), (token_stride, head_stride, 1), 1024 + ahead)
+    place = lambda heads, start: {start + t * token_stride + h * head_stride + c for t in range(tokens) for h in range(heads) for c in range(64)}
+    assert place(4, 0) & place(2, ahead)
+    k = torch.zeros(tokens, 2, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="k_out must not share memory with q"):
+        fused_qk_norm_rope(q, k, k_out=k_out)
+    # read only, and beside it: what such rows hold is what their copy holds
+    apart = torch.zeros(tokens, 2, 64, dtype=torch.bfloat16, device=DEV)
+    buffer.normal_()
+    got, same = fused_qk_norm_rope(q, k, k_out=apart)
+    assert same.data_ptr() == apart.data_ptr() and torch.equal(got, q)
