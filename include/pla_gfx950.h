@@ -493,10 +493,10 @@ int pla_kda_prefill_halved_sequences(const int32_t* raw_cu_seqlens, int N, int T
  * batch has context[n] cached and query[n] new tokens and owns row mapping[n] (NULL: n) of block_table [table_rows, table_cols],
  * of which held_blocks[row] entries are in use.  Index vectors are dense int32 or int64 (is_int64 flags).
  *   Blocks held beyond ceil((context + query) / block_size) go back on the stack free_blocks[0 .. *free_count), in the order of
- *   the batch, then of the row (those that find it full, at free_capacity, are nobody's from then on); then missing ones come off it in that order.  An entry is granted if the running sum of what
- *   entries ask for, its own included, is on the stack (after the returns), and changes nothing if not.  Refused as well, and
- *   asking for nothing: negative lengths, query > token_capacity, positions beyond the row, rows outside the table, a row that an
- *   earlier entry names, token rows that end beyond token_capacity.
+ *   the batch, then of the row (those that find it full, at free_capacity, are nobody's from then on); then missing ones come off
+ *   it in that order.  An entry is granted if the running sum of what entries ask for, its own included, is on the stack (after
+ *   the returns), and changes nothing if not.  Refused as well, and asking for nothing: negative lengths, query > token_capacity,
+ *   positions beyond the row, rows outside the table, a row that an earlier entry names, token rows that end beyond token_capacity.
  *   offsets [batch + 1] running sum of the query lengths in 0 .. token_capacity (others count 0), at most token_capacity;
  *   seq_lens [batch] context + query, 0 if refused; positions and slots [token_capacity]: of token rows of granted entries, 0 and
  *   -1 of all others.  With a mapping at most 8192 table rows.  Outputs and the four tables share no memory with the inputs.
@@ -536,7 +536,8 @@ int64_t pla_paged_attention_workspace_bytes(int batch, int HQ, int HKV, int head
  *   offsets [batch + 1]: rows of request n's window, 1 .. max_query_len (at most 32) tokens (NULL: row n); a request whose
  *       window is empty, longer or outside [0, tokens) is passed over.  seq_lens [batch]: cached tokens, window included.
  *   token j of m sees positions below seq_len - m + j + 1 whose block is in the cache; a row that sees none is zeros.
- *   out = softmax(scale q k^T) v [* sigmoid(gate)], weights in two parts of act_dtype, all else float32, one rounding.  Calls that overlap in time need workspaces of their own.
+ *   out = softmax(scale q k^T) v [* sigmoid(gate)], weights in two parts of act_dtype, all else float32, one rounding.  Calls that
+ *   overlap in time need workspaces of their own.
  */
 int pla_paged_attention_launch(
     const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,

@@ -978,7 +978,8 @@ static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query
   l.runs = (int64_t)batch * HKV * l.row_blocks;
   // Wavefronts alone from a run for every 32 of them on: D 128 with 64 runs 21.8 us together and 21.1 alone, with 32 19.8 and 20.7; D 64
   // with 128 runs 22.3 and 22.3, with 64 17.0 and 18.6; D 256 with 32 runs 26.6 and 22.6, with 16 18.9 and 19.0.  But not where every
-  // run is one tile and gets a workgroup: then no run is cut, and no join runs (64 requests of one head, D 128, up to 112 keys, 13.3 and 9.1).
+  // run is one tile and gets a workgroup: then no run is cut, and no join runs (64 requests of one head, D 128, up to 112 keys, 13.3
+  // alone and 9.1).
   // A run counts a unit more than it has: without it 200 ragged windows (4 heads, D 64) take 60.2 us, with it 53.0, with two 52.4
   // (but the 256 requests above 249 in place of 245).
   const int64_t most = 256 * residency(D, l.row_tiles);
