@@ -1,0 +1,522 @@
+"""Prompts, quantised caches and shared prefixes for the softmax-attention layers between a model's linear-attention layers.
+
+Five operations, each timed as a serving program calls it:
+
+  prompt   causal attention of whole prompts, packed one after the other, over their own keys and values
+  chunk    the same for a part of a prompt whose earlier tokens stand in the paged cache
+  store8   norms, position rotation and the write of keys and values into a paged cache of 8-bit numbers with a scale a head
+  decode8  attention of one new token, or of a window of draft tokens, over such a cache
+  prefix   attention of new tokens over a prefix that all requests of the batch share, and over what each has of its own
+
+Prompt lengths, batch sizes, draft windows and heads lie in the ranges of the prefill and decode cases of this framework's
+linear-attention layers, with which these operators share their batches.  ``own`` chooses between the framework's entry points and
+a plain form of elementary torch operations.  Lengths follow from the case, everything else from the seed.
+"""
+import math
+import random
+from types import SimpleNamespace
+
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+E4M3 = torch.float8_e4m3fn
+LARGEST = 448.0                                              # of e4m3
+LEAST = 1e-30                                                # magnitude that a head's scale starts from
+EPS = 1e-6
+
+
+# ---- cases ------------------------------------------------------------------------------------------------------
+
+def listed():
+    return [
+        # first messages of a few chats: launch and latency count
+        dict(name="prompt_chats_b5", op="prompt", batch=5, lo=12, hi=150, ctx=0, HQ=16, HKV=2, D=128, gate=False, act="bf16"),
+        # prompts of eight users of very different lengths, about 32 000 tokens
+        dict(name="prompt_ragged_b8", op="prompt", batch=8, lo=512, hi=8192, ctx=0, HQ=32, HKV=8, D=128, gate=False, act="bf16"),
+        # one long document
+        dict(name="prompt_long_t32768", op="prompt", batch=1, lo=32768, hi=32768, ctx=0, HQ=16, HKV=2, D=128, gate=False, act="bf16"),
+        # large heads with an output gate, two documents of odd lengths
+        dict(name="prompt_gated_b2", op="prompt", batch=2, lo=4001, hi=9001, ctx=0, HQ=16, HKV=2, D=256, gate=True, act="bf16"),
+        # a part of a long prompt: 1500 new tokens over 60 000 that are cached
+        dict(name="chunk_context_b1", op="chunk", batch=1, lo=1500, hi=1500, ctx=60000, HQ=32, HKV=8, D=128, block=16, gate=False, act="bf16"),
+        # a step that takes in parts of many prompts: small heads without sharing
+        dict(name="chunk_mixed_b18", op="chunk", batch=18, lo=33, hi=700, ctx=9000, HQ=10, HKV=10, D=64, block=64, gate=False, act="fp16"),
+        # a few concurrent chats: launch and latency count
+        dict(name="store8_decode_b8", op="store8", tokens=8, HQ=16, HKV=2, D=128, rot=128, interleaved=False, norm=True, block=16, act="bf16"),
+        # a prompt's tokens
+        dict(name="store8_prefill_t8192", op="store8", tokens=8192, HQ=32, HKV=8, D=128, rot=128, interleaved=False, norm=True, block=64, act="bf16"),
+        # the ordinary decode step of a full batch
+        dict(name="decode8_b256", op="decode8", batch=256, lo=300, hi=4000, window=1, ragged=False, HQ=32, HKV=8, D=128, block=64, gate=False, act="bf16"),
+        # verify of draft windows of up to four tokens, large gated heads
+        dict(name="decode8_verify_b40", op="decode8", batch=40, lo=500, hi=30000, window=4, ragged=True, HQ=16, HKV=2, D=256, block=16, gate=True, act="bf16"),
+        # chats under one instruction text
+        dict(name="prefix_chats_b64", op="prefix", batch=64, lo=40, hi=1500, prefix=8000, window=1, ragged=False, HQ=32, HKV=8, D=128, block=16, gate=False, act="bf16"),
+        # verify of draft windows of requests about one document whose end lies inside a block
+        dict(name="prefix_verify_b100", op="prefix", batch=100, lo=8, hi=900, prefix=30011, window=4, ragged=True, HQ=16, HKV=2, D=128, block=64, gate=True, act="bf16"),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 0.5)))))))
+
+
+HEADS = ((8, 1), (8, 8), (16, 2), (10, 10), (16, 16), (32, 4), (32, 8), (28, 4), (5, 5), (15, 3))
+PRODUCTS = 32768 * 32769 // 2 * 16 * 128                     # of the long document, one of its two matrix products
+
+
+def draw(rng):
+    op = rng.choice(("prompt", "prompt", "chunk", "store8", "decode8", "prefix"))
+    act = rng.choice(("bf16", "bf16", "fp16"))
+    block = rng.choice((16, 16, 32, 64, 80, 528))
+    HQ, HKV = rng.choice(HEADS)
+    D = rng.choice((64, 128, 128, 256))
+    if op in ("prompt", "chunk"):
+        # up to half of what the long document takes
+        ctx = 0 if op == "prompt" and rng.random() < 0.7 else _log_int(rng, 1, 60000)
+        per = PRODUCTS // 2 // (HQ * D)
+        most = min(32768, int(math.sqrt(ctx * ctx + 2 * per)) - ctx)              # tokens of one request
+        hi = _log_int(rng, 1, max(1, most))
+        batch = _log_int(rng, 1, max(1, min(64, per // (hi * (ctx + (hi + 1) // 2)), 400000 // (hi + ctx))))
+        c = dict(op=op, batch=batch, lo=_log_int(rng, 1, hi), hi=hi, ctx=ctx, HQ=HQ, HKV=HKV, D=D, gate=rng.random() < 0.3, act=act)
+        return c if op == "prompt" else dict(c, block=block)
+    if op == "store8":
+        rot = rng.choice((0, D, D, D // 2, D // 4))
+        return dict(op=op, tokens=_log_int(rng, 1, 8192 * 32 * 128 // (HQ * D)), HQ=HQ, HKV=HKV, D=D, rot=rot, interleaved=rng.random() < 0.5,
+                    norm=rot == 0 or rng.random() < 0.7, block=block, act=act)
+    window = rng.choice((1, 1, 1, 2, 4, 8, 17, 32))
+    if op == "decode8":
+        keys = min(256 * 1400 * 8 * 128 // (HKV * D), 40 * 8000 * 4 * 32 * 256 // (window * HQ * D))
+        lo = _log_int(rng, 1, min(4000, keys))
+        hi = _log_int(rng, lo, min(60000, keys))
+        return dict(op=op, batch=_log_int(rng, 1, max(1, min(300, keys // hi))), lo=lo, hi=hi, window=window, ragged=window > 1 and rng.random() < 0.5,
+                    HQ=HQ, HKV=HKV, D=D, block=block, gate=rng.random() < 0.4, act=act)
+    prefix = _log_int(rng, 1, 60000)
+    batch = _log_int(rng, 1, max(1, min(200, 800 // window, 400 * 30000 * 16 // (window * prefix * HQ))))
+    lo = _log_int(rng, 1, 400)
+    return dict(op=op, batch=batch, lo=lo, hi=_log_int(rng, lo, 3000), prefix=prefix, window=window, ragged=window > 1 and rng.random() < 0.5,
+                HQ=HQ, HKV=HKV, D=D, block=block, gate=rng.random() < 0.4, act=act)
+
+
+def _spread(rng, n, lo, hi):
+    """n lengths between lo and hi, even over their logarithm."""
+    return [min(hi, max(lo, int(math.exp(rng.uniform(math.log(lo + 1), math.log(hi + 1))) - 0.5))) for _ in range(n)]
+
+
+def _case_rng(c):
+    return random.Random(str(sorted((k, v) for k, v in c.items() if k != "name")))
+
+
+def _prompt_lengths(c):
+    """(all keys, new tokens) of every request; of a context of up to ctx tokens every request has another part."""
+    rng = _case_rng(c)
+    new = _spread(rng, c["batch"], c["lo"], c["hi"])
+    if not c["ctx"]:
+        return [(m, m) for m in new]
+    before = [c["ctx"]] if c["batch"] == 1 else [rng.randint(0, c["ctx"]) for _ in new]
+    return [(a + m, m) for a, m in zip(before, new)]
+
+
+def _window_lengths(c):
+    """(cached tokens with the window, window) of every request; one of a larger batch has nothing cached."""
+    rng = _case_rng(c)
+    out = []
+    for n, length in enumerate(_spread(rng, c["batch"], c["lo"], c["hi"])):
+        window = rng.randint(0 if n else 1, c["window"]) if c["ragged"] else c["window"]
+        out.append((max(length, window) if n != 6 or not c["ragged"] else 0, window))
+    return out
+
+
+# ---- inputs -----------------------------------------------------------------------------------------------------
+
+class _Draw:
+    """Seeded draws on the GPU."""
+
+    def __init__(self, seed):
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self.g = torch.Generator(device=self.device).manual_seed(seed)
+
+    def normal(self, *shape, dtype=torch.float32, scale=1.0):
+        return torch.empty(*shape, dtype=dtype, device=self.device).normal_(0.0, scale, generator=self.g)
+
+    def permutation(self, n):
+        return torch.randperm(n, generator=self.g, device=self.device).to(torch.int32)
+
+    def ints(self, values):
+        return torch.tensor(values, dtype=torch.int32, device=self.device)
+
+
+def _offsets(counts):
+    out = [0]
+    for n in counts:
+        out.append(out[-1] + n)
+    return out
+
+
+def _pages(r, pages):
+    """A block table of a long-running service, its blocks in no order, block 0 kept aside, and the blocks of its cache."""
+    cols, total = max(pages) + 1, sum(pages) + 1
+    order, count = 1 + r.permutation(total), r.ints(pages)
+    start, grid = count.cumsum(0) - count, torch.arange(cols, device=r.device)[None, :]
+    return torch.where(grid < count[:, None], order[(start[:, None] + grid).clamp(max=total - 1)], 0).to(torch.int32), total + 1
+
+
+def _prepare_prompt(c, r):
+    lengths = _prompt_lengths(c)
+    HQ, HKV, D, act = c["HQ"], c["HKV"], c["D"], DTYPES[c["act"]]
+    tokens, keys = sum(m for _, m in lengths), sum(a for a, _ in lengths)
+    s = SimpleNamespace(case=c, lengths=lengths, scale=D ** -0.5, offsets=r.ints(_offsets(m for _, m in lengths)), k=None, k_cache=None)
+    # queries that look at some keys more than at others
+    s.q = r.normal(tokens, HQ, D, dtype=act, scale=1.5)
+    if c["op"] == "prompt":
+        # keys and values lie in one row, as a projection leaves them
+        both = r.normal(keys, 2 * HKV, D, dtype=act)
+        s.k, s.v = both[:, :HKV], both[:, HKV:]
+        s.key_offsets = r.ints(_offsets(a for a, _ in lengths)) if c["ctx"] else None
+    else:
+        s.table, blocks = _pages(r, [-(-a // c["block"]) for a, _ in lengths])
+        cache = r.normal(blocks, 2, c["block"], HKV, D, dtype=act)
+        s.k_cache, s.v_cache = cache[:, 0], cache[:, 1]
+        s.seq_lens = r.ints([a for a, _ in lengths])
+    s.gate = r.normal(tokens, HQ, D, dtype=act) if c["gate"] else None
+    s.out = torch.zeros(tokens, HQ, D, dtype=act, device=r.device)
+    return s
+
+
+def _prepare_store8(c, r):
+    T, HQ, HKV, D, act = c["tokens"], c["HQ"], c["HKV"], c["D"], DTYPES[c["act"]]
+    blocks = -(-T // c["block"]) + 3
+    # one projection row: q, k, v
+    row = r.normal(T, (HQ + 2 * HKV) * D, dtype=act)
+    s = SimpleNamespace(case=c, q=row[:, :HQ * D].view(T, HQ, D), k=row[:, HQ * D:(HQ + HKV) * D].view(T, HKV, D),
+                        v=row[:, (HQ + HKV) * D:].view(T, HKV, D), q_weight=None, k_weight=None, positions=None, inv_freq=None, factor=1.0)
+    if c["norm"]:
+        s.q_weight, s.k_weight = r.normal(D, dtype=act, scale=0.1), r.normal(D, dtype=act, scale=0.1)     # about an offset of one
+    if c["rot"]:
+        s.positions = torch.randint(0, 1 << 20, (T,), generator=r.g, device=r.device, dtype=torch.int32)
+        exponent = torch.arange(0, c["rot"], 2, device=r.device, dtype=torch.float64) / c["rot"]
+        s.inv_freq, s.factor = (1e6 ** -exponent).to(torch.float32), 1.125
+    s.k_cache, s.v_cache = (torch.zeros(blocks, c["block"], HKV, D, device=r.device).to(E4M3) for _ in range(2))
+    s.k_scales, s.v_scales = (torch.zeros(blocks, HKV, c["block"], device=r.device) for _ in range(2))
+    s.slots = torch.randperm(blocks * c["block"], generator=r.g, device=r.device)[:T].contiguous()
+    s.slots[T - T // 16:] = -1                               # padding of a captured step
+    s.q_out = torch.zeros(T, HQ, D, dtype=act, device=r.device)
+    return s
+
+
+def _prepare_windows(c, r):
+    lengths = _window_lengths(c)
+    HQ, HKV, D, bs, act = c["HQ"], c["HKV"], c["D"], c["block"], DTYPES[c["act"]]
+    pages = [-(-a // bs) for a, _ in lengths]
+    shared = -(-c["prefix"] // bs) if c["op"] == "prefix" else 0
+    table, blocks = _pages(r, pages + [shared])
+    tokens = sum(w for _, w in lengths)
+    s = SimpleNamespace(case=c, table=table[:-1], seq_lens=r.ints([a for a, _ in lengths]), scale=D ** -0.5, k_scales=None, v_scales=None,
+                        offsets=None if c["window"] == 1 else r.ints(_offsets(w for _, w in lengths)), prefix_blocks=None, prefix_len=None)
+    if c["op"] == "prefix":
+        s.prefix_blocks, s.prefix_len = table[-1, :shared].contiguous(), r.ints([c["prefix"]])
+        cache = r.normal(blocks, 2, bs, HKV, D, dtype=act)
+        s.k_cache, s.v_cache = cache[:, 0], cache[:, 1]
+    else:
+        # heads whose largest magnitude is 4 deviations or less; scales differ from key to key
+        s.k_cache, s.v_cache = (r.normal(blocks, bs, HKV, D, dtype=act, scale=112.0).clamp_(-LARGEST, LARGEST).to(E4M3) for _ in range(2))
+        s.k_scales, s.v_scales = (torch.empty(blocks, HKV, bs, device=r.device).uniform_(0.006, 0.012, generator=r.g) for _ in range(2))
+    s.q = r.normal(tokens, HQ, D, dtype=act, scale=1.5)
+    s.gate = r.normal(tokens, HQ, D, dtype=act) if c["gate"] else None
+    s.out = torch.zeros(tokens, HQ, D, dtype=act, device=r.device)
+    return s
+
+
+def prepare(case, seed):
+    r = _Draw(seed)
+    return {"prompt": _prepare_prompt, "chunk": _prepare_prompt, "store8": _prepare_store8}.get(case["op"], _prepare_windows)(case, r)
+
+
+# ---- one pass ---------------------------------------------------------------------------------------------------
+
+def _plain_prompt(s):
+    c = s.case
+    HKV, D = c["HKV"], c["D"]
+    G = c["HQ"] // HKV
+    token = key = 0
+    for n, (length, new) in enumerate(s.lengths):
+        if s.k_cache is None:
+            k, v = s.k[key:key + length], s.v[key:key + length]
+        else:
+            pages = s.table[n, :-(-length // c["block"])].long()
+            k, v = (x[pages].flatten(0, 1)[:length] for x in (s.k_cache, s.v_cache))
+        k, v = k.permute(1, 2, 0).float().contiguous(), v.transpose(0, 1).float().contiguous()     # [HKV, D, length], [HKV, length, D]
+        # as many rows at a time as have 2 GB of scores
+        rows = max(1, int(5e8 / (length * c["HQ"])))
+        for j in range(0, new, rows):
+            m = min(rows, new - j)
+            sees = length - new + j + m                      # keys that the last of these tokens sees
+            at = slice(token + j, token + j + m)
+            q = s.q[at].float().view(m, HKV, G, D).permute(1, 0, 2, 3).reshape(HKV, m * G, D)
+            score = torch.matmul(q, k[:, :, :sees].contiguous()).view(HKV, m, G, sees).mul_(s.scale)
+            behind = torch.arange(sees, device=q.device)[None, :] > torch.arange(sees - m, sees, device=q.device)[:, None]
+            score.masked_fill_(behind[None, :, None, :], -math.inf)
+            weight = score.sub_(score.amax(-1, keepdim=True)).exp_()
+            o = torch.matmul(weight.view(HKV, m * G, sees), v[:, :sees]).view(HKV, m, G, D) / weight.sum(-1, keepdim=True)
+            o = o.permute(1, 0, 2, 3).reshape(m, c["HQ"], D)
+            s.out[at] = (o if s.gate is None else o / (1.0 + torch.exp(-s.gate[at].float()))).to(s.q.dtype)
+        token, key = token + new, key + length
+    return s.out
+
+
+def _run_prompt(s):
+    if not own:
+        return _plain_prompt(s)
+    if s.case["op"] == "prompt":
+        from pla_amd.prefill.attention import packed_attention_fwd
+        return packed_attention_fwd(s.q, s.k, s.v, s.offsets, cu_seqlens_k=s.key_offsets, scale=s.scale, output_gate=s.gate, out=s.out)
+    from pla_amd.decode.paged import paged_attention_prefill
+    return paged_attention_prefill(s.q, s.k_cache, s.v_cache, s.table, s.seq_lens, s.offsets, scale=s.scale, output_gate=s.gate, out=s.out)
+
+
+def _plain_heads(s, x, weight):
+    """Norm and rotation of one tensor of heads, in 32 bits; angles in 64."""
+    c = s.case
+    y = x.float()
+    if weight is not None:
+        y = y * torch.rsqrt((y * y).mean(-1, keepdim=True) + EPS) * (weight.float() + 1.0)
+    if c["rot"]:
+        angle = s.positions.double()[:, None] * s.inv_freq.double()[None, :]
+        cos, sin = ((f(angle) * s.factor).float()[:, None, :] for f in (torch.cos, torch.sin))
+        turned, rest = y[..., :c["rot"]], y[..., c["rot"]:]
+        if c["interleaved"]:
+            a, b = turned[..., 0::2], turned[..., 1::2]
+            turned = torch.stack([a * cos - b * sin, b * cos + a * sin], dim=-1).flatten(-2)
+        else:
+            a, b = turned[..., :c["rot"] // 2], turned[..., c["rot"] // 2:]
+            turned = torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+        y = torch.cat([turned, rest], dim=-1)
+    return y
+
+
+def _run_store8(s):
+    c = s.case
+    if own:
+        from pla_amd.decode.paged import fused_qk_norm_rope
+        fused_qk_norm_rope(s.q, s.k, s.positions, q_weight=s.q_weight, k_weight=s.k_weight, eps=EPS, weight_offset=1.0,
+                           inv_freq=s.inv_freq, attention_factor=s.factor, interleaved=c["interleaved"], q_out=s.q_out,
+                           v=s.v, k_cache=s.k_cache, v_cache=s.v_cache, slot_mapping=s.slots, k_scales=s.k_scales, v_scales=s.v_scales)
+    else:
+        s.q_out.copy_(_plain_heads(s, s.q, s.q_weight))
+        kept, at = s.slots >= 0, s.slots.clamp(min=0)
+        at = torch.where(kept, at, at[0])                    # rows of padding write back what stands at the first stored slot
+        block, place = at // c["block"], at % c["block"]
+        for cache, scales, x in ((s.k_cache, s.k_scales, _plain_heads(s, s.k, s.k_weight)), (s.v_cache, s.v_scales, s.v.float())):
+            scale = x.abs().amax(-1).clamp(min=LEAST) / LARGEST
+            code = (x / scale[..., None]).to(E4M3).view(torch.uint8)
+            cache.view(torch.uint8)[block, place] = torch.where(kept[:, None, None], code, code[0])
+            scales[block, :, place] = torch.where(kept[:, None], scale, scale[0])
+    return s.q_out, s.k_cache, s.v_cache, s.k_scales, s.v_scales
+
+
+def _plain_windows(s):
+    c = s.case
+    HQ, HKV, D, bs, W = c["HQ"], c["HKV"], c["D"], c["block"], c["window"]
+    G = HQ // HKV
+    N, cols = s.table.shape
+    out = torch.zeros_like(s.q)
+    P = 0
+    if s.prefix_len is not None:
+        P = c["prefix"]
+        pages = s.prefix_blocks.long()
+        prefix_k = s.k_cache[pages].flatten(0, 1)[:P].permute(1, 2, 0).float().contiguous()
+        prefix_v = s.v_cache[pages].flatten(0, 1)[:P].transpose(0, 1).float().contiguous()
+    # as many requests at a time as fit 2 GB of widened keys, or of scores
+    group = max(1, int(5e8 / max(cols * bs * HKV * max(D, W * G), W * HQ * P)))
+    for n0 in range(0, N, group):
+        pages = s.table[n0:n0 + group].long()
+        n, L = pages.size(0), cols * bs
+        if s.k_scales is None:
+            k, v = s.k_cache[pages].float(), s.v_cache[pages].float()
+        else:
+            k, v = (x.view(torch.uint8)[pages].view(E4M3).float() * y[pages].transpose(2, 3)[..., None]
+                    for x, y in ((s.k_cache, s.k_scales), (s.v_cache, s.v_scales)))
+        k = k.view(n, L, HKV, D).permute(0, 2, 3, 1).contiguous()
+        v = v.view(n, L, HKV, D).permute(0, 2, 1, 3).contiguous()
+        length = s.seq_lens[n0:n0 + n].long()
+        if s.offsets is None:
+            begin = torch.arange(n0, n0 + n, device=k.device)
+            count = torch.ones_like(begin)
+        else:
+            begin, end = s.offsets[n0:n0 + n].long(), s.offsets[n0 + 1:n0 + n + 1].long()
+            count = end - begin
+        j = torch.arange(W, device=k.device)
+        real = j[None, :] < count[:, None]                                        # [n, W]
+        at = (begin[:, None] + j[None, :]).clamp(max=s.q.size(0) - 1)
+        q = s.q[at].float().view(n, W, HKV, G, D).permute(0, 2, 1, 3, 4).reshape(n, HKV, W * G, D)
+        score = torch.matmul(q, k) * s.scale                                      # [n, HKV, W G, L]
+        limit = (length[:, None] - count[:, None] + j[None, :] + 1)               # keys of its own that a token sees
+        seen = torch.arange(L, device=k.device)[None, None, :] < limit[:, :, None]
+        seen = seen.repeat_interleave(G, dim=1)[:, None]
+        score = torch.where(seen, score, -math.inf)
+        top = score.amax(-1, keepdim=True)
+        if P:
+            # all requests' rows over the same keys
+            rows = q.transpose(0, 1).reshape(HKV, n * W * G, D)
+            before = (torch.matmul(rows, prefix_k) * s.scale).view(HKV, n, W * G, P).transpose(0, 1)
+            before_top = before.amax(-1, keepdim=True)
+            top = torch.where(top == -math.inf, top, torch.maximum(top, before_top))              # a row without a token of its own is none
+        zero = torch.where(top == -math.inf, 0.0, top)
+        weight = torch.where(seen, torch.exp(score - zero), 0.0)
+        total = weight.sum(-1, keepdim=True)
+        # what stands behind a request's end, or in the pages of another, has no weight and must not count
+        v = torch.where((torch.arange(L, device=k.device)[None, :] < length[:, None])[:, None, :, None], v, 0.0)
+        o = torch.matmul(weight, v)
+        if P:
+            weight = torch.where(top == -math.inf, 0.0, torch.exp(before - zero))
+            total = total + weight.sum(-1, keepdim=True)
+            weight = weight.transpose(0, 1).reshape(HKV, n * W * G, P)
+            o = o + torch.matmul(weight, prefix_v).view(HKV, n, W * G, D).transpose(0, 1)
+        o = o / torch.where(total == 0, 1.0, total)
+        o = o.view(n, HKV, W, G, D).permute(0, 2, 1, 3, 4).reshape(n, W, HQ, D)
+        if s.gate is not None:
+            o = o / (1.0 + torch.exp(-s.gate[at].float()))
+        out.index_put_((torch.where(real, at, begin[:, None].clamp(max=s.q.size(0) - 1)),),
+                       torch.where(real[:, :, None, None], o.to(s.q.dtype), 0.0).to(s.q.dtype), accumulate=True)
+    s.out.copy_(out)
+    return s.out
+
+
+def _run_windows(s):
+    if not own:
+        return _plain_windows(s)
+    from pla_amd.decode.paged import paged_attention_decode
+    if s.case["op"] == "decode8":
+        return paged_attention_decode(s.q, s.k_cache, s.v_cache, s.table, s.seq_lens, query_start_loc=s.offsets, max_query_len=s.case["window"],
+                                      scale=s.scale, output_gate=s.gate, out=s.out, k_scales=s.k_scales, v_scales=s.v_scales)
+    return paged_attention_decode(s.q, s.k_cache, s.v_cache, s.table, s.seq_lens, query_start_loc=s.offsets, max_query_len=s.case["window"],
+                                  scale=s.scale, output_gate=s.gate, out=s.out, prefix_blocks=s.prefix_blocks, prefix_len=s.prefix_len)
+
+
+def run(state):
+    return {"prompt": _run_prompt, "chunk": _run_prompt, "store8": _run_store8}.get(state.case["op"], _run_windows)(state)
+
+
+# ---- what a pass cannot do without ------------------------------------------------------------------------------
+
+def work(case):
+    c = case
+    heads = c["HQ"] * c["D"]
+    if c["op"] == "store8":
+        T, stored = c["tokens"], c["tokens"] - c["tokens"] // 16
+        # q there and back; k and v in 16 bits, back in 8 with a scale; position and slot
+        return {"bytes": 4 * T * heads + stored * c["HKV"] * (6 * c["D"] + 8) + T * ((4 if c["rot"] else 0) + 8),
+                "flops": T * (c["HQ"] + c["HKV"]) * c["D"] * (3 * bool(c["rot"]) + 4 * c["norm"]) + 4 * stored * c["HKV"] * c["D"]}
+    if c["op"] in ("prompt", "chunk"):
+        lengths = _prompt_lengths(c)
+        keys, tokens = sum(a for a, _ in lengths), sum(m for _, m in lengths)
+        pairs = sum(m * (a - m) + m * (m + 1) // 2 for a, m in lengths)
+        pages = sum(-(-a // c["block"]) for a, _ in lengths) if c["op"] == "chunk" else 0
+        return {"bytes": keys * c["HKV"] * c["D"] * 4 + tokens * heads * (6 if c["gate"] else 4) + 4 * pages + 8 * len(lengths), "flops": 4 * pairs * heads}
+    lengths = _window_lengths(c)
+    keys, tokens = sum(a for a, w in lengths if w), sum(w for _, w in lengths)
+    pairs = sum(max(0, a - w + j + 1) for a, w in lengths for j in range(w))
+    small = 4 * (keys // c["block"] + len(lengths)) + tokens * heads * (6 if c["gate"] else 4)
+    if c["op"] == "decode8":
+        return {"bytes": keys * c["HKV"] * (2 * c["D"] + 8) + small, "flops": 4 * pairs * heads}
+    rows = sum(w for a, w in lengths if a)
+    return {"bytes": (keys + c["prefix"]) * c["HKV"] * c["D"] * 4 + small, "flops": 4 * (pairs + rows * c["prefix"]) * heads}
+
+
+# ---- the definition in 64 bits ----------------------------------------------------------------------------------
+
+def _exact_rows(q, k, v, sees, scale):
+    """q [m, G, D] over k, v [n, D] in 64 bits; token j sees the first sees + j keys."""
+    m, G, D = q.shape
+    p = (q.double().reshape(m * G, D) @ k.double().t().contiguous()).view(m, G, -1) * scale
+    p = p.masked_fill(torch.ones(m, k.size(0), dtype=torch.bool, device=q.device).triu(sees)[:, None, :], -math.inf)
+    return (torch.softmax(p, dim=-1).view(m * G, -1) @ v.double()).view(m, G, D)
+
+
+def _exact_prompt(s):
+    c = s.case
+    G = c["HQ"] // c["HKV"]
+    out = torch.zeros(s.q.shape, dtype=torch.float64, device=s.q.device)
+    token = key = 0
+    for n, (length, new) in enumerate(s.lengths):
+        at = torch.arange(length, device=s.q.device)
+        for h in range(c["HKV"]):
+            if c["op"] == "prompt":
+                k, v = s.k[key:key + length, h], s.v[key:key + length, h]
+            else:
+                page = s.table[n].long()[at // c["block"]]
+                k, v = (x[page, at % c["block"], h] for x in (s.k_cache, s.v_cache))
+            step = max(1, int(2e8 / (length * G)))
+            for j in range(0, new, step):
+                m, last = min(step, new - j), length - new + min(j + step, new)
+                out[token + j:token + j + m, h * G:(h + 1) * G] = _exact_rows(
+                    s.q[token + j:token + j + m, h * G:(h + 1) * G], k[:last], v[:last], length - new + j + 1, s.scale)
+        token, key = token + new, key + length
+    return out if s.gate is None else out * torch.sigmoid(s.gate.double())
+
+
+def _exact_store8(s):
+    """Numbers before they are rounded to 8 bits, with their scales."""
+    c = s.case
+
+    def heads(x, weight):
+        x = x.double()
+        if weight is not None:
+            x = x / torch.sqrt(x.square().mean(-1, keepdim=True) + EPS) * (1.0 + weight.double())
+        if c["rot"]:
+            half = c["rot"] // 2
+            first = torch.arange(0, c["rot"], 2) if c["interleaved"] else torch.arange(half)
+            second = first + (1 if c["interleaved"] else half)
+            turn = torch.polar(torch.full((1, half), s.factor, dtype=torch.float64, device=x.device),
+                               s.positions.double()[:, None] * s.inv_freq.double())
+            z = torch.complex(x[..., first], x[..., second]) * turn[:, None, :]
+            x[..., first], x[..., second] = z.real, z.imag
+        return x
+
+    stored = int((s.slots >= 0).sum())                       # the others stand at the end
+    block, place = s.slots[:stored] // c["block"], s.slots[:stored] % c["block"]
+    caches, scales = [], []
+    for x in (heads(s.k, s.k_weight), s.v.double()):
+        x = x[:stored]
+        top = x.abs().amax(-1).clamp(min=LEAST) / LARGEST
+        caches.append(torch.zeros(s.k_cache.shape, dtype=torch.float64, device=x.device).index_put_((block, place), x / top[..., None]))
+        wide = torch.zeros(s.k_scales.shape, dtype=torch.float64, device=x.device).transpose(1, 2).contiguous()
+        scales.append(wide.index_put_((block, place), top).transpose(1, 2).contiguous())
+    return heads(s.q, s.q_weight), *caches, *scales
+
+
+def _exact_windows(s):
+    c = s.case
+    G, bs = c["HQ"] // c["HKV"], c["block"]
+    out = torch.zeros(s.q.shape, dtype=torch.float64, device=s.q.device)
+
+    def keys(pages, length, h):
+        at = torch.arange(length, device=s.q.device)
+        page, place = pages.long()[at // bs], at % bs
+        if s.k_scales is None:
+            return [x[page, place, h].double() for x in (s.k_cache, s.v_cache)]
+        return [x.view(torch.uint8)[page, place, h].view(E4M3).double() * y[page, h, place].double()[:, None]
+                for x, y in ((s.k_cache, s.k_scales), (s.v_cache, s.v_scales))]
+
+    for h in range(c["HKV"]):
+        P = c.get("prefix", 0)
+        before = keys(s.prefix_blocks, P, h) if P else None
+        token = 0
+        for n, (length, window) in enumerate(_window_lengths(c)):
+            if window and length:
+                k, v = keys(s.table[n], length, h)
+                if P:
+                    k, v = torch.cat([before[0], k]), torch.cat([before[1], v])
+                at = slice(token, token + window)
+                out[at, h * G:(h + 1) * G] = _exact_rows(s.q[at, h * G:(h + 1) * G], k, v, P + length - window + 1, s.scale)
+            token += window
+    return out if s.gate is None else out * torch.sigmoid(s.gate.double())
+
+
+def exact(case, seed):
+    # about as many small products as take twenty seconds
+    if case["op"] in ("decode8", "prefix") and case["batch"] * case["HKV"] > 10000:
+        return None
+    s = prepare(case, seed)
+    return {"prompt": _exact_prompt, "chunk": _exact_prompt, "store8": _exact_store8}.get(case["op"], _exact_windows)(s)
