@@ -271,7 +271,7 @@ def _run_prompt(s):
     if s.case["op"] == "prompt":
         from pla_amd.prefill.attention import packed_attention_fwd
         return packed_attention_fwd(s.q, s.k, s.v, s.offsets, cu_seqlens_k=s.key_offsets, scale=s.scale, output_gate=s.gate, out=s.out)
-    from pla_amd.decode.paged import paged_attention_prefill
+    from pla_amd.prefill.attention import paged_attention_prefill
     return paged_attention_prefill(s.q, s.k_cache, s.v_cache, s.table, s.seq_lens, s.offsets, scale=s.scale, output_gate=s.gate, out=s.out)
 
 
