@@ -559,6 +559,36 @@ int pla_paged_attention_segments(
     const int32_t* offsets, const int32_t* seq_lens, int batch, int tokens, int HQ, int HKV, int head_dim, int max_query_len,
     int64_t positions, int worker, int64_t* segments, int capacity);
 
+/* Workspace bytes (16-byte aligned; 0: none) of the two prompt launches below; keys: rows of k, or table_cols * block_size.  -1: not a
+ * valid shape. */
+int64_t pla_prompt_attention_workspace_bytes(int batch, int64_t tokens, int HQ, int HKV, int head_dim, int64_t keys);
+
+/*
+ * Causal attention of packed sequences over packed keys (no counterpart in the reference).
+ *   q, out, gate (NULL: none) [tokens,HQ,D], k, v [keys,HKV,D] in act_dtype (PLA_BF16 or PLA_F16) with (token, head) strides, multiples
+ *       of 8 elements, pointers 16-byte aligned, token strides of k and v below 2^24, D 64, 128 or 256, HQ a multiple of HKV
+ *   offsets [batch + 1]: rows of each sequence; key_offsets [batch + 1]: rows of its keys (NULL: the same).  A sequence that is empty or
+ *       not within [0, tokens) and [0, keys) is passed over.
+ *   token j of m with n keys sees the first n - m + j + 1; a row that sees none is zeros.
+ *   out = softmax(scale q k^T) v [* sigmoid(gate)], weights rounded to act_dtype, all else float32.  Calls that overlap in time need
+ *   workspaces of their own.
+ */
+int pla_prompt_attention_launch(
+    const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+    const void* offsets, int offsets_wide, const void* key_offsets, int key_offsets_wide, const void* gate, int64_t gate_token, int64_t gate_head,
+    void* out, int64_t out_token, int64_t out_head, float scale, int batch, int tokens, int64_t keys, int HQ, int HKV, int head_dim, int act_dtype,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The same over a paged cache, as pla_paged_attention_launch has it, for windows of any length at the end of seq_lens[n] cached tokens.
+ */
+int pla_paged_prompt_attention_launch(
+    const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache, int64_t kv_block, int64_t kv_token, int64_t kv_head,
+    int blocks, int block_size, const int32_t* block_table, int64_t table_row_stride, int table_rows, int table_cols,
+    const void* mapping, int mapping_wide, const void* offsets, int offsets_wide, const void* seq_lens, int seq_lens_wide,
+    const void* gate, int64_t gate_token, int64_t gate_head, void* out, int64_t out_token, int64_t out_head,
+    float scale, int batch, int tokens, int HQ, int HKV, int head_dim, int act_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 /*
  * Rows of the 128-row state tile a wavefront owns (8, 16 or 32) that a k-last launch with
  * rows_per_wave = 0 takes for a shape: the row count the auto-tuner measured for the nearest batch size

@@ -141,6 +141,17 @@ SIGNATURES = {
         _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
         _c_f, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
         _c_p, _c_i64, _c_p],
+    "pla_prompt_attention_launch": [
+        _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+        _c_p, _c_int, _c_p, _c_int, _c_p, _c_i64, _c_i64,
+        _c_p, _c_i64, _c_i64, _c_f, _c_int, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int,
+        _c_p, _c_i64, _c_p],
+    "pla_paged_prompt_attention_launch": [
+        _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64,
+        _c_int, _c_int, _c_p, _c_i64, _c_int, _c_int,
+        _c_p, _c_int, _c_p, _c_int, _c_p, _c_int,
+        _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+        _c_f, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_i64, _c_p],
 }
 
 _lib = None
@@ -174,6 +185,8 @@ def load():
     lib.pla_kda_prefill_workspace_bytes.argtypes = [_c_int, _c_int, _c_int]
     lib.pla_paged_attention_workspace_bytes.restype = _c_i64
     lib.pla_paged_attention_workspace_bytes.argtypes = [_c_int, _c_int, _c_int, _c_int, _c_int, _c_i64]
+    lib.pla_prompt_attention_workspace_bytes.restype = _c_i64
+    lib.pla_prompt_attention_workspace_bytes.argtypes = [_c_int, _c_i64, _c_int, _c_int, _c_int, _c_i64]
     lib.pla_tuned_rows_per_wave.restype = _c_int
     lib.pla_tuned_rows_per_wave.argtypes = [_c_int] * 7
     for name, argtypes in SIGNATURES.items():

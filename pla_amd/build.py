@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libpla_gfx950.so")
 OBJ_DIR = os.path.join(HERE, "build")
 
 SOURCES = ["api.hip", "decode_k_last.hip", "decode_kda_mega.hip", "decode_kda_replay.hip", "commit_plan.hip", "prefill_gdn.hip", "prefill_kda.hip",
-           "paged_plan.hip", "qk_norm_rope.hip", "paged_attention.hip"]
+           "paged_plan.hip", "qk_norm_rope.hip", "paged_attention.hip", "prompt_attention.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-inline-asm",

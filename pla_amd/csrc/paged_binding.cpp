@@ -203,6 +203,17 @@ void cache_form(const Tensor& t, const char* name, int64_t heads, int64_t D, at:
   TORCH_CHECK(t.size(0) * t.size(1) <= INT32_MAX, name, " must have at most 2^31 - 1 slots");
 }
 
+// Caches that attention reads.
+void cache_pair(const Tensor& k_cache, const Tensor& v_cache, int64_t heads, int64_t D, at::ScalarType type) {
+  cache_form(k_cache, "k_cache", heads, D, type);
+  cache_form(v_cache, "v_cache", heads, D, type);
+  TORCH_CHECK(v_cache.sizes() == k_cache.sizes() && step(v_cache, 0) == step(k_cache, 0) && step(v_cache, 1) == step(k_cache, 1) &&
+                  step(v_cache, 2) == step(k_cache, 2),
+              "k_cache and v_cache must have the same shape and strides");
+  TORCH_CHECK(k_cache.size(1) % 16 == 0, "block_size must be a multiple of 16, got ", k_cache.size(1));
+  TORCH_CHECK(step(k_cache, 1) < (1 << 24), "the caches' token stride must be below 2^24");
+}
+
 // ---- norms, rotation, cache write --------------------------------------------------------------------------------
 
 std::tuple<Tensor, OptTensor> fused_qk_norm_rope(
@@ -297,13 +308,7 @@ Tensor paged_attention_decode(
   TORCH_CHECK(k_cache.dim() == 4, "k_cache must be [blocks, block_size, heads, head_dim]");
   const int64_t HKV = k_cache.size(2), block_size = k_cache.size(1);
   TORCH_CHECK(HKV > 0 && HQ >= HKV && HQ % HKV == 0, "query heads must be a positive multiple of key-value heads, got ", HQ, " and ", HKV);
-  cache_form(k_cache, "k_cache", HKV, D, type);
-  cache_form(v_cache, "v_cache", HKV, D, type);
-  TORCH_CHECK(v_cache.sizes() == k_cache.sizes() && step(v_cache, 0) == step(k_cache, 0) && step(v_cache, 1) == step(k_cache, 1) &&
-                  step(v_cache, 2) == step(k_cache, 2),
-              "k_cache and v_cache must have the same shape and strides");
-  TORCH_CHECK(block_size % 16 == 0, "block_size must be a multiple of 16, got ", block_size);
-  TORCH_CHECK(step(k_cache, 1) < (1 << 24), "the caches' token stride must be below 2^24");
+  cache_pair(k_cache, v_cache, HKV, D, type);
   block_table_form(block_table);
   const int64_t rows = block_table.size(0), cols = block_table.size(1);
   TORCH_CHECK(cols * block_size <= (1 << 30), "a row of the block table must hold at most 2^30 positions");
@@ -343,6 +348,105 @@ Tensor paged_attention_decode(
   return out;
 }
 
+// ---- prompts -----------------------------------------------------------------------------------------------------
+
+// Heads of q and of a tensor with key-value heads.
+void query_heads(int64_t HQ, int64_t HKV) {
+  TORCH_CHECK(HKV > 0 && HQ >= HKV && HQ % HKV == 0, "query heads must be a positive multiple of key-value heads, got ", HQ, " and ", HKV);
+}
+
+Tensor packed_attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets_in, const OptTensor& key_offsets_in,
+                            std::optional<double> scale, const OptTensor& output_gate, const OptTensor& out_in) {
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3, "q and k must be [tokens, heads, head_dim]");
+  const int64_t T = q.size(0), HQ = q.size(1), D = q.size(2), keys = k.size(0), HKV = k.size(1);
+  TORCH_CHECK(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got ", D);
+  const int act = act_code(q, "q");
+  const at::ScalarType type = q.scalar_type();
+  query_heads(HQ, HKV);
+  head_rows(q, "q", T, HQ, D, type);
+  head_rows(k, "k", keys, HKV, D, type);
+  head_rows(v, "v", keys, HKV, D, type);
+  TORCH_CHECK(step(k, 0) < (1 << 24) && step(v, 0) < (1 << 24), "the token strides of k and v must be below 2^24");
+  TORCH_CHECK(offsets_in.dim() == 1 && offsets_in.numel() >= 1, "cu_seqlens must be an int32 or int64 vector of at least one entry");
+  const int64_t batch = offsets_in.numel() - 1;
+  const Tensor offsets = index_vector(offsets_in, "cu_seqlens", batch + 1);
+  OptTensor key_offsets;
+  if (key_offsets_in) key_offsets = index_vector(*key_offsets_in, "cu_seqlens_k", batch + 1);
+  else TORCH_CHECK(keys == T, "without cu_seqlens_k there is a key for every token: ", T, " tokens, ", keys, " keys");
+  TORCH_CHECK(T * HQ <= (1 << 30) && keys <= INT32_MAX - 1024, "too many rows");
+  const int sequences = count(batch, "sequences");
+  TORCH_CHECK(!scale || finite(*scale), "scale must be finite");
+  if (output_gate) head_rows(*output_gate, "output_gate", T, HQ, D, type);
+  if (out_in) head_rows(*out_in, "out", T, HQ, D, type);
+  const OptTensor qt(q), kt(k), vt(v), off(offsets);
+  on_one_gpu(q, "q", {{"k", &kt}, {"v", &vt}, {"cu_seqlens", &off}, {"cu_seqlens_k", &key_offsets}, {"output_gate", &output_gate}, {"out", &out_in}});
+  apart({{"out", &out_in}}, {{"q", &qt}, {"k", &kt}, {"v", &vt}, {"cu_seqlens", &off}, {"cu_seqlens_k", &key_offsets}, {"output_gate", &output_gate}});
+
+  const c10::DeviceGuard guard(q.device());
+  Tensor out = out_in ? *out_in : at::empty({T, HQ, D}, q.options());
+  if (bypass() || T == 0 || batch == 0) return out;
+  const int64_t bytes = pla_prompt_attention_workspace_bytes(sequences, T, (int)HQ, (int)HKV, (int)D, keys);
+  TORCH_CHECK(bytes >= 0, pla_last_error());
+  Tensor workspace;
+  if (bytes > 0) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+  launched(pla_prompt_attention_launch(
+      q.data_ptr(), step(q, 0), step(q, 1), k.data_ptr(), step(k, 0), step(k, 1), v.data_ptr(), step(v, 0), step(v, 1), offsets.data_ptr(),
+      wide(offsets), ptr(key_offsets), wide(key_offsets), ptr(output_gate), step(output_gate, 0), step(output_gate, 1), out.data_ptr(), step(out, 0),
+      step(out, 1), (float)scale.value_or(1.0 / std::sqrt((double)D)), sequences, (int)T, keys, (int)HQ, (int)HKV, (int)D, act,
+      bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(q)));
+  return out;
+}
+
+Tensor paged_attention_prefill(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens_in,
+                               const Tensor& offsets_in, const OptTensor& request_indices, std::optional<double> scale,
+                               const OptTensor& output_gate, const OptTensor& out_in) {
+  TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head_dim]");
+  const int64_t T = q.size(0), HQ = q.size(1), D = q.size(2);
+  TORCH_CHECK(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got ", D);
+  const int act = act_code(q, "q");
+  const at::ScalarType type = q.scalar_type();
+  head_rows(q, "q", T, HQ, D, type);
+  TORCH_CHECK(k_cache.dim() == 4, "k_cache must be [blocks, block_size, heads, head_dim]");
+  const int64_t HKV = k_cache.size(2), block_size = k_cache.size(1);
+  query_heads(HQ, HKV);
+  cache_pair(k_cache, v_cache, HKV, D, type);
+  block_table_form(block_table);
+  const int64_t rows = block_table.size(0), cols = block_table.size(1);
+  TORCH_CHECK(cols * block_size <= (1 << 30), "a row of the block table must hold at most 2^30 positions");
+  TORCH_CHECK(seq_lens_in.dim() == 1, "seq_lens must be an int32 or int64 vector");
+  const int64_t batch = seq_lens_in.numel();
+  const Tensor seq_lens = index_vector(seq_lens_in, "seq_lens", batch), offsets = index_vector(offsets_in, "query_start_loc", batch + 1);
+  OptTensor mapping;
+  if (request_indices) mapping = index_vector(*request_indices, "request_indices", batch);
+  else TORCH_CHECK(batch <= rows, "more requests than rows of the block table");
+  TORCH_CHECK(T * HQ <= (1 << 30), "too many rows");
+  const int requests = count(batch, "requests"), table_rows = count(rows, "rows of the block table");
+  TORCH_CHECK(!scale || finite(*scale), "scale must be finite");
+  if (output_gate) head_rows(*output_gate, "output_gate", T, HQ, D, type);
+  if (out_in) head_rows(*out_in, "out", T, HQ, D, type);
+  const OptTensor qt(q), kt(k_cache), vt(v_cache), table(block_table), lens(seq_lens), off(offsets);
+  on_one_gpu(q, "q", {{"k_cache", &kt}, {"v_cache", &vt}, {"block_table", &table}, {"seq_lens", &lens}, {"query_start_loc", &off},
+                      {"request_indices", &mapping}, {"output_gate", &output_gate}, {"out", &out_in}});
+  apart({{"out", &out_in}}, {{"q", &qt}, {"k_cache", &kt}, {"v_cache", &vt}, {"block_table", &table}, {"seq_lens", &lens},
+                             {"query_start_loc", &off}, {"request_indices", &mapping}, {"output_gate", &output_gate}});
+
+  const c10::DeviceGuard guard(q.device());
+  Tensor out = out_in ? *out_in : at::empty({T, HQ, D}, q.options());
+  if (bypass() || T == 0 || batch == 0) return out;
+  const int64_t bytes = pla_prompt_attention_workspace_bytes(requests, T, (int)HQ, (int)HKV, (int)D, cols * block_size);
+  TORCH_CHECK(bytes >= 0, pla_last_error());
+  Tensor workspace;
+  if (bytes > 0) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+  launched(pla_paged_prompt_attention_launch(
+      q.data_ptr(), step(q, 0), step(q, 1), k_cache.data_ptr(), v_cache.data_ptr(), step(k_cache, 0), step(k_cache, 1),
+      step(k_cache, 2), (int)k_cache.size(0), (int)block_size, block_table.data_ptr<int32_t>(), table_pitch(block_table), table_rows,
+      (int)cols, ptr(mapping), wide(mapping), offsets.data_ptr(), wide(offsets), seq_lens.data_ptr(), wide(seq_lens), ptr(output_gate),
+      step(output_gate, 0), step(output_gate, 1), out.data_ptr(), step(out, 0), step(out, 1),
+      (float)scale.value_or(1.0 / std::sqrt((double)D)), requests, (int)T, (int)HQ, (int)HKV, (int)D, act,
+      bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(q)));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -350,4 +454,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_kv_plan", &paged_kv_plan);
   m.def("fused_qk_norm_rope", &fused_qk_norm_rope);
   m.def("paged_attention_decode", &paged_attention_decode);
+  m.def("packed_attention_fwd", &packed_attention_fwd);
+  m.def("paged_attention_prefill", &paged_attention_prefill);
 }

@@ -11,6 +11,8 @@ needs besides the linear-attention operators; it has no counterpart in the refer
 ``rotary_frequencies``      the rotation's frequencies, plain or scaled for long contexts.
 ``paged_attention_decode``  attention of one new token, or of a window of up to 32 draft tokens, over the paged cache.
 
+Longer windows, prompts and parts of them: ``pla.prefill.attention.paged_attention_prefill``.
+
 All checks live in the compiled layer (``pla.decode.paged._C``), raise RuntimeError and come before any launch.  Nothing is read
 back from the device, so every call can be captured in a graph.  ``PLA_SANITY_CHECK=1`` adds checks of values (they read device
 memory and are skipped under capture).

@@ -58,18 +58,18 @@ def check_slots(slot_mapping, k_cache):
         _fail("fused_qk_norm_rope", "two tokens name one slot")
 
 
-def check_attention(q, k_cache, block_table, seq_lens, query_start_loc, request_indices, max_query_len):
+def check_attention(q, k_cache, block_table, seq_lens, query_start_loc, request_indices, max_query_len, op="paged_attention_decode"):
     if (_capturing() or not _formed(block_table, seq_lens, query_start_loc, request_indices) or k_cache.dim() < 2 or q.dim() < 1 or
             k_cache.size(1) < 1 or (query_start_loc is not None and query_start_loc.numel() != seq_lens.numel() + 1)):
         return
-    op, (rows, cols) = "paged_attention_decode", block_table.shape
+    rows, cols = block_table.shape
     blocks, block_size = k_cache.shape[:2]
     lengths = seq_lens.tolist()
     offsets = list(range(len(lengths) + 1)) if query_start_loc is None else query_start_loc.tolist()
     index = list(range(len(lengths))) if request_indices is None else request_indices.tolist()
     if offsets[0] != 0 or any(b < a for a, b in zip(offsets, offsets[1:])) or offsets[-1] > q.size(0):
         _fail(op, "query_start_loc must start at 0, not decrease and stay within q")
-    if any(b - a > max_query_len for a, b in zip(offsets, offsets[1:])):
+    if max_query_len is not None and any(b - a > max_query_len for a, b in zip(offsets, offsets[1:])):
         _fail(op, "a window is longer than max_query_len")
     if any(not 0 <= x < rows for x in index):
         _fail(op, "request_indices must be rows of the block table")
@@ -79,3 +79,18 @@ def check_attention(q, k_cache, block_table, seq_lens, query_start_loc, request_
             _fail(op, "a sequence length is negative or passes the block table")
         if any(not 0 <= b < blocks for b in table[row][:-(-length // block_size)]):
             _fail(op, "a block of the table is not in the cache")
+
+
+def check_packed(q, k, cu_seqlens, cu_seqlens_k):
+    if _capturing() or not _formed(None, cu_seqlens, cu_seqlens_k) or q.dim() < 1 or k.dim() < 1 or cu_seqlens.numel() < 1:
+        return
+    op = "packed_attention_fwd"
+    offsets = cu_seqlens.tolist()
+    key_offsets = offsets if cu_seqlens_k is None else cu_seqlens_k.tolist()
+    if len(key_offsets) != len(offsets):
+        return
+    for name, x, rows in (("cu_seqlens", offsets, q.size(0)), ("cu_seqlens_k", key_offsets, k.size(0))):
+        if x[0] != 0 or any(b < a for a, b in zip(x, x[1:])) or x[-1] > rows:
+            _fail(op, f"{name} must start at 0, not decrease and stay within its tensor")
+    if any(d - c < b - a for a, b, c, d in zip(offsets, offsets[1:], key_offsets, key_offsets[1:])):
+        _fail(op, "a sequence has fewer keys than tokens")
