@@ -524,6 +524,19 @@ int pla_qk_norm_rope_launch(
     void* q_out, void* k_out, void* k_cache, void* v_cache, const void* slots, int slots_wide, int blocks, int block_size,
     int tokens, int HQ, int HKV, int D, int act_dtype, void* stream);
 
+/*
+ * The same with k_cache and v_cache (NULL: no values) of e4m3 numbers of 8 bits, whose strides are multiples of 16, and a float32 scale
+ * for each head of a token: max(largest magnitude, 1e-30) / 448, numbers rounded to nearest from the float32 quotient.
+ *   k_scales, v_scales: [blocks][HKV][block_size] with dense places; scale_strides [4]: (block, head) of both, in elements
+ *   A NaN stays one; an infinity makes what its head stands for NaN.
+ */
+int pla_qk_norm_rope_fp8_launch(
+    const void* q, const void* k, const void* v, const int64_t* strides, const void* positions, int positions_wide,
+    const void* q_weight, const void* k_weight, int weights_f32, float eps, float weight_offset,
+    const float* inv_freq, int rotary_dim, float attention_factor, int interleaved,
+    void* q_out, void* k_out, void* k_cache, void* v_cache, float* k_scales, float* v_scales, const int64_t* scale_strides,
+    const void* slots, int slots_wide, int blocks, int block_size, int tokens, int HQ, int HKV, int D, int act_dtype, void* stream);
+
 /* Workspace bytes (16-byte aligned; 0: none) of pla_paged_attention_launch, positions = table_cols * block_size; -1: not a valid shape. */
 int64_t pla_paged_attention_workspace_bytes(int batch, int HQ, int HKV, int head_dim, int max_query_len, int64_t positions);
 
@@ -558,6 +571,41 @@ int pla_paged_attention_launch(
 int pla_paged_attention_segments(
     const int32_t* offsets, const int32_t* seq_lens, int batch, int tokens, int HQ, int HKV, int head_dim, int max_query_len,
     int64_t positions, int worker, int64_t* segments, int capacity);
+
+/*
+ * The same over caches of e4m3 numbers with float32 scales as pla_qk_norm_rope_fp8_launch writes them: cache strides multiples of 16,
+ * k_scales and v_scales [blocks][HKV][block_size] with common (block, head) strides, multiples of 4 elements, 16-byte aligned; values
+ * of scales that are read are not negative.  Numbers are widened without an error; keys' scales multiply scores, values' scales weights,
+ * which meet the values in two parts of bf16.  Workspace as pla_paged_attention_launch.
+ */
+int pla_paged_attention_fp8_launch(
+    const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,
+    int64_t kv_block, int64_t kv_token, int64_t kv_head, int blocks, int block_size,
+    const float* k_scales, const float* v_scales, int64_t scale_block, int64_t scale_head,
+    const int32_t* block_table, int64_t table_row_stride, int table_rows, int table_cols,
+    const void* mapping, int mapping_wide, const void* offsets, int offsets_wide, const void* seq_lens, int seq_lens_wide,
+    const void* gate, int64_t gate_token, int64_t gate_head, void* out, int64_t out_token, int64_t out_head,
+    float scale, int batch, int tokens, int max_query_len, int HQ, int HKV, int head_dim, int act_dtype,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of pla_paged_attention_prefix_launch, prefix_positions = prefix_pages * block_size; -1: not a valid shape. */
+int64_t pla_paged_attention_prefix_workspace_bytes(int batch, int tokens, int HQ, int HKV, int head_dim, int max_query_len, int64_t positions,
+                                                   int64_t prefix_positions);
+
+/*
+ * pla_paged_attention_launch where all token rows also see a prefix that stands before their own keys: the first prefix_len[0] (int32 or
+ * int64, on the device; at most prefix_pages * block_size) positions of prefix_blocks int32 [prefix_pages], read once for the whole batch.
+ * A row that sees no key of its own is zeros.  Weights of the prefix are rounded to act_dtype.
+ */
+int pla_paged_attention_prefix_launch(
+    const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,
+    int64_t kv_block, int64_t kv_token, int64_t kv_head, int blocks, int block_size,
+    const int32_t* prefix_blocks, int prefix_pages, const void* prefix_len, int prefix_len_wide,
+    const int32_t* block_table, int64_t table_row_stride, int table_rows, int table_cols,
+    const void* mapping, int mapping_wide, const void* offsets, int offsets_wide, const void* seq_lens, int seq_lens_wide,
+    const void* gate, int64_t gate_token, int64_t gate_head, void* out, int64_t out_token, int64_t out_head,
+    float scale, int batch, int tokens, int max_query_len, int HQ, int HKV, int head_dim, int act_dtype,
+    void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Workspace bytes (16-byte aligned; 0: none) of the two prompt launches below; keys: rows of k, or table_cols * block_size.  -1: not a
  * valid shape. */

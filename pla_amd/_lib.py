@@ -141,6 +141,30 @@ SIGNATURES = {
         _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
         _c_f, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
         _c_p, _c_i64, _c_p],
+    "pla_qk_norm_rope_fp8_launch": [
+        _c_p, _c_p, _c_p, _c_p, _c_p, _c_int,
+        _c_p, _c_p, _c_int, _c_f, _c_f,
+        _c_p, _c_int, _c_f, _c_int,
+        _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_int, _c_int, _c_int,
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_p],
+    "pla_paged_attention_fp8_launch": [
+        _c_p, _c_i64, _c_i64, _c_p, _c_p,
+        _c_i64, _c_i64, _c_i64, _c_int, _c_int,
+        _c_p, _c_p, _c_i64, _c_i64,
+        _c_p, _c_i64, _c_int, _c_int,
+        _c_p, _c_int, _c_p, _c_int, _c_p, _c_int,
+        _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+        _c_f, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+        _c_p, _c_i64, _c_p],
+    "pla_paged_attention_prefix_launch": [
+        _c_p, _c_i64, _c_i64, _c_p, _c_p,
+        _c_i64, _c_i64, _c_i64, _c_int, _c_int,
+        _c_p, _c_int, _c_p, _c_int,
+        _c_p, _c_i64, _c_int, _c_int,
+        _c_p, _c_int, _c_p, _c_int, _c_p, _c_int,
+        _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+        _c_f, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+        _c_p, _c_i64, _c_p],
     "pla_prompt_attention_launch": [
         _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
         _c_p, _c_int, _c_p, _c_int, _c_p, _c_i64, _c_i64,
@@ -185,6 +209,8 @@ def load():
     lib.pla_kda_prefill_workspace_bytes.argtypes = [_c_int, _c_int, _c_int]
     lib.pla_paged_attention_workspace_bytes.restype = _c_i64
     lib.pla_paged_attention_workspace_bytes.argtypes = [_c_int, _c_int, _c_int, _c_int, _c_int, _c_i64]
+    lib.pla_paged_attention_prefix_workspace_bytes.restype = _c_i64
+    lib.pla_paged_attention_prefix_workspace_bytes.argtypes = [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_i64]
     lib.pla_prompt_attention_workspace_bytes.restype = _c_i64
     lib.pla_prompt_attention_workspace_bytes.argtypes = [_c_int, _c_i64, _c_int, _c_int, _c_int, _c_i64]
     lib.pla_tuned_rows_per_wave.restype = _c_int

@@ -36,6 +36,7 @@
 #include "decode_common.h"
 #include "mfma_bf16.h"
 #include "paged_schedule.h"
+#include "prompt_attention.h"
 
 namespace pla {
 
@@ -49,7 +50,8 @@ struct PagedRun {
 
 struct PagedAttention {
   const uint16_t* q; int64_t q_token, q_head;
-  const uint16_t *k, *v; int64_t kv_block, kv_token, kv_head;
+  const void *k, *v; int64_t kv_block, kv_token, kv_head;         // 16 bits a number, or 8
+  const float *k_scales, *v_scales; int64_t scale_block, scale_head;     // of numbers of 8 bits: [block][head][place]
   const int32_t* table; int64_t table_row;
   const void* mapping; int mapping_wide;
   const void* offsets; int offsets_wide;          // NULL: token row n is request n
@@ -62,6 +64,9 @@ struct PagedAttention {
   float scale_log2;
   int by_run, row_blocks;                         // runs in pieces are listed by run, or by worker; row blocks of the longest window
   float* partial; float2* tops; PagedRun* runs;
+  // attention over a prefix that all rows share, in pieces: outputs and their references and sums [piece][token][query head]
+  const float* prefix; const float2* prefix_tops;
+  const void* prefix_len; int prefix_len_wide, prefix_splits; int64_t prefix_positions;
 
   __device__ int64_t at(const void* base, int wide, int64_t i) const {
     return wide ? static_cast<const int64_t*>(base)[i] : (int64_t) static_cast<const int32_t*>(base)[i];
@@ -91,6 +96,25 @@ template <> __device__ __forceinline__ f32x4_t mfma_act<f16_t>(bf16x8_t a, bf16x
 
 template <typename act_t> constexpr float WEIGHT_SHIFT = 0.f;
 template <> constexpr float WEIGHT_SHIFT<f16_t> = 14.f;
+
+// What a cache holds: numbers of the queries' type, or e4m3 numbers of 8 bits with a factor a key and head.  The latter are widened to
+// the queries' type for the scores and to bf16 for the values, both without an error; keys' factors go to the scores and values' to the
+// weights, so a weight may be larger than one there, which bf16 holds.
+struct e4m3_t { uint8_t bits; };
+template <typename act_t, typename kv_t> struct Cached { using raw_t = uint16_t; using value_t = act_t; static constexpr bool SCALED = false; };
+template <typename act_t> struct Cached<act_t, e4m3_t> { using raw_t = uint8_t; using value_t = bf16_t; static constexpr bool SCALED = true; };
+// Two of the four numbers of a word, widened.
+template <typename T> __device__ __forceinline__ uint32_t widen2(uint32_t word, int second);
+template <> __device__ __forceinline__ uint32_t widen2<bf16_t>(uint32_t word, int second) {
+  return second ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.f, false));
+}
+template <> __device__ __forceinline__ uint32_t widen2<f16_t>(uint32_t word, int second) {
+  return second ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, false));
+}
+template <typename act_t> __device__ __forceinline__ float cached_number(const uint16_t* p) { return to_float(act_t{*p}); }
+template <typename act_t> __device__ __forceinline__ float cached_number(const uint8_t* p) { return __builtin_amdgcn_cvt_f32_fp8((int)*p, 0); }
 
 // Over the four lanes that hold a query's scores.
 __device__ __forceinline__ float query_max(float x) {
@@ -132,47 +156,74 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 template <int D> struct ValueWords { static constexpr int N = D == 64 ? 2 : 4; };      // 32-bit words of a lane's channels, a chunk
 
 // Keys in flight, values in flight and the state of the rows of one wavefront.
-template <typename act_t, int D, int RT>
+template <typename act_t, typename kv_t, int D, int RT>
 struct Wave {
+  using raw_t = typename Cached<act_t, kv_t>::raw_t;
+  static constexpr bool SCALED = Cached<act_t, kv_t>::SCALED;
   static constexpr int STEPS = D / 32;                        // of the contraction of K Q^T
   static constexpr int WORDS = ValueWords<D>::N, CHUNKS = D == 256 ? 2 : 1, TILES = 2 * WORDS;
   static constexpr int LANE_CHANNELS = 2 * WORDS;             // channels of a value that a lane loads, a chunk of 16 times as many
-  u32x4_t k[2][STEPS];
-  uint32_t v[8][CHUNKS][WORDS];
+  static constexpr int KEY_LOADS = SCALED ? STEPS / 2 : STEPS, RAW_WORDS = SCALED ? WORDS / 2 : WORDS;
+  u32x4_t k[2][KEY_LOADS];
+  uint32_t v[8][CHUNKS][RAW_WORDS];
+  f32x4_t k_scale[SCALED ? 2 : 1], v_scale[SCALED ? 2 : 1];   // of the lane's keys
   f32x4_t o[RT][CHUNKS][TILES];
   float top[RT], sum[RT];
   int limit[RT];
   int set_aside;                                              // first key of the step whose partly seen values are added at the end, + 1 if those
                                                               // of the next are too (a wavefront alone may have both), or -1
+  __device__ __forceinline__ bf16x8_t key(int h, int c) const {
+    if constexpr (SCALED) {
+      u32x4_t x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = widen2<act_t>(k[h][c / 2][2 * (c & 1) + i / 2], i & 1);
+      return __builtin_bit_cast(bf16x8_t, x);
+    } else {
+      return __builtin_bit_cast(bf16x8_t, k[h][c]);
+    }
+  }
+  __device__ __forceinline__ uint32_t value(int i, int c, int j) const {
+    if constexpr (SCALED) return widen2<bf16_t>(v[i][c][j / 2], j & 1);
+    else return v[i][c][j];
+  }
 };
 
-template <typename act_t, int D, int RT>
-__device__ __forceinline__ void load_keys(Wave<act_t, D, RT>& w, const uint16_t* base, const int64_t (&place)[2], uint32_t lane_offset) {
+// Where the two halves of a step's keys lie, in elements from the caches' and from the factors' start.
+struct Places { int64_t at[2], scale[2]; };
+
+template <typename W, typename raw_t>
+__device__ __forceinline__ void load_keys(W& w, const raw_t* base, const float* scales, const Places& place, uint32_t lane_offset) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const auto p = as_global(reinterpret_cast<const char*>(base + place[h]));
+    const auto p = as_global(reinterpret_cast<const char*>(base + place.at[h]));
 #pragma unroll
-    for (int c = 0; c < Wave<act_t, D, RT>::STEPS; ++c) w.k[h][c] = *reinterpret_cast<global_ptr<const u32x4_t>>(p + lane_offset + 64 * c);
+    for (int c = 0; c < W::KEY_LOADS; ++c) w.k[h][c] = *reinterpret_cast<global_ptr<const u32x4_t>>(p + lane_offset + 64 * c);
+    if constexpr (W::SCALED) w.k_scale[h] = *reinterpret_cast<global_ptr<const f32x4_t>>(as_global(scales + place.scale[h]) + 4 * ((threadIdx.x & 63) >> 4));
   }
 }
 
-template <typename act_t, int D, int RT>
-__device__ __forceinline__ void load_values(Wave<act_t, D, RT>& w, const uint16_t* base, const int64_t (&place)[2], uint32_t lane_offset,
-                                            int64_t token_bytes) {
+template <typename W, typename raw_t>
+__device__ __forceinline__ void load_values(W& w, const raw_t* base, const float* scales, const Places& place, uint32_t lane_offset, int64_t token_bytes) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const auto p = as_global(reinterpret_cast<const char*>(base + place[i / 4])) + (i & 3) * token_bytes;
+    const auto p = as_global(reinterpret_cast<const char*>(base + place.at[i / 4])) + (i & 3) * token_bytes;
 #pragma unroll
-    for (int c = 0; c < Wave<act_t, D, RT>::CHUNKS; ++c) {
-      if constexpr (Wave<act_t, D, RT>::WORDS == 4) {
+    for (int c = 0; c < W::CHUNKS; ++c) {
+      if constexpr (W::RAW_WORDS == 4) {
         const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<global_ptr<const u32x4_t>>(p + lane_offset + 256 * c));
 #pragma unroll
         for (int y = 0; y < 4; ++y) w.v[i][c][y] = x[y];
-      } else {
-        const u32x2_t x = __builtin_nontemporal_load(reinterpret_cast<global_ptr<const u32x2_t>>(p + lane_offset));
+      } else if constexpr (W::RAW_WORDS == 2) {
+        const u32x2_t x = __builtin_nontemporal_load(reinterpret_cast<global_ptr<const u32x2_t>>(p + lane_offset + 128 * c));
         w.v[i][c][0] = x[0]; w.v[i][c][1] = x[1];
+      } else {
+        w.v[i][c][0] = __builtin_nontemporal_load(reinterpret_cast<global_ptr<const uint32_t>>(p + lane_offset));
       }
     }
+  }
+  if constexpr (W::SCALED) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) w.v_scale[h] = *reinterpret_cast<global_ptr<const f32x4_t>>(as_global(scales + place.scale[h]) + 4 * ((threadIdx.x & 63) >> 4));
   }
 }
 
@@ -187,12 +238,16 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
   return __is_same(act_t, bf16_t) ? (pair & 0x7f807f80u) + 0x00800080u : (pair & 0x7c007c00u) + 0x04000400u;
 }
 
+// The same of words of four numbers of 8 bits, of which the NaN is the one with all bits set but the sign; bit 7, 15, 23 or 31.
+__device__ __forceinline__ uint32_t not_a_number8(uint32_t word) { return (word & 0x7f7f7f7fu) + 0x01010101u; }
+
 // One step of a wavefront: scores of 32 keys from key0 on, their weights, and the weighted values.  `next`: issues the loads of
 // the step after (keys once these are used, values once those are).
-template <typename act_t, int D, int RT, typename Queries, typename NextKeys, typename NextValues>
-__device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, float scale_log2, const bool (&there)[2],
+template <typename act_t, typename kv_t, int D, int RT, typename Queries, typename NextKeys, typename NextValues>
+__device__ __forceinline__ void attend(Wave<act_t, kv_t, D, RT>& w, Queries queries, float scale_log2, const bool (&there)[2],
                                        int key0, int least, int end, NextKeys next_keys, NextValues next_values) {
-  using W = Wave<act_t, D, RT>;
+  using W = Wave<act_t, kv_t, D, RT>;
+  using value_t = typename Cached<act_t, kv_t>::value_t;
   const int kb = (threadIdx.x & 63) >> 4;
   f32x4_t s[RT][2];
 #pragma unroll
@@ -203,9 +258,14 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
     for (int t = 0; t < RT; ++t) {
       const bf16x8_t q = __builtin_bit_cast(bf16x8_t, queries(t, c));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) s[t][h] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, w.k[h][c]), q, s[t][h]);
+      for (int h = 0; h < 2; ++h) s[t][h] = mfma_act<act_t>(w.key(h, c), q, s[t][h]);
     }
     if (D == 256) __builtin_amdgcn_sched_barrier(0);          // queries of all steps at once would not fit the registers
+  }
+  f32x4_t factor[2];                              // of the lane's keys, to the scores
+  if constexpr (W::SCALED) {
+    factor[0] = w.k_scale[0] * scale_log2;
+    factor[1] = w.k_scale[1] * scale_log2;
   }
   next_keys();
 
@@ -216,7 +276,7 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
   for (int t = 0; t < RT; ++t) {
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = s[t][i / 4][i & 3] * scale_log2;
+    for (int i = 0; i < 8; ++i) x[i] = s[t][i / 4][i & 3] * (W::SCALED ? factor[i / 4][i & 3] : scale_log2);
     if (masked) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = sees(t, i) ? x[i] : -INFINITY;
@@ -232,7 +292,7 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
         for (int j = 0; j < W::TILES; ++j) w.o[t][c][j] *= f;
       w.top[t] = top;
     }
-    const float zero = (top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>;
+    const float zero = (top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<value_t>;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - zero);
     u32x4_t a, b;
@@ -240,7 +300,14 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
     for (int i = 0; i < 4; ++i) {
       w.sum[t] += x[2 * i] + x[2 * i + 1];
       uint32_t first, second;
-      weight_parts<act_t>(x[2 * i], x[2 * i + 1], first, second);
+      if constexpr (W::SCALED) {
+        // numbers of 8 bits have no infinity that a weight of zero would hide
+        const float y0 = x[2 * i] * w.v_scale[i / 2][2 * (i & 1)], y1 = x[2 * i + 1] * w.v_scale[i / 2][2 * (i & 1) + 1];
+        first = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y1), __builtin_bit_cast(uint32_t, y0), 0x07060302u);
+        second = pack2<bf16_t>(y0 - lo16<bf16_t>(first), y1 - hi16<bf16_t>(first));
+      } else {
+        weight_parts<act_t>(x[2 * i], x[2 * i + 1], first, second);
+      }
       a[i] = first;
       b[i] = second;
     }
@@ -275,9 +342,9 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
 #pragma unroll
         for (int c = 0; c < W::CHUNKS; ++c)
 #pragma unroll
-          for (int j = 0; j < W::WORDS; ++j) odd |= partly ? not_finite<act_t>(w.v[i][c][j]) : 0u;
+          for (int j = 0; j < W::RAW_WORDS; ++j) odd |= !partly ? 0u : W::SCALED ? not_a_number8(w.v[i][c][j]) : not_finite<act_t>(w.v[i][c][j]);
       }
-      if (__ballot((odd & 0x80008000u) != 0) != 0) {
+      if (__ballot((odd & (W::SCALED ? 0x80808080u : 0x80008000u)) != 0) != 0) {
         stop = least;
         w.set_aside = w.set_aside < 0 ? key0 : w.set_aside | 1;
       }
@@ -296,11 +363,11 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
     for (int j = 0; j < W::TILES; ++j) {
       u32x4_t a;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(w.v[2 * i + 1][c][j / 2], w.v[2 * i][c][j / 2], select[j & 1][i]);
+      for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(w.value(2 * i + 1, c, j / 2), w.value(2 * i, c, j / 2), select[j & 1][i]);
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        w.o[t][c][j] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, a), high[t], w.o[t][c][j]);
-        w.o[t][c][j] = mfma_act<act_t>(__builtin_bit_cast(bf16x8_t, a), low[t], w.o[t][c][j]);
+        w.o[t][c][j] = mfma_act<value_t>(__builtin_bit_cast(bf16x8_t, a), high[t], w.o[t][c][j]);
+        w.o[t][c][j] = mfma_act<value_t>(__builtin_bit_cast(bf16x8_t, a), low[t], w.o[t][c][j]);
       }
     }
   next_values();
@@ -308,23 +375,30 @@ __device__ __forceinline__ void attend(Wave<act_t, D, RT>& w, Queries queries, f
 
 // The weighted values of keys [first, last) into the D / TEAM channels of a row that a thread has (the sum has the weights already);
 // the TEAM threads of a row form its scores together.
-template <typename act_t, int D, int TEAM>
+template <typename act_t, typename kv_t, int D, int TEAM>
 __device__ __forceinline__ void add_set_aside(const PagedAttention& p, const PagedRequest& req, int kv_head, int row, int channel,
                                               const int32_t* pages, int first, int last, float top, float (&o)[D / TEAM]) {
   const int j = paged_quotient(p.shape.by_group, row), head = kv_head * p.shape.group + row - j * p.shape.group;
   const uint16_t* q = p.q + (req.begin + j) * p.q_token + head * p.q_head + channel;
+  using cached = Cached<act_t, kv_t>;
+  using value_t = typename cached::value_t;
+  const auto *keys = static_cast<const typename cached::raw_t*>(p.k), *values = static_cast<const typename cached::raw_t*>(p.v);
   last = min(last, paged_limit(p.shape, req, row));
   for (int key = first; key < last; ++key) {
-    const int page = paged_quotient(p.page_of, key);
-    int64_t at = paged_place(pages[page], key - page * p.block_size, p.blocks, p.kv_block, p.kv_token);
+    const int page = paged_quotient(p.page_of, key), place = key - page * p.block_size;
+    int64_t at = paged_place(pages[page], place, p.blocks, p.kv_block, p.kv_token);
     if (at < 0) continue;
     at += kv_head * p.kv_head + channel;
     float score = 0.f;
-    for (int i = 0; i < D / TEAM; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
-    score = (TEAM == 16 ? row16_allreduce(score) : row32_allreduce(score)) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
-    const float weight = fmaxf(__builtin_amdgcn_exp2f(score), LEAST_PART<act_t>);
+    for (int i = 0; i < D / TEAM; ++i) score = fmaf(to_float(act_t{q[i]}), cached_number<act_t>(keys + at + i), score);
+    score = TEAM == 16 ? row16_allreduce(score) : row32_allreduce(score);
+    const int64_t scale = cached::SCALED ? pages[page] * p.scale_block + kv_head * p.scale_head + place : 0;
+    if constexpr (cached::SCALED) score *= p.k_scales[scale];
+    score = score * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<value_t>);
+    float weight = fmaxf(__builtin_amdgcn_exp2f(score), LEAST_PART<value_t>);
+    if constexpr (cached::SCALED) weight *= p.v_scales[scale];
 #pragma unroll
-    for (int i = 0; i < D / TEAM; ++i) o[i] = fmaf(weight, to_float(act_t{p.v[at + i]}), o[i]);
+    for (int i = 0; i < D / TEAM; ++i) o[i] = fmaf(weight, cached_number<act_t>(values + at + i), o[i]);
   }
 }
 
@@ -361,9 +435,49 @@ struct Part {
   const int32_t* pages;
 };
 
+// What a row has of the prefix, joined with what it has of its own keys: first the common reference and the factors of what stands in
+// registers, then a piece at a time.  A row that sees no key of its own (sum 0) has no part in the prefix.
+struct PrefixPieces {
+  int pieces;                                     // 0: none
+  float reference, own;
+  int64_t row, step;                              // of the row in the first piece, to the next piece
+};
+template <typename value_t>
+__device__ __forceinline__ PrefixPieces prefix_pieces(const PagedAttention& p, int64_t token, int head, float top, float& sum) {
+  PrefixPieces x{0, top - WEIGHT_SHIFT<value_t>, 1.f, 0, 0};
+  if (!p.prefix_tops || sum == 0.f) return x;
+  const int64_t length = p.at(p.prefix_len, p.prefix_len_wide, 0);
+  const int keys = (int)(length < 0 ? 0 : length < p.prefix_positions ? length : p.prefix_positions), heads = p.shape.heads * p.shape.group;
+  x.pieces = keys == 0 ? 0 : prompt_share(keys, p.prefix_splits).pieces;
+  x.step = (int64_t)p.shape.tokens * heads;
+  x.row = token * heads + head;
+  const float before = x.reference;
+  for (int i = 0; i < x.pieces; ++i) x.reference = fmaxf(x.reference, p.prefix_tops[x.row + i * x.step].x);
+  x.own = rescale(before, x.reference);
+  sum *= x.own;
+  for (int i = 0; i < x.pieces; ++i) {
+    const float2 y = p.prefix_tops[x.row + i * x.step];
+    sum = fmaf(y.y, rescale(y.x, x.reference), sum);
+  }
+  return x;
+}
+template <int CHANNELS>
+__device__ __forceinline__ void add_prefix(const PagedAttention& p, const PrefixPieces& x, int D, int channel, float (&o)[CHANNELS]) {
+  if (x.pieces == 0) return;
+#pragma unroll
+  for (int i = 0; i < CHANNELS; ++i) o[i] *= x.own;
+  for (int n = 0; n < x.pieces; ++n) {
+    const float f = rescale(p.prefix_tops[x.row + n * x.step].x, x.reference);
+    const float* part = p.prefix + (x.row + n * x.step) * D + channel;
+#pragma unroll
+    for (int i = 0; i < CHANNELS; ++i) o[i] = fmaf(part[i], f, o[i]);
+  }
+}
+
 // CHANNELS channels of a row's output from their sums.
-template <typename act_t, int CHANNELS>
-__device__ __forceinline__ void write_row(const PagedAttention& p, int64_t token, int head, int channel, float sum, const float (&o)[CHANNELS]) {
+template <typename act_t, int D, int CHANNELS>
+__device__ __forceinline__ void write_row(const PagedAttention& p, int64_t token, int head, int channel, float top, float sum, float (&o)[CHANNELS]) {
+  if (p.prefix_tops) add_prefix(p, prefix_pieces<act_t>(p, token, head, top, sum), D, channel, o);
   const float norm = sum == 0.f ? 0.f : 1.0f / sum;         // no key: zeros
   uint32_t word[CHANNELS / 2];
 #pragma unroll
@@ -383,25 +497,32 @@ __device__ __forceinline__ void write_row(const PagedAttention& p, int64_t token
 
 // The same as add_set_aside for all 16 rows at once, by a wavefront alone: lane (r, kb) has a quarter of row r's channels, from
 // `o` on in LDS.  row < 0: none.
-template <typename act_t, int D>
+template <typename act_t, typename kv_t, int D>
 __device__ __forceinline__ void add_set_aside_alone(const PagedAttention& p, const PagedRequest& req, int kv_head, int row, int kb,
                                                     const int32_t* pages, int first, int last, float top, float* o) {
   const int j = row < 0 ? 0 : paged_quotient(p.shape.by_group, row), head = kv_head * p.shape.group + (row < 0 ? 0 : row - j * p.shape.group);
   const uint16_t* q = p.q + (req.begin + j) * p.q_token + head * p.q_head + kb * (D / 4);
+  using cached = Cached<act_t, kv_t>;
+  using value_t = typename cached::value_t;
+  const auto *keys = static_cast<const typename cached::raw_t*>(p.k), *values = static_cast<const typename cached::raw_t*>(p.v);
   const int limit = row < 0 ? 0 : paged_limit(p.shape, req, row);
   for (int key = first; key < last; ++key) {
-    const int page = paged_quotient(p.page_of, key);
-    int64_t at = paged_place(pages[page], key - page * p.block_size, p.blocks, p.kv_block, p.kv_token);
+    const int page = paged_quotient(p.page_of, key), place = key - page * p.block_size;
+    int64_t at = paged_place(pages[page], place, p.blocks, p.kv_block, p.kv_token);
     if (at < 0) continue;
     at += kv_head * p.kv_head + kb * (D / 4);
     float score = 0.f;
 #pragma nounroll
-    for (int i = 0; i < D / 4; ++i) score = fmaf(to_float(act_t{q[i]}), to_float(act_t{p.k[at + i]}), score);
-    score = query_sum(score) * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<act_t>);
+    for (int i = 0; i < D / 4; ++i) score = fmaf(to_float(act_t{q[i]}), cached_number<act_t>(keys + at + i), score);
+    score = query_sum(score);
+    const int64_t scale = cached::SCALED ? pages[page] * p.scale_block + kv_head * p.scale_head + place : 0;
+    if constexpr (cached::SCALED) score *= p.k_scales[scale];
+    score = score * p.scale_log2 - ((top == -INFINITY ? 0.f : top) - WEIGHT_SHIFT<value_t>);
     if (key >= limit) continue;
-    const float weight = fmaxf(__builtin_amdgcn_exp2f(score), LEAST_PART<act_t>);
+    float weight = fmaxf(__builtin_amdgcn_exp2f(score), LEAST_PART<value_t>);
+    if constexpr (cached::SCALED) weight *= p.v_scales[scale];
 #pragma nounroll
-    for (int i = 0; i < D / 4; ++i) o[kb * (D / 4) + i] = fmaf(weight, to_float(act_t{p.v[at + i]}), o[kb * (D / 4) + i]);
+    for (int i = 0; i < D / 4; ++i) o[kb * (D / 4) + i] = fmaf(weight, cached_number<act_t>(values + at + i), o[kb * (D / 4) + i]);
   }
 }
 
@@ -489,9 +610,10 @@ struct PieceOfRun {
   int64_t last;                           // unit of the line
 };
 
-template <typename act_t, int D, int RT, bool ALONE>
+template <typename act_t, typename kv_t, int D, int RT, bool ALONE>
 __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) / 4) void paged_attention_kernel(const PagedAttention p) {
-  using W = Wave<act_t, D, RT>;
+  using W = Wave<act_t, kv_t, D, RT>;
+  using raw_t = typename W::raw_t;
   constexpr int WAVES = waves(D, RT), THREADS = 64 * WAVES, TILE = 32 * WAVES;
   constexpr int TEAM = THREADS / 16, CHANNELS = D / TEAM;       // threads that put a row's outputs together, and channels of each
   constexpr int PITCH = D + 4;                    // floats of a row in LDS: rows of a quad of lanes start in different banks
@@ -517,8 +639,12 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
   const int start = ALONE ? wave : 0;
   int n = __builtin_amdgcn_readfirstlane(room.index[start]);
 
-  const uint32_t key_lane = (uint32_t)(r * p.kv_token + 8 * kb) * 2;
-  const uint32_t value_lane = (uint32_t)(4 * kb * p.kv_token + W::LANE_CHANNELS * r) * 2;
+  const uint32_t key_lane = (uint32_t)(r * p.kv_token) * sizeof(raw_t) + 16 * kb;
+  const uint32_t value_lane = (uint32_t)(4 * kb * p.kv_token + W::LANE_CHANNELS * r) * sizeof(raw_t);
+  auto keys_of = [&](int head) { return static_cast<const raw_t*>(p.k) + head * p.kv_head; };
+  auto values_of = [&](int head) { return static_cast<const raw_t*>(p.v) + head * p.kv_head; };
+  auto key_scales_of = [&](int head) { return W::SCALED ? p.k_scales + head * p.scale_head : nullptr; };
+  auto value_scales_of = [&](int head) { return W::SCALED ? p.v_scales + head * p.scale_head : nullptr; };
 
   // The part of the stretch at `at` in request n, `req`.
   auto part_at = [&](const PagedRequest& req, const PagedStart& at) {
@@ -569,13 +695,14 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     }
     return x;
   };
-  auto place_of = [&](const Part& a, int step, const Entries& x, int64_t (&place)[2], bool (&there)[2]) {
+  auto place_of = [&](const Part& a, int step, const Entries& x, Places& place, bool (&there)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int key = a.key + step * STRIDE + 16 * h;
-      place[h] = paged_place(x.block[h], key - paged_quotient(p.page_of, key) * p.block_size, p.blocks, p.kv_block, p.kv_token);
-      there[h] = a.steps > 0 && key < a.end && place[h] >= 0;
-      if (!there[h]) place[h] = 0;
+      const int key = a.key + step * STRIDE + 16 * h, at = key - paged_quotient(p.page_of, key) * p.block_size;
+      place.at[h] = paged_place(x.block[h], at, p.blocks, p.kv_block, p.kv_token);
+      there[h] = a.steps > 0 && key < a.end && place.at[h] >= 0;
+      if (!there[h]) place.at[h] = 0;
+      place.scale[h] = W::SCALED && there[h] ? x.block[h] * p.scale_block + at : 0;
     }
   };
   // The queries: a wavefront alone keeps its operands, row r at channels 32 c + 8 kb, in registers.  Together a thread has pieces of
@@ -583,7 +710,8 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
   auto load_queries = [&](const Part& a, u32x4_t (&x)[MINE]) {
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
-      const int piece = tid + THREADS * i, row = ALONE ? r : piece / (D / 8), channel = ALONE ? 32 * i + 8 * kb : piece % (D / 8) * 8;
+      const int piece = tid + THREADS * i, row = ALONE ? r : piece / (D / 8);
+      const int channel = !ALONE ? piece % (D / 8) * 8 : W::SCALED ? 64 * (i / 2) + 16 * kb + 8 * (i & 1) : 32 * i + 8 * kb;
       x[i] = u32x4_t{0, 0, 0, 0};
       if (row < a.rows) {
         const int j = paged_quotient(p.shape.by_group, a.row0 + row), g = a.row0 + row - j * p.shape.group;
@@ -595,13 +723,15 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
       const int piece = tid + THREADS * i, row = piece / (D / 8), chunk = piece % (D / 8);
-      if (piece < PIECES) queries[((row >> 4) * W::STEPS + (chunk >> 2)) * 64 + 16 * (chunk & 3) + (row & 15)] = x[i];
+      // chunks of a step: those whose keys lie in one load of a lane (of 8-bit numbers, which are half as long, every other chunk)
+      const int step = W::SCALED ? (chunk >> 3) * 2 + (chunk & 1) : chunk >> 2, group = W::SCALED ? chunk >> 1 & 3 : chunk & 3;
+      if (piece < PIECES) queries[((row >> 4) * W::STEPS + step) * 64 + 16 * group + (row & 15)] = x[i];
     }
   };
 
   W w;
   u32x4_t q_words[MINE];
-  int64_t place[2], next_place[2];
+  Places place, next_place;
   bool there[2], next_there[2];
   if (ALONE && lane < 2) left[lane][wave] = PieceOfRun{};
   if (!ALONE || unit < stretch_end) {
@@ -610,10 +740,10 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
   const Entries entries = look_up(a, 0);
   if (a.steps > 0) {
     place_of(a, 0, entries, place, there);
-    load_keys(w, p.k + a.seg.head * p.kv_head, place, key_lane);
+    load_keys(w, keys_of(a.seg.head), key_scales_of(a.seg.head), place, key_lane);
   }
   load_queries(a, q_words);
-  if (a.steps > 0) load_values(w, p.v + a.seg.head * p.kv_head, place, value_lane, p.kv_token * 2);
+  if (a.steps > 0) load_values(w, values_of(a.seg.head), value_scales_of(a.seg.head), place, value_lane, p.kv_token * sizeof(raw_t));
   u32x4_t q_now[ALONE ? MINE : 1];
   if constexpr (ALONE) {
 #pragma unroll
@@ -658,21 +788,22 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       // The very last step fetches some block's first keys, the same for all, from the caches: a branch around the loads costs the
       // compiler the registers.
       // The entries for the step after next are asked for behind the keys of the next: a wait for queries in LDS is one for them too.
-      const int64_t head = (more ? a.seg.head : b.seg.head) * p.kv_head;
+      const int head = more ? a.seg.head : b.seg.head;
       attend(w, query, p.scale_log2, there, a.key + step * STRIDE, a.least, a.end,
              [&] {
                place_of(more ? a : b, more ? step + 1 : 0, coming, next_place, next_there);
-               load_keys(w, p.k + head, next_place, key_lane);
+               load_keys(w, keys_of(head), key_scales_of(head), next_place, key_lane);
                coming = step + 2 < a.steps ? look_up(a, step + 2) : look_up(b, 0);
              },
-             [&] { load_values(w, p.v + head, next_place, value_lane, p.kv_token * 2); });
+             [&] { load_values(w, values_of(head), value_scales_of(head), next_place, value_lane, p.kv_token * sizeof(raw_t)); });
+      place = next_place;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) { place[h] = next_place[h]; there[h] = next_there[h]; }
+      for (int h = 0; h < 2; ++h) there[h] = next_there[h];
     }
     if (a.steps == 0 && b.steps > 0) {
       place_of(b, 0, coming, place, there);
-      load_keys(w, p.k + b.seg.head * p.kv_head, place, key_lane);
-      load_values(w, p.v + b.seg.head * p.kv_head, place, value_lane, p.kv_token * 2);
+      load_keys(w, keys_of(b.seg.head), key_scales_of(b.seg.head), place, key_lane);
+      load_values(w, values_of(b.seg.head), value_scales_of(b.seg.head), place, value_lane, p.kv_token * sizeof(raw_t));
     }
 
     if constexpr (ALONE) {
@@ -694,7 +825,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
         float* mine = &outs[1][wave][r][0];               // not in use before the wavefront's last run
         park(mine);
         own_lds_order();
-        add_set_aside_alone<act_t, D>(p, a.req, a.seg.head, r < a.rows ? row : -1, kb, a.pages, max(w.set_aside & ~31, a.least),
+        add_set_aside_alone<act_t, kv_t, D>(p, a.req, a.seg.head, r < a.rows ? row : -1, kb, a.pages, max(w.set_aside & ~31, a.least),
                                       min((w.set_aside & ~31) + (w.set_aside & 1 ? 64 : 32), a.end), w.top[0], mine);
         own_lds_order();
 #pragma unroll
@@ -707,8 +838,22 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       }
       if (a.seg.tiles == a.req.tiles) {
         if (r < a.rows) {
-          const float norm = sum == 0.f ? 0.f : 1.0f / sum;         // no key: zeros
           const int64_t token = a.req.begin + j;
+          if (p.prefix_tops) {
+            const PrefixPieces pieces = prefix_pieces<act_t>(p, token, head, w.top[0], sum);
+#pragma unroll
+            for (int c = 0; c < W::CHUNKS; ++c)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float y[W::TILES];
+#pragma unroll
+                for (int x = 0; x < W::TILES; ++x) y[x] = w.o[0][c][x][e];
+                add_prefix(p, pieces, D, channel_of(c, e), y);
+#pragma unroll
+                for (int x = 0; x < W::TILES; ++x) w.o[0][c][x][e] = y[x];
+              }
+          }
+          const float norm = sum == 0.f ? 0.f : 1.0f / sum;         // no key: zeros
 #pragma unroll
           for (int c = 0; c < W::CHUNKS; ++c)
 #pragma unroll
@@ -782,10 +927,10 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
         const int row = a.row0 + 16 * t + out_row;
         for (int x = 0; x < WAVES; ++x)
           if (aside[x] >= 0)
-            add_set_aside<act_t, D, TEAM>(p, a.req, a.seg.head, row, out_channel, a.pages, max(aside[x], a.least), min(aside[x] + 32, a.end), row_top, o);
+            add_set_aside<act_t, kv_t, D, TEAM>(p, a.req, a.seg.head, row, out_channel, a.pages, max(aside[x], a.least), min(aside[x] + 32, a.end), row_top, o);
         if (a.seg.slot < 0) {
           const int j = paged_quotient(p.shape.by_group, row), head = a.seg.head * p.shape.group + row - j * p.shape.group;
-          write_row<act_t, CHANNELS>(p, a.req.begin + j, head, out_channel, row_sum, o);
+          write_row<act_t, D, CHANNELS>(p, a.req.begin + j, head, out_channel, row_top, row_sum, o);
         } else {
           const int64_t at = (int64_t)a.seg.slot * (16 * RT) + 16 * t + out_row;
 #pragma unroll
@@ -853,7 +998,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
         }
         if (g >= 0 && !open) {
           const int row = row0 + mine, j = paged_quotient(p.shape.by_group, row), head = run.head * p.shape.group + row - j * p.shape.group;
-          write_row<act_t, 8>(p, run.begin + j, head, channel, row_sum, o);
+          write_row<act_t, D, 8>(p, run.begin + j, head, channel, row_top, row_sum, o);
         } else {
           const int64_t at = (int64_t)(2 * worker + (g >= 0)) * 16 + mine;
           float4* dst = reinterpret_cast<float4*>(p.partial + at * D + channel);
@@ -939,11 +1084,14 @@ __global__ __launch_bounds__(64 * WAVES) void paged_join_kernel(const PagedAtten
       }
     }
     if (!PER_ROW || wave == 0) {
-      const float norm = sum == 0.f ? 0.f : 1.0f / sum;
       float x[LANE];
 #pragma unroll
+      for (int c = 0; c < LANE; ++c) x[c] = o[c];
+      if (p.prefix_tops) add_prefix(p, prefix_pieces<act_t>(p, token, head, top, sum), D, LANE * lane, x);
+      const float norm = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
       for (int c = 0; c < LANE; ++c) {
-        x[c] = o[c] * norm;
+        x[c] *= norm;
         if (p.gate) x[c] *= 1.0f / (1.0f + __expf(-to_float(act_t{gate[c]})));
       }
       uint16_t* dst = p.out + token * p.out_token + head * p.out_head + LANE * lane;
@@ -1005,16 +1153,23 @@ static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query
   return l;
 }
 
-template <typename act_t, int D>
+template <typename act_t, typename kv_t, int D>
 static void launch_paged_attention(const PagedAttention& p, const PagedLaunch& l, hipStream_t s) {
-  if (l.alone) paged_attention_kernel<act_t, D, 1, true><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
-  else if (l.row_tiles == 1) paged_attention_kernel<act_t, D, 1, false><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
-  else if (l.row_tiles == 2) paged_attention_kernel<act_t, D, 2, false><<<l.workers, 64 * waves(D, 2), 0, s>>>(p);
-  else if constexpr (D != 256) paged_attention_kernel<act_t, D, 4, false><<<l.workers, 64 * waves(D, 4), 0, s>>>(p);
+  if (l.alone) paged_attention_kernel<act_t, kv_t, D, 1, true><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
+  else if (l.row_tiles == 1) paged_attention_kernel<act_t, kv_t, D, 1, false><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
+  else if (l.row_tiles == 2) paged_attention_kernel<act_t, kv_t, D, 2, false><<<l.workers, 64 * waves(D, 2), 0, s>>>(p);
+  else if constexpr (D != 256) paged_attention_kernel<act_t, kv_t, D, 4, false><<<l.workers, 64 * waves(D, 4), 0, s>>>(p);
   if (!l.split) return;
   const dim3 grid((unsigned)(l.by_run ? l.runs : l.workers), l.join_rows);
   if (l.per_row) paged_join_kernel<act_t, D, true, 16><<<grid, 1024, 0, s>>>(p);
   else paged_join_kernel<act_t, D, false, 4><<<grid, 256, 0, s>>>(p);
+}
+
+template <typename act_t, typename kv_t>
+static void launch_paged_attention(const PagedAttention& p, const PagedLaunch& l, int D, hipStream_t s) {
+  if (D == 64) launch_paged_attention<act_t, kv_t, 64>(p, l, s);
+  else if (D == 128) launch_paged_attention<act_t, kv_t, 128>(p, l, s);
+  else launch_paged_attention<act_t, kv_t, 256>(p, l, s);
 }
 
 static int check_shape(int batch, int HQ, int HKV, int D, int max_query, int64_t positions) {
@@ -1072,15 +1227,28 @@ extern "C" int pla_paged_attention_segments(
   return found;
 }
 
-extern "C" int pla_paged_attention_launch(
+namespace pla {
+
+// What a call has beyond the plain one: factors of a cache of 8-bit numbers, a prefix that all rows share.
+struct PagedExtras {
+  const float *k_scales, *v_scales;
+  int64_t scale_block, scale_head;
+  const int32_t* prefix_blocks;
+  int prefix_pages;
+  const void* prefix_len;
+  int prefix_len_wide;
+};
+
+static int64_t prefix_bytes(const PromptLaunch& l, int64_t tokens, int HQ, int D) { return prompt_bytes(l, tokens, HQ, D, true); }
+
+static int paged_attention(
     const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,
     int64_t kv_block, int64_t kv_token, int64_t kv_head, int blocks, int block_size,
     const int32_t* block_table, int64_t table_row_stride, int table_rows, int table_cols,
     const void* mapping, int mapping_wide, const void* offsets, int offsets_wide, const void* seq_lens, int seq_lens_wide,
     const void* gate, int64_t gate_token, int64_t gate_head, void* out, int64_t out_token, int64_t out_head,
-    float scale, int batch, int tokens, int max_query_len, int HQ, int HKV, int head_dim, int act_dtype,
+    float scale, int batch, int tokens, int max_query_len, int HQ, int HKV, int head_dim, int act_dtype, const PagedExtras& extras,
     void* workspace, int64_t workspace_bytes, void* stream) {
-  using namespace pla;
   PLA_REQUIRE(block_size > 0 && block_size % 16 == 0, "block_size must be a multiple of 16");
   const int64_t positions = (int64_t)table_cols * block_size;
   if (const int bad = check_shape(batch, HQ, HKV, head_dim, max_query_len, positions)) return bad;
@@ -1093,31 +1261,137 @@ extern "C" int pla_paged_attention_launch(
   PLA_REQUIRE(q && k_cache && v_cache && seq_lens && out, "null tensor pointer");
   PLA_REQUIRE(block_table || table_rows == 0 || table_cols == 0, "null tensor pointer");
   PLA_REQUIRE(blocks > 0, "the cache must hold a block");
+  const bool scaled = extras.k_scales != nullptr;
   for (const int64_t s : {q_token, q_head, kv_block, kv_token, kv_head, gate_token, gate_head, out_token, out_head})
     PLA_REQUIRE(s % 8 == 0, "rows must be 16-byte aligned");
   for (const void* x : {q, k_cache, v_cache, gate, (const void*)out})
     PLA_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0, "rows must be 16-byte aligned");
+  if (scaled) {
+    for (const int64_t s : {kv_block, kv_token, kv_head}) PLA_REQUIRE(s % 16 == 0, "rows must be 16-byte aligned");
+    PLA_REQUIRE(extras.v_scales && extras.scale_block % 4 == 0 && extras.scale_head % 4 == 0 &&
+                    (reinterpret_cast<uintptr_t>(extras.k_scales) | reinterpret_cast<uintptr_t>(extras.v_scales)) % 16 == 0,
+                "scales of a block's head must be 16-byte aligned");
+  }
   PLA_REQUIRE(kv_token >= 0 && kv_token < (1 << 24), "the cache's token stride must be below 2^24");
   const PagedLaunch l = paged_launch(batch, HQ, HKV, head_dim, max_query_len, positions);
-  PLA_REQUIRE(workspace_bytes >= l.bytes && (l.bytes == 0 || workspace), "workspace too small: %lld bytes needed", (long long)l.bytes);
-  PLA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be 16-byte aligned");
   char* ws = static_cast<char*>(workspace);
-  const PagedAttention p{(const uint16_t*)q, q_token, q_head, (const uint16_t*)k_cache, (const uint16_t*)v_cache, kv_block, kv_token,
-                         kv_head, block_table, table_row_stride, mapping, mapping_wide, offsets, offsets_wide, seq_lens, seq_lens_wide,
-                         (const uint16_t*)gate, gate_token, gate_head, (uint16_t*)out, out_token, out_head,
-                         PagedShape{HKV, HQ / HKV, paged_divisor(HQ / HKV), bits_of(l.rows), bits_of(l.tile), l.units, l.extra, max_query_len, tokens, positions},
-                         batch, blocks, block_size, table_rows, paged_divisor(block_size), scale * 1.44269504088896341f, l.by_run, l.row_blocks,
-                         l.split ? reinterpret_cast<float*>(ws) : nullptr, l.split ? reinterpret_cast<float2*>(ws + l.tops_at) : nullptr,
-                         l.split ? reinterpret_cast<PagedRun*>(ws + l.runs_at) : nullptr};
+  PLA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be 16-byte aligned");
+  PagedAttention p{};
+  int64_t taken = 0;
+  if (extras.prefix_len) {
+    PLA_REQUIRE(!scaled, "a shared prefix stands in a cache of the queries' type");
+    PLA_REQUIRE(extras.prefix_pages >= 0 && (int64_t)extras.prefix_pages * block_size <= (1 << 30), "a prefix must have at most 2^30 positions");
+    PLA_REQUIRE(extras.prefix_blocks || extras.prefix_pages == 0, "null tensor pointer");
+    if (const int bad = check_prompt(1, tokens, HQ, HKV, head_dim)) return bad;
+    PromptAttention x{};
+    x.q = (const uint16_t*)q; x.q_token = q_token; x.q_head = q_head;
+    x.k = (const uint16_t*)k_cache; x.k_token = kv_token; x.k_head = kv_head;
+    x.v = (const uint16_t*)v_cache; x.v_token = kv_token; x.v_head = kv_head;
+    x.kv_block = kv_block; x.blocks = blocks; x.block_size = block_size; x.page_of = paged_divisor(block_size);
+    x.table = extras.prefix_blocks; x.table_rows = extras.prefix_pages ? 1 : 0;
+    x.lengths = extras.prefix_len; x.lengths_wide = extras.prefix_len_wide;
+    x.batch = 1; x.tokens = tokens; x.heads = HKV; x.group = HQ / HKV; x.by_group = paged_divisor(HQ / HKV);
+    x.positions = (int64_t)extras.prefix_pages * block_size;
+    const PromptLaunch prompt = prompt_launch(1, tokens, HQ, HKV, head_dim, x.positions);
+    taken = prefix_bytes(prompt, tokens, HQ, head_dim);
+    if (const int bad = launch_prompt(x, prompt, true, HQ, head_dim, scale, act_dtype, workspace, workspace_bytes - l.bytes, static_cast<hipStream_t>(stream)))
+      return bad;
+    p.prefix = reinterpret_cast<const float*>(ws);
+    p.prefix_tops = reinterpret_cast<const float2*>(ws + prompt_tops_at(prompt, tokens, HQ, head_dim));
+    p.prefix_len = extras.prefix_len; p.prefix_len_wide = extras.prefix_len_wide;
+    p.prefix_splits = prompt.splits; p.prefix_positions = x.positions;
+  }
+  PLA_REQUIRE(workspace_bytes >= taken + l.bytes && (taken + l.bytes == 0 || workspace), "workspace too small: %lld bytes needed", (long long)(taken + l.bytes));
+  ws += taken;
+  p.q = (const uint16_t*)q; p.q_token = q_token; p.q_head = q_head;
+  p.k = k_cache; p.v = v_cache; p.kv_block = kv_block; p.kv_token = kv_token; p.kv_head = kv_head;
+  p.k_scales = extras.k_scales; p.v_scales = extras.v_scales; p.scale_block = extras.scale_block; p.scale_head = extras.scale_head;
+  p.table = block_table; p.table_row = table_row_stride;
+  p.mapping = mapping; p.mapping_wide = mapping_wide;
+  p.offsets = offsets; p.offsets_wide = offsets_wide;
+  p.lengths = seq_lens; p.lengths_wide = seq_lens_wide;
+  p.gate = (const uint16_t*)gate; p.gate_token = gate_token; p.gate_head = gate_head;
+  p.out = (uint16_t*)out; p.out_token = out_token; p.out_head = out_head;
+  p.shape = PagedShape{HKV, HQ / HKV, paged_divisor(HQ / HKV), bits_of(l.rows), bits_of(l.tile), l.units, l.extra, max_query_len, tokens, positions};
+  p.batch = batch; p.blocks = blocks; p.block_size = block_size; p.table_rows = table_rows;
+  p.page_of = paged_divisor(block_size);
+  p.scale_log2 = scale * 1.44269504088896341f;
+  p.by_run = l.by_run; p.row_blocks = l.row_blocks;
+  if (l.split) {
+    p.partial = reinterpret_cast<float*>(ws);
+    p.tops = reinterpret_cast<float2*>(ws + l.tops_at);
+    p.runs = reinterpret_cast<PagedRun*>(ws + l.runs_at);
+  }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (act_dtype == PLA_BF16) {
-    if (head_dim == 64) launch_paged_attention<bf16_t, 64>(p, l, s);
-    else if (head_dim == 128) launch_paged_attention<bf16_t, 128>(p, l, s);
-    else launch_paged_attention<bf16_t, 256>(p, l, s);
+    if (scaled) launch_paged_attention<bf16_t, e4m3_t>(p, l, head_dim, s);
+    else launch_paged_attention<bf16_t, bf16_t>(p, l, head_dim, s);
   } else {
-    if (head_dim == 64) launch_paged_attention<f16_t, 64>(p, l, s);
-    else if (head_dim == 128) launch_paged_attention<f16_t, 128>(p, l, s);
-    else launch_paged_attention<f16_t, 256>(p, l, s);
+    if (scaled) launch_paged_attention<f16_t, e4m3_t>(p, l, head_dim, s);
+    else launch_paged_attention<f16_t, f16_t>(p, l, head_dim, s);
   }
   return check_launch("paged_attention_kernel");
+}
+
+}  // namespace pla
+
+extern "C" int pla_paged_attention_launch(
+    const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,
+    int64_t kv_block, int64_t kv_token, int64_t kv_head, int blocks, int block_size,
+    const int32_t* block_table, int64_t table_row_stride, int table_rows, int table_cols,
+    const void* mapping, int mapping_wide, const void* offsets, int offsets_wide, const void* seq_lens, int seq_lens_wide,
+    const void* gate, int64_t gate_token, int64_t gate_head, void* out, int64_t out_token, int64_t out_head,
+    float scale, int batch, int tokens, int max_query_len, int HQ, int HKV, int head_dim, int act_dtype,
+    void* workspace, int64_t workspace_bytes, void* stream) {
+  return pla::paged_attention(q, q_token, q_head, k_cache, v_cache, kv_block, kv_token, kv_head, blocks, block_size, block_table, table_row_stride,
+                              table_rows, table_cols, mapping, mapping_wide, offsets, offsets_wide, seq_lens, seq_lens_wide, gate, gate_token,
+                              gate_head, out, out_token, out_head, scale, batch, tokens, max_query_len, HQ, HKV, head_dim, act_dtype,
+                              pla::PagedExtras{}, workspace, workspace_bytes, stream);
+}
+
+extern "C" int pla_paged_attention_fp8_launch(
+    const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,
+    int64_t kv_block, int64_t kv_token, int64_t kv_head, int blocks, int block_size,
+    const float* k_scales, const float* v_scales, int64_t scale_block, int64_t scale_head,
+    const int32_t* block_table, int64_t table_row_stride, int table_rows, int table_cols,
+    const void* mapping, int mapping_wide, const void* offsets, int offsets_wide, const void* seq_lens, int seq_lens_wide,
+    const void* gate, int64_t gate_token, int64_t gate_head, void* out, int64_t out_token, int64_t out_head,
+    float scale, int batch, int tokens, int max_query_len, int HQ, int HKV, int head_dim, int act_dtype,
+    void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace pla;
+  PLA_REQUIRE(k_scales && v_scales, "null tensor pointer");
+  PagedExtras extras{};
+  extras.k_scales = k_scales; extras.v_scales = v_scales; extras.scale_block = scale_block; extras.scale_head = scale_head;
+  return paged_attention(q, q_token, q_head, k_cache, v_cache, kv_block, kv_token, kv_head, blocks, block_size, block_table, table_row_stride,
+                         table_rows, table_cols, mapping, mapping_wide, offsets, offsets_wide, seq_lens, seq_lens_wide, gate, gate_token,
+                         gate_head, out, out_token, out_head, scale, batch, tokens, max_query_len, HQ, HKV, head_dim, act_dtype,
+                         extras, workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t pla_paged_attention_prefix_workspace_bytes(int batch, int tokens, int HQ, int HKV, int head_dim, int max_query_len, int64_t positions,
+                                                              int64_t prefix_positions) {
+  using namespace pla;
+  if (check_shape(batch, HQ, HKV, head_dim, max_query_len, positions) || check_prompt(1, tokens, HQ, HKV, head_dim) || prefix_positions < 0) return -1;
+  if (batch == 0 || tokens == 0) return 0;
+  return paged_launch(batch, HQ, HKV, head_dim, max_query_len, positions).bytes +
+         prefix_bytes(prompt_launch(1, tokens, HQ, HKV, head_dim, prefix_positions), tokens, HQ, head_dim);
+}
+
+extern "C" int pla_paged_attention_prefix_launch(
+    const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,
+    int64_t kv_block, int64_t kv_token, int64_t kv_head, int blocks, int block_size,
+    const int32_t* prefix_blocks, int prefix_pages, const void* prefix_len, int prefix_len_wide,
+    const int32_t* block_table, int64_t table_row_stride, int table_rows, int table_cols,
+    const void* mapping, int mapping_wide, const void* offsets, int offsets_wide, const void* seq_lens, int seq_lens_wide,
+    const void* gate, int64_t gate_token, int64_t gate_head, void* out, int64_t out_token, int64_t out_head,
+    float scale, int batch, int tokens, int max_query_len, int HQ, int HKV, int head_dim, int act_dtype,
+    void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace pla;
+  PLA_REQUIRE(prefix_len, "null tensor pointer");
+  PagedExtras extras{};
+  extras.prefix_blocks = prefix_blocks; extras.prefix_pages = prefix_pages; extras.prefix_len = prefix_len; extras.prefix_len_wide = prefix_len_wide;
+  return paged_attention(q, q_token, q_head, k_cache, v_cache, kv_block, kv_token, kv_head, blocks, block_size, block_table, table_row_stride,
+                         table_rows, table_cols, mapping, mapping_wide, offsets, offsets_wide, seq_lens, seq_lens_wide, gate, gate_token,
+                         gate_head, out, out_token, out_head, scale, batch, tokens, max_query_len, HQ, HKV, head_dim, act_dtype,
+                         extras, workspace, workspace_bytes, stream);
 }

@@ -197,10 +197,20 @@ void cache_form(const Tensor& t, const char* name, int64_t heads, int64_t D, at:
   TORCH_CHECK(t.dim() == 4 && t.size(2) == heads && t.size(3) == D, name, " must be [blocks, block_size, ", heads, ", ", D, "], got ", t.sizes());
   TORCH_CHECK(t.scalar_type() == act, name, " must be ", act, ", got ", t.scalar_type());
   TORCH_CHECK(t.size(0) > 0 && t.size(1) > 0, name, " must hold at least one block");
-  TORCH_CHECK(t.stride(3) == 1 && step(t, 0) % 8 == 0 && step(t, 1) % 8 == 0 && step(t, 2) % 8 == 0 &&
+  const int64_t unit = 16 / t.element_size();
+  TORCH_CHECK(t.stride(3) == 1 && step(t, 0) % unit == 0 && step(t, 1) % unit == 0 && step(t, 2) % unit == 0 &&
                   reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
               name, " must have dense channels and 16-byte aligned rows");
   TORCH_CHECK(t.size(0) * t.size(1) <= INT32_MAX, name, " must have at most 2^31 - 1 slots");
+}
+
+// Scales of a cache of 8-bit numbers, [blocks, heads, block_size] float32.
+void scales_form(const Tensor& t, const char* name, const Tensor& cache) {
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == cache.size(0) && t.size(1) == cache.size(2) && t.size(2) == cache.size(1), name, " must be [",
+              cache.size(0), ", ", cache.size(2), ", ", cache.size(1), "], got ", t.sizes());
+  TORCH_CHECK(t.scalar_type() == at::kFloat, name, " must be float32, got ", t.scalar_type());
+  TORCH_CHECK((t.size(2) == 1 || t.stride(2) == 1) && step(t, 0) % 4 == 0 && step(t, 1) % 4 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              name, " must have dense places and 16-byte aligned heads");
 }
 
 // Caches that attention reads.
@@ -219,7 +229,8 @@ void cache_pair(const Tensor& k_cache, const Tensor& v_cache, int64_t heads, int
 std::tuple<Tensor, OptTensor> fused_qk_norm_rope(
     const Tensor& q, const Tensor& k, const OptTensor& positions_in, const OptTensor& q_weight, const OptTensor& k_weight, double eps,
     double weight_offset, const OptTensor& inv_freq, double attention_factor, bool interleaved, const OptTensor& q_out_in,
-    const OptTensor& k_out_in, const OptTensor& v, const OptTensor& k_cache, const OptTensor& v_cache, const OptTensor& slots_in) {
+    const OptTensor& k_out_in, const OptTensor& v, const OptTensor& k_cache, const OptTensor& v_cache, const OptTensor& slots_in,
+    const OptTensor& k_scales, const OptTensor& v_scales) {
   TORCH_CHECK(q.dim() == 3 && k.dim() == 3, "q and k must be [tokens, heads, head_dim]");
   const int64_t T = q.size(0), HQ = q.size(1), HKV = k.size(1), D = q.size(2);
   TORCH_CHECK(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got ", D);
@@ -251,13 +262,18 @@ std::tuple<Tensor, OptTensor> fused_qk_norm_rope(
   TORCH_CHECK(k_cache.has_value() == slots_in.has_value(), "k_cache and slot_mapping come together");
   TORCH_CHECK(v_cache.has_value() == v.has_value() && (!v || k_cache), "v comes with v_cache, and both with k_cache");
   OptTensor slots;
+  const at::ScalarType stored = k_scales ? at::kFloat8_e4m3fn : type;
+  TORCH_CHECK(!k_scales || k_cache, "k_scales come with k_cache");
+  TORCH_CHECK(v_scales.has_value() == (k_scales.has_value() && v.has_value()), "v_scales come with v and k_scales");
   if (k_cache) {
-    cache_form(*k_cache, "k_cache", HKV, D, type);
+    cache_form(*k_cache, "k_cache", HKV, D, stored);
+    if (k_scales) scales_form(*k_scales, "k_scales", *k_cache);
     slots = index_vector(*slots_in, "slot_mapping", T);
   }
   if (v) {
     head_rows(*v, "v", T, HKV, D, type);
-    cache_form(*v_cache, "v_cache", HKV, D, type);
+    cache_form(*v_cache, "v_cache", HKV, D, stored);
+    if (v_scales) scales_form(*v_scales, "v_scales", *v_cache);
     TORCH_CHECK(v_cache->size(0) == k_cache->size(0) && v_cache->size(1) == k_cache->size(1), "k_cache and v_cache must have the same blocks");
   }
   if (q_out_in) head_rows(*q_out_in, "q_out", T, HQ, D, type);
@@ -265,11 +281,11 @@ std::tuple<Tensor, OptTensor> fused_qk_norm_rope(
   const OptTensor qt(q), kt(k);
   on_one_gpu(q, "q", {{"k", &kt}, {"v", &v}, {"positions", &positions}, {"q_weight", &q_weight}, {"k_weight", &k_weight},
                       {"inv_freq", &inv_freq}, {"q_out", &q_out_in}, {"k_out", &k_out_in}, {"k_cache", &k_cache},
-                      {"v_cache", &v_cache}, {"slot_mapping", &slots}});
+                      {"v_cache", &v_cache}, {"slot_mapping", &slots}, {"k_scales", &k_scales}, {"v_scales", &v_scales}});
   // in place: the very rows of the input, each of which one group of lanes reads and writes
   const bool q_in_place = q_out_in && same_rows(*q_out_in, q), k_in_place = k_out_in && same_rows(*k_out_in, k);
   const OptTensor none, other_q = q_in_place ? none : qt, other_k = k_in_place ? none : kt;
-  apart({{"q_out", &q_out_in}, {"k_out", &k_out_in}, {"k_cache", &k_cache}, {"v_cache", &v_cache}},
+  apart({{"q_out", &q_out_in}, {"k_out", &k_out_in}, {"k_cache", &k_cache}, {"v_cache", &v_cache}, {"k_scales", &k_scales}, {"v_scales", &v_scales}},
         {{"q", &other_q}, {"k", &other_k}, {"v", &v}, {"positions", &positions}, {"q_weight", &q_weight}, {"k_weight", &k_weight},
          {"inv_freq", &inv_freq}, {"slot_mapping", &slots}});
   TORCH_CHECK(!q_in_place || !may_overlap(*q_out_in, k), "q_out must not share memory with k");
@@ -284,12 +300,22 @@ std::tuple<Tensor, OptTensor> fused_qk_norm_rope(
                                step(k_out, 0), step(k_out, 1), step(k_cache, 0), step(k_cache, 1), step(k_cache, 2),
                                step(v_cache, 0), step(v_cache, 1), step(v_cache, 2)};
   const bool f32 = (q_weight && q_weight->scalar_type() == at::kFloat) || (k_weight && k_weight->scalar_type() == at::kFloat);
-  launched(pla_qk_norm_rope_launch(
-      q.data_ptr(), k.data_ptr(), ptr(v), strides, ptr(positions), wide(positions), ptr(q_weight), ptr(k_weight), f32 ? 1 : 0, (float)eps,
-      (float)weight_offset, inv_freq ? inv_freq->data_ptr<float>() : nullptr, (int)rot, (float)attention_factor, interleaved ? 1 : 0,
-      q_out.data_ptr(), k_out ? k_out->data_ptr() : nullptr, k_cache ? k_cache->data_ptr() : nullptr,
-      v_cache ? v_cache->data_ptr() : nullptr, ptr(slots), wide(slots), k_cache ? (int)k_cache->size(0) : 0,
-      k_cache ? (int)k_cache->size(1) : 0, (int)T, (int)HQ, (int)HKV, (int)D, act, stream_of(q)));
+  const float* frequencies = inv_freq ? inv_freq->data_ptr<float>() : nullptr;
+  void *k_to = k_out ? k_out->data_ptr() : nullptr, *k_cached = k_cache ? k_cache->data_ptr() : nullptr, *v_cached = v_cache ? v_cache->data_ptr() : nullptr;
+  const int blocks = k_cache ? (int)k_cache->size(0) : 0, block_size = k_cache ? (int)k_cache->size(1) : 0;
+  if (k_scales) {
+    const int64_t scale_strides[4] = {step(k_scales, 0), step(k_scales, 1), step(v_scales, 0), step(v_scales, 1)};
+    launched(pla_qk_norm_rope_fp8_launch(
+        q.data_ptr(), k.data_ptr(), ptr(v), strides, ptr(positions), wide(positions), ptr(q_weight), ptr(k_weight), f32 ? 1 : 0, (float)eps,
+        (float)weight_offset, frequencies, (int)rot, (float)attention_factor, interleaved ? 1 : 0, q_out.data_ptr(), k_to, k_cached, v_cached,
+        k_scales->data_ptr<float>(), v_scales ? v_scales->data_ptr<float>() : nullptr, scale_strides, ptr(slots), wide(slots), blocks, block_size,
+        (int)T, (int)HQ, (int)HKV, (int)D, act, stream_of(q)));
+  } else {
+    launched(pla_qk_norm_rope_launch(
+        q.data_ptr(), k.data_ptr(), ptr(v), strides, ptr(positions), wide(positions), ptr(q_weight), ptr(k_weight), f32 ? 1 : 0, (float)eps,
+        (float)weight_offset, frequencies, (int)rot, (float)attention_factor, interleaved ? 1 : 0, q_out.data_ptr(), k_to, k_cached, v_cached,
+        ptr(slots), wide(slots), blocks, block_size, (int)T, (int)HQ, (int)HKV, (int)D, act, stream_of(q)));
+  }
   return {q_out, k_out};
 }
 
@@ -298,7 +324,8 @@ std::tuple<Tensor, OptTensor> fused_qk_norm_rope(
 Tensor paged_attention_decode(
     const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens_in,
     const OptTensor& offsets_in, const OptTensor& request_indices, int64_t max_query_len, std::optional<double> scale,
-    const OptTensor& output_gate, const OptTensor& out_in) {
+    const OptTensor& output_gate, const OptTensor& out_in, const OptTensor& k_scales, const OptTensor& v_scales, const OptTensor& prefix_blocks,
+    const OptTensor& prefix_len_in) {
   TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head_dim]");
   const int64_t T = q.size(0), HQ = q.size(1), D = q.size(2);
   TORCH_CHECK(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got ", D);
@@ -308,7 +335,22 @@ Tensor paged_attention_decode(
   TORCH_CHECK(k_cache.dim() == 4, "k_cache must be [blocks, block_size, heads, head_dim]");
   const int64_t HKV = k_cache.size(2), block_size = k_cache.size(1);
   TORCH_CHECK(HKV > 0 && HQ >= HKV && HQ % HKV == 0, "query heads must be a positive multiple of key-value heads, got ", HQ, " and ", HKV);
-  cache_pair(k_cache, v_cache, HKV, D, type);
+  TORCH_CHECK(k_scales.has_value() == v_scales.has_value(), "k_scales and v_scales come together");
+  cache_pair(k_cache, v_cache, HKV, D, k_scales ? at::kFloat8_e4m3fn : type);
+  if (k_scales) {
+    scales_form(*k_scales, "k_scales", k_cache);
+    scales_form(*v_scales, "v_scales", v_cache);
+    TORCH_CHECK(step(k_scales, 0) == step(v_scales, 0) && step(k_scales, 1) == step(v_scales, 1), "k_scales and v_scales must have the same strides");
+  }
+  TORCH_CHECK(prefix_blocks.has_value() == prefix_len_in.has_value(), "prefix_blocks and prefix_len come together");
+  TORCH_CHECK(!prefix_blocks || !k_scales, "a shared prefix stands in a cache of q's type");
+  OptTensor prefix_len;
+  if (prefix_blocks) {
+    TORCH_CHECK(prefix_blocks->dim() == 1 && prefix_blocks->scalar_type() == at::kInt && prefix_blocks->is_contiguous(), "prefix_blocks must be a contiguous int32 vector");
+    TORCH_CHECK(prefix_blocks->numel() * block_size <= (1 << 30), "a prefix must have at most 2^30 positions");
+    prefix_len = index_vector(*prefix_len_in, "prefix_len", 1);
+    TORCH_CHECK(T * HQ <= (1 << 30), "too many rows");
+  }
   block_table_form(block_table);
   const int64_t rows = block_table.size(0), cols = block_table.size(1);
   TORCH_CHECK(cols * block_size <= (1 << 30), "a row of the block table must hold at most 2^30 positions");
@@ -327,24 +369,37 @@ Tensor paged_attention_decode(
   if (out_in) head_rows(*out_in, "out", T, HQ, D, type);
   const OptTensor qt(q), kt(k_cache), vt(v_cache), table(block_table), lens(seq_lens);
   on_one_gpu(q, "q", {{"k_cache", &kt}, {"v_cache", &vt}, {"block_table", &table}, {"seq_lens", &lens}, {"query_start_loc", &offsets},
-                      {"request_indices", &mapping}, {"output_gate", &output_gate}, {"out", &out_in}});
+                      {"request_indices", &mapping}, {"output_gate", &output_gate}, {"out", &out_in}, {"k_scales", &k_scales}, {"v_scales", &v_scales},
+                      {"prefix_blocks", &prefix_blocks}, {"prefix_len", &prefix_len}});
   apart({{"out", &out_in}}, {{"q", &qt}, {"k_cache", &kt}, {"v_cache", &vt}, {"block_table", &table}, {"seq_lens", &lens},
-                             {"query_start_loc", &offsets}, {"request_indices", &mapping}, {"output_gate", &output_gate}});
+                             {"query_start_loc", &offsets}, {"request_indices", &mapping}, {"output_gate", &output_gate}, {"k_scales", &k_scales},
+                             {"v_scales", &v_scales}, {"prefix_blocks", &prefix_blocks}, {"prefix_len", &prefix_len}});
 
   const c10::DeviceGuard guard(q.device());
   Tensor out = out_in ? *out_in : at::empty({T, HQ, D}, q.options());
   if (bypass() || T == 0 || batch == 0) return out;
-  const int64_t bytes = pla_paged_attention_workspace_bytes(requests, heads, (int)HKV, (int)D, (int)max_query_len, cols * block_size);
+  const int64_t positions = cols * block_size;
+  const int64_t bytes = prefix_len ? pla_paged_attention_prefix_workspace_bytes(requests, tokens, heads, (int)HKV, (int)D, (int)max_query_len, positions,
+                                                                                prefix_blocks->numel() * block_size)
+                                   : pla_paged_attention_workspace_bytes(requests, heads, (int)HKV, (int)D, (int)max_query_len, positions);
   TORCH_CHECK(bytes >= 0, pla_last_error());
   Tensor workspace;
   if (bytes > 0) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
-  launched(pla_paged_attention_launch(
-      q.data_ptr(), step(q, 0), step(q, 1), k_cache.data_ptr(), v_cache.data_ptr(), step(k_cache, 0), step(k_cache, 1),
-      step(k_cache, 2), (int)k_cache.size(0), (int)block_size, block_table.data_ptr<int32_t>(), table_pitch(block_table), table_rows,
-      (int)cols, ptr(mapping), wide(mapping), ptr(offsets), wide(offsets), seq_lens.data_ptr(), wide(seq_lens), ptr(output_gate),
-      step(output_gate, 0), step(output_gate, 1), out.data_ptr(), step(out, 0), step(out, 1),
-      (float)scale.value_or(1.0 / std::sqrt((double)D)), requests, tokens, (int)max_query_len, heads, (int)HKV, (int)D, act,
-      bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(q)));
+  const float factor = (float)scale.value_or(1.0 / std::sqrt((double)D));
+  void* ws = bytes > 0 ? workspace.data_ptr() : nullptr;
+  const auto launch = [&](auto entry, auto... extras) {
+    launched(entry(q.data_ptr(), step(q, 0), step(q, 1), k_cache.data_ptr(), v_cache.data_ptr(), step(k_cache, 0), step(k_cache, 1), step(k_cache, 2),
+                   (int)k_cache.size(0), (int)block_size, extras..., block_table.data_ptr<int32_t>(), table_pitch(block_table), table_rows, (int)cols,
+                   ptr(mapping), wide(mapping), ptr(offsets), wide(offsets), seq_lens.data_ptr(), wide(seq_lens), ptr(output_gate),
+                   step(output_gate, 0), step(output_gate, 1), out.data_ptr(), step(out, 0), step(out, 1), factor, requests, tokens,
+                   (int)max_query_len, heads, (int)HKV, (int)D, act, ws, bytes, stream_of(q)));
+  };
+  if (k_scales)
+    launch(pla_paged_attention_fp8_launch, k_scales->data_ptr<float>(), v_scales->data_ptr<float>(), step(k_scales, 0), step(k_scales, 1));
+  else if (prefix_len)
+    launch(pla_paged_attention_prefix_launch, prefix_blocks->data_ptr<int32_t>(), (int)prefix_blocks->numel(), prefix_len->data_ptr(), wide(prefix_len));
+  else
+    launch(pla_paged_attention_launch);
   return out;
 }
 

@@ -37,5 +37,12 @@ PLA_HD PromptShare prompt_share(int keys, int splits) {
 
 struct PromptLaunch { int rows; int64_t blocks; int splits; };          // rows of a block, blocks at most, pieces of a block's keys at most
 PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, int64_t keys);
+int check_prompt(int batch, int64_t tokens, int HQ, int HKV, int D);
+// Workspace of the pieces: where their references and sums start behind the outputs, and all of it (`always`: where there is one piece too).
+int64_t prompt_tops_at(const PromptLaunch& l, int64_t tokens, int HQ, int D);
+int64_t prompt_bytes(const PromptLaunch& l, int64_t tokens, int HQ, int D, bool always);
+// Checks what is left of the arguments and launches.
+int launch_prompt(PromptAttention p, const PromptLaunch& l, bool paged, int HQ, int D, float scale, int act, void* workspace, int64_t workspace_bytes,
+                  hipStream_t s);
 
 }  // namespace pla

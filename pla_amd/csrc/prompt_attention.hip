@@ -511,7 +511,7 @@ PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, in
   return l;
 }
 
-static int check_prompt(int batch, int64_t tokens, int HQ, int HKV, int D) {
+int check_prompt(int batch, int64_t tokens, int HQ, int HKV, int D) {
   PLA_REQUIRE(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got %d", D);
   PLA_REQUIRE(HKV > 0 && HQ >= HKV && HQ % HKV == 0, "query heads must be a positive multiple of key-value heads");
   PLA_REQUIRE(batch >= 0 && tokens >= 0 && tokens * HQ <= (1 << 30), "too many rows");
@@ -519,13 +519,12 @@ static int check_prompt(int batch, int64_t tokens, int HQ, int HKV, int D) {
   return 0;
 }
 
-// Bytes of the pieces of a call: outputs, then maxima and sums.
-static int64_t prompt_tops_at(const PromptLaunch& l, int64_t tokens, int HQ, int D) { return l.splits * tokens * HQ * D * 4; }
-static int64_t prompt_bytes(const PromptLaunch& l, int64_t tokens, int HQ, int D, bool always) {
+int64_t prompt_tops_at(const PromptLaunch& l, int64_t tokens, int HQ, int D) { return l.splits * tokens * HQ * D * 4; }
+int64_t prompt_bytes(const PromptLaunch& l, int64_t tokens, int HQ, int D, bool always) {
   return l.splits > 1 || always ? (prompt_tops_at(l, tokens, HQ, D) + l.splits * tokens * HQ * 8 + 255) / 256 * 256 : 0;
 }
 
-static int launch_prompt(PromptAttention p, const PromptLaunch& l, bool paged, int HQ, int D, float scale, int act, void* workspace, int64_t workspace_bytes,
+int launch_prompt(PromptAttention p, const PromptLaunch& l, bool paged, int HQ, int D, float scale, int act, void* workspace, int64_t workspace_bytes,
                          hipStream_t s) {
   const int64_t bytes = prompt_bytes(l, p.tokens, HQ, D, !p.offsets);
   PLA_REQUIRE(workspace_bytes >= bytes && (bytes == 0 || workspace), "workspace too small: %lld bytes needed", (long long)bytes);

@@ -34,7 +34,9 @@ struct QkNormRope {
   const float* inv_freq; int rot; float attention_factor; int interleaved;
   uint16_t *q_out, *k_out;
   int64_t qo_token, qo_head, ko_token, ko_head;
-  uint16_t *k_cache, *v_cache;
+  void *k_cache, *v_cache;            // 16 bits a number, or 8
+  float *k_scales, *v_scales;         // of numbers of 8 bits: [block][head][place]
+  int64_t ks_block, ks_head, vs_block, vs_head;
   int64_t kc_block, kc_token, kc_head, vc_block, vc_token, vc_head;
   const void* slots; int slots_wide; int block, cache_slots;
   int tokens, HQ, HKV;
@@ -51,6 +53,38 @@ __device__ __forceinline__ float lanes_allreduce(float x) {
   x += dpp_mov<0x4E>(x);
   x += dpp_mov<0x141>(x);
   return x;
+}
+
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float x) {
+  x = fmaxf(x, dpp_mov<0xB1>(x));
+  x = fmaxf(x, dpp_mov<0x4E>(x));
+  x = fmaxf(x, dpp_mov<0x141>(x));
+  if constexpr (LANES >= 16) x = fmaxf(x, dpp_mov<0x140>(x));
+  if constexpr (LANES == 32) {
+    const LanePair r = swap_rows16(x);
+    x = fmaxf(r.lo, r.hi);
+  }
+  return x;
+}
+
+// A head in numbers of 8 bits: its largest magnitude becomes the largest e4m3 number, 448, and the others are rounded to nearest.  Returns the
+// eight numbers of this lane; `scale` is what the numbers stand for multiples of.  A NaN stays one, an infinity makes its head one.  The
+// scale starts from 1e-30, so that it has all its digits and a head of zeros has one.
+constexpr float LARGEST_E4M3 = 448.f, LEAST_MAGNITUDE = 1e-30f;
+template <int LANES>
+__device__ __forceinline__ uint2 quantise8(const float (&x)[8], float& scale) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+  scale = fmaxf(lanes_max<LANES>(top), LEAST_MAGNITUDE) / LARGEST_E4M3;
+  const float by = 1.0f / scale;
+  uint2 y;
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * by, x[1] * by, 0, false);
+  y.x = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * by, x[3] * by, w, true);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4] * by, x[5] * by, 0, false);
+  y.y = __builtin_amdgcn_cvt_pk_fp8_f32(x[6] * by, x[7] * by, w, true);
+  return y;
 }
 
 template <typename act_t>
@@ -99,7 +133,7 @@ __device__ __forceinline__ float part_of_turn(int64_t position, float frequency)
 constexpr int64_t PAST_CACHES = 48ll << 20;
 constexpr int WAVES_RESIDENT = 8192;  // on the chip, about
 
-template <typename act_t, int D, bool PAST>
+template <typename act_t, int D, bool PAST, bool CACHE8>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
   constexpr int LANES = D / 8, HEADS = 64 / LANES, AHEAD = 2;            // heads of a step, steps whose rows are asked for together
   __shared__ __align__(16) float turn[4][2][D / 2];                      // cosines and sines of a wavefront's token
@@ -198,12 +232,13 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
       if (step >= end) break;
       const int kind = kind_of(step), h = head_of(step, kind);
       uint4 result = now[a];
+      float x[8];
       if (kind < 2) {
         if (kind != prepared) {
           prepare(kind);
           prepared = kind;
         }
-        float x[8], y[8];
+        float y[8];
         widen8<act_t>(now[a], x);
         if (split) {
           uint4 other;
@@ -229,14 +264,31 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
         }
         result = make_uint4(pack2<act_t>(x[0], x[1]), pack2<act_t>(x[2], x[3]), pack2<act_t>(x[4], x[5]), pack2<act_t>(x[6], x[7]));
       }
+      // (all lanes of a row go through here: its heads are whole groups of them)
+      uint2 eight = {0, 0};
+      float scale = 0.f;
+      if constexpr (CACHE8) {
+        if (kind && slot >= 0) {
+          if (kind == 2) widen8<act_t>(now[a], x);
+          eight = quantise8<LANES>(x, scale);
+        }
+      }
       if (h >= (kind == 0 ? p.HQ : p.HKV)) continue;
       if (kind == 0) {
         store_row(p.q_out + token * p.qo_token + h * p.qo_head, result);
       } else {
         if (kind == 1 && p.k_out) store_row(p.k_out + token * p.ko_token + h * p.ko_head, result);
-        if (slot >= 0)
-          store_row(kind == 1 ? p.k_cache + block * p.kc_block + place * p.kc_token + h * p.kc_head
-                              : p.v_cache + block * p.vc_block + place * p.vc_token + h * p.vc_head, result);
+        if (slot >= 0) {
+          const int64_t at = kind == 1 ? block * p.kc_block + place * p.kc_token + h * p.kc_head : block * p.vc_block + place * p.vc_token + h * p.vc_head;
+          if constexpr (CACHE8) {
+            uint8_t* row = static_cast<uint8_t*>(kind == 1 ? p.k_cache : p.v_cache) + at + channel;
+            if (PAST) __builtin_nontemporal_store(__builtin_bit_cast(uint64_t, eight), reinterpret_cast<uint64_t*>(row));
+            else *reinterpret_cast<uint2*>(row) = eight;
+            if (lane == 0) (kind == 1 ? p.k_scales + block * p.ks_block + h * p.ks_head : p.v_scales + block * p.vs_block + h * p.vs_head)[place] = scale;
+          } else {
+            store_row(static_cast<uint16_t*>(kind == 1 ? p.k_cache : p.v_cache) + at, result);
+          }
+        }
       }
     }
   }
@@ -253,8 +305,13 @@ static void launch_qk_norm_rope(QkNormRope p, hipStream_t s) {
   p.chunk = (int)(share < p.steps ? share : p.steps);
   p.chunks = (p.steps + p.chunk - 1) / p.chunk;
   const dim3 grid((unsigned)(((int64_t)p.tokens * p.chunks + 3) / 4));
-  if ((int64_t)p.tokens * (p.HQ + p.HKV) * D * 2 > PAST_CACHES) qk_norm_rope_kernel<act_t, D, true><<<grid, 256, 0, s>>>(p);
-  else qk_norm_rope_kernel<act_t, D, false><<<grid, 256, 0, s>>>(p);
+  if ((int64_t)p.tokens * (p.HQ + p.HKV) * D * 2 > PAST_CACHES) {
+    if (p.k_scales) qk_norm_rope_kernel<act_t, D, true, true><<<grid, 256, 0, s>>>(p);
+    else qk_norm_rope_kernel<act_t, D, true, false><<<grid, 256, 0, s>>>(p);
+  } else {
+    if (p.k_scales) qk_norm_rope_kernel<act_t, D, false, true><<<grid, 256, 0, s>>>(p);
+    else qk_norm_rope_kernel<act_t, D, false, false><<<grid, 256, 0, s>>>(p);
+  }
 }
 
 template <typename act_t>
@@ -264,15 +321,13 @@ static void launch_qk_norm_rope(const QkNormRope& p, int D, hipStream_t s) {
   else launch_qk_norm_rope<act_t, 256>(p, s);
 }
 
-}  // namespace pla
-
-extern "C" int pla_qk_norm_rope_launch(
+// scale_strides [4]: (block, head) of k_scales and v_scales; NULL where the caches have the activations' type.
+static int qk_norm_rope(
     const void* q, const void* k, const void* v, const int64_t* strides, const void* positions, int positions_wide,
     const void* q_weight, const void* k_weight, int weights_f32, float eps, float weight_offset,
     const float* inv_freq, int rotary_dim, float attention_factor, int interleaved,
-    void* q_out, void* k_out, void* k_cache, void* v_cache, const void* slots, int slots_wide, int blocks, int block_size,
-    int tokens, int HQ, int HKV, int D, int act_dtype, void* stream) {
-  using namespace pla;
+    void* q_out, void* k_out, void* k_cache, void* v_cache, float* k_scales, float* v_scales, const int64_t* scale_strides,
+    const void* slots, int slots_wide, int blocks, int block_size, int tokens, int HQ, int HKV, int D, int act_dtype, void* stream) {
   PLA_REQUIRE(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got %d", D);
   PLA_REQUIRE(act_dtype == PLA_BF16 || act_dtype == PLA_F16, "activations must be bf16 or fp16");
   PLA_REQUIRE(tokens >= 0 && HQ > 0 && HKV > 0, "invalid token or head counts");
@@ -285,19 +340,50 @@ extern "C" int pla_qk_norm_rope_launch(
   PLA_REQUIRE((k_cache != nullptr) == (slots != nullptr) && (v_cache == nullptr || (v && k_cache)),
               "k_cache and slots come together, v_cache with v and both");
   PLA_REQUIRE(k_cache || k_out, "keys need a cache or an output");
+  if (scale_strides) {
+    PLA_REQUIRE(k_cache && k_scales && (v_cache != nullptr) == (v_scales != nullptr), "a cache of 8-bit numbers needs scales");
+    for (int i = 10; i < 16; ++i) PLA_REQUIRE(strides[i] % 16 == 0, "rows must be 16-byte aligned");
+  }
   PLA_REQUIRE(k_cache == nullptr || (blocks >= 0 && block_size > 0 && (int64_t)blocks * block_size <= INT32_MAX),
               "a cache must have at most 2^31 - 1 slots");
   for (int i = 0; i < 16; ++i) PLA_REQUIRE(strides[i] % 8 == 0, "rows must be 16-byte aligned");
   for (const void* x : {q, k, v, q_weight, k_weight, (const void*)q_out, (const void*)k_out, (const void*)k_cache, (const void*)v_cache})
     PLA_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0, "rows must be 16-byte aligned");
   const int64_t* t = strides;
+  const int64_t none[4] = {0, 0, 0, 0}, *u = scale_strides ? scale_strides : none;
   const QkNormRope p{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, t[0], t[1], t[2], t[3], t[4], t[5],
                      positions, positions_wide, q_weight, k_weight, weights_f32, eps, weight_offset, inv_freq, rotary_dim,
                      attention_factor, interleaved, (uint16_t*)q_out, (uint16_t*)k_out, t[6], t[7], t[8], t[9],
-                     (uint16_t*)k_cache, (uint16_t*)v_cache, t[10], t[11], t[12], t[13], t[14], t[15],
+                     k_cache, v_cache, k_scales, v_scales, u[0], u[1], u[2], u[3], t[10], t[11], t[12], t[13], t[14], t[15],
                      slots, slots_wide, block_size, k_cache ? blocks * block_size : 0, tokens, HQ, HKV, 0, 0, 0, 0, 0};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (act_dtype == PLA_BF16) launch_qk_norm_rope<bf16_t>(p, D, s);
   else launch_qk_norm_rope<f16_t>(p, D, s);
   return check_launch("qk_norm_rope_kernel");
+}
+
+}  // namespace pla
+
+extern "C" int pla_qk_norm_rope_launch(
+    const void* q, const void* k, const void* v, const int64_t* strides, const void* positions, int positions_wide,
+    const void* q_weight, const void* k_weight, int weights_f32, float eps, float weight_offset,
+    const float* inv_freq, int rotary_dim, float attention_factor, int interleaved,
+    void* q_out, void* k_out, void* k_cache, void* v_cache, const void* slots, int slots_wide, int blocks, int block_size,
+    int tokens, int HQ, int HKV, int D, int act_dtype, void* stream) {
+  return pla::qk_norm_rope(q, k, v, strides, positions, positions_wide, q_weight, k_weight, weights_f32, eps, weight_offset, inv_freq, rotary_dim,
+                           attention_factor, interleaved, q_out, k_out, k_cache, v_cache, nullptr, nullptr, nullptr, slots, slots_wide, blocks,
+                           block_size, tokens, HQ, HKV, D, act_dtype, stream);
+}
+
+extern "C" int pla_qk_norm_rope_fp8_launch(
+    const void* q, const void* k, const void* v, const int64_t* strides, const void* positions, int positions_wide,
+    const void* q_weight, const void* k_weight, int weights_f32, float eps, float weight_offset,
+    const float* inv_freq, int rotary_dim, float attention_factor, int interleaved,
+    void* q_out, void* k_out, void* k_cache, void* v_cache, float* k_scales, float* v_scales, const int64_t* scale_strides,
+    const void* slots, int slots_wide, int blocks, int block_size, int tokens, int HQ, int HKV, int D, int act_dtype, void* stream) {
+  using namespace pla;
+  PLA_REQUIRE(scale_strides, "null tensor pointer");
+  return qk_norm_rope(q, k, v, strides, positions, positions_wide, q_weight, k_weight, weights_f32, eps, weight_offset, inv_freq, rotary_dim,
+                      attention_factor, interleaved, q_out, k_out, k_cache, v_cache, k_scales, v_scales, scale_strides, slots, slots_wide, blocks,
+                      block_size, tokens, HQ, HKV, D, act_dtype, stream);
 }

@@ -7,9 +7,10 @@ needs besides the linear-attention operators; it has no counterpart in the refer
 ``paged_kv_plan``           block tables, slot map, positions and offsets of a step, from the requests' lengths, on the GPU.  Its
                             ``query_start_loc`` is the one ``kda_replay_verify`` takes, its block table the one that
                             ``KDAReplayCommitContext.commit`` takes in align mode.
-``fused_qk_norm_rope``      norms of queries and keys for each head, position rotation and write into the paged cache.
+``fused_qk_norm_rope``      norms of queries and keys for each head, position rotation and write into the paged cache, of 16 or 8 bits.
 ``rotary_frequencies``      the rotation's frequencies, plain or scaled for long contexts.
-``paged_attention_decode``  attention of one new token, or of a window of up to 32 draft tokens, over the paged cache.
+``paged_attention_decode``  attention of one new token, or of a window of up to 32 draft tokens, over the paged cache, and over a prefix
+                            that all requests share.
 
 Longer windows, prompts and parts of them: ``pla.prefill.attention.paged_attention_prefill``.
 
@@ -143,7 +144,7 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, factor=1.0, original_length=
 
 def fused_qk_norm_rope(q, k, positions=None, *, q_weight=None, k_weight=None, eps=1e-6, weight_offset=0.0, inv_freq=None,
                        attention_factor=1.0, interleaved=False, q_out=None, k_out=None, v=None, k_cache=None, v_cache=None,
-                       slot_mapping: Optional[torch.Tensor] = None):
+                       slot_mapping: Optional[torch.Tensor] = None, k_scales=None, v_scales=None):
     """Norms the heads of q [T, HQ, D] and k [T, HKV, D], turns them by their positions, stores k and v [T, HKV, D].
 
     bf16 or fp16, D 64, 128 or 256; rows are views with any 16-byte aligned token and head strides.  All in float32, one rounding.
@@ -155,6 +156,9 @@ def fused_qk_norm_rope(q, k, positions=None, *, q_weight=None, k_weight=None, ep
     store     with k_cache (and v, v_cache) [blocks, block_size, HKV, D] and slot_mapping [T] (int32 or int64), token t goes to
               slot ``block * block_size + place``; a slot that is negative or past the cache is nowhere.  No two tokens may
               name one slot.
+    8 bits    with k_scales (and v_scales) [blocks, HKV, block_size] float32 the caches are torch.float8_e4m3fn: a head of a token is
+              stored as x / scale, rounded once from float32 to nearest, with scale max(largest |x|, 1e-30) / 448 beside it.  A NaN
+              stays one, an infinity makes what its head stands for NaN.
 
     Returns (q_out, k_out): ``k_out`` is made if neither it nor a cache is given, and else what was passed.  q_out and k_out may be
     q and k themselves (the same rows), and share memory with nothing else.
@@ -163,11 +167,12 @@ def fused_qk_norm_rope(q, k, positions=None, *, q_weight=None, k_weight=None, ep
         from ._sanity import check_slots
         check_slots(slot_mapping, k_cache)
     return _compiled().fused_qk_norm_rope(q, k, positions, q_weight, k_weight, eps, weight_offset, inv_freq, attention_factor,
-                                          interleaved, q_out, k_out, v, k_cache, v_cache, slot_mapping)
+                                          interleaved, q_out, k_out, v, k_cache, v_cache, slot_mapping, k_scales, v_scales)
 
 
 def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, query_start_loc=None, request_indices=None,
-                           max_query_len=1, scale=None, output_gate=None, out=None):
+                           max_query_len=1, scale=None, output_gate=None, out=None, k_scales=None, v_scales=None,
+                           prefix_blocks=None, prefix_len=None):
     """Attention of new tokens over a paged cache that holds their keys and values already.
 
     q [T, HQ, D] (bf16 or fp16; D 64, 128 or 256; HQ a multiple of HKV), caches [blocks, block_size, HKV, D] of one shape and
@@ -183,6 +188,14 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, query_
     before it.
     ``request_indices`` [N]: rows of the block table, n without it.
 
+    Caches of 8-bit numbers (torch.float8_e4m3fn) come with ``k_scales`` and ``v_scales`` as ``fused_qk_norm_rope`` writes them, of common
+    strides, none negative.  Numbers and scales are used as they are, without a rounding of their product.
+
+    A prefix that all requests share, such as one instruction text, stands in blocks of its own, which no request's row of the table names:
+    the first ``prefix_len`` [1] (int32 or int64, on the device) positions of ``prefix_blocks`` int32 [pages].  Every row that sees a
+    position of its own sees the whole prefix too, before them (positions of new tokens count on from its end); keys and values of the
+    prefix are read once for the whole batch.  Its weights are rounded once to q's type.  Not with 8-bit caches.
+
     scale (default D^-0.5) applies to the scores; output_gate [T, HQ, D] multiplies the result by its sigmoid.  Scores, their
     maxima and sums and the outputs are float32; weights meet the values in two parts of q's type (off by 2^-16 of themselves at most,
     fp16 2^-22), outputs are rounded once.  Returns ``out`` [T, HQ, D], which shares memory with no input.  Results do not depend on
@@ -192,4 +205,4 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, query_
         from ._sanity import check_attention
         check_attention(q, k_cache, block_table, seq_lens, query_start_loc, request_indices, max_query_len)
     return _compiled().paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, query_start_loc, request_indices,
-                                              max_query_len, scale, output_gate, out)
+                                              max_query_len, scale, output_gate, out, k_scales, v_scales, prefix_blocks, prefix_len)
