@@ -51,7 +51,6 @@ struct PagedRun {
 struct PagedAttention {
   const uint16_t* q; int64_t q_token, q_head;
   const void *k, *v; int64_t kv_block, kv_token, kv_head;         // 16 bits a number, or 8
-  const float *k_scales, *v_scales; int64_t scale_block, scale_head;     // of numbers of 8 bits: [block][head][place]
   const int32_t* table; int64_t table_row;
   const void* mapping; int mapping_wide;
   const void* offsets; int offsets_wide;          // NULL: token row n is request n
@@ -64,6 +63,7 @@ struct PagedAttention {
   float scale_log2;
   int by_run, row_blocks;                         // runs in pieces are listed by run, or by worker; row blocks of the longest window
   float* partial; float2* tops; PagedRun* runs;
+  const float *k_scales, *v_scales; int64_t scale_block, scale_head;     // of numbers of 8 bits: [block][head][place]
   // attention over a prefix that all rows share, in pieces: outputs and their references and sums [piece][token][query head]
   const float* prefix; const float2* prefix_tops;
   const void* prefix_len; int prefix_len_wide, prefix_splits; int64_t prefix_positions;
@@ -188,25 +188,24 @@ struct Wave {
   }
 };
 
-// Where the two halves of a step's keys lie, in elements from the caches' and from the factors' start.
-struct Places { int64_t at[2], scale[2]; };
-
+// Keys and values from where the two halves of a step's keys lie (`place`, and `at` of their factors), in elements.
 template <typename W, typename raw_t>
-__device__ __forceinline__ void load_keys(W& w, const raw_t* base, const float* scales, const Places& place, uint32_t lane_offset) {
+__device__ __forceinline__ void load_keys(W& w, const raw_t* base, const float* scales, const int64_t (&place)[2], const int64_t (&at)[2], uint32_t lane_offset) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const auto p = as_global(reinterpret_cast<const char*>(base + place.at[h]));
+    const auto p = as_global(reinterpret_cast<const char*>(base + place[h]));
 #pragma unroll
     for (int c = 0; c < W::KEY_LOADS; ++c) w.k[h][c] = *reinterpret_cast<global_ptr<const u32x4_t>>(p + lane_offset + 64 * c);
-    if constexpr (W::SCALED) w.k_scale[h] = *reinterpret_cast<global_ptr<const f32x4_t>>(as_global(scales + place.scale[h]) + 4 * ((threadIdx.x & 63) >> 4));
+    if constexpr (W::SCALED) w.k_scale[h] = *reinterpret_cast<global_ptr<const f32x4_t>>(as_global(scales + at[h]) + 4 * ((threadIdx.x & 63) >> 4));
   }
 }
 
 template <typename W, typename raw_t>
-__device__ __forceinline__ void load_values(W& w, const raw_t* base, const float* scales, const Places& place, uint32_t lane_offset, int64_t token_bytes) {
+__device__ __forceinline__ void load_values(W& w, const raw_t* base, const float* scales, const int64_t (&place)[2], const int64_t (&at)[2], uint32_t lane_offset,
+                                            int64_t token_bytes) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const auto p = as_global(reinterpret_cast<const char*>(base + place.at[i / 4])) + (i & 3) * token_bytes;
+    const auto p = as_global(reinterpret_cast<const char*>(base + place[i / 4])) + (i & 3) * token_bytes;
 #pragma unroll
     for (int c = 0; c < W::CHUNKS; ++c) {
       if constexpr (W::RAW_WORDS == 4) {
@@ -223,7 +222,7 @@ __device__ __forceinline__ void load_values(W& w, const raw_t* base, const float
   }
   if constexpr (W::SCALED) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) w.v_scale[h] = *reinterpret_cast<global_ptr<const f32x4_t>>(as_global(scales + place.scale[h]) + 4 * ((threadIdx.x & 63) >> 4));
+    for (int h = 0; h < 2; ++h) w.v_scale[h] = *reinterpret_cast<global_ptr<const f32x4_t>>(as_global(scales + at[h]) + 4 * ((threadIdx.x & 63) >> 4));
   }
 }
 
@@ -445,7 +444,7 @@ struct PrefixPieces {
 template <typename value_t>
 __device__ __forceinline__ PrefixPieces prefix_pieces(const PagedAttention& p, int64_t token, int head, float top, float& sum) {
   PrefixPieces x{0, top - WEIGHT_SHIFT<value_t>, 1.f, 0, 0};
-  if (!p.prefix_tops || sum == 0.f) return x;
+  if (sum == 0.f) return x;
   const int64_t length = p.at(p.prefix_len, p.prefix_len_wide, 0);
   const int keys = (int)(length < 0 ? 0 : length < p.prefix_positions ? length : p.prefix_positions), heads = p.shape.heads * p.shape.group;
   x.pieces = keys == 0 ? 0 : prompt_share(keys, p.prefix_splits).pieces;
@@ -475,9 +474,9 @@ __device__ __forceinline__ void add_prefix(const PagedAttention& p, const Prefix
 }
 
 // CHANNELS channels of a row's output from their sums.
-template <typename act_t, int D, int CHANNELS>
+template <typename act_t, int D, bool PREFIX, int CHANNELS>
 __device__ __forceinline__ void write_row(const PagedAttention& p, int64_t token, int head, int channel, float top, float sum, float (&o)[CHANNELS]) {
-  if (p.prefix_tops) add_prefix(p, prefix_pieces<act_t>(p, token, head, top, sum), D, channel, o);
+  if constexpr (PREFIX) add_prefix(p, prefix_pieces<act_t>(p, token, head, top, sum), D, channel, o);
   const float norm = sum == 0.f ? 0.f : 1.0f / sum;         // no key: zeros
   uint32_t word[CHANNELS / 2];
 #pragma unroll
@@ -610,7 +609,7 @@ struct PieceOfRun {
   int64_t last;                           // unit of the line
 };
 
-template <typename act_t, typename kv_t, int D, int RT, bool ALONE>
+template <typename act_t, typename kv_t, int D, int RT, bool ALONE, bool PREFIX>
 __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) / 4) void paged_attention_kernel(const PagedAttention p) {
   using W = Wave<act_t, kv_t, D, RT>;
   using raw_t = typename W::raw_t;
@@ -641,8 +640,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
 
   const uint32_t key_lane = (uint32_t)(r * p.kv_token) * sizeof(raw_t) + 16 * kb;
   const uint32_t value_lane = (uint32_t)(4 * kb * p.kv_token + W::LANE_CHANNELS * r) * sizeof(raw_t);
-  auto keys_of = [&](int head) { return static_cast<const raw_t*>(p.k) + head * p.kv_head; };
-  auto values_of = [&](int head) { return static_cast<const raw_t*>(p.v) + head * p.kv_head; };
+  const raw_t *keys = static_cast<const raw_t*>(p.k), *values = static_cast<const raw_t*>(p.v);
   auto key_scales_of = [&](int head) { return W::SCALED ? p.k_scales + head * p.scale_head : nullptr; };
   auto value_scales_of = [&](int head) { return W::SCALED ? p.v_scales + head * p.scale_head : nullptr; };
 
@@ -695,14 +693,14 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     }
     return x;
   };
-  auto place_of = [&](const Part& a, int step, const Entries& x, Places& place, bool (&there)[2]) {
+  auto place_of = [&](const Part& a, int step, const Entries& x, int64_t (&place)[2], int64_t (&at)[2], bool (&there)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int key = a.key + step * STRIDE + 16 * h, at = key - paged_quotient(p.page_of, key) * p.block_size;
-      place.at[h] = paged_place(x.block[h], at, p.blocks, p.kv_block, p.kv_token);
-      there[h] = a.steps > 0 && key < a.end && place.at[h] >= 0;
-      if (!there[h]) place.at[h] = 0;
-      place.scale[h] = W::SCALED && there[h] ? x.block[h] * p.scale_block + at : 0;
+      const int key = a.key + step * STRIDE + 16 * h;
+      place[h] = paged_place(x.block[h], key - paged_quotient(p.page_of, key) * p.block_size, p.blocks, p.kv_block, p.kv_token);
+      there[h] = a.steps > 0 && key < a.end && place[h] >= 0;
+      if (!there[h]) place[h] = 0;
+      if constexpr (W::SCALED) at[h] = there[h] ? x.block[h] * p.scale_block + key - paged_quotient(p.page_of, key) * p.block_size : 0;
     }
   };
   // The queries: a wavefront alone keeps its operands, row r at channels 32 c + 8 kb, in registers.  Together a thread has pieces of
@@ -731,7 +729,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
 
   W w;
   u32x4_t q_words[MINE];
-  Places place, next_place;
+  int64_t place[2], next_place[2], scale_at[2] = {0, 0}, next_scale_at[2] = {0, 0};
   bool there[2], next_there[2];
   if (ALONE && lane < 2) left[lane][wave] = PieceOfRun{};
   if (!ALONE || unit < stretch_end) {
@@ -739,11 +737,11 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
   Part a = part_at(first_request, paged_start(first_request, __builtin_amdgcn_readfirstlane(room.offset[start])));
   const Entries entries = look_up(a, 0);
   if (a.steps > 0) {
-    place_of(a, 0, entries, place, there);
-    load_keys(w, keys_of(a.seg.head), key_scales_of(a.seg.head), place, key_lane);
+    place_of(a, 0, entries, place, scale_at, there);
+    load_keys(w, keys + a.seg.head * p.kv_head, key_scales_of(a.seg.head), place, scale_at, key_lane);
   }
   load_queries(a, q_words);
-  if (a.steps > 0) load_values(w, values_of(a.seg.head), value_scales_of(a.seg.head), place, value_lane, p.kv_token * sizeof(raw_t));
+  if (a.steps > 0) load_values(w, values + a.seg.head * p.kv_head, value_scales_of(a.seg.head), place, scale_at, value_lane, p.kv_token * (int)sizeof(raw_t));
   u32x4_t q_now[ALONE ? MINE : 1];
   if constexpr (ALONE) {
 #pragma unroll
@@ -788,22 +786,22 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       // The very last step fetches some block's first keys, the same for all, from the caches: a branch around the loads costs the
       // compiler the registers.
       // The entries for the step after next are asked for behind the keys of the next: a wait for queries in LDS is one for them too.
-      const int head = more ? a.seg.head : b.seg.head;
+      const int kv_head = more ? a.seg.head : b.seg.head;
+      const int64_t head = (more ? a.seg.head : b.seg.head) * p.kv_head;
       attend(w, query, p.scale_log2, there, a.key + step * STRIDE, a.least, a.end,
              [&] {
-               place_of(more ? a : b, more ? step + 1 : 0, coming, next_place, next_there);
-               load_keys(w, keys_of(head), key_scales_of(head), next_place, key_lane);
+               place_of(more ? a : b, more ? step + 1 : 0, coming, next_place, next_scale_at, next_there);
+               load_keys(w, keys + head, key_scales_of(kv_head), next_place, next_scale_at, key_lane);
                coming = step + 2 < a.steps ? look_up(a, step + 2) : look_up(b, 0);
              },
-             [&] { load_values(w, values_of(head), value_scales_of(head), next_place, value_lane, p.kv_token * sizeof(raw_t)); });
-      place = next_place;
+             [&] { load_values(w, values + head, value_scales_of(kv_head), next_place, next_scale_at, value_lane, p.kv_token * (int)sizeof(raw_t)); });
 #pragma unroll
-      for (int h = 0; h < 2; ++h) there[h] = next_there[h];
+      for (int h = 0; h < 2; ++h) { place[h] = next_place[h]; scale_at[h] = next_scale_at[h]; there[h] = next_there[h]; }
     }
     if (a.steps == 0 && b.steps > 0) {
-      place_of(b, 0, coming, place, there);
-      load_keys(w, keys_of(b.seg.head), key_scales_of(b.seg.head), place, key_lane);
-      load_values(w, values_of(b.seg.head), value_scales_of(b.seg.head), place, value_lane, p.kv_token * sizeof(raw_t));
+      place_of(b, 0, coming, place, scale_at, there);
+      load_keys(w, keys + b.seg.head * p.kv_head, key_scales_of(b.seg.head), place, scale_at, key_lane);
+      load_values(w, values + b.seg.head * p.kv_head, value_scales_of(b.seg.head), place, scale_at, value_lane, p.kv_token * (int)sizeof(raw_t));
     }
 
     if constexpr (ALONE) {
@@ -839,7 +837,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       if (a.seg.tiles == a.req.tiles) {
         if (r < a.rows) {
           const int64_t token = a.req.begin + j;
-          if (p.prefix_tops) {
+          if constexpr (PREFIX) {
             const PrefixPieces pieces = prefix_pieces<act_t>(p, token, head, w.top[0], sum);
 #pragma unroll
             for (int c = 0; c < W::CHUNKS; ++c)
@@ -930,7 +928,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
             add_set_aside<act_t, kv_t, D, TEAM>(p, a.req, a.seg.head, row, out_channel, a.pages, max(aside[x], a.least), min(aside[x] + 32, a.end), row_top, o);
         if (a.seg.slot < 0) {
           const int j = paged_quotient(p.shape.by_group, row), head = a.seg.head * p.shape.group + row - j * p.shape.group;
-          write_row<act_t, D, CHANNELS>(p, a.req.begin + j, head, out_channel, row_top, row_sum, o);
+          write_row<act_t, D, PREFIX, CHANNELS>(p, a.req.begin + j, head, out_channel, row_top, row_sum, o);
         } else {
           const int64_t at = (int64_t)a.seg.slot * (16 * RT) + 16 * t + out_row;
 #pragma unroll
@@ -998,7 +996,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
         }
         if (g >= 0 && !open) {
           const int row = row0 + mine, j = paged_quotient(p.shape.by_group, row), head = run.head * p.shape.group + row - j * p.shape.group;
-          write_row<act_t, D, 8>(p, run.begin + j, head, channel, row_top, row_sum, o);
+          write_row<act_t, D, PREFIX, 8>(p, run.begin + j, head, channel, row_top, row_sum, o);
         } else {
           const int64_t at = (int64_t)(2 * worker + (g >= 0)) * 16 + mine;
           float4* dst = reinterpret_cast<float4*>(p.partial + at * D + channel);
@@ -1018,7 +1016,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
 // Pieces of a run to its output: a workgroup a run and every gridDim.y-th of its rows.  The wavefronts share the rows, or
 // (PER_ROW; many pieces) the pieces of a row; a lane has D / 64 channels.  Everything that a row takes is asked for at once, as
 // far as it is no more than AHEAD pieces a wavefront.
-template <typename act_t, int D, bool PER_ROW, int WAVES>
+template <typename act_t, int D, bool PER_ROW, int WAVES, bool PREFIX>
 __global__ __launch_bounds__(64 * WAVES) void paged_join_kernel(const PagedAttention p) {
   constexpr int LANE = D / 64, AHEAD = !PER_ROW ? 8 : D == 256 ? 10 : 18;
   typedef float lane_t __attribute__((ext_vector_type(LANE)));
@@ -1087,7 +1085,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_join_kernel(const PagedAtten
       float x[LANE];
 #pragma unroll
       for (int c = 0; c < LANE; ++c) x[c] = o[c];
-      if (p.prefix_tops) add_prefix(p, prefix_pieces<act_t>(p, token, head, top, sum), D, LANE * lane, x);
+      if constexpr (PREFIX) add_prefix(p, prefix_pieces<act_t>(p, token, head, top, sum), D, LANE * lane, x);
       const float norm = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
       for (int c = 0; c < LANE; ++c) {
@@ -1153,23 +1151,29 @@ static PagedLaunch paged_launch(int batch, int HQ, int HKV, int D, int max_query
   return l;
 }
 
-template <typename act_t, typename kv_t, int D>
+template <typename act_t, typename kv_t, int D, bool PREFIX>
 static void launch_paged_attention(const PagedAttention& p, const PagedLaunch& l, hipStream_t s) {
-  if (l.alone) paged_attention_kernel<act_t, kv_t, D, 1, true><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
-  else if (l.row_tiles == 1) paged_attention_kernel<act_t, kv_t, D, 1, false><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
-  else if (l.row_tiles == 2) paged_attention_kernel<act_t, kv_t, D, 2, false><<<l.workers, 64 * waves(D, 2), 0, s>>>(p);
-  else if constexpr (D != 256) paged_attention_kernel<act_t, kv_t, D, 4, false><<<l.workers, 64 * waves(D, 4), 0, s>>>(p);
+  if (l.alone) paged_attention_kernel<act_t, kv_t, D, 1, true, PREFIX><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
+  else if (l.row_tiles == 1) paged_attention_kernel<act_t, kv_t, D, 1, false, PREFIX><<<l.workers, 64 * waves(D, 1), 0, s>>>(p);
+  else if (l.row_tiles == 2) paged_attention_kernel<act_t, kv_t, D, 2, false, PREFIX><<<l.workers, 64 * waves(D, 2), 0, s>>>(p);
+  else if constexpr (D != 256) paged_attention_kernel<act_t, kv_t, D, 4, false, PREFIX><<<l.workers, 64 * waves(D, 4), 0, s>>>(p);
   if (!l.split) return;
   const dim3 grid((unsigned)(l.by_run ? l.runs : l.workers), l.join_rows);
-  if (l.per_row) paged_join_kernel<act_t, D, true, 16><<<grid, 1024, 0, s>>>(p);
-  else paged_join_kernel<act_t, D, false, 4><<<grid, 256, 0, s>>>(p);
+  if (l.per_row) paged_join_kernel<act_t, D, true, 16, PREFIX><<<grid, 1024, 0, s>>>(p);
+  else paged_join_kernel<act_t, D, false, 4, PREFIX><<<grid, 256, 0, s>>>(p);
 }
 
-template <typename act_t, typename kv_t>
+template <typename act_t, typename kv_t, bool PREFIX>
 static void launch_paged_attention(const PagedAttention& p, const PagedLaunch& l, int D, hipStream_t s) {
-  if (D == 64) launch_paged_attention<act_t, kv_t, 64>(p, l, s);
-  else if (D == 128) launch_paged_attention<act_t, kv_t, 128>(p, l, s);
-  else launch_paged_attention<act_t, kv_t, 256>(p, l, s);
+  if (D == 64) launch_paged_attention<act_t, kv_t, 64, PREFIX>(p, l, s);
+  else if (D == 128) launch_paged_attention<act_t, kv_t, 128, PREFIX>(p, l, s);
+  else launch_paged_attention<act_t, kv_t, 256, PREFIX>(p, l, s);
+}
+template <typename act_t>
+static void launch_paged_attention(const PagedAttention& p, const PagedLaunch& l, int D, hipStream_t s) {
+  if (p.k_scales) launch_paged_attention<act_t, e4m3_t, false>(p, l, D, s);
+  else if (p.prefix_tops) launch_paged_attention<act_t, act_t, true>(p, l, D, s);
+  else launch_paged_attention<act_t, act_t, false>(p, l, D, s);
 }
 
 static int check_shape(int batch, int HQ, int HKV, int D, int max_query, int64_t positions) {
@@ -1323,13 +1327,8 @@ static int paged_attention(
     p.runs = reinterpret_cast<PagedRun*>(ws + l.runs_at);
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (act_dtype == PLA_BF16) {
-    if (scaled) launch_paged_attention<bf16_t, e4m3_t>(p, l, head_dim, s);
-    else launch_paged_attention<bf16_t, bf16_t>(p, l, head_dim, s);
-  } else {
-    if (scaled) launch_paged_attention<f16_t, e4m3_t>(p, l, head_dim, s);
-    else launch_paged_attention<f16_t, f16_t>(p, l, head_dim, s);
-  }
+  if (act_dtype == PLA_BF16) launch_paged_attention<bf16_t>(p, l, head_dim, s);
+  else launch_paged_attention<f16_t>(p, l, head_dim, s);
   return check_launch("paged_attention_kernel");
 }
 

@@ -35,13 +35,13 @@ struct QkNormRope {
   uint16_t *q_out, *k_out;
   int64_t qo_token, qo_head, ko_token, ko_head;
   void *k_cache, *v_cache;            // 16 bits a number, or 8
-  float *k_scales, *v_scales;         // of numbers of 8 bits: [block][head][place]
-  int64_t ks_block, ks_head, vs_block, vs_head;
   int64_t kc_block, kc_token, kc_head, vc_block, vc_token, vc_head;
   const void* slots; int slots_wide; int block, cache_slots;
   int tokens, HQ, HKV;
   int q_steps, k_steps, steps;        // of a token: for queries, for keys, and with those for values
   int chunk, chunks;                  // steps a wavefront, wavefronts a token
+  float *k_scales, *v_scales;         // of numbers of 8 bits: [block][head][place]
+  int64_t ks_block, ks_head, vs_block, vs_head;
 };
 
 template <int LANES>
@@ -232,13 +232,13 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
       if (step >= end) break;
       const int kind = kind_of(step), h = head_of(step, kind);
       uint4 result = now[a];
-      float x[8];
+      [[maybe_unused]] float full[8];               // of a key or value, before it is rounded
       if (kind < 2) {
         if (kind != prepared) {
           prepare(kind);
           prepared = kind;
         }
-        float y[8];
+        float x[8], y[8];
         widen8<act_t>(now[a], x);
         if (split) {
           uint4 other;
@@ -262,6 +262,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
           const float along = x[i] * straight[i];
           x[i] = (turns ? fmaf(y[i], cross[i], along) : along) * rstd;
         }
+        if constexpr (CACHE8) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) full[i] = x[i];
+        }
         result = make_uint4(pack2<act_t>(x[0], x[1]), pack2<act_t>(x[2], x[3]), pack2<act_t>(x[4], x[5]), pack2<act_t>(x[6], x[7]));
       }
       // (all lanes of a row go through here: its heads are whole groups of them)
@@ -269,8 +273,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
       float scale = 0.f;
       if constexpr (CACHE8) {
         if (kind && slot >= 0) {
-          if (kind == 2) widen8<act_t>(now[a], x);
-          eight = quantise8<LANES>(x, scale);
+          if (kind == 2) widen8<act_t>(now[a], full);
+          eight = quantise8<LANES>(full, scale);
         }
       }
       if (h >= (kind == 0 ? p.HQ : p.HKV)) continue;
@@ -278,16 +282,16 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRope p) {
         store_row(p.q_out + token * p.qo_token + h * p.qo_head, result);
       } else {
         if (kind == 1 && p.k_out) store_row(p.k_out + token * p.ko_token + h * p.ko_head, result);
-        if (slot >= 0) {
-          const int64_t at = kind == 1 ? block * p.kc_block + place * p.kc_token + h * p.kc_head : block * p.vc_block + place * p.vc_token + h * p.vc_head;
-          if constexpr (CACHE8) {
-            uint8_t* row = static_cast<uint8_t*>(kind == 1 ? p.k_cache : p.v_cache) + at + channel;
-            if (PAST) __builtin_nontemporal_store(__builtin_bit_cast(uint64_t, eight), reinterpret_cast<uint64_t*>(row));
-            else *reinterpret_cast<uint2*>(row) = eight;
-            if (lane == 0) (kind == 1 ? p.k_scales + block * p.ks_block + h * p.ks_head : p.v_scales + block * p.vs_block + h * p.vs_head)[place] = scale;
-          } else {
-            store_row(static_cast<uint16_t*>(kind == 1 ? p.k_cache : p.v_cache) + at, result);
-          }
+        if constexpr (CACHE8) {
+          if (slot < 0) continue;
+          uint8_t* row = kind == 1 ? static_cast<uint8_t*>(p.k_cache) + block * p.kc_block + place * p.kc_token + h * p.kc_head
+                                   : static_cast<uint8_t*>(p.v_cache) + block * p.vc_block + place * p.vc_token + h * p.vc_head;
+          if (PAST) __builtin_nontemporal_store(__builtin_bit_cast(uint64_t, eight), reinterpret_cast<uint64_t*>(row + channel));
+          else *reinterpret_cast<uint2*>(row + channel) = eight;
+          if (lane == 0) (kind == 1 ? p.k_scales + block * p.ks_block + h * p.ks_head : p.v_scales + block * p.vs_block + h * p.vs_head)[place] = scale;
+        } else if (slot >= 0) {
+          store_row(kind == 1 ? static_cast<uint16_t*>(p.k_cache) + block * p.kc_block + place * p.kc_token + h * p.kc_head
+                              : static_cast<uint16_t*>(p.v_cache) + block * p.vc_block + place * p.vc_token + h * p.vc_head, result);
         }
       }
     }
@@ -354,8 +358,9 @@ static int qk_norm_rope(
   const QkNormRope p{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, t[0], t[1], t[2], t[3], t[4], t[5],
                      positions, positions_wide, q_weight, k_weight, weights_f32, eps, weight_offset, inv_freq, rotary_dim,
                      attention_factor, interleaved, (uint16_t*)q_out, (uint16_t*)k_out, t[6], t[7], t[8], t[9],
-                     k_cache, v_cache, k_scales, v_scales, u[0], u[1], u[2], u[3], t[10], t[11], t[12], t[13], t[14], t[15],
-                     slots, slots_wide, block_size, k_cache ? blocks * block_size : 0, tokens, HQ, HKV, 0, 0, 0, 0, 0};
+                     k_cache, v_cache, t[10], t[11], t[12], t[13], t[14], t[15],
+                     slots, slots_wide, block_size, k_cache ? blocks * block_size : 0, tokens, HQ, HKV, 0, 0, 0, 0, 0,
+                     k_scales, v_scales, u[0], u[1], u[2], u[3]};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (act_dtype == PLA_BF16) launch_qk_norm_rope<bf16_t>(p, D, s);
   else launch_qk_norm_rope<f16_t>(p, D, s);
