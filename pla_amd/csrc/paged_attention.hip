@@ -64,9 +64,8 @@ struct PagedAttention {
   int by_run, row_blocks;                         // runs in pieces are listed by run, or by worker; row blocks of the longest window
   float* partial; float2* tops; PagedRun* runs;
   const float *k_scales, *v_scales; int64_t scale_block, scale_head;     // of numbers of 8 bits: [block][head][place]
-  // attention over a prefix that all rows share, in pieces: outputs and their references and sums [piece][token][query head]
+  // attention over a prefix that all rows share: outputs and their references and sums [token][query head]
   const float* prefix; const float2* prefix_tops;
-  const void* prefix_len; int prefix_len_wide, prefix_splits; int64_t prefix_positions;
 
   __device__ int64_t at(const void* base, int wide, int64_t i) const {
     return wide ? static_cast<const int64_t*>(base)[i] : (int64_t) static_cast<const int32_t*>(base)[i];
@@ -434,49 +433,34 @@ struct Part {
   const int32_t* pages;
 };
 
-// What a row has of the prefix, joined with what it has of its own keys: first the common reference and the factors of what stands in
-// registers, then a piece at a time.  A row that sees no key of its own (sum 0) has no part in the prefix.
-struct PrefixPieces {
-  int pieces;                                     // 0: none
-  float reference, own;
-  int64_t row, step;                              // of the row in the first piece, to the next piece
+// What a row has of the prefix, joined with what it has of its own keys: a common reference and the factors of both.  A row that sees no
+// key of its own (sum 0) has no part in the prefix.
+struct PrefixPart {
+  int64_t row;                                    // of the prefix's outputs
+  float own, prefix;
 };
 template <typename value_t>
-__device__ __forceinline__ PrefixPieces prefix_pieces(const PagedAttention& p, int64_t token, int head, float top, float& sum) {
-  PrefixPieces x{0, top - WEIGHT_SHIFT<value_t>, 1.f, 0, 0};
-  if (sum == 0.f) return x;
-  const int64_t length = p.at(p.prefix_len, p.prefix_len_wide, 0);
-  const int keys = (int)(length < 0 ? 0 : length < p.prefix_positions ? length : p.prefix_positions), heads = p.shape.heads * p.shape.group;
-  x.pieces = keys == 0 ? 0 : prompt_share(keys, p.prefix_splits).pieces;
-  x.step = (int64_t)p.shape.tokens * heads;
-  x.row = token * heads + head;
-  const float before = x.reference;
-  for (int i = 0; i < x.pieces; ++i) x.reference = fmaxf(x.reference, p.prefix_tops[x.row + i * x.step].x);
-  x.own = rescale(before, x.reference);
-  sum *= x.own;
-  for (int i = 0; i < x.pieces; ++i) {
-    const float2 y = p.prefix_tops[x.row + i * x.step];
-    sum = fmaf(y.y, rescale(y.x, x.reference), sum);
-  }
+__device__ __forceinline__ PrefixPart prefix_part(const PagedAttention& p, int64_t token, int head, float top, float& sum) {
+  PrefixPart x{token * (p.shape.heads * p.shape.group) + head, 1.f, 0.f};
+  const float2 y = p.prefix_tops[x.row];
+  if (sum == 0.f || y.x == -INFINITY) return x;
+  const float mine = top - WEIGHT_SHIFT<value_t>, reference = fmaxf(mine, y.x);
+  x.own = rescale(mine, reference);
+  x.prefix = rescale(y.x, reference);
+  sum = fmaf(y.y, x.prefix, sum * x.own);
   return x;
 }
 template <int CHANNELS>
-__device__ __forceinline__ void add_prefix(const PagedAttention& p, const PrefixPieces& x, int D, int channel, float (&o)[CHANNELS]) {
-  if (x.pieces == 0) return;
+__device__ __forceinline__ void add_prefix(const PagedAttention& p, const PrefixPart& x, int D, int channel, float (&o)[CHANNELS]) {
+  const float* part = p.prefix + x.row * D + channel;
 #pragma unroll
-  for (int i = 0; i < CHANNELS; ++i) o[i] *= x.own;
-  for (int n = 0; n < x.pieces; ++n) {
-    const float f = rescale(p.prefix_tops[x.row + n * x.step].x, x.reference);
-    const float* part = p.prefix + (x.row + n * x.step) * D + channel;
-#pragma unroll
-    for (int i = 0; i < CHANNELS; ++i) o[i] = fmaf(part[i], f, o[i]);
-  }
+  for (int i = 0; i < CHANNELS; ++i) o[i] = x.prefix == 0.f ? o[i] : fmaf(part[i], x.prefix, o[i] * x.own);
 }
 
 // CHANNELS channels of a row's output from their sums.
 template <typename act_t, int D, bool PREFIX, int CHANNELS>
 __device__ __forceinline__ void write_row(const PagedAttention& p, int64_t token, int head, int channel, float top, float sum, float (&o)[CHANNELS]) {
-  if constexpr (PREFIX) add_prefix(p, prefix_pieces<act_t>(p, token, head, top, sum), D, channel, o);
+  if constexpr (PREFIX) add_prefix(p, prefix_part<act_t>(p, token, head, top, sum), D, channel, o);
   const float norm = sum == 0.f ? 0.f : 1.0f / sum;         // no key: zeros
   uint32_t word[CHANNELS / 2];
 #pragma unroll
@@ -838,7 +822,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
         if (r < a.rows) {
           const int64_t token = a.req.begin + j;
           if constexpr (PREFIX) {
-            const PrefixPieces pieces = prefix_pieces<act_t>(p, token, head, w.top[0], sum);
+            const PrefixPart part = prefix_part<act_t>(p, token, head, w.top[0], sum);
 #pragma unroll
             for (int c = 0; c < W::CHUNKS; ++c)
 #pragma unroll
@@ -846,7 +830,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
                 float y[W::TILES];
 #pragma unroll
                 for (int x = 0; x < W::TILES; ++x) y[x] = w.o[0][c][x][e];
-                add_prefix(p, pieces, D, channel_of(c, e), y);
+                add_prefix(p, part, D, channel_of(c, e), y);
 #pragma unroll
                 for (int x = 0; x < W::TILES; ++x) w.o[0][c][x][e] = y[x];
               }
@@ -1085,7 +1069,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_join_kernel(const PagedAtten
       float x[LANE];
 #pragma unroll
       for (int c = 0; c < LANE; ++c) x[c] = o[c];
-      if constexpr (PREFIX) add_prefix(p, prefix_pieces<act_t>(p, token, head, top, sum), D, LANE * lane, x);
+      if constexpr (PREFIX) add_prefix(p, prefix_part<act_t>(p, token, head, top, sum), D, LANE * lane, x);
       const float norm = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
       for (int c = 0; c < LANE; ++c) {
@@ -1243,8 +1227,6 @@ struct PagedExtras {
   int prefix_len_wide;
 };
 
-static int64_t prefix_bytes(const PromptLaunch& l, int64_t tokens, int HQ, int D) { return prompt_bytes(l, tokens, HQ, D, true); }
-
 static int paged_attention(
     const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,
     int64_t kv_block, int64_t kv_token, int64_t kv_head, int blocks, int block_size,
@@ -1296,14 +1278,12 @@ static int paged_attention(
     x.lengths = extras.prefix_len; x.lengths_wide = extras.prefix_len_wide;
     x.batch = 1; x.tokens = tokens; x.heads = HKV; x.group = HQ / HKV; x.by_group = paged_divisor(HQ / HKV);
     x.positions = (int64_t)extras.prefix_pages * block_size;
-    const PromptLaunch prompt = prompt_launch(1, tokens, HQ, HKV, head_dim, x.positions);
-    taken = prefix_bytes(prompt, tokens, HQ, head_dim);
-    if (const int bad = launch_prompt(x, prompt, true, HQ, head_dim, scale, act_dtype, workspace, workspace_bytes - l.bytes, static_cast<hipStream_t>(stream)))
+    const PromptLaunch prompt = prompt_launch(1, tokens, HQ, HKV, head_dim, x.positions, true);
+    taken = prompt.bytes;
+    if (const int bad = launch_prompt(x, prompt, true, head_dim, scale, act_dtype, workspace, workspace_bytes - l.bytes, static_cast<hipStream_t>(stream)))
       return bad;
-    p.prefix = reinterpret_cast<const float*>(ws);
-    p.prefix_tops = reinterpret_cast<const float2*>(ws + prompt_tops_at(prompt, tokens, HQ, head_dim));
-    p.prefix_len = extras.prefix_len; p.prefix_len_wide = extras.prefix_len_wide;
-    p.prefix_splits = prompt.splits; p.prefix_positions = x.positions;
+    p.prefix = reinterpret_cast<const float*>(ws + prompt.rows_at);
+    p.prefix_tops = reinterpret_cast<const float2*>(ws + prompt.row_tops_at);
   }
   PLA_REQUIRE(workspace_bytes >= taken + l.bytes && (taken + l.bytes == 0 || workspace), "workspace too small: %lld bytes needed", (long long)(taken + l.bytes));
   ws += taken;
@@ -1373,7 +1353,7 @@ extern "C" int64_t pla_paged_attention_prefix_workspace_bytes(int batch, int tok
   if (check_shape(batch, HQ, HKV, head_dim, max_query_len, positions) || check_prompt(1, tokens, HQ, HKV, head_dim) || prefix_positions < 0) return -1;
   if (batch == 0 || tokens == 0) return 0;
   return paged_launch(batch, HQ, HKV, head_dim, max_query_len, positions).bytes +
-         prefix_bytes(prompt_launch(1, tokens, HQ, HKV, head_dim, prefix_positions), tokens, HQ, head_dim);
+         prompt_launch(1, tokens, HQ, HKV, head_dim, prefix_positions, true).bytes;
 }
 
 extern "C" int pla_paged_attention_prefix_launch(

@@ -7,6 +7,15 @@
 namespace pla {
 
 constexpr int PROMPT_KEYS = 64;           // of a tile
+constexpr int PROMPT_ROWS = 128;          // of a block: query heads of a key-value head, token by token
+
+// A row block of a sequence and a piece of its keys, as a workgroup takes them.
+struct PromptItem {
+  int n, row0, rows;                      // sequence; first row of the block, rows of the block that are there (0: no item)
+  int window, keys;                       // tokens and keys of the sequence
+  int pieces, piece, first;               // of the block's keys at most, this one, item of the first
+  int64_t begin, key_begin;               // first token row, first key (dense)
+};
 
 struct PromptAttention {
   const uint16_t* q; int64_t q_token, q_head;
@@ -23,26 +32,43 @@ struct PromptAttention {
   int batch, tokens, heads, group; PagedDivisor by_group;
   int64_t positions;                              // dense: rows of k; paged: positions of a row of the table
   float scale_log2; uint32_t flip;                // of the magnitude of the scale; sign bits of a pair of query values
-  int splits;
-  float* partial; float2* tops;                   // pieces: [split][token][query head]
+  int items, least;                               // pieces that a head's keys are cut into (0: not at all), tiles of one at least
+  int slots, slot_rows;                           // of the workspace, for each head; rows of one
+  PromptItem* plan;                               // of all slots, where a call over sequences is split
+  float* partial; float2* tops;                   // a slot an item and head: outputs, references and sums of its rows
+  float* rows; float2* row_tops;                  // a prefix: the same of each row [token][query head], joined
 };
 
-// Key tiles of a row block that sees `keys` keys: `pieces` workgroups have `tiles` each, the last one what is left.
+// How keys are dealt out.  A call of many row blocks has a workgroup for each, the longest of a sequence first.  Where there are fewer, a
+// block's keys are cut into pieces, so that the blocks of a long sequence do not go on when all others are done: as many as make the whole
+// batch, were all blocks of a sequence as long as its last one, about `items` pieces of equal size, none under `least` tiles.  Pieces of
+// different blocks begin at the same keys, so that the caches hold them for all.  The batch's lengths stand on the device, so it is there
+// that the size is worked out; the host knows that blocks and pieces together are no more than blocks + items.
+PLA_HD int prompt_tiles(int keys) { return (int)(((int64_t)keys + PROMPT_KEYS - 1) / PROMPT_KEYS); }
+PLA_HD int prompt_piece(int items, int64_t total, int least) {
+  if (items <= 0) return INT32_MAX;
+  const int64_t even = paged_divide(total + items - 1, items);
+  return (int)(even < least ? least : even < INT32_MAX ? even : INT32_MAX);
+}
+PLA_HD int prompt_pieces(int tiles, int most) { return tiles <= most ? 1 : (tiles - 1) / most + 1; }
+// A block of `tiles` tiles in at most `most` pieces: `pieces` workgroups (one for nothing) have `tiles` each, the last one what is left.
 struct PromptShare { int tiles, pieces; };
-PLA_HD PromptShare prompt_share(int keys, int splits) {
-  const int tiles = (int)(((int64_t)keys + PROMPT_KEYS - 1) / PROMPT_KEYS);
-  const int even = (tiles + splits - 1) / splits, each = splits == 1 || even >= 4 ? even : 4;
+PLA_HD PromptShare prompt_share(int tiles, int most, int least) {
+  const int even = (tiles + most - 1) / most, each = most == 1 || even >= least ? even : least;
   return {each, tiles <= each ? 1 : (tiles + each - 1) / each};
 }
 
-struct PromptLaunch { int rows; int64_t blocks; int splits; };          // rows of a block, blocks at most, pieces of a block's keys at most
-PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, int64_t keys);
+constexpr int PROMPT_PLAN = 2048;         // sequences of a call that is split at most
+constexpr PLA_HD int prompt_residency(int D) { return D == 256 ? 1 : D == 64 ? 3 : 2; }       // workgroups a CU
+struct PromptLaunch {
+  int64_t blocks, items, pieces;                  // row blocks at most, workgroups a head, pieces (0: not split) that a head's keys are cut into
+  int least, slot_rows, join_rows;
+  bool split;
+  int64_t tops_at, plan_at, rows_at, row_tops_at, bytes;   // workspace
+};
+PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, int64_t keys, bool prefix);
 int check_prompt(int batch, int64_t tokens, int HQ, int HKV, int D);
-// Workspace of the pieces: where their references and sums start behind the outputs, and all of it (`always`: where there is one piece too).
-int64_t prompt_tops_at(const PromptLaunch& l, int64_t tokens, int HQ, int D);
-int64_t prompt_bytes(const PromptLaunch& l, int64_t tokens, int HQ, int D, bool always);
 // Checks what is left of the arguments and launches.
-int launch_prompt(PromptAttention p, const PromptLaunch& l, bool paged, int HQ, int D, float scale, int act, void* workspace, int64_t workspace_bytes,
-                  hipStream_t s);
+int launch_prompt(PromptAttention p, const PromptLaunch& l, bool paged, int D, float scale, int act, void* workspace, int64_t workspace_bytes, hipStream_t s);
 
 }  // namespace pla

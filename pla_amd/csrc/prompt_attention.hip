@@ -2,8 +2,36 @@
 //
 //   o = sum_p softmax_p(scale q.k_p) v_p  [* sigmoid(gate)]      over the keys p < keys - window + j + 1
 //
-// for token j of a window of `window` tokens at the end of `keys` keys.  The query heads of a key-value head and the tokens of the
-// window are the rows of one product, so keys and values are read once for all of them.
+// for token j of a window of `window` tokens at the end of `keys` keys; and of all token rows over one prefix, whose outputs the attention
+// over their own keys goes on with.  The query heads of a key-value head and the tokens of the window are the rows of one product, in
+// blocks of 128, 32 a wavefront, so a tile of 64 keys and values is fetched once for them.
+//
+//   S^T = K Q^T    keys are the rows: lane (query, half) gets the scores of its query at keys 8 i + 4 half .. + 3 of 32,
+//   O^T = V^T P^T  which is the operand that the second product wants, if its contraction runs over the keys in that order; the values
+//                  come out of LDS in it by transposing reads.  No weight crosses a lane, a query's maximum and sum cross one.
+//
+// Queries and outputs stay in registers (32 x 32 x 16 products), keys and values go to LDS past the registers, the next tile's under this
+// one's products.  A row of LDS is put in an order in which both kinds of reads meet no bank twice (none counted; in the plain order of
+// granules 33 % of the LDS's cycles were such, and one prompt of 32 768 tokens took 4090 us in place of 3940).  The loads of operands
+// are issued four ahead of the products that take them (3990 us against 4096 where the compiler puts them right before; one prompt of 4000
+// and one of 9000 tokens with heads of 256 channels 847 against 923).
+//
+// Two workgroups a CU (heads of 64: three; 256: one, whose registers and tiles fill it), so that one's products run under the other's
+// exponentials: 64 queries a wavefront, which halves the reads of LDS but leaves room for one workgroup, take 5080 us.  Products and
+// exponentials of one wavefront in a software pipeline, values a tile behind, gain nothing on top (3960).
+//
+// Bound by the matrix cores and, at their rate, by the power that they may draw: one prompt of 32 768 tokens (16 + 2 heads of 128) runs
+// at 1.1 PFLOP/s with the clock at 1.8 GHz, a product of two 16 384 x 16 384 matrices of the library at 1.37.  Half of a heads-of-64 tile's
+// time are exponentials, sums and roundings.
+//
+// The maximum is not followed as long as it grows by less than 2^8: the weights, in 32 bits until they are rounded, hold what it may be behind,
+// and the outputs need no factor then.  Weights are rounded once, to the queries' type, to meet the values (off by half a step of it, as
+// the outputs are by their own rounding; two parts would cost half as many products again).  fp16 weights are scaled by 2^7, so that the
+// smallest that count are not subnormal and the largest, 2^15, is finite.
+//
+// Infinite and NaN values: a weight of zero times one is NaN, where the formula has no product (a key that the row does not see) or an
+// infinite one (a weight that is zero only in 32 bits).  The loop does not look for them.  Where an output comes out infinite or NaN the
+// workgroup runs once more, with such values taken out of the product and brought in row by row.
 
 #include "decode_common.h"
 #include "prefill_common.h"
@@ -21,13 +49,6 @@ template <> __device__ __forceinline__ f32x16_t mfma32<bf16_t>(bf16x8_t a, bf16x
 template <> __device__ __forceinline__ f32x16_t mfma32<f16_t>(bf16x8_t a, bf16x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
-
-// A row block of a sequence, as a workgroup takes it.
-struct PromptBlock {
-  int n, row0, rows;                      // sequence; first row of the block, rows of the block that are there
-  int window, keys;                       // tokens and keys of the sequence
-  int64_t begin, key_begin;               // first token row, first key (dense)
-};
 
 __device__ __forceinline__ int64_t prompt_index(const void* base, int wide, int64_t i) {
   return wide ? static_cast<const int64_t*>(base)[i] : (int64_t) static_cast<const int32_t*>(base)[i];
@@ -57,51 +78,152 @@ __device__ __forceinline__ void prompt_sequence(const PromptAttention& p, int n,
   keys = (int)length;
 }
 
-// Row block `index` of the call.  Blocks of a sequence stand last one first: it has the most keys, and the shortest end the call.
-template <int ROWS, bool PAGED>
-__device__ __forceinline__ bool prompt_block(const PromptAttention& p, int index, PromptBlock& b) {
+__device__ __forceinline__ int prompt_blocks(const PromptAttention& p, int window) { return (int)(((int64_t)window * p.group + PROMPT_ROWS - 1) / PROMPT_ROWS); }
+
+// Row block `index` of a call that is not split.  Blocks of a sequence stand last one first: it has the most keys, and the shortest end the
+// call.
+template <bool PAGED>
+__device__ __forceinline__ bool prompt_block(const PromptAttention& p, int index, PromptItem& b) {
   const int lane = threadIdx.x & 63;
-  if (PAGED && !p.offsets) {              // all token rows over one prefix
-    const int64_t length = prompt_index(p.lengths, p.lengths_wide, 0);
-    b = PromptBlock{0, index * ROWS, 0, p.tokens, (int)(length < 0 ? 0 : length < p.positions ? length : p.positions), 0, 0};
-    b.rows = min(ROWS, b.window * p.group - b.row0);
-    return b.rows > 0;
-  }
   for (int base = 0; base < p.batch; base += 64) {
     int64_t begin = 0, key_begin = 0;
     int window = 0, keys = 0;
     if (base + lane < p.batch) prompt_sequence<PAGED>(p, base + lane, begin, window, key_begin, keys);
-    const int mine = (int)(((int64_t)window * p.group + ROWS - 1) / ROWS);
-    int64_t below = mine;
+    // (sequences that share rows may come to more blocks than there are workgroups)
+    const int mine = prompt_blocks(p, window);
+    int below = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t x = __shfl_up(below, d);
-      if (lane >= d) below += x;
+      const int x = __shfl_up(below, d);
+      if (lane >= d) below = min(below + x, 1 << 30);
     }
-    const int64_t all = lane_value(below, 63);
+    const int all = __builtin_amdgcn_readlane(below, 63);
     if (index >= all) {
-      index -= (int)all;
+      index -= all;
       continue;
     }
     const int at = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(below > index)) - 1);
-    const int left = (int)lane_value(below, at) - 1 - index;
     b.n = base + at;
     b.window = __builtin_amdgcn_readlane(window, at);
     b.keys = __builtin_amdgcn_readlane(keys, at);
     b.begin = lane_value(begin, at);
     b.key_begin = lane_value(key_begin, at);
-    b.row0 = left * ROWS;
-    b.rows = min(ROWS, b.window * p.group - b.row0);
+    b.row0 = (__builtin_amdgcn_readlane(below, at) - 1 - index) * PROMPT_ROWS;
+    b.rows = min(PROMPT_ROWS, b.window * p.group - b.row0);
+    b.pieces = 1;
+    b.piece = b.first = 0;
     return true;
   }
   return false;
 }
 
+// Through the scalar cache: nothing writes the plan any more.
+__device__ __forceinline__ PromptItem planned_item(const PromptAttention& p, int index) {
+  typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+  const scalar_ptr x = (scalar_ptr) reinterpret_cast<const int32_t*>(p.plan + index);
+  auto wide = [&](int i) { return (int64_t)((uint64_t)(uint32_t)x[i] | (uint64_t)(uint32_t)x[i + 1] << 32); };
+  return PromptItem{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], wide(8), wide(10)};
+}
+
+// Item `index` of a call over one prefix, whose blocks are alike; BY_BLOCK: its row block `index`.
+template <bool BY_BLOCK>
+__device__ __forceinline__ bool prefix_item(const PromptAttention& p, int index, PromptItem& b) {
+  const int64_t length = prompt_index(p.lengths, p.lengths_wide, 0);
+  const int keys = (int)(length < 0 ? 0 : length < p.positions ? length : p.positions), blocks = prompt_blocks(p, p.tokens), tiles = prompt_tiles(keys);
+  const int pieces = prompt_pieces(tiles, prompt_piece(p.items, (int64_t)blocks * tiles, p.least));
+  const int rank = BY_BLOCK ? index : index / pieces;
+  if (rank >= blocks) return false;
+  const int row0 = rank * PROMPT_ROWS;
+  b = PromptItem{0, row0, min(PROMPT_ROWS, p.tokens * p.group - row0), p.tokens, keys, pieces, BY_BLOCK ? 0 : index - rank * pieces, rank * pieces, 0, 0};
+  return true;
+}
+
 // Keys that row `row` of a sequence sees (they are the first ones).  Keys without a page count as ones that nobody sees.
-__device__ __forceinline__ int prompt_limit(const PromptAttention& p, const PromptBlock& b, int row) {
+__device__ __forceinline__ int prompt_limit(const PromptAttention& p, const PromptItem& b, int row) {
   const int64_t limit = p.offsets ? (int64_t)b.keys - b.window + paged_quotient(p.by_group, row) + 1 : b.keys;
   const int64_t most = b.keys < p.positions ? b.keys : p.positions;
   return (int)(limit < 0 ? 0 : limit < most ? limit : most);
+}
+
+// The items of a call that is split, block by block, the last one of a sequence first.  One workgroup; the host has seen to it that there are
+// no more than PROMPT_PLAN sequences.
+template <bool PAGED>
+__global__ __launch_bounds__(1024) void prompt_plan_kernel(const PromptAttention p) {
+  __shared__ int first[PROMPT_PLAN + 1], pieces_of[PROMPT_PLAN];
+  __shared__ int64_t sums[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // of `x` over all threads before this one; `all`: over all
+  auto scan = [&](int64_t x, int64_t& all) {
+    int64_t below = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t y = __shfl_up(below, d);
+      if (lane >= d) below += y;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = below;
+    __syncthreads();
+    int64_t before = 0;
+    all = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) before += sums[w];
+      all += sums[w];
+    }
+    return before + below - x;
+  };
+  constexpr int EACH = PROMPT_PLAN / 1024;
+  int64_t begin, key_begin, total = 0;
+  int window[EACH], tiles[EACH], keys;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    window[i] = tiles[i] = 0;
+    if (EACH * tid + i < p.batch) {
+      prompt_sequence<PAGED>(p, EACH * tid + i, begin, window[i], key_begin, keys);
+      tiles[i] = prompt_tiles((int)(keys < p.positions ? keys : p.positions));
+    }
+    total += (int64_t)prompt_blocks(p, window[i]) * tiles[i];
+  }
+  int64_t all, items = 0;
+  scan(total, all);
+  const int most = prompt_piece(p.items, all, p.least);
+  int pieces[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    pieces[i] = prompt_pieces(tiles[i], most);
+    items += (int64_t)prompt_blocks(p, window[i]) * pieces[i];
+  }
+  int64_t at = scan(items, all);
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    // (sequences that share rows may come to more items than there is room for)
+    first[EACH * tid + i] = (int)(at < p.slots ? at : p.slots);
+    pieces_of[EACH * tid + i] = pieces[i];
+    at += (int64_t)prompt_blocks(p, window[i]) * pieces[i];
+  }
+  if (tid == 0) first[PROMPT_PLAN] = (int)(all < p.slots ? all : p.slots);
+  __syncthreads();
+  const int count = first[PROMPT_PLAN];
+  for (int i = tid; i < p.slots; i += 1024) {
+    PromptItem b{};
+    if (i < count) {
+      int low = 0, high = PROMPT_PLAN - 1;        // the last sequence that starts at or before i
+      while (low < high) {
+        const int mid = (low + high + 1) >> 1;
+        if (first[mid] <= i) low = mid;
+        else high = mid - 1;
+      }
+      b.n = low;
+      prompt_sequence<PAGED>(p, low, b.begin, b.window, b.key_begin, b.keys);
+      b.pieces = pieces_of[low];
+      const int rank = (i - first[low]) / b.pieces;
+      b.piece = i - first[low] - rank * b.pieces;
+      b.first = i - b.piece;
+      b.row0 = (prompt_blocks(p, b.window) - 1 - rank) * PROMPT_ROWS;
+      b.rows = min(PROMPT_ROWS, b.window * p.group - b.row0);
+      if (b.first + b.pieces > p.slots) b.rows = 0;
+    }
+    p.plan[i] = b;
+  }
 }
 
 template <typename act_t> constexpr float PROMPT_SHIFT = 0.f;
@@ -133,197 +255,144 @@ template <typename act_t> __device__ __forceinline__ uint32_t all_exponent(uint3
   return ((pair & mask) == mask ? 0xffffu : 0u) | ((pair >> 16 & mask) == mask ? 0xffff0000u : 0u);
 }
 
-template <typename act_t, int D, int QT, bool PAGED>
-__global__ __launch_bounds__(256, QT * D <= 128 ? 2 : 1) void prompt_attention_kernel(const PromptAttention p) {
-  constexpr int ROWS = 128 * QT, STEPS = D / 16, TILES = D / 32, PITCH = 2 * D, TILE = PROMPT_KEYS * PITCH;
-  constexpr int LANES = PITCH / 16, ROWS_A_COPY = 64 / LANES, COPIES = 16 / ROWS_A_COPY;           // of the 16 keys that a wavefront copies
-  __shared__ __align__(1024) unsigned char tiles[2][2][TILE];
+template <typename act_t, int D, bool PAGED>
+__global__ __launch_bounds__(256, prompt_residency(D)) void prompt_attention_kernel(const PromptAttention p) {
+  constexpr int KEYS = PROMPT_KEYS, STEPS = D / 16, TILES = D / 32, PITCH = 2 * D, TILE = KEYS * PITCH;
+  constexpr int LANES = PITCH / 16, ROWS_A_COPY = 64 / LANES, COPIES = 16 / ROWS_A_COPY;           // of 16 keys or values, by a wavefront
+  __shared__ __align__(1024) unsigned char tiles[2][2][TILE];         // keys and values
   __shared__ uint32_t there[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
-  const int pieces = p.heads * p.splits, index = blockIdx.x / pieces, rest = blockIdx.x - index * pieces, head = rest / p.splits, split = rest - head * p.splits;
-  PromptBlock b;
-  if (!prompt_block<ROWS, PAGED>(p, index, b)) return;
-  const int end = prompt_limit(p, b, b.row0 + b.rows - 1);
-  const PromptShare share = prompt_share(end, p.splits);
-  const int first_tile = split * share.tiles, last_tile = min(first_tile + share.tiles, (end + PROMPT_KEYS - 1) / PROMPT_KEYS);
-  if (split >= share.pieces) return;
+  const int index = blockIdx.x / p.heads, head = blockIdx.x - index * p.heads;
+  PromptItem b;
+  if (p.plan) b = planned_item(p, index);
+  else if (!(PAGED && !p.offsets ? prefix_item<false>(p, index, b) : prompt_block<PAGED>(p, index, b))) return;
+  if (b.rows == 0) return;
+  const int tiles_seen = prompt_tiles(prompt_limit(p, b, b.row0 + b.rows - 1));
+  const PromptShare share = prompt_share(tiles_seen, b.pieces, p.least);
+  if (b.piece >= share.pieces) return;
+  const int first_tile = b.piece * share.tiles, last_tile = min(first_tile + share.tiles, tiles_seen);
+  const int copy_row = lane / LANES, granule = lane % LANES;
+  auto key_swizzle = [](int r) { return D == 64 ? (r >> 1 & 3) | (r >> 4 & 1) << 2 : (r & 7) | (r >> 4 & 1) << 3; };
+  auto value_swizzle = [](int r) { return D == 64 ? 4 * (r >> 1 & 1) : 4 * (r & 3); };
+  // Copies: wavefront w has keys and values 16 w .. + 15 of a tile.
+  uint32_t k_off[COPIES], v_off[COPIES];
+#pragma unroll
+  for (int c = 0; c < COPIES; ++c) {
+    const int r = ROWS_A_COPY * c + copy_row;
+    k_off[c] = (uint32_t)(r * p.k_token * 2) + 16 * (granule ^ key_swizzle(16 * wave + r));
+    v_off[c] = (uint32_t)(r * p.v_token * 2) + 16 * (granule ^ value_swizzle(r));
+  }
+  const uint32_t lds = lds_address(&tiles[0][0][0]);
+  // Operands: K rows are keys, lane (col, half) reads granule 2 s + half of key 32 t + col; values four keys and sixteen channels a
+  // group of 16 lanes.
+  const uint32_t k_at = lds + col * PITCH + 16 * (half ^ key_swizzle(col));
+  const int v_row = 4 * half + ((lane & 15) >> 2);
+  const uint32_t v_at = lds + TILE + v_row * PITCH + 16 * ((2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) ^ value_swizzle(v_row)) + 8 * (lane & 1);
 
   // This wavefront's rows; those past the end repeat the last one.
-  int row[QT], limit[QT];
-  bf16x8_t q[QT][STEPS];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    row[t] = b.row0 + min(32 * (QT * wave + t) + col, b.rows - 1);
-    limit[t] = prompt_limit(p, b, row[t]);
-    const int j = paged_quotient(p.by_group, row[t]), g = row[t] - j * p.group;
-    const uint16_t* src = p.q + (b.begin + j) * p.q_token + (int64_t)(head * p.group + g) * p.q_head + 8 * half;
+  const int row = b.row0 + min(32 * wave + col, b.rows - 1), limit = prompt_limit(p, b, row);
+  const int j = paged_quotient(p.by_group, row), query_head = head * p.group + row - j * p.group;
+  const int64_t token = b.begin + j;
+  const bool real = 32 * wave + col < b.rows, mine = 32 * wave < b.rows;
+  bf16x8_t q[STEPS];
+  {
+    const uint16_t* src = p.q + token * p.q_token + query_head * p.q_head + 8 * half;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       u32x4_t x = *reinterpret_cast<const u32x4_t*>(src + 16 * s);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] ^= p.flip;
-      q[t][s] = __builtin_bit_cast(bf16x8_t, x);
+      q[s] = __builtin_bit_cast(bf16x8_t, x);
     }
   }
-  const int least = __builtin_amdgcn_readfirstlane(prompt_limit(p, b, b.row0 + min(32 * QT * wave, b.rows - 1)));
-  const int most = __builtin_amdgcn_readfirstlane(prompt_limit(p, b, b.row0 + min(32 * QT * (wave + 1), b.rows) - 1));
-  const bool mine = 32 * QT * wave < b.rows;      // the wavefront has rows at all
-
-  // Copies: wavefront w has keys 16 w .. + 15 of a tile.
-  const int copy_row = lane / LANES, granule = lane % LANES;
-  auto copy_swizzle_k = [&](int r) { return D == 64 ? r >> 1 & 7 : r & 15; };
-  auto copy_swizzle_v = [&](int r) { return D == 64 ? 2 * (r >> 1 & 3) : 2 * (r & 7); };
-  uint32_t k_off[COPIES], v_off[COPIES];
-#pragma unroll
-  for (int c = 0; c < COPIES; ++c) {
-    const int r = ROWS_A_COPY * c + copy_row;
-    k_off[c] = (uint32_t)(r * p.k_token * 2) + 16 * (granule ^ copy_swizzle_k(r));
-    v_off[c] = (uint32_t)(r * p.v_token * 2) + 16 * (granule ^ copy_swizzle_v(r));
-  }
-  const uint32_t lds = lds_address(&tiles[0][0][0]);
-  int64_t table_row = 0;
+  const int least = __builtin_amdgcn_readfirstlane(prompt_limit(p, b, b.row0 + min(32 * wave, b.rows - 1)));
+  const int most = __builtin_amdgcn_readfirstlane(prompt_limit(p, b, b.row0 + min(32 * wave + 31, b.rows - 1)));
   bool has_row = true;
   const int32_t* pages = nullptr;
   if constexpr (PAGED) {
-    table_row = p.mapping ? prompt_index(p.mapping, p.mapping_wide, b.n) : b.n;
+    const int64_t table_row = p.mapping ? prompt_index(p.mapping, p.mapping_wide, b.n) : b.n;
     has_row = table_row >= 0 && table_row < p.table_rows;
     pages = uniform_pointer(p.table + (has_row ? table_row : 0) * p.table_row);
   }
-  const int sequence_keys = min((int64_t)b.keys, p.positions);
-  auto group_of = [&](int tile) { return min(tile * PROMPT_KEYS + 16 * wave, max(sequence_keys - 1, 0) & ~15); };
+  const int keys = min((int64_t)b.keys, p.positions);
+  auto group_of = [&](int tile) { return min(tile * KEYS + 16 * wave, max(keys - 1, 0) & ~15); };
   auto page_entry = [&](int tile) {
-    if (!PAGED || !has_row || sequence_keys == 0) return -1;
+    if (!PAGED || !has_row || keys == 0) return -1;
     return *(const __attribute__((address_space(4))) int32_t*)(pages + paged_quotient(p.page_of, group_of(tile)));
   };
+  // A tile's keys and values; those behind the sequence repeat its last one.
+  const uint16_t* k_base = p.k + head * p.k_head + (PAGED ? 0 : b.key_begin * p.k_token);
+  const uint16_t* v_base = p.v + head * p.v_head + (PAGED ? 0 : b.key_begin * p.v_token);
   auto copy_tile = [&](int tile, int buffer, int entry) {
+    const uint32_t to = lds + buffer * 2 * TILE + wave * 16 * PITCH;
     const int key0 = group_of(tile);
-    int last = sequence_keys - 1 - key0;          // of the 16 keys; those behind repeat it
-    const uint16_t *k, *v;
+    int last = keys - 1 - key0;
+    uint64_t k_at = (uint64_t)(uint32_t)key0 * (uint32_t)p.k_token, v_at = (uint64_t)(uint32_t)key0 * (uint32_t)p.v_token;
     if constexpr (PAGED) {
       const bool ok = entry >= 0 && entry < p.blocks;
       const int place = key0 - paged_quotient(p.page_of, key0) * p.block_size;
-      const int64_t at = ok ? entry * p.kv_block + place * p.k_token : 0;
-      k = p.k + at + head * p.k_head;
-      v = p.v + at + head * p.v_head;
-      if (!ok) last = 15;
+      k_at = ok ? entry * p.kv_block + (uint64_t)(uint32_t)place * (uint32_t)p.k_token : 0;
+      v_at = k_at;
+      last = ok ? last : 15;
       if (lane == 0) reinterpret_cast<unsigned char*>(&there[buffer])[wave] = ok;
-    } else {
-      k = p.k + (b.key_begin + key0) * p.k_token + head * p.k_head;
-      v = p.v + (b.key_begin + key0) * p.v_token + head * p.v_head;
     }
-    const uint32_t to = lds + buffer * 2 * TILE + wave * 16 * PITCH;
-    const char *kb = uniform_pointer(reinterpret_cast<const char*>(k)), *vb = uniform_pointer(reinterpret_cast<const char*>(v));
+    const char *k_from = uniform_pointer(reinterpret_cast<const char*>(k_base + k_at)), *v_from = uniform_pointer(reinterpret_cast<const char*>(v_base + v_at));
     if (last >= 15) {
 #pragma unroll
-      for (int c = 0; c < COPIES; ++c) dma16(kb, k_off[c], to + 1024 * c);
+      for (int c = 0; c < COPIES; ++c) dma16(k_from, k_off[c], to + 1024 * c);
 #pragma unroll
-      for (int c = 0; c < COPIES; ++c) dma16(vb, v_off[c], to + TILE + 1024 * c);
+      for (int c = 0; c < COPIES; ++c) dma16(v_from, v_off[c], to + TILE + 1024 * c);
     } else {
 #pragma unroll
       for (int c = 0; c < COPIES; ++c) {
-        const int r = ROWS_A_COPY * c + copy_row, back = max(r - last, 0);
-        dma16(kb, k_off[c] - (uint32_t)(back * p.k_token * 2), to + 1024 * c);
-        dma16(vb, v_off[c] - (uint32_t)(back * p.v_token * 2), to + TILE + 1024 * c);
+        const int back = max(ROWS_A_COPY * c + copy_row - last, 0);
+        dma16(k_from, k_off[c] - (uint32_t)(back * p.k_token * 2), to + 1024 * c);
+        dma16(v_from, v_off[c] - (uint32_t)(back * p.v_token * 2), to + TILE + 1024 * c);
       }
     }
   };
-  // Operands: K rows are keys, lane (col, half) reads granule 2 s + half of key 32 t + col; values four keys and sixteen channels a
-  // group of 16 lanes.
-  const uint32_t k_at = lds + col * PITCH + 16 * (half ^ copy_swizzle_k(col));
-  const int v_row = 4 * half + ((lane & 15) >> 2);
-  const uint32_t v_at = lds + TILE + v_row * PITCH + 16 * ((2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) ^ copy_swizzle_v(v_row)) + 8 * (lane & 1);
-
-  f32x16_t o[QT][TILES];
-  float top[QT], sum[QT];
+  f32x16_t o[TILES];
+  float top, sum;
 
   auto pass = [&](auto careful) {
     constexpr bool CAREFUL = decltype(careful)::value;
+    top = -INFINITY;
+    sum = 0.f;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      top[t] = -INFINITY;
-      sum[t] = 0.f;
+    for (int c = 0; c < TILES; ++c)
 #pragma unroll
-      for (int c = 0; c < TILES; ++c)
+      for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
+    auto sees = [&](int key0, uint32_t flags, int h, int i) {
+      const int key = 32 * h + 8 * (i / 4) + 4 * half + (i & 3);
+      return (key0 + key < limit) & ((flags >> (8 * (2 * h + i / 8)) & 1) != 0);
+    };
+    constexpr int HALVES = KEYS / 32;
+    constexpr uint32_t ALL = 0x01010101u;
+    f32x16_t s[HALVES];
+    auto scores = [&](int buffer) {
+      const uint32_t kb = k_at + buffer * 2 * TILE;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[t][c][i] = 0.f;
-    }
-    int entry = page_entry(first_tile);
-    if (first_tile < last_tile) copy_tile(first_tile, 0, entry);
-    entry = page_entry(first_tile + 1);
-    for (int tile = first_tile; tile < last_tile; ++tile) {
-      const int buffer = (tile - first_tile) & 1, key0 = tile * PROMPT_KEYS;
-      wait_vmcnt<0>();
-      lds_barrier();
-      if (tile + 1 < last_tile) {
-        copy_tile(tile + 1, buffer ^ 1, entry);
-        entry = page_entry(tile + 2);
-      }
-      if (!mine || key0 >= most) continue;
-      uint32_t flags = 0x01010101u;
-      if constexpr (PAGED) flags = __builtin_amdgcn_readfirstlane(there[buffer]);
-      const uint32_t kb = k_at + buffer * 2 * TILE, vb = v_at + buffer * 2 * TILE;
-      f32x16_t s[QT][2];
+      for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[t][h][i] = 0.f;
+        for (int i = 0; i < 16; ++i) s[h][i] = 0.f;
 #pragma unroll
       for (int c = 0; c < STEPS; ++c)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const bf16x8_t k = lds_operand((kb ^ (32u * c)) + h * 32 * PITCH);
+        for (int h = 0; h < HALVES; ++h) s[h] = mfma32<act_t>(lds_operand((kb ^ (32u * c)) + h * 32 * PITCH), q[c], s[h]);
+      if constexpr (!CAREFUL) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-          for (int t = 0; t < QT; ++t) s[t][h] = mfma32<act_t>(k, q[t][c], s[t][h]);
+        for (int i = 0; i < STEPS * HALVES - 4; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-      const bool masked = key0 + PROMPT_KEYS > least || flags != 0x01010101u;
-      auto sees = [&](int t, int h, int i) {
-        const int key = 32 * h + 8 * (i / 4) + 4 * half + (i & 3);
-        return (key0 + key < limit[t]) & ((flags >> (8 * (2 * h + i / 8)) & 1) != 0);
-      };
-      bf16x8_t weight[QT][4];
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        if (masked) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[t][h][i] = sees(t, h, i) ? s[t][h][i] : -INFINITY;
-        }
-        float high = fmaxf(s[t][0][0], s[t][1][0]);
-#pragma unroll
-        for (int i = 1; i < 16; ++i) high = fmaxf(fmaxf(s[t][0][i], s[t][1][i]), high);
-        high = halves_max(high) * p.scale_log2;
-        if (__ballot(high > top[t] + PROMPT_SLACK) != 0) {
-          const float now = fmaxf(top[t], high), f = step_factor(top[t], now);
-          top[t] = now;
-          sum[t] *= f;
-#pragma unroll
-          for (int c = 0; c < TILES; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[t][c][i] *= f;
-        }
-        const float zero = (top[t] == -INFINITY ? 0.f : top[t]) - PROMPT_SHIFT<act_t>;
-        float part[2] = {0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            s[t][h][i] = __builtin_amdgcn_exp2f(fmaf(s[t][h][i], p.scale_log2, -zero));
-            part[h] += s[t][h][i];
-          }
-        sum[t] += part[0] + part[1];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          u32x4_t w;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = pack2<act_t>(s[t][x / 2][8 * (x & 1) + 2 * i], s[t][x / 2][8 * (x & 1) + 2 * i + 1]);
-          weight[t][x] = __builtin_bit_cast(bf16x8_t, w);
-        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
       }
+    };
+    auto product = [&](int buffer, int key0, uint32_t flags, const bf16x8_t (&weight)[2 * HALVES]) {
+      const uint32_t vb = v_at + buffer * 2 * TILE;
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+      for (int x = 0; x < 2 * HALVES; ++x)
 #pragma unroll
         for (int c = 0; c < TILES; ++c) {
           const uint32_t at = (vb ^ (64u * c)) + 16 * x * PITCH;
@@ -348,59 +417,105 @@ __global__ __launch_bounds__(256, QT * D <= 128 ? 2 : 1) void prompt_attention_k
             }
             v = __builtin_bit_cast(bf16x8_t, w);
             if (__ballot(any != 0) != 0) {
+              u32x4_t marks;
 #pragma unroll
-              for (int t = 0; t < QT; ++t) {
-                u32x4_t marks;
+              for (int i = 0; i < 4; ++i)
+                marks[i] = one & ((sees(key0, flags, x / 2, 8 * (x & 1) + 2 * i) ? 0xffffu : 0u) | (sees(key0, flags, x / 2, 8 * (x & 1) + 2 * i + 1) ? 0xffff0000u : 0u));
+              f32x16_t up, down;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  marks[i] = one & ((sees(t, x / 2, 8 * (x & 1) + 2 * i) ? 0xffffu : 0u) | (sees(t, x / 2, 8 * (x & 1) + 2 * i + 1) ? 0xffff0000u : 0u));
-                f32x16_t up, down;
+              for (int i = 0; i < 16; ++i) up[i] = down[i] = 0.f;
+              up = mfma32<act_t>(__builtin_bit_cast(bf16x8_t, plus), __builtin_bit_cast(bf16x8_t, marks), up);
+              down = mfma32<act_t>(__builtin_bit_cast(bf16x8_t, minus), __builtin_bit_cast(bf16x8_t, marks), down);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) up[i] = down[i] = 0.f;
-                up = mfma32<act_t>(__builtin_bit_cast(bf16x8_t, plus), __builtin_bit_cast(bf16x8_t, marks), up);
-                down = mfma32<act_t>(__builtin_bit_cast(bf16x8_t, minus), __builtin_bit_cast(bf16x8_t, marks), down);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[t][c][i] += (up[i] > 0.f ? INFINITY : 0.f) + (down[i] > 0.f ? -INFINITY : 0.f);
-              }
+              for (int i = 0; i < 16; ++i) o[c][i] += (up[i] > 0.f ? INFINITY : 0.f) + (down[i] > 0.f ? -INFINITY : 0.f);
             }
           }
-#pragma unroll
-          for (int t = 0; t < QT; ++t) o[t][c] = mfma32<act_t>(v, weight[t][x], o[t][c]);
+          o[c] = mfma32<act_t>(v, weight[x], o[c]);
         }
+    };
+    // Scores to weights, with the sum; returns the factor of what was summed before.
+    auto raise = [&](int key0, uint32_t flags) {
+      if (key0 + KEYS > least || flags != ALL) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[h][i] = sees(key0, flags, h, i) ? s[h][i] : -INFINITY;
+      }
+      float high = fmaxf(s[0][0], s[HALVES - 1][0]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) high = fmaxf(fmaxf(s[0][i], s[HALVES - 1][i]), high);
+      high = halves_max(high) * p.scale_log2;
+      const float now = high > top + PROMPT_SLACK ? high : top, f = step_factor(top, now);
+      top = now;
+      return f;
+    };
+    auto weigh = [&](float f, bf16x8_t (&weight)[2 * HALVES]) {
+      const float zero = (top == -INFINITY ? 0.f : top) - PROMPT_SHIFT<act_t>;
+      float part[2] = {sum * f, 0.f};
+#pragma unroll
+      for (int x = 0; x < 2 * HALVES; ++x) {
+        u32x4_t w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float low = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x & 1) + 2 * i], p.scale_log2, -zero));
+          const float high = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x & 1) + 2 * i + 1], p.scale_log2, -zero));
+          part[0] += low;
+          part[1] += high;
+          w[i] = pack2<act_t>(low, high);
+        }
+        weight[x] = __builtin_bit_cast(bf16x8_t, w);
+      }
+      sum = part[0] + part[1];
+    };
+    int entry = page_entry(first_tile);
+    if (first_tile < last_tile) copy_tile(first_tile, 0, entry);
+    entry = page_entry(first_tile + 1);
+    for (int tile = first_tile; tile < last_tile; ++tile) {
+      const int buffer = (tile - first_tile) & 1, key0 = tile * KEYS;
+      wait_vmcnt<0>();
+      lds_barrier();
+      if (tile + 1 < last_tile) {
+        copy_tile(tile + 1, buffer ^ 1, entry);
+        entry = page_entry(tile + 2);
+      }
+      if (!mine || key0 >= most) continue;
+      uint32_t flags = ALL;
+      if constexpr (PAGED) flags = __builtin_amdgcn_readfirstlane(there[buffer]);
+      scores(buffer);
+      const float f = raise(key0, flags);
+      if (__ballot(f != 1.f) != 0) {
+#pragma unroll
+        for (int c = 0; c < TILES; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[c][i] *= f;
+      }
+      bf16x8_t weight[2 * HALVES];
+      weigh(f, weight);
+      product(buffer, key0, flags, weight);
     }
   };
   pass(std::false_type{});
   // A NaN may be one of the formula's, or an infinite or NaN value whose weight is zero: once more, with such values apart.
   float check = 0.f;
 #pragma unroll
-  for (int t = 0; t < QT; ++t)
+  for (int c = 0; c < TILES; ++c)
 #pragma unroll
-    for (int c = 0; c < TILES; ++c)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) check += o[t][c][i] * 0.f;
+    for (int i = 0; i < 16; ++i) check += o[c][i] * 0.f;
   if (__syncthreads_or(check != check)) pass(std::true_type{});
   if (!mine) return;
-
+  const float total = halves_sum(sum);
+  if (share.pieces > 1 || !p.offsets) {
+    const int64_t at = share.pieces == 1 ? token * (p.heads * p.group) + query_head
+                                         : ((int64_t)(b.first + b.piece) * p.heads + head) * p.slot_rows + 32 * wave + col;
+    float* to = (share.pieces == 1 ? p.rows : p.partial) + at * D;
+    if (real) {
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const bool real = 32 * (QT * wave + t) + col < b.rows;
-    const int j = paged_quotient(p.by_group, row[t]), g = row[t] - j * p.group;
-    const int64_t token = b.begin + j;
-    const int query_head = head * p.group + g;
-    const float total = halves_sum(sum[t]);
-    if (p.tops && (share.pieces > 1 || !p.offsets)) {
-      const int64_t at = ((int64_t)split * p.tokens + token) * (p.heads * p.group) + query_head;
-      if (real) {
+      for (int c = 0; c < TILES; ++c)
 #pragma unroll
-        for (int c = 0; c < TILES; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<float4*>(p.partial + at * D + 32 * c + 8 * i + 4 * half) =
-                float4{o[t][c][4 * i], o[t][c][4 * i + 1], o[t][c][4 * i + 2], o[t][c][4 * i + 3]};
-        if (half == 0) p.tops[at] = float2{top[t] - PROMPT_SHIFT<act_t>, total};
-      }
-      continue;
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(to + 32 * c + 8 * i + 4 * half) = float4{o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]};
+      if (half == 0) (share.pieces == 1 ? p.row_tops : p.tops)[at] = float2{top - PROMPT_SHIFT<act_t>, total};
     }
+  } else {
     const float norm = total == 0.f ? 0.f : 1.0f / total;         // no key: zeros
 #pragma unroll
     for (int c = 0; c < TILES; ++c)
@@ -410,7 +525,7 @@ __global__ __launch_bounds__(256, QT * D <= 128 ? 2 : 1) void prompt_attention_k
         float y[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float low = o[t][c][8 * x + i], high = o[t][c][8 * x + 4 + i];
+          const float low = o[c][8 * x + i], high = o[c][8 * x + 4 + i];
           const auto w = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, low), __builtin_bit_cast(uint32_t, high), false, false);
           const uint32_t first = w[0], second = w[1];
           y[i] = __builtin_bit_cast(float, first) * norm;
@@ -432,31 +547,54 @@ __global__ __launch_bounds__(256, QT * D <= 128 ? 2 : 1) void prompt_attention_k
   }
 }
 
-// Pieces of a row block to its output: a wavefront a row at a time, a lane D / 64 channels.
-template <typename act_t, int D, int ROWS, bool PAGED>
+// Pieces of a row block to its output, or (a prefix) to one piece for each row: a wavefront a row at a time, a lane D / 64 channels.
+template <typename act_t, int D>
 __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptAttention p) {
-  constexpr int LANE = D / 64;
+  constexpr int LANE = D / 64, AHEAD = 8;
   typedef float lane_t __attribute__((ext_vector_type(LANE)));
   const int index = blockIdx.x / p.heads, head = blockIdx.x - index * p.heads;
-  PromptBlock b;
-  if (!prompt_block<ROWS, PAGED>(p, index, b)) return;
-  const PromptShare share = prompt_share(prompt_limit(p, b, b.row0 + b.rows - 1), p.splits);
+  PromptItem b;
+  if (p.plan) b = planned_item(p, index);
+  else if (!prefix_item<true>(p, index, b)) return;
+  if (b.rows == 0 || b.piece != 0 || b.pieces < 2) return;
+  const PromptShare share = prompt_share(prompt_tiles(prompt_limit(p, b, b.row0 + b.rows - 1)), b.pieces, p.least);
   if (share.pieces < 2) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int r = blockIdx.y * 4 + wave; r < b.rows; r += 4 * gridDim.y) {
     const int j = paged_quotient(p.by_group, b.row0 + r), query_head = head * p.group + b.row0 + r - j * p.group;
-    const int64_t token = b.begin + j;
+    const int64_t token = b.begin + j, first = ((int64_t)b.first * p.heads + head) * p.slot_rows + r, step = (int64_t)p.heads * p.slot_rows;
     float top = -INFINITY, sum = 0.f;
     lane_t o = {};
-    for (int s = 0; s < share.pieces; ++s) {
-      const int64_t at = ((int64_t)s * p.tokens + token) * (p.heads * p.group) + query_head;
-      const float2 y = p.tops[at];
-      const lane_t x = *reinterpret_cast<const lane_t*>(p.partial + at * D + LANE * lane);
-      const float now = fmaxf(top, y.x), back = step_factor(top, now), f = step_factor(y.x, now);
-      sum = fmaf(y.y, f, sum * back);
+    for (int i = 0; i < share.pieces; i += AHEAD) {
+      float2 y[AHEAD];
+      lane_t x[AHEAD];
 #pragma unroll
-      for (int c = 0; c < LANE; ++c) o[c] = fmaf(x[c], f, o[c] * back);
+      for (int a = 0; a < AHEAD; ++a) {
+        const int64_t at = first + min(i + a, share.pieces - 1) * step;
+        y[a] = p.tops[at];
+        x[a] = *reinterpret_cast<const lane_t*>(p.partial + at * D + LANE * lane);
+      }
+      float now = top;
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) now = fmaxf(now, y[a].x);          // one piece twice does no harm here
+      const float back = step_factor(top, now);
+      sum *= back;
+      o *= back;
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const bool counts = i + a < share.pieces;
+        const float f = step_factor(y[a].x, now);
+        sum = counts ? fmaf(y[a].y, f, sum) : sum;
+#pragma unroll
+        for (int c = 0; c < LANE; ++c) o[c] = counts ? fmaf(x[a][c], f, o[c]) : o[c];
+      }
       top = now;
+    }
+    if (!p.offsets) {
+      const int64_t at = token * (p.heads * p.group) + query_head;
+      *reinterpret_cast<lane_t*>(p.rows + at * D + LANE * lane) = o;
+      if (lane == 0) p.row_tops[at] = float2{top, sum};
+      continue;
     }
     const float norm = sum == 0.f ? 0.f : 1.0f / sum;
     float y[LANE];
@@ -474,16 +612,9 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptAttention 
 
 template <typename act_t, int D, bool PAGED>
 static void launch_prompt(const PromptAttention& p, const PromptLaunch& l, hipStream_t s) {
-  const dim3 grid((unsigned)(l.blocks * p.heads * l.splits));
-  if constexpr (D != 256) {
-    if (l.rows == 256) prompt_attention_kernel<act_t, D, 2, PAGED><<<grid, 256, 0, s>>>(p);
-  }
-  if (l.rows == 128) prompt_attention_kernel<act_t, D, 1, PAGED><<<grid, 256, 0, s>>>(p);
-  if (l.splits > 1 && p.offsets) {
-    const dim3 join((unsigned)(l.blocks * p.heads), (unsigned)(l.rows / 16));
-    if (l.rows == 256) prompt_join_kernel<act_t, D, 256, PAGED><<<join, 256, 0, s>>>(p);
-    else prompt_join_kernel<act_t, D, 128, PAGED><<<join, 256, 0, s>>>(p);
-  }
+  if (p.plan) prompt_plan_kernel<PAGED><<<1, 1024, 0, s>>>(p);
+  prompt_attention_kernel<act_t, D, PAGED><<<dim3((unsigned)(l.items * p.heads)), 256, 0, s>>>(p);
+  if (l.split) prompt_join_kernel<act_t, D><<<dim3((unsigned)((p.plan ? l.items : l.blocks) * p.heads), (unsigned)l.join_rows), 256, 0, s>>>(p);
 }
 template <bool PAGED>
 static void launch_prompt(const PromptAttention& p, const PromptLaunch& l, int D, int act, hipStream_t s) {
@@ -498,16 +629,36 @@ static void launch_prompt(const PromptAttention& p, const PromptLaunch& l, int D
   }
 }
 
-PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, int64_t keys) {
+PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, int64_t keys, bool prefix) {
   PromptLaunch l{};
   const int64_t rows = tokens * (HQ / HKV);
-  l.rows = D != 256 && (rows / 256 + batch) * HKV >= 256 ? 256 : 128;
   // a sequence has a block that is not full, and there are no more blocks than rows
-  l.blocks = rows / l.rows + batch;
+  l.blocks = prefix ? (rows + PROMPT_ROWS - 1) / PROMPT_ROWS : rows / PROMPT_ROWS + batch;
   if (l.blocks > rows) l.blocks = rows;
-  const int64_t groups = l.blocks * HKV, most = (keys + 4 * PROMPT_KEYS - 1) / (4 * PROMPT_KEYS);
-  l.splits = (int)(groups >= 256 ? 1 : (511 / groups < most ? 511 / groups : most));
-  if (l.splits < 1) l.splits = 1;
+  l.least = prefix ? 4 : 8;
+  // Pieces and blocks together fill the chip twice, or (few rows over a prefix) once: an unequal end costs less than twice the pieces, which
+  // are written and read again.  1500 tokens over 60 000 keys 1542 us (three times 1572, four 1574, not split 1650), eighteen parts of
+  // prompts with heads of 64 145 (155, 169, 163).
+  const int64_t room = 256 * prompt_residency(D), fill = (prefix && l.blocks * HKV <= room / 2 ? 1 : 2) * room / HKV - l.blocks;
+  l.split = prefix || (l.blocks * HKV < 2 * room && batch <= PROMPT_PLAN && keys > 2 * l.least * PROMPT_KEYS);
+  l.pieces = !l.split ? 0 : fill > 1 ? fill : 1;
+  l.items = l.blocks + l.pieces;
+  l.slot_rows = (int)(rows < PROMPT_ROWS ? rows : PROMPT_ROWS);
+  // Rows of a block at once: all where few blocks have many pieces (64 chats over 8000 keys 62.6 us, a quarter at once 72).
+  l.join_rows = (l.slot_rows + (prefix ? 3 : 15)) / (prefix ? 4 : 16);
+  if (l.split) {
+    int64_t at = l.items * HKV * l.slot_rows * D * 4;
+    auto take = [&](int64_t bytes) {
+      const int64_t here = at;
+      at += (bytes + 255) / 256 * 256;
+      return here;
+    };
+    l.tops_at = take(l.items * HKV * l.slot_rows * 8);
+    l.plan_at = take(prefix ? 0 : l.items * (int64_t)sizeof(PromptItem));
+    l.rows_at = take(prefix ? tokens * HQ * D * 4 : 0);
+    l.row_tops_at = take(prefix ? tokens * HQ * 8 : 0);
+    l.bytes = at;
+  }
   return l;
 }
 
@@ -515,19 +666,13 @@ int check_prompt(int batch, int64_t tokens, int HQ, int HKV, int D) {
   PLA_REQUIRE(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got %d", D);
   PLA_REQUIRE(HKV > 0 && HQ >= HKV && HQ % HKV == 0, "query heads must be a positive multiple of key-value heads");
   PLA_REQUIRE(batch >= 0 && tokens >= 0 && tokens * HQ <= (1 << 30), "too many rows");
-  PLA_REQUIRE((tokens * (HQ / HKV) / 128 + batch) * HKV < (1 << 24), "too many sequences");
+  PLA_REQUIRE((tokens * (HQ / HKV) / PROMPT_ROWS + batch) * HKV < (1 << 23), "too many sequences");
   return 0;
 }
 
-int64_t prompt_tops_at(const PromptLaunch& l, int64_t tokens, int HQ, int D) { return l.splits * tokens * HQ * D * 4; }
-int64_t prompt_bytes(const PromptLaunch& l, int64_t tokens, int HQ, int D, bool always) {
-  return l.splits > 1 || always ? (prompt_tops_at(l, tokens, HQ, D) + l.splits * tokens * HQ * 8 + 255) / 256 * 256 : 0;
-}
-
-int launch_prompt(PromptAttention p, const PromptLaunch& l, bool paged, int HQ, int D, float scale, int act, void* workspace, int64_t workspace_bytes,
+int launch_prompt(PromptAttention p, const PromptLaunch& l, bool paged, int D, float scale, int act, void* workspace, int64_t workspace_bytes,
                          hipStream_t s) {
-  const int64_t bytes = prompt_bytes(l, p.tokens, HQ, D, !p.offsets);
-  PLA_REQUIRE(workspace_bytes >= bytes && (bytes == 0 || workspace), "workspace too small: %lld bytes needed", (long long)bytes);
+  PLA_REQUIRE(workspace_bytes >= l.bytes && (l.bytes == 0 || workspace), "workspace too small: %lld bytes needed", (long long)l.bytes);
   PLA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be 16-byte aligned");
   for (const int64_t x : {p.q_token, p.q_head, p.k_token, p.k_head, p.v_token, p.v_head, p.kv_block, p.gate_token, p.gate_head, p.out_token, p.out_head})
     PLA_REQUIRE(x % 8 == 0, "rows must be 16-byte aligned");
@@ -538,10 +683,18 @@ int launch_prompt(PromptAttention p, const PromptLaunch& l, bool paged, int HQ, 
   // leaves finite scores equal.
   p.flip = scale < 0.f ? 0x80008000u : 0u;
   p.scale_log2 = scale == 0.f ? 1e-38f : fabsf(scale) * 1.44269504088896341f;
-  p.splits = l.splits;
-  char* ws = static_cast<char*>(workspace);
-  p.partial = bytes ? reinterpret_cast<float*>(ws) : nullptr;
-  p.tops = bytes ? reinterpret_cast<float2*>(ws + prompt_tops_at(l, p.tokens, HQ, D)) : nullptr;
+  p.items = (int)l.pieces;
+  p.least = l.least;
+  p.slots = (int)l.items;
+  p.slot_rows = l.slot_rows;
+  if (l.split) {
+    char* ws = static_cast<char*>(workspace);
+    p.partial = reinterpret_cast<float*>(ws);
+    p.tops = reinterpret_cast<float2*>(ws + l.tops_at);
+    p.plan = p.offsets ? reinterpret_cast<PromptItem*>(ws + l.plan_at) : nullptr;
+    p.rows = reinterpret_cast<float*>(ws + l.rows_at);
+    p.row_tops = reinterpret_cast<float2*>(ws + l.row_tops_at);
+  }
   if (paged) launch_prompt<true>(p, l, D, act, s);
   else launch_prompt<false>(p, l, D, act, s);
   return check_launch("prompt_attention_kernel");
@@ -553,7 +706,7 @@ extern "C" int64_t pla_prompt_attention_workspace_bytes(int batch, int64_t token
   using namespace pla;
   if (check_prompt(batch, tokens, HQ, HKV, head_dim) || keys < 0) return -1;
   if (batch == 0 || tokens == 0) return 0;
-  return prompt_bytes(prompt_launch(batch, tokens, HQ, HKV, head_dim, keys), tokens, HQ, head_dim, false);
+  return prompt_launch(batch, tokens, HQ, HKV, head_dim, keys, false).bytes;
 }
 
 extern "C" int pla_prompt_attention_launch(
@@ -577,7 +730,7 @@ extern "C" int pla_prompt_attention_launch(
   p.out = (uint16_t*)out; p.out_token = out_token; p.out_head = out_head;
   p.batch = batch; p.tokens = tokens; p.heads = HKV; p.group = HQ / HKV; p.by_group = paged_divisor(HQ / HKV);
   p.positions = keys;
-  return launch_prompt(p, prompt_launch(batch, tokens, HQ, HKV, head_dim, keys), false, HQ, head_dim, scale, act_dtype, workspace, workspace_bytes,
+  return launch_prompt(p, prompt_launch(batch, tokens, HQ, HKV, head_dim, keys, false), false, head_dim, scale, act_dtype, workspace, workspace_bytes,
                        static_cast<hipStream_t>(stream));
 }
 
@@ -612,6 +765,6 @@ extern "C" int pla_paged_prompt_attention_launch(
   p.out = (uint16_t*)out; p.out_token = out_token; p.out_head = out_head;
   p.batch = batch; p.tokens = tokens; p.heads = HKV; p.group = HQ / HKV; p.by_group = paged_divisor(HQ / HKV);
   p.positions = positions;
-  return launch_prompt(p, prompt_launch(batch, tokens, HQ, HKV, head_dim, positions), true, HQ, head_dim, scale, act_dtype, workspace, workspace_bytes,
+  return launch_prompt(p, prompt_launch(batch, tokens, HQ, HKV, head_dim, positions, false), true, head_dim, scale, act_dtype, workspace, workspace_bytes,
                        static_cast<hipStream_t>(stream));
 }
