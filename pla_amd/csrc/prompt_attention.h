@@ -63,7 +63,7 @@ constexpr PLA_HD int prompt_residency(int D) { return D == 256 ? 1 : D == 64 ? 3
 struct PromptLaunch {
   int64_t blocks, items, pieces;                  // row blocks at most, workgroups a head, pieces (0: not split) that a head's keys are cut into
   int least, slot_rows, join_rows;
-  bool split;
+  bool split, plan;                               // whether keys are cut into pieces, whether the items are listed
   int64_t tops_at, plan_at, rows_at, row_tops_at, bytes;   // workspace
 };
 PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, int64_t keys, bool prefix);

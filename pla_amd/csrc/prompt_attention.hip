@@ -80,7 +80,7 @@ __device__ __forceinline__ void prompt_sequence(const PromptAttention& p, int n,
 
 __device__ __forceinline__ int prompt_blocks(const PromptAttention& p, int window) { return (int)(((int64_t)window * p.group + PROMPT_ROWS - 1) / PROMPT_ROWS); }
 
-// Row block `index` of a call that is not split.  Blocks of a sequence stand last one first: it has the most keys, and the shortest end the
+// Row block `index` of a call without a list of them.  Blocks of a sequence stand last one first: it has the most keys, and the shortest end the
 // call.
 template <bool PAGED>
 __device__ __forceinline__ bool prompt_block(const PromptAttention& p, int index, PromptItem& b) {
@@ -145,7 +145,7 @@ __device__ __forceinline__ int prompt_limit(const PromptAttention& p, const Prom
   return (int)(limit < 0 ? 0 : limit < most ? limit : most);
 }
 
-// The items of a call that is split, block by block, the last one of a sequence first.  One workgroup; the host has seen to it that there are
+// The list of a call's items, block by block, the last one of a sequence first.  One workgroup; the host has seen to it that there are
 // no more than PROMPT_PLAN sequences.
 template <bool PAGED>
 __global__ __launch_bounds__(1024) void prompt_plan_kernel(const PromptAttention p) {
@@ -492,6 +492,15 @@ __global__ __launch_bounds__(256, prompt_residency(D)) void prompt_attention_ker
       bf16x8_t weight[2 * HALVES];
       weigh(f, weight);
       product(buffer, key0, flags, weight);
+      if constexpr (!CAREFUL && D == 256) {       // (827 -> 815 us; smaller heads, of which a CU has more wavefronts, gain nothing)
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+#pragma unroll
+        for (int i = 0; i < 2 * HALVES * TILES - 4; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
+      }
     }
   };
   pass(std::false_type{});
@@ -643,18 +652,21 @@ PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, in
   l.split = prefix || (l.blocks * HKV < 2 * room && batch <= PROMPT_PLAN && keys > 2 * l.least * PROMPT_KEYS);
   l.pieces = !l.split ? 0 : fill > 1 ? fill : 1;
   l.items = l.blocks + l.pieces;
+  // A list of the items: for pieces, and where every workgroup would look through many sequences for its own (prompts of 64 tokens, 16 + 2
+  // heads: 128 of them 28.5 us with a list and 25.2 without, 300 54 and 61, 1000 161 and 279), unless it is long itself.
+  l.plan = !prefix && (l.split || (batch > 192 && batch <= PROMPT_PLAN && l.blocks <= 8192));
   l.slot_rows = (int)(rows < PROMPT_ROWS ? rows : PROMPT_ROWS);
   // Rows of a block at once: all where few blocks have many pieces (64 chats over 8000 keys 62.6 us, a quarter at once 72).
   l.join_rows = (l.slot_rows + (prefix ? 3 : 15)) / (prefix ? 4 : 16);
-  if (l.split) {
-    int64_t at = l.items * HKV * l.slot_rows * D * 4;
+  if (l.split || l.plan) {
+    int64_t at = l.split ? l.items * HKV * l.slot_rows * D * 4 : 0;
     auto take = [&](int64_t bytes) {
       const int64_t here = at;
       at += (bytes + 255) / 256 * 256;
       return here;
     };
-    l.tops_at = take(l.items * HKV * l.slot_rows * 8);
-    l.plan_at = take(prefix ? 0 : l.items * (int64_t)sizeof(PromptItem));
+    l.tops_at = take(l.split ? l.items * HKV * l.slot_rows * 8 : 0);
+    l.plan_at = take(l.plan ? l.items * (int64_t)sizeof(PromptItem) : 0);
     l.rows_at = take(prefix ? tokens * HQ * D * 4 : 0);
     l.row_tops_at = take(prefix ? tokens * HQ * 8 : 0);
     l.bytes = at;
@@ -687,11 +699,11 @@ int launch_prompt(PromptAttention p, const PromptLaunch& l, bool paged, int D, f
   p.least = l.least;
   p.slots = (int)l.items;
   p.slot_rows = l.slot_rows;
-  if (l.split) {
+  if (l.split || l.plan) {
     char* ws = static_cast<char*>(workspace);
     p.partial = reinterpret_cast<float*>(ws);
     p.tops = reinterpret_cast<float2*>(ws + l.tops_at);
-    p.plan = p.offsets ? reinterpret_cast<PromptItem*>(ws + l.plan_at) : nullptr;
+    p.plan = l.plan ? reinterpret_cast<PromptItem*>(ws + l.plan_at) : nullptr;
     p.rows = reinterpret_cast<float*>(ws + l.rows_at);
     p.row_tops = reinterpret_cast<float2*>(ws + l.row_tops_at);
   }

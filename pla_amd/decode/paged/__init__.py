@@ -202,7 +202,8 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, query_
     timing.
     """
     if _sanity_enabled():
-        from ._sanity import check_attention
+        from ._sanity import check_attention, check_prefix
         check_attention(q, k_cache, block_table, seq_lens, query_start_loc, request_indices, max_query_len)
+        check_prefix(k_cache, prefix_blocks, prefix_len)
     return _compiled().paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, query_start_loc, request_indices,
                                               max_query_len, scale, output_gate, out, k_scales, v_scales, prefix_blocks, prefix_len)

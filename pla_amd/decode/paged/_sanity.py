@@ -81,6 +81,16 @@ def check_attention(q, k_cache, block_table, seq_lens, query_start_loc, request_
             _fail(op, "a block of the table is not in the cache")
 
 
+def check_prefix(k_cache, prefix_blocks, prefix_len):
+    if prefix_blocks is None or prefix_len is None or _capturing() or not _formed(None, prefix_blocks, prefix_len) or prefix_len.numel() != 1 or k_cache.dim() < 2:
+        return
+    op, length, block_size = "paged_attention_decode", prefix_len.item(), k_cache.size(1)
+    if not 0 <= length <= prefix_blocks.numel() * block_size:
+        _fail(op, "prefix_len is negative or passes prefix_blocks")
+    if any(not 0 <= b < k_cache.size(0) for b in prefix_blocks[:-(-length // block_size)].tolist()):
+        _fail(op, "a block of the prefix is not in the cache")
+
+
 def check_packed(q, k, cu_seqlens, cu_seqlens_k):
     if _capturing() or not _formed(None, cu_seqlens, cu_seqlens_k) or q.dim() < 1 or k.dim() < 1 or cu_seqlens.numel() < 1:
         return

@@ -40,7 +40,7 @@ def paged_attention_prefill(q, k_cache, v_cache, block_table, seq_lens, query_st
     earlier tokens are cached, or both in one batch.
 
     Arguments, masks and what becomes of entries that are out of range are those of ``pla.decode.paged.paged_attention_decode``, with
-    ``query_start_loc`` [N+1] always given and no longest window.  Windows of up to 32 tokens are better off there: it is made for few
+    ``query_start_loc`` [N+1] always given, no longest window, and caches of q's type.  Windows of up to 32 tokens are better off there: it is made for few
     rows, and keeps twice the digits of a weight.
     """
     if _paged._sanity_enabled():

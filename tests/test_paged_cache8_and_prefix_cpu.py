@@ -117,3 +117,17 @@ def test_workspace_of_a_prefix_is_host_arithmetic():
     # one piece is kept even of a prefix of no pages
     assert size(3, 3, 4, 2, 128, 1, 4096, 0) >= plain(3, 4, 2, 128, 1, 4096) + 3 * 4 * (128 * 4 + 8)
     assert size(64, 64, 32, 8, 128, 1, 4096, 1 << 16) == size(64, 64, 32, 8, 128, 1, 4096, 16)          # the length stands on the device
+
+
+def test_sanity_mode_names_a_prefix_that_would_be_cut_or_left_out(monkeypatch):
+    ints = lambda *x: torch.tensor(x, **_INTS)
+    monkeypatch.setenv("PLA_SANITY_CHECK", "1")
+    for blocks, length, message in ((ints(1, 2), ints(33), "passes prefix_blocks"), (ints(1, 2), ints(-1), "negative"), (ints(1, 5), ints(17), "not in the cache"),
+                                    (ints(-1, 2), ints(1), "not in the cache")):
+        with pytest.raises(RuntimeError, match=r"PLA_SANITY_CHECK \[paged_attention_decode\]: .*" + message):
+            paged_attention_decode(**_prefix_args(prefix_blocks=blocks, prefix_len=length))
+    for blocks, length in ((ints(1, 5), ints(16)), (ints(1, 2), ints(0)), (ints(), ints(0))):
+        with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+            paged_attention_decode(**_prefix_args(prefix_blocks=blocks, prefix_len=length))
+    with pytest.raises(RuntimeError, match="prefix_len must have 1 entries"):
+        paged_attention_decode(**_prefix_args(prefix_len=ints(1, 2)))

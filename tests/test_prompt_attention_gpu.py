@@ -102,7 +102,7 @@ def test_short_prompts_of_every_length(D, act, HQ, HKV, gated, strided):
 
 @pytest.mark.parametrize("lens, HQ, HKV, D, act", [
     ([2500], 16, 2, 128, "bf16"), ([1], 16, 2, 64, "fp16"), ([1999, 3, 1000], 32, 8, 128, "fp16"), ([1537], 10, 10, 64, "bf16"), ([901, 2048], 8, 1, 256, "bf16"),
-    ([40] * 150, 4, 4, 128, "bf16"), ([777], 15, 3, 256, "fp16"), ([2100], 32, 32, 64, "fp16")])
+    ([40] * 150, 4, 4, 128, "bf16"), ([3, 0, 70, 1] * 90, 4, 1, 64, "fp16"), ([2] * 2100, 2, 1, 64, "bf16"), ([9, 0] * 150 + [1500], 8, 8, 128, "bf16"), ([777], 15, 3, 256, "fp16"), ([2100], 32, 32, 64, "fp16")])
 def test_longer_prompts(lens, HQ, HKV, D, act):
     _check_packed(lens, HQ, HKV, D, act, seed=sum(lens), wide=torch.int64)
 
@@ -153,8 +153,25 @@ def test_rows_of_no_sequence_and_sequences_that_are_passed_over():
     packed_attention_fwd(q, k, v, _ints([0, 9, 20]), cu_seqlens_k=_ints([0, 40, 51]), out=out)
     assert (out[9:] == 5).all() and (out[:9] != 5).any()
     assert packed_attention_fwd(q[:0], k[:0], v[:0], _ints([0, 0])).shape == (0, 4, 128)
+    assert (packed_attention_fwd(q, k[:0], v[:0], _ints([0, 20, 50]), cu_seqlens_k=_ints([0, 0, 0])) == 0).all()         # no keys at all
     packed_attention_fwd(q, k, v, _ints([0]), out=out)
     assert (out[9:] == 5).all()
+
+
+@pytest.mark.parametrize("T, N", [(50, 40), (3000, 30), (600, 1500)])
+def test_sequences_that_share_rows_stay_within_bounds(T, N):
+    """Not a call to make, but one that ends: offsets go forth and back, so that sequences come to more row blocks than T and N allow."""
+    from pla.prefill.attention import packed_attention_fwd
+    q, k, v = _randn(1, T, 8, 64, dtype=torch.bfloat16), _randn(2, 9000, 2, 64, dtype=torch.bfloat16), _randn(3, 9000, 2, 64, dtype=torch.bfloat16)
+    offsets, keys = [], []
+    for n in range(N + 1):
+        offsets.append(0 if n % 2 == 0 else T)
+        keys.append(0 if n % 2 == 0 else 9000)
+    out = torch.full_like(q, 5.0)
+    packed_attention_fwd(q, k, v, _ints(offsets), cu_seqlens_k=_ints(keys), out=out)
+    torch.cuda.synchronize()
+    # the sequence (it is always the same one) that stands first has been taken
+    _close(out[-1:], *_reference(q[-1:], k, v, 64 ** -0.5))
 
 
 def _formula(q, k, v, scale):
