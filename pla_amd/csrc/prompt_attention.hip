@@ -645,11 +645,13 @@ PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, in
   l.blocks = prefix ? (rows + PROMPT_ROWS - 1) / PROMPT_ROWS : rows / PROMPT_ROWS + batch;
   if (l.blocks > rows) l.blocks = rows;
   l.least = prefix ? 4 : 8;
-  // Pieces and blocks together fill the chip twice, or (few rows over a prefix) once: an unequal end costs less than twice the pieces, which
-  // are written and read again.  1500 tokens over 60 000 keys 1542 us (three times 1572, four 1574, not split 1650), eighteen parts of
-  // prompts with heads of 64 145 (155, 169, 163).
-  const int64_t room = 256 * prompt_residency(D), fill = (prefix && l.blocks * HKV <= room / 2 ? 1 : 2) * room / HKV - l.blocks;
-  l.split = prefix || (l.blocks * HKV < 2 * room && batch <= PROMPT_PLAN && keys > 2 * l.least * PROMPT_KEYS);
+  // Pieces and blocks together fill the chip twice: an unequal end costs less than twice the pieces, which are written and read again.  1500
+  // tokens over 60 000 keys 1542 us (three times 1572, four 1574, not split 1650), eighteen parts of prompts with heads of 64 145 (155, 169,
+  // 163).  A prefix's blocks are alike and end together: once (100 windows of four over 30 000 keys 96 us, twice 115), with very few rows,
+  // whose pieces are as large as the prefix, half (64 chats over 8000 keys, 8 heads, 57.4, once 61.1; the windows 104).
+  const int64_t room = 256 * prompt_residency(D), groups = l.blocks * HKV;
+  const int64_t fill = (!prefix || groups > room / 2 ? 2 * room : groups > room / 32 ? room : room / 2) / HKV - l.blocks;
+  l.split = prefix || (groups < 2 * room && batch <= PROMPT_PLAN && keys > 2 * l.least * PROMPT_KEYS);
   l.pieces = !l.split ? 0 : fill > 1 ? fill : 1;
   l.items = l.blocks + l.pieces;
   // A list of the items: for pieces, and where every workgroup would look through many sequences for its own (prompts of 64 tokens, 16 + 2
