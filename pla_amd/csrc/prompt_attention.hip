@@ -31,7 +31,8 @@
 //
 // Infinite and NaN values: a weight of zero times one is NaN, where the formula has no product (a key that the row does not see) or an
 // infinite one (a weight that is zero only in 32 bits).  The loop does not look for them.  Where an output comes out infinite or NaN the
-// workgroup runs once more, with such values taken out of the product and brought in row by row.
+// workgroup runs once more, with such values taken out of the product and brought in row by row.  Finite values whose sum is not come that
+// way too (bf16 reaches 3.4e38, as FP32 does): the weights are scaled by 2^-28 there, which changes no other result.
 
 #include "decode_common.h"
 #include "prefill_common.h"
@@ -229,6 +230,8 @@ __global__ __launch_bounds__(1024) void prompt_plan_kernel(const PromptAttention
 template <typename act_t> constexpr float PROMPT_SHIFT = 0.f;
 template <> constexpr float PROMPT_SHIFT<f16_t> = 7.f;
 constexpr float PROMPT_SLACK = 8.f;
+template <typename act_t> constexpr float PROMPT_ROOM = 0.f;        // of a second run's weights: 2^20 of the largest values are finite
+template <> constexpr float PROMPT_ROOM<bf16_t> = 28.f;
 
 // The factor from maximum `m` to maximum `top` >= m; equal infinities are no step.  Never zero: an infinite output stays one.
 __device__ __forceinline__ float step_factor(float m, float top) { return m == top ? 1.f : fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-126f); }
@@ -457,8 +460,12 @@ __global__ __launch_bounds__(256, prompt_residency(D)) void prompt_attention_ker
         u32x4_t w;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float low = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x & 1) + 2 * i], p.scale_log2, -zero));
-          const float high = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x & 1) + 2 * i + 1], p.scale_log2, -zero));
+          float low = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x & 1) + 2 * i], p.scale_log2, -zero));
+          float high = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x & 1) + 2 * i + 1], p.scale_log2, -zero));
+          if constexpr (CAREFUL && PROMPT_ROOM<act_t> != 0.f) {
+            low *= __builtin_ldexpf(1.f, -(int)PROMPT_ROOM<act_t>);
+            high *= __builtin_ldexpf(1.f, -(int)PROMPT_ROOM<act_t>);
+          }
           part[0] += low;
           part[1] += high;
           w[i] = pack2<act_t>(low, high);
@@ -502,6 +509,7 @@ __global__ __launch_bounds__(256, prompt_residency(D)) void prompt_attention_ker
         __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
       }
     }
+    top -= PROMPT_SHIFT<act_t> - (CAREFUL ? PROMPT_ROOM<act_t> : 0.f);
   };
   pass(std::false_type{});
   // A NaN may be one of the formula's, or an infinite or NaN value whose weight is zero: once more, with such values apart.
@@ -522,7 +530,7 @@ __global__ __launch_bounds__(256, prompt_residency(D)) void prompt_attention_ker
       for (int c = 0; c < TILES; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(to + 32 * c + 8 * i + 4 * half) = float4{o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]};
-      if (half == 0) (share.pieces == 1 ? p.row_tops : p.tops)[at] = float2{top - PROMPT_SHIFT<act_t>, total};
+      if (half == 0) (share.pieces == 1 ? p.row_tops : p.tops)[at] = float2{top, total};
     }
   } else {
     const float norm = total == 0.f ? 0.f : 1.0f / total;         // no key: zeros
@@ -557,9 +565,10 @@ __global__ __launch_bounds__(256, prompt_residency(D)) void prompt_attention_ker
 }
 
 // Pieces of a row block to its output, or (a prefix) to one piece for each row: a wavefront a row at a time, a lane D / 64 channels.
+// Four pieces are in flight (parts of prompts with heads of 64, three or four pieces a block, 142 us; eight, twice the loads, 149).
 template <typename act_t, int D>
 __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptAttention p) {
-  constexpr int LANE = D / 64, AHEAD = 8;
+  constexpr int LANE = D / 64, AHEAD = 4;
   typedef float lane_t __attribute__((ext_vector_type(LANE)));
   const int index = blockIdx.x / p.heads, head = blockIdx.x - index * p.heads;
   PromptItem b;
@@ -679,7 +688,7 @@ PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, in
 int check_prompt(int batch, int64_t tokens, int HQ, int HKV, int D) {
   PLA_REQUIRE(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got %d", D);
   PLA_REQUIRE(HKV > 0 && HQ >= HKV && HQ % HKV == 0, "query heads must be a positive multiple of key-value heads");
-  PLA_REQUIRE(batch >= 0 && tokens >= 0 && tokens * HQ <= (1 << 30), "too many rows");
+  PLA_REQUIRE(batch >= 0 && tokens >= 0 && tokens <= (1 << 30) / HQ, "too many rows");
   PLA_REQUIRE((tokens * (HQ / HKV) / PROMPT_ROWS + batch) * HKV < (1 << 23), "too many sequences");
   return 0;
 }

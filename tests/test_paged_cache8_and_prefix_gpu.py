@@ -300,6 +300,46 @@ def test_what_is_written_is_read():
         context = [c + n for c, n in zip(context, new)]
 
 
+def test_captured_stores_and_reads_of_8_bits():
+    """Two graphs of a step (store, then attention) on two streams, replayed over other slots and lengths."""
+    from pla.decode.paged import fused_qk_norm_rope, paged_attention_decode
+    N, HQ, HKV, D, bs, pages = 6, 8, 2, 128, 16, 80
+    table = torch.randperm(N * pages, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(torch.int32).view(N, pages)
+    steps = []
+    for g in range(2):
+        caches = [torch.randint(0, 120, (N * pages, bs, HKV, D), dtype=torch.uint8, device=DEV, generator=torch.Generator(device=DEV).manual_seed(g)).view(E4M3) for _ in range(2)]
+        scales = [torch.rand(N * pages, HKV, bs, device=DEV) * 0.01 for _ in range(2)]
+        q, k, v = _randn(g, N, HQ, D, dtype=torch.bfloat16), _randn(g + 4, N, HKV, D, dtype=torch.bfloat16), _randn(g + 8, N, HKV, D, dtype=torch.bfloat16)
+        slots, lens, out = torch.full((N,), -1, dtype=torch.int64, device=DEV), torch.zeros(N, dtype=torch.int32, device=DEV), torch.zeros_like(q)
+
+        def call(caches, scales, out, q=q, k=k, v=v, slots=slots, lens=lens):
+            turned, _ = fused_qk_norm_rope(q, k, v=v, k_cache=caches[0], v_cache=caches[1], slot_mapping=slots, k_scales=scales[0], v_scales=scales[1])
+            return paged_attention_decode(turned, caches[0], caches[1], table, lens, k_scales=scales[0], v_scales=scales[1], out=out)
+        call(caches, scales, out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(caches, scales, out)
+        steps.append((graph, torch.cuda.Stream(), caches, scales, slots, lens, out, call))
+    for lengths in ([1, 2, 16, 17, 1200, 0], [1280, 1280, 3, 40, 900, 77], [0, 0, 0, 0, 0, 0], [33, 1000, 1000, 1, 7, 1279]):
+        expected = []
+        for graph, stream, caches, scales, slots, lens, out, call in steps:
+            last = [(n, x - 1) for n, x in enumerate(lengths)]
+            slots.copy_(torch.tensor([table[n, p // bs].item() * bs + p % bs if p >= 0 else -1 for n, p in last], device=DEV))
+            lens.copy_(_ints(lengths))
+            out.fill_(9.0)
+            mine = [c.view(torch.uint8).clone().view(E4M3) for c in caches], [x.clone() for x in scales]
+            expected.append((mine, call(*mine, torch.zeros_like(out))))
+        torch.cuda.synchronize()
+        for graph, stream, *_ in steps:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, caches, scales, _, _, out, _), (mine, ref) in zip(steps, expected):
+            assert torch.equal(out, ref) and (out[[n for n, x in enumerate(lengths) if x == 0]] == 0).all()
+            for a, b in zip(caches + scales, mine[0] + mine[1]):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_shared_memory_of_scales_is_refused():
     from pla.decode.paged import fused_qk_norm_rope, paged_attention_decode
     q, k, v = (_randn(i, 4, 2, 64, dtype=torch.bfloat16) for i in range(3))

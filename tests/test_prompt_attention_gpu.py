@@ -140,6 +140,23 @@ def test_scores_that_rise_along_the_keys():
         _close(got, *_reference(q, k, v, D ** -0.5))
 
 
+@pytest.mark.parametrize("D, act", [(64, "bf16"), (128, "bf16"), (256, "bf16"), (128, "fp16")])
+@pytest.mark.parametrize("tokens, keys", [(300, 300), (3, 9000)])
+def test_the_largest_values(D, act, tokens, keys):
+    """Values up to half of the type's largest, under weights and sums that pass FP32 with them where they are not scaled."""
+    from pla.prefill.attention import packed_attention_fwd
+    dtype = DTYPES[act]
+    q, k, v = _randn(1, tokens, 4, D, dtype=dtype), _randn(2, keys, 2, D, dtype=dtype), (torch.tanh(_randn(3, keys, 2, D)) * torch.finfo(dtype).max / 2).to(dtype)
+    q[..., 0] = 4.0
+    k[..., 0] = (torch.arange(keys, device=DEV) % 300 * D ** 0.5 / 200).to(k.dtype)[:, None]
+    k[keys // 3] = float("nan") if tokens == keys else 1.0                # an infinite sum next to a token that is not finite
+    got = packed_attention_fwd(q, k, v, _ints([0, tokens]), cu_seqlens_k=_ints([0, keys]))
+    first = keys // 3 if tokens == keys else tokens                       # rows before the token
+    ref, slack = _reference(q[:first], k[:keys - tokens + first], v[:keys - tokens + first], D ** -0.5)
+    _close(got[:first], ref, slack)
+    assert got[first:].isnan().all()
+
+
 def test_rows_of_no_sequence_and_sequences_that_are_passed_over():
     from pla.prefill.attention import packed_attention_fwd
     q, k, v = _randn(1, 50, 4, 128, dtype=torch.bfloat16), _randn(2, 50, 2, 128, dtype=torch.bfloat16), _randn(3, 50, 2, 128, dtype=torch.bfloat16)
