@@ -340,6 +340,24 @@ def test_captured_stores_and_reads_of_8_bits():
                 assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+def test_8_bits_past_32_bits():
+    """The last blocks of a cache of more than 2^32 numbers against the same tokens in a small one, bit for bit."""
+    from pla.decode.paged import fused_qk_norm_rope, paged_attention_decode
+    N, HQ, HKV, D, bs, pages, far = 3, 16, 8, 128, 16, 30, 264_000
+    q, k, v = (_randn(i, N * 16 * pages, h, D, dtype=torch.bfloat16) for i, h in ((1, HQ), (2, HKV), (3, HKV)))
+    results = []
+    for blocks, base in ((N * pages, 0), (far, far - N * pages)):
+        caches = [torch.empty(blocks, bs, HKV, D, dtype=torch.uint8, device=DEV).view(E4M3) for _ in range(2)]
+        scales = [torch.empty(blocks, HKV, bs, device=DEV) for _ in range(2)]
+        fused_qk_norm_rope(q, k, v=v, k_cache=caches[0], v_cache=caches[1], slot_mapping=torch.arange(N * 16 * pages, device=DEV) + base * bs, k_scales=scales[0], v_scales=scales[1])
+        table = (torch.arange(N * pages, dtype=torch.int32, device=DEV) + base).view(N, pages)
+        results.append([paged_attention_decode(q[:N * m], caches[0], caches[1], table, _ints([480, 77, 300]), query_start_loc=_ints([0, m, 2 * m, 3 * m]), max_query_len=m,
+                                               k_scales=scales[0], v_scales=scales[1]) for m in (1, 4, 32)])
+    assert far * bs * HKV * D > 2 ** 32
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and a.isfinite().all()
+
+
 def test_shared_memory_of_scales_is_refused():
     from pla.decode.paged import fused_qk_norm_rope, paged_attention_decode
     q, k, v = (_randn(i, 4, 2, 64, dtype=torch.bfloat16) for i in range(3))

@@ -122,6 +122,32 @@ def test_few_rows_over_many_keys_are_split_and_joined(tokens, keys, HQ, HKV, D, 
     _check_packed([tokens, 1, tokens], HQ, HKV, D, act, keys=[keys, 70, 300], seed=keys)
 
 
+@pytest.mark.parametrize("HQ, HKV, D, act", [(130, 1, 64, "bf16"), (300, 1, 128, "fp16"), (258, 2, 256, "bf16")])
+def test_more_query_heads_than_rows_of_a_block(HQ, HKV, D, act):
+    _check_packed([1, 70, 0, 3], HQ, HKV, D, act, gated=True, seed=HQ)
+    _check_packed([2, 1], HQ, HKV, D, act, keys=[3000, 1], seed=HQ)
+
+
+def test_nothing_to_do_and_no_keys_at_all():
+    from pla.prefill.attention import packed_attention_fwd, paged_attention_prefill
+    q, none = _randn(1, 5, 4, 128, dtype=torch.bfloat16), torch.empty(0, 2, 128, dtype=torch.bfloat16, device=DEV)
+    assert (packed_attention_fwd(q, none, none, _ints([0, 2, 5]), cu_seqlens_k=_ints([0, 0, 0])) == 0).all()
+    out = torch.full_like(q, 3.0)
+    assert packed_attention_fwd(q, none, none, _ints([0]), cu_seqlens_k=_ints([0]), out=out) is out and (out == 3).all()
+    assert packed_attention_fwd(q[:0], none, none, _ints([0, 0])).shape == (0, 4, 128)
+    cache = _randn(2, 3, 16, 2, 128, dtype=torch.bfloat16)
+    got = paged_attention_prefill(q, cache, cache, torch.zeros(2, 0, dtype=torch.int32, device=DEV), _ints([7, 3]), _ints([0, 2, 5]))
+    assert (got == 0).all()                                               # no page of the table
+    table = _ints([[0, 1], [2, 2]])
+    paged_attention_prefill(q, cache, cache, table, _ints([]), _ints([0]), out=out)
+    assert (out == 3).all()
+    k = cache.view(48, 2, 128)
+    got = paged_attention_prefill(q, cache, cache, table, _ints([20, 30, 18]), _ints([0, 2, 3, 5]), request_indices=_ints([0, 1, 0]))   # one row of the table twice
+    keys = torch.cat([k[:20], k[32:], k[32:46], k[:18]])
+    for (a, b), x in zip(((0, 2), (2, 3), (3, 5)), keys.split([20, 30, 18])):
+        _close(got[a:b], *_reference(q[a:b], x, x, 128 ** -0.5))
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-20, 3.0])
 @pytest.mark.parametrize("act, D", [("bf16", 128), ("fp16", 64)])
 def test_other_scales(scale, act, D):
