@@ -454,7 +454,7 @@ template <typename value_t>
 __device__ __forceinline__ PrefixPart prefix_part(const PagedAttention& p, int64_t token, int head, float top, float& sum) {
   PrefixPart x{token * (p.shape.heads * p.shape.group) + head, 1.f, 0.f};
   const float2 y = p.prefix_tops[x.row];
-  if (sum == 0.f || y.x == -INFINITY) return x;
+  if (sum == 0.f) return x;
   const float mine = top - WEIGHT_SHIFT<value_t>, reference = fmaxf(mine, y.x);
   x.own = rescale(mine, reference);
   x.prefix = rescale(y.x, reference);
