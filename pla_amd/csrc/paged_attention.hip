@@ -444,6 +444,11 @@ struct Part {
   const int32_t* pages;
 };
 
+// With a prefix it matters whether a row sees a key of its own at all: if it sees some whose scores are all minus infinity, it is the
+// attention over the prefix, if none, zeros.  So such sums are not left at zero but made this, which nothing is added to that it would
+// change: beside any other maximum it is zero.
+constexpr float SUM_OF_NOTHING = 0x1p-126f;
+
 // What a row has of the prefix, joined with what it has of its own keys: a common reference and the factors of both.  A row that sees no
 // key of its own (sum 0) has no part in the prefix.
 struct PrefixPart {
@@ -459,6 +464,7 @@ __device__ __forceinline__ PrefixPart prefix_part(const PagedAttention& p, int64
   x.own = rescale(mine, reference);
   x.prefix = rescale(y.x, reference);
   sum = fmaf(y.y, x.prefix, sum * x.own);
+  if (reference == -INFINITY && sum == sum) sum = 0.f;      // nothing in the prefix either
   return x;
 }
 template <int CHANNELS>
@@ -757,6 +763,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     } else {
       b.steps = 0;
     }
+    [[maybe_unused]] int first_key = INT32_MAX;   // with a page, of those that this wavefront has; pages hold whole sixteens
     // entries of the step after the one in flight
     Entries coming = a.steps > 1 ? look_up(a, 1) : look_up(b, 0);
     w.set_aside = -1;
@@ -778,6 +785,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
       if ((step + (blockIdx.x >> 8)) & 1) __builtin_amdgcn_s_setprio(1);
       else __builtin_amdgcn_s_setprio(0);
       const bool more = step + 1 < a.steps;
+      if constexpr (PREFIX) first_key = min(first_key, there[0] ? a.key + step * STRIDE : there[1] ? a.key + step * STRIDE + 16 : INT32_MAX);
       // The very last step fetches some block's first keys, the same for all, from the caches: a branch around the loads costs the
       // compiler the registers.
       // The entries for the step after next are asked for behind the keys of the next: a wait for queries in LDS is one for them too.
@@ -802,6 +810,7 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     if constexpr (ALONE) {
       const int row = a.row0 + r, j = paged_quotient(p.shape.by_group, row), head = a.seg.head * p.shape.group + row - j * p.shape.group;
       float sum = query_sum(w.sum[0]);
+      if constexpr (PREFIX) sum = sum == 0.f && first_key < w.limit[0] ? SUM_OF_NOTHING : sum;
       // this lane's channels of row r: LANE_CHANNELS at a time from these on
       auto channel_of = [&](int c, int e) { return 128 * c + W::LANE_CHANNELS * (4 * kb + e); };
       auto park = [&](float* to) {
@@ -879,7 +888,8 @@ __global__ __launch_bounds__(64 * waves(D, RT), residency(D, RT) * waves(D, RT) 
     // The wavefronts' rows together.
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const float sum = query_sum(w.sum[t]);
+      float sum = query_sum(w.sum[t]);
+      if constexpr (PREFIX) sum = sum == 0.f && first_key < w.limit[t] ? SUM_OF_NOTHING : sum;
       if (kb == 0) tops[0][wave][16 * t + r] = float2{w.top[t], sum};
     }
     if (lane == 0) aside[wave] = w.set_aside;

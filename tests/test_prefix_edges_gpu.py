@@ -41,3 +41,35 @@ def test_keys_of_a_prefix_that_are_all_nan(D, act, HQ, HKV, prefix, crowd):
         caches[0][pages, :, 1] = math.nan
         got = _call(q, caches, table, lengths, prefix, crowd).view(4, HKV, HQ // HKV, D)
         assert torch.isnan(got[[0, 1, 3], 1]).all() and torch.isfinite(got[:, 0]).all() and torch.isfinite(got[:, 2:]).all()
+
+
+@pytest.mark.parametrize("D, act, HQ, HKV", SHAPES)
+@pytest.mark.parametrize("prefix", [1, 200, 9000])
+def test_own_keys_whose_scores_are_all_minus_infinity(D, act, HQ, HKV, prefix, crowd):
+    """Such a row sees keys of its own, all of weight zero: it is the attention over the prefix."""
+    lengths, windows = [1, 40, 7000, 60, 20, 2, 300], [1, 3, 2, 1, 1, 4, 4]
+    caches, table, kept = _cache16(lengths + [prefix], HKV, D, 16, act, seed=D)
+    for n, length in enumerate(lengths):
+        for page in range(-(-length // 16)):
+            caches[0][table[n, page].long(), :, :, 0] = -math.inf
+    block, place = _place(table, 6, 299)
+    caches[0][block, place, :, 0] = 0.5                      # the last token of the last request sees another one
+    table[3, 1:3] = caches[0].size(0)                        # some pages are missing,
+    table[4, :2] = -1                                        # all pages are
+    q = _randn(5, sum(windows), HQ, D, dtype=DTYPES[act], scale=1.5)
+    q[..., 0] = 4.0
+    got = _call(q, caches, table, lengths, prefix, crowd, windows)
+    u = torch.finfo(q.dtype).eps / 2
+    parts = torch.full((prefix,), u * (1 + 2 * u), dtype=torch.float64, device=DEV)
+    first = _offsets(windows)
+    zeros = [first[4], first[5], first[5] + 1]               # no pages; tokens before the first of their own
+    for row in range(sum(windows) - 1):
+        if row in zeros:
+            assert (got[row] == 0).all(), row
+        else:
+            _close(got[row:row + 1], *_rows_reference(q[row:row + 1], kept[0][-1], kept[1][-1], D ** -0.5, parts))
+    k, v = (torch.cat([kept[i][-1], caches[i][block, place][None]]) for i in range(2))
+    parts = torch.cat([parts, torch.full((1,), 2.0 ** -15, dtype=torch.float64, device=DEV)])
+    _close(got[-1:], *_rows_reference(q[-1:], k, v, D ** -0.5, parts))
+    # without a prefix in sight as before: zeros
+    assert (_call(q, caches, table, lengths, 0, crowd, windows)[:-1] == 0).all()
