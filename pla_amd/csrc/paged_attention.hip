@@ -452,26 +452,30 @@ constexpr float SUM_OF_NOTHING = 0x1p-126f;
 // What a row has of the prefix, joined with what it has of its own keys: a common reference and the factors of both.  A row that sees no
 // key of its own (sum 0) has no part in the prefix.
 struct PrefixPart {
-  int64_t row;                                    // of the prefix's outputs
+  int64_t row;                                    // of the prefix's outputs, -1: no part
   float own, prefix;
 };
 template <typename value_t>
 __device__ __forceinline__ PrefixPart prefix_part(const PagedAttention& p, int64_t token, int head, float top, float& sum) {
   PrefixPart x{token * (p.shape.heads * p.shape.group) + head, 1.f, 0.f};
   const float2 y = p.prefix_tops[x.row];
-  if (sum == 0.f) return x;
+  if (sum == 0.f) {
+    x.row = -1;
+    return x;
+  }
   const float mine = top - WEIGHT_SHIFT<value_t>, reference = fmaxf(mine, y.x);
-  x.own = rescale(mine, reference);
-  x.prefix = rescale(y.x, reference);
+  x.own = step_factor(mine, reference);
+  x.prefix = step_factor(y.x, reference);
   sum = fmaf(y.y, x.prefix, sum * x.own);
   if (reference == -INFINITY && sum == sum) sum = 0.f;      // nothing in the prefix either
   return x;
 }
 template <int CHANNELS>
 __device__ __forceinline__ void add_prefix(const PagedAttention& p, const PrefixPart& x, int D, int channel, float (&o)[CHANNELS]) {
+  if (x.row < 0) return;
   const float* part = p.prefix + x.row * D + channel;
 #pragma unroll
-  for (int i = 0; i < CHANNELS; ++i) o[i] = x.prefix == 0.f ? o[i] : fmaf(part[i], x.prefix, o[i] * x.own);
+  for (int i = 0; i < CHANNELS; ++i) o[i] = add_brought(brought(o[i], x.own), part[i], x.prefix);
 }
 
 // CHANNELS channels of a row's output from their sums.

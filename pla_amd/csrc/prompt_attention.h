@@ -58,6 +58,13 @@ PLA_HD PromptShare prompt_share(int tiles, int most, int least) {
   return {each, tiles <= each ? 1 : (tiles + each - 1) / each};
 }
 
+// Parts of a row's sums are brought from their maximum `m` to a common one, `top` >= m (equal infinities are no step).  The factor may
+// come out zero: then a finite part has nothing left (a value of 1e38 times the smallest number would not be nothing), an infinite one
+// stays, as the formula's weights are never zero.
+__device__ __forceinline__ float step_factor(float m, float top) { return m == top ? 1.f : __builtin_amdgcn_exp2f(m - top); }
+__device__ __forceinline__ float brought(float x, float f) { return f > 0.f || x - x == 0.f ? x * f : x; }
+__device__ __forceinline__ float add_brought(float sum, float x, float f) { return f > 0.f || x - x == 0.f ? fmaf(x, f, sum) : sum + x; }
+
 constexpr int PROMPT_PLAN = 2048;         // sequences of a call that is split at most
 constexpr PLA_HD int prompt_residency(int D) { return D == 256 ? 1 : D == 64 ? 3 : 2; }       // workgroups a CU
 struct PromptLaunch {

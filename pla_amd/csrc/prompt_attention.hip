@@ -233,9 +233,6 @@ constexpr float PROMPT_SLACK = 8.f;
 template <typename act_t> constexpr float PROMPT_ROOM = 0.f;        // of a second run's weights: 2^20 of the largest values are finite
 template <> constexpr float PROMPT_ROOM<bf16_t> = 28.f;
 
-// The factor from maximum `m` to maximum `top` >= m; equal infinities are no step.  Never zero: an infinite output stays one.
-__device__ __forceinline__ float step_factor(float m, float top) { return m == top ? 1.f : fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-126f); }
-
 __device__ __forceinline__ float halves_max(float x) {
   const LanePair a = swap_halves(x);
   return fmaxf(a.lo, a.hi);
@@ -494,7 +491,7 @@ __global__ __launch_bounds__(256, prompt_residency(D)) void prompt_attention_ker
 #pragma unroll
         for (int c = 0; c < TILES; ++c)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[c][i] *= f;
+          for (int i = 0; i < 16; ++i) o[c][i] = CAREFUL ? brought(o[c][i], f) : o[c][i] * f;         // (zero times an infinity: there is another run)
       }
       bf16x8_t weight[2 * HALVES];
       weigh(f, weight);
@@ -597,14 +594,15 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptAttention 
       for (int a = 0; a < AHEAD; ++a) now = fmaxf(now, y[a].x);          // one piece twice does no harm here
       const float back = step_factor(top, now);
       sum *= back;
-      o *= back;
+#pragma unroll
+      for (int c = 0; c < LANE; ++c) o[c] = brought(o[c], back);
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) {
         const bool counts = i + a < share.pieces;
         const float f = step_factor(y[a].x, now);
         sum = counts ? fmaf(y[a].y, f, sum) : sum;
 #pragma unroll
-        for (int c = 0; c < LANE; ++c) o[c] = counts ? fmaf(x[a][c], f, o[c]) : o[c];
+        for (int c = 0; c < LANE; ++c) o[c] = counts ? add_brought(o[c], x[a][c], f) : o[c];
       }
       top = now;
     }

@@ -73,3 +73,33 @@ def test_own_keys_whose_scores_are_all_minus_infinity(D, act, HQ, HKV, prefix, c
     _close(got[-1:], *_rows_reference(q[-1:], k, v, D ** -0.5, parts))
     # without a prefix in sight as before: zeros
     assert (_call(q, caches, table, lengths, 0, crowd, windows)[:-1] == 0).all()
+
+
+@pytest.mark.parametrize("D, HQ, HKV", [(128, 8, 2), (64, 4, 4), (256, 8, 1)])
+@pytest.mark.parametrize("prefix, own", [(3, 5), (700, 300), (9000, 7000)])
+@pytest.mark.parametrize("far", ["prefix", "own"])
+def test_large_values_under_weights_of_nothing(D, HQ, HKV, prefix, own, far, crowd):
+    """Values of 1e38 under weights of exp(-300) are nothing beside ones of 1, infinite ones are infinite all the same."""
+    caches, table, kept = _cache16([own, prefix], HKV, D, 16, "bf16", seed=3)
+    q = _randn(5, 1, HQ, D, dtype=torch.bfloat16)
+    q[..., 0] = 4.0
+    n, length = (1, prefix) if far == "prefix" else (0, own)
+    near = 1 - n
+    pages = [table[i, :-(-x // 16)].long() for i, x in enumerate((own, prefix))]
+    caches[0][pages[near], :, :, 0] = 75.0 * D ** 0.5        # 300 more than the others' scores
+    caches[0][pages[n], :, :, 0] = 0.0
+    kept[0][near][..., 0] = 75.0 * D ** 0.5
+    sane = kept[1][near]
+    if far == "prefix":
+        caches[1][pages[n], :, :, 5] = 1e38
+    else:                                                    # (own keys' sums are 32 bits wide, several such values pass them)
+        block, place = _place(table, n, length // 2)
+        caches[1][block, place, :, 5] = 1e38
+    got = _call(q, caches, table, [own], prefix, crowd)
+    u = 2.0 ** -8 * (1 + 2 ** -7)
+    parts = torch.full((sane.size(0),), u, dtype=torch.float64, device=DEV)
+    _close(got, *_rows_reference(q, kept[0][near], sane, D ** -0.5, parts))
+    block, place = _place(table, n, length - 1)
+    caches[1][block, place, :, 7] = -math.inf
+    got = _call(q, caches, table, [own], prefix, crowd)
+    assert (got[..., 7] == -math.inf).all() and torch.isfinite(got[..., :7]).all() and torch.isfinite(got[..., 8:]).all()
