@@ -464,8 +464,8 @@ __device__ __forceinline__ PrefixPart prefix_part(const PagedAttention& p, int64
     return x;
   }
   const float mine = top - WEIGHT_SHIFT<value_t>, reference = fmaxf(mine, y.x);
-  x.own = step_factor(mine, reference);
-  x.prefix = step_factor(y.x, reference);
+  x.own = 0.5f * step_factor(mine, reference);          // half of each, as the sum of two numbers may pass 32 bits
+  x.prefix = 0.5f * step_factor(y.x, reference);
   sum = fmaf(y.y, x.prefix, sum * x.own);
   if (reference == -INFINITY && sum == sum) sum = 0.f;      // nothing in the prefix either
   return x;

@@ -578,33 +578,49 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptAttention 
   for (int r = blockIdx.y * 4 + wave; r < b.rows; r += 4 * gridDim.y) {
     const int j = paged_quotient(p.by_group, b.row0 + r), query_head = head * p.group + b.row0 + r - j * p.group;
     const int64_t token = b.begin + j, first = ((int64_t)b.first * p.heads + head) * p.slot_rows + r, step = (int64_t)p.heads * p.slot_rows;
-    float top = -INFINITY, sum = 0.f;
-    lane_t o = {};
-    for (int i = 0; i < share.pieces; i += AHEAD) {
-      float2 y[AHEAD];
-      lane_t x[AHEAD];
+    float top, sum;
+    lane_t o;
+    auto put_together = [&](float room) {
+      top = -INFINITY;
+      sum = 0.f;
+      o = lane_t{};
+      for (int i = 0; i < share.pieces; i += AHEAD) {
+        float2 y[AHEAD];
+        lane_t x[AHEAD];
 #pragma unroll
-      for (int a = 0; a < AHEAD; ++a) {
-        const int64_t at = first + min(i + a, share.pieces - 1) * step;
-        y[a] = p.tops[at];
-        x[a] = *reinterpret_cast<const lane_t*>(p.partial + at * D + LANE * lane);
+        for (int a = 0; a < AHEAD; ++a) {
+          const int64_t at = first + min(i + a, share.pieces - 1) * step;
+          y[a] = p.tops[at];
+          x[a] = *reinterpret_cast<const lane_t*>(p.partial + at * D + LANE * lane);
+        }
+        float now = top;
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) now = fmaxf(now, y[a].x);          // one piece twice does no harm here
+        const float back = step_factor(top, now);
+        sum *= back;
+#pragma unroll
+        for (int c = 0; c < LANE; ++c) o[c] = brought(o[c], back);
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+          const bool counts = i + a < share.pieces;
+          const float f = step_factor(y[a].x, now) * room;
+          sum = counts ? fmaf(y[a].y, f, sum) : sum;
+#pragma unroll
+          for (int c = 0; c < LANE; ++c) o[c] = counts ? add_brought(o[c], x[a][c], f) : o[c];
+        }
+        top = now;
       }
-      float now = top;
+    };
+    put_together(1.f);
+    if constexpr (PROMPT_ROOM<act_t> != 0.f) {
+      // Finite pieces whose sum is not: once more, scaled as a piece's own sums are.
+      float check = 0.f;
 #pragma unroll
-      for (int a = 0; a < AHEAD; ++a) now = fmaxf(now, y[a].x);          // one piece twice does no harm here
-      const float back = step_factor(top, now);
-      sum *= back;
-#pragma unroll
-      for (int c = 0; c < LANE; ++c) o[c] = brought(o[c], back);
-#pragma unroll
-      for (int a = 0; a < AHEAD; ++a) {
-        const bool counts = i + a < share.pieces;
-        const float f = step_factor(y[a].x, now);
-        sum = counts ? fmaf(y[a].y, f, sum) : sum;
-#pragma unroll
-        for (int c = 0; c < LANE; ++c) o[c] = counts ? add_brought(o[c], x[a][c], f) : o[c];
+      for (int c = 0; c < LANE; ++c) check += o[c] * 0.f;
+      if (__ballot(check != check) != 0) {
+        put_together(__builtin_ldexpf(1.f, -(int)PROMPT_ROOM<act_t>));
+        top += PROMPT_ROOM<act_t>;
       }
-      top = now;
     }
     if (!p.offsets) {
       const int64_t at = token * (p.heads * p.group) + query_head;

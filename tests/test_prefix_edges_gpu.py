@@ -76,6 +76,22 @@ def test_own_keys_whose_scores_are_all_minus_infinity(D, act, HQ, HKV, prefix, c
 
 
 @pytest.mark.parametrize("D, HQ, HKV", [(128, 8, 2), (64, 4, 4), (256, 8, 1)])
+@pytest.mark.parametrize("prefix, own, value", [(2, 1, 1.5e38), (500, 300, 6e35), (500, 300, -6e35), (9000, 7000, 2.5e34)])
+def test_sums_of_prefix_and_own_keys_that_pass_32_bits_together(D, HQ, HKV, prefix, own, value, crowd):
+    caches, table, _ = _cache16([own, prefix], HKV, D, 16, "bf16")
+    for n, length in enumerate((own, prefix)):
+        for page in range(-(-length // 16)):
+            caches[1][table[n, page].long(), :, :, :D // 2] = value
+            caches[1][table[n, page].long(), :, :, D // 2:] = 0.375
+    q = torch.zeros(1, HQ, D, dtype=torch.bfloat16, device=DEV)
+    got = _call(q, caches, table, [own], prefix, crowd).double()
+    # equal weights of equal values: sums of n products, a division, one rounding
+    want = torch.tensor(value, dtype=torch.bfloat16).item()
+    assert ((got[..., :D // 2] - want).abs() <= abs(want) * (2 ** -8 + (prefix + own + 32) * 2 ** -24)).all()
+    assert ((got[..., D // 2:] - 0.375).abs() <= 0.375 * (2 ** -8 + (prefix + own + 32) * 2 ** -24)).all()
+
+
+@pytest.mark.parametrize("D, HQ, HKV", [(128, 8, 2), (64, 4, 4), (256, 8, 1)])
 @pytest.mark.parametrize("prefix, own", [(3, 5), (700, 300), (9000, 7000)])
 @pytest.mark.parametrize("far", ["prefix", "own"])
 def test_large_values_under_weights_of_nothing(D, HQ, HKV, prefix, own, far, crowd):

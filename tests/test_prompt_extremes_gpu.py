@@ -9,6 +9,19 @@ from test_prompt_attention_gpu import DEV, DTYPES, _close, _ints, _randn, _refer
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("tokens, keys, value", [(3, 9000, 5e35), (3, 9000, -5e35), (40, 30000, 4e35), (1, 3000, 6e35)])
+def test_pieces_whose_sums_pass_32_bits_together(D, tokens, keys, value):
+    from pla.prefill.attention import packed_attention_fwd
+    q, k, v = (torch.zeros(tokens if h == 4 else keys, h, D, dtype=torch.bfloat16, device=DEV) for h in (4, 2, 2))
+    k.normal_()
+    v[..., :D // 2], v[..., D // 2:] = value, 0.375
+    got = packed_attention_fwd(q, k, v, _ints([0, tokens]), cu_seqlens_k=_ints([0, keys])).double()
+    # equal weights of equal values: sums of n products, a division, one rounding
+    for x, want in ((got[..., :D // 2], v[0, 0, 0].item()), (got[..., D // 2:], 0.375)):
+        assert ((x - want).abs() <= abs(want) * (2 ** -8 + (keys + 32) * 2 ** -24)).all()
+
+
 @pytest.mark.parametrize("D, act", [(64, "bf16"), (128, "bf16"), (256, "bf16"), (128, "fp16")])
 @pytest.mark.parametrize("tokens, keys", [(300, 300), (3, 9000)])
 def test_large_values_under_weights_of_nothing(D, act, tokens, keys):
