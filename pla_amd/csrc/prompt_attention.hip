@@ -716,10 +716,10 @@ int launch_prompt(PromptAttention p, const PromptLaunch& l, bool paged, int D, f
   for (const void* x : {(const void*)p.q, (const void*)p.k, (const void*)p.v, (const void*)p.gate, (const void*)p.out})
     PLA_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0, "rows must be 16-byte aligned");
   PLA_REQUIRE(p.k_token >= 0 && p.k_token < (1 << 24) && p.v_token >= 0 && p.v_token < (1 << 24), "token strides of keys and values must be below 2^24");
-  // The kernel takes a maximum of scores before it scales them: the sign goes to the queries, and a scale of zero becomes one that
-  // leaves finite scores equal.
+  // The kernel takes a maximum of scores before it scales them: the sign goes to the queries, and a scale of zero becomes the smallest
+  // number, which leaves finite scores equal (to 2^-20) and masked ones at minus infinity.
   p.flip = scale < 0.f ? 0x80008000u : 0u;
-  p.scale_log2 = scale == 0.f ? 1e-38f : fabsf(scale) * 1.44269504088896341f;
+  p.scale_log2 = scale == 0.f ? 0x1p-149f : fabsf(scale) * 1.44269504088896341f;
   p.items = (int)l.pieces;
   p.least = l.least;
   p.slots = (int)l.items;

@@ -39,3 +39,15 @@ def test_large_values_under_weights_of_nothing(D, act, tokens, keys):
     v[9, :, 7] = -math.inf
     got = call()
     assert (got[rows, :, 7] == -math.inf).all() and torch.isfinite(got[rows, :, :7]).all() and torch.isfinite(got[rows, :, 8:]).all() and n > 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("tokens, keys", [(300, 300), (3, 9000)])
+def test_a_scale_of_zero_makes_all_finite_scores_equal(D, tokens, keys):
+    from pla.prefill.attention import packed_attention_fwd
+    q, k, v = _randn(1, tokens, 4, D, dtype=torch.bfloat16), _randn(2, keys, 2, D, dtype=torch.bfloat16), _randn(3, keys, 2, D, dtype=torch.bfloat16)
+    q[..., 0] = 1e19
+    k[::3, :, 0], k[1::3, :, 0] = 1.5e19, -1.5e19
+    got = packed_attention_fwd(q, k, v, _ints([0, tokens]), cu_seqlens_k=_ints([0, keys]), scale=0.0)
+    zero = torch.zeros_like(q)
+    _close(got, *_reference(zero, k * 0, v, 1.0))
