@@ -82,7 +82,8 @@ def check_attention(q, k_cache, block_table, seq_lens, query_start_loc, request_
 
 
 def check_prefix(k_cache, prefix_blocks, prefix_len):
-    if prefix_blocks is None or prefix_len is None or _capturing() or not _formed(None, prefix_blocks, prefix_len) or prefix_len.numel() != 1 or k_cache.dim() < 2:
+    if (prefix_blocks is None or prefix_len is None or _capturing() or not _formed(None, prefix_blocks, prefix_len) or prefix_len.numel() != 1 or
+            k_cache.dim() < 2 or k_cache.size(1) < 1):
         return
     op, length, block_size = "paged_attention_decode", prefix_len.item(), k_cache.size(1)
     if not 0 <= length <= prefix_blocks.numel() * block_size:
