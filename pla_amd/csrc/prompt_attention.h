@@ -43,7 +43,8 @@ struct PromptAttention {
 // block's keys are cut into pieces, so that the blocks of a long sequence do not go on when all others are done: as many as make the whole
 // batch, were all blocks of a sequence as long as its last one, about `items` pieces of equal size, none under `least` tiles.  Pieces of
 // different blocks begin at the same keys, so that the caches hold them for all.  The batch's lengths stand on the device, so it is there
-// that the size is worked out; the host knows that blocks and pieces together are no more than blocks + items.
+// that the size is worked out; the host knows that blocks and pieces together are no more than blocks + items, nor than the blocks and,
+// for each, every `least` tiles of the keys behind its first.
 PLA_HD int prompt_tiles(int keys) { return (int)(((int64_t)keys + PROMPT_KEYS - 1) / PROMPT_KEYS); }
 PLA_HD int prompt_piece(int items, int64_t total, int least) {
   if (items <= 0) return INT32_MAX;
@@ -68,7 +69,7 @@ __device__ __forceinline__ float add_brought(float sum, float x, float f) { retu
 constexpr int PROMPT_PLAN = 2048;         // sequences of a call that is split at most
 constexpr PLA_HD int prompt_residency(int D) { return D == 256 ? 1 : D == 64 ? 3 : 2; }       // workgroups a CU
 struct PromptLaunch {
-  int64_t blocks, items, pieces;                  // row blocks at most, workgroups a head, pieces (0: not split) that a head's keys are cut into
+  int64_t blocks, items, pieces;                  // row blocks at most, workgroups a head, pieces (0: not split) to cut a head's keys into
   int least, slot_rows, join_rows;
   bool split, plan;                               // whether keys are cut into pieces, whether the items are listed
   int64_t tops_at, plan_at, rows_at, row_tops_at, bytes;   // workspace
