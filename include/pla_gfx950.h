@@ -595,7 +595,7 @@ int64_t pla_paged_attention_prefix_workspace_bytes(int batch, int tokens, int HQ
 /*
  * pla_paged_attention_launch where all token rows also see a prefix that stands before their own keys: the first prefix_len[0] (int32 or
  * int64, on the device; at most prefix_pages * block_size) positions of prefix_blocks int32 [prefix_pages], read once for the whole batch.
- * A row that sees no key of its own is zeros.  Weights of the prefix are rounded to act_dtype.
+ * A row that sees no key of its own is zeros.  Weights of the prefix are rounded to act_dtype.  All `tokens` rows of q are taken over it.
  */
 int pla_paged_attention_prefix_launch(
     const void* q, int64_t q_token, int64_t q_head, const void* k_cache, const void* v_cache,

@@ -36,12 +36,12 @@
 // Caches of 8-bit numbers (e4m3) with a scale a token and head are widened to the queries' type on the way to the matrix instructions,
 // which is exact; a key's scale multiplies its scores, a value's scale its weights, which then go in two parts of bf16 with either type of
 // queries, as a scale may be anything FP32 holds.  2 D + 8 bytes a key and head: 256 requests of 300 to 4000 keys (D 128, 8 heads) 143 us
-// (5.4 TB/s) against 245 over 16 bits; 40 windows of four over 500 to 30 000 keys (D 256, 2 heads, 32 rows) 77 against 87, where
-// widening and products take as long as the memory.
+// (5.4 TB/s) against 245 over 16 bits; 40 windows of four over 500 to 30 000 keys (D 256, 2 heads, 32 rows) 77 against 87: of the one
+// wavefront's cycles on a SIMD 40 % issue vector instructions there and 30 % wait for keys, LDS or a barrier, with nothing to cover them.
 //
 // A prefix that all requests share is attended to first, for all token rows together (the kernel over prompts, which reads it once), and what
 // it gives for a row, (maximum, sum, outputs) in FP32, is put in where a run's rows or pieces are put together: 64 requests of 40 to 1500
-// keys after a prefix of 8000 (D 128, 8 heads) 57 us, 27 of them for the prefix and 31 for the own keys.  It is compiled in apart (PREFIX):
+// keys after a prefix of 8000 (D 128, 8 heads) 56 us, 27 of them for the prefix and 28 for the own keys.  It is compiled in apart (PREFIX):
 // as a branch it cost calls without a prefix 1.4 us of 30.
 
 #include "decode_common.h"

@@ -32,7 +32,9 @@
 // Infinite and NaN values: a weight of zero times one is NaN, where the formula has no product (a key that the row does not see) or an
 // infinite one (a weight that is zero only in 32 bits).  The loop does not look for them.  Where an output comes out infinite or NaN the
 // workgroup runs once more, with such values taken out of the product and brought in row by row.  Finite values whose sum is not come that
-// way too (bf16 reaches 3.4e38, as FP32 does): the weights are scaled by 2^-28 there, which changes no other result.
+// way too (bf16 reaches 3.4e38, as FP32 does): the weights are scaled by 2^-28 there, which changes no other result but those below 2^-98,
+// of which digits are lost.  So does the join.  Of a prefix all rows of q are taken, and an infinite or NaN row of no request has its
+// workgroup run twice as well (64 such rows beside 64 chats over a prefix of 8000 keys 90 us, finite ones 59, none 49).
 
 #include "decode_common.h"
 #include "prefill_common.h"
@@ -670,8 +672,14 @@ PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, in
   l.least = prefix ? 4 : 8;
   // Pieces and blocks together fill the chip twice: an unequal end costs less than twice the pieces, which are written and read again.  1500
   // tokens over 60 000 keys 1542 us (three times 1572, four 1574, not split 1650), eighteen parts of prompts with heads of 64 145 (155, 169,
-  // 163).  A prefix's blocks are alike and end together: once (100 windows of four over 30 000 keys 96 us, twice 115), with very few rows,
-  // whose pieces are as large as the prefix, half (64 chats over 8000 keys, 8 heads, 57.4, once 61.1; the windows 104).
+  // 163).  A prefix's blocks are alike and end together: once (100 windows of four over 30 000 keys 96 us, twice 115, half 104), with very few
+  // rows, whose pieces are as large as the prefix, half: 64 chats over 8000 keys, 32 + 8 heads of 128, 49.5, once 52.7; heads of 64 44.4 and
+  // 43.7, of 256 (16 chats) 56.6 and 51.9.  Above the line: 96 chats, heads of 128, half 62.8, once 63.8; 64, heads of 256, 94.8 and 79.6.
+  //
+  // Whether keys are cut is decided by what the host knows, all keys of the call or the positions of a row of the table.  With 16 + 2 heads of
+  // 128: 100 tokens over 1100 keys 29.8 us (not split 24.8), 1500 30.6 (31.2), 2000 32.8 (39.8), 4000 41 (72); heads of 256 over 1500 41.5
+  // (56.7).  It costs where no sequence is long, or its blocks fill the chip by half: nine prompts of 120 tokens 18.2 (8.7), one of 1100
+  // 37.6 (24.9), of 3000 85 (61), of 5000 124 (114).  From 513 keys on, rather than 1025: 100 tokens over 900 29.2 (20.8).
   const int64_t room = 256 * prompt_residency(D), groups = l.blocks * HKV;
   const int64_t fill = (!prefix || groups > room / 2 ? 2 * room : groups > room / 32 ? room : room / 2) / HKV - l.blocks;
   l.split = prefix || (groups < 2 * room && batch <= PROMPT_PLAN && keys > 2 * l.least * PROMPT_KEYS);

@@ -157,8 +157,8 @@ def fused_qk_norm_rope(q, k, positions=None, *, q_weight=None, k_weight=None, ep
               slot ``block * block_size + place``; a slot that is negative or past the cache is nowhere.  No two tokens may
               name one slot.
     8 bits    with k_scales (and v_scales) [blocks, HKV, block_size] float32 the caches are torch.float8_e4m3fn: a head of a token is
-              stored as x / scale, rounded once from float32 to nearest, with scale max(largest |x|, 1e-30) / 448 beside it.  A NaN
-              stays one, an infinity makes what its head stands for NaN.
+              stored as x / scale, rounded once from float32 to nearest, with scale max(largest |x|, 1e-30) / 448 beside it: off by
+              2^-4 of itself or 2^-10 of the scale, whichever is more.  A NaN stays one, an infinity makes what its head stands for NaN.
 
     Returns (q_out, k_out): ``k_out`` is made if neither it nor a cache is given, and else what was passed.  q_out and k_out may be
     q and k themselves (the same rows), and share memory with nothing else.
@@ -194,12 +194,14 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, query_
     A prefix that all requests share, such as one instruction text, stands in blocks of its own, which no request's row of the table names:
     the first ``prefix_len`` [1] (int32 or int64, on the device) positions of ``prefix_blocks`` int32 [pages].  Every row that sees a
     position of its own sees the whole prefix too, before them (positions of new tokens count on from its end); keys and values of the
-    prefix are read once for the whole batch.  Its weights are rounded once to q's type.  Not with 8-bit caches.
+    prefix are read once for the whole batch.  Its weights are rounded once to q's type.  Not with 8-bit caches.  Rows of q that belong
+    to no request are taken over the prefix as well, to no result: keep them few, and finite (else parts of the prefix are gone through twice).
 
     scale (default D^-0.5) applies to the scores; output_gate [T, HQ, D] multiplies the result by its sigmoid.  Scores, their
     maxima and sums and the outputs are float32; weights meet the values in two parts of q's type (off by 2^-16 of themselves at most,
-    fp16 2^-22), outputs are rounded once.  Returns ``out`` [T, HQ, D], which shares memory with no input.  Results do not depend on
-    timing.
+    fp16 2^-22; over 8-bit caches 2^-16), outputs are rounded once.  A key of a 16-bit cache that a row sees has a weight of at least 2^-125
+    (fp16 2^-37) of the row's largest, so an infinite value there counts.  Sums of weights no larger than one times the values have
+    to stay within float32.  Returns ``out`` [T, HQ, D], which shares memory with no input.  Results do not depend on timing.
     """
     if _sanity_enabled():
         from ._sanity import check_attention, check_prefix

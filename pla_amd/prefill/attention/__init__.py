@@ -21,7 +21,7 @@ def packed_attention_fwd(q, k, v, cu_seqlens, *, cu_seqlens_k=None, scale=None, 
     and v, or those of ``cu_seqlens_k`` where it has other, say earlier, keys too: token j of m with n keys sees the first n - m + j + 1.
     A row that sees nothing is zeros.  A sequence that is empty or not within the tensors is passed over, and rows of no sequence are
     left as they are (anything, where ``out`` is made here); no two sequences may share a row of q.  A key or value that is infinite or
-    NaN reaches no token before it.
+    NaN reaches no token before it.  (``PLA_SANITY_CHECK=1`` takes a sequence of fewer keys than tokens for a mistake and names it.)
 
     scale (default D^-0.5) applies to the scores; output_gate [T, HQ, D] multiplies the result by its sigmoid.  Softmax statistics and
     sums are float32; weights are rounded once to q's type before they meet the values (off by half a step of it, as much as the
