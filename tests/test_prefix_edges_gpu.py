@@ -119,3 +119,17 @@ def test_large_values_under_weights_of_nothing(D, HQ, HKV, prefix, own, far, cro
     caches[1][block, place, :, 7] = -math.inf
     got = _call(q, caches, table, [own], prefix, crowd)
     assert (got[..., 7] == -math.inf).all() and torch.isfinite(got[..., :7]).all() and torch.isfinite(got[..., 8:]).all()
+
+
+@pytest.mark.parametrize("D, act, HQ, HKV", SHAPES)
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_rows_of_no_request_may_hold_anything(D, act, HQ, HKV, value, crowd):
+    lengths, windows, prefix = [50, 300, 1, 9], [2, 3, 1, 0], 4001
+    caches, table, _ = _cache16(lengths + [prefix], HKV, D, 16, act, seed=D)
+    q = _randn(5, 40, HQ, D, dtype=DTYPES[act], scale=1.5)
+    sane = _call(q[:6], caches, table, lengths, prefix, crowd, windows)
+    q[6:] = value
+    out = torch.full_like(q, 5.0)
+    _call(q, caches, table, lengths, prefix, crowd, windows, out=out)
+    assert (out[6:] == 5).all()
+    torch.testing.assert_close(out[:6].float(), sane.float(), atol=2 ** -7, rtol=2 ** -6)       # other pieces, so other roundings
