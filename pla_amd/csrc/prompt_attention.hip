@@ -686,7 +686,7 @@ PromptLaunch prompt_launch(int batch, int64_t tokens, int HQ, int HKV, int D, in
   l.pieces = !l.split ? 0 : fill > 1 ? fill : 1;
   // Room for them, and workgroups: no block has more pieces than its keys have `least` tiles for, whatever the chip could take.  (A
   // prefix has room for any length.)
-  const int64_t allowed = l.blocks * ((prompt_tiles((int)keys) - 1) / l.least);
+  const int64_t allowed = l.blocks * (((keys + PROMPT_KEYS - 1) / PROMPT_KEYS - 1) / l.least);
   l.items = l.blocks + (!prefix && l.pieces > allowed ? allowed : l.pieces);
   // A list of the items: for pieces, and where every workgroup would look through many sequences for its own (prompts of 64 tokens, 16 + 2
   // heads: 128 of them 28.5 us with a list and 25.2 without, 300 54 and 61, 1000 161 and 279), unless it is long itself.

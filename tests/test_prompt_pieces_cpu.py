@@ -13,3 +13,9 @@ def test_no_more_than_the_keys_can_be_cut_into(batch, tokens, HQ, HKV, D, keys):
     most = slots * (4 * D + 8) + items * 48                   # outputs, maxima and sums; the list
     size = _lib.load().pla_prompt_attention_workspace_bytes(batch, tokens, HQ, HKV, D, keys)
     assert 0 < size <= most + 3 * 256
+
+
+def test_more_keys_never_take_less():
+    size = _lib.load().pla_prompt_attention_workspace_bytes
+    sizes = [size(12, 1200, 16, 2, 128, keys) for keys in (1200, 2000, 30000, 2 ** 30, 2 ** 31, 2 ** 32 + 70, 2 ** 40)]
+    assert sizes == sorted(sizes) and sizes[0] < sizes[1]
